@@ -189,16 +189,18 @@ def _plain_append(st):
     return [st.k_pages, st.v_pages]
 
 
-def _gather(pages, table, length, page):
-    x = pages[table[: -(-length // page)].long()].float()  # [n, Hkv, page, D]
-    return x.permute(1, 0, 2, 3).reshape(x.shape[1], -1, x.shape[3])[:, :length]
+def _gather(pages, table, page):
+    """The pages of some sequences side by side, [sequences, Hkv, keys, D]."""
+    x = pages[table.long()].float()  # [sequences, n, Hkv, page, D]
+    return x.permute(0, 2, 1, 3, 4).reshape(x.shape[0], x.shape[2], -1, x.shape[4])
 
 
-def _part(q, keys, values, visible):
-    """Largest score, sum and products of exponentials of rows against some keys; visible: None or [rows, keys]."""
-    s = torch.matmul(q, keys.transpose(1, 2))
-    if visible is not None:
-        s = s.masked_fill(~visible, -math.inf)
+def _part(st, q, table, last):
+    """Largest score, sum and products of exponentials of the rows q, [sequences, Hkv, rows, D], against the pages of their sequences;
+    last: the last key each of them sees, [sequences, rows]."""
+    keys, values = (_gather(p, table, st.case["page"]) for p in (st.k_pages, st.v_pages))
+    s = torch.matmul(q, keys.transpose(2, 3))
+    s = s.masked_fill(torch.arange(s.shape[3], device=s.device) > last[:, None, :, None], -math.inf)
     m = s.amax(-1, keepdim=True)
     e = torch.exp(s - m)
     return m, e.sum(-1, keepdim=True), torch.matmul(e, values)
@@ -214,27 +216,27 @@ def _plain_attend(st):
         q = _rotate(q, st.cos[prefix + pos][:, None], st.sin[prefix + pos][:, None])
     if case["qk_norm"]:
         q = _unit(q)
-    q = q * st.gain / math.sqrt(D)
-    q = q.unflatten(1, (Hkv, rep)).permute(1, 0, 2, 3)  # [Hkv, T, rep, D]
-    o = torch.empty_like(q)
+    q = (q * st.gain / math.sqrt(D)).unflatten(1, (Hkv, rep))  # [T, Hkv, rep, D]
+    if case["step"] == "token":
+        m, l, y = _part(st, q, st.block_table, pos[:, None].expand(-1, rep))
+    else:  # ragged rows: one sequence after the other
+        parts = []
+        for b, length in enumerate(st.lens):
+            rows = slice(st.starts[b], st.starts[b + 1])
+            some = _part(st, q[None, rows].transpose(1, 2).flatten(2, 3), st.block_table[b:b + 1, : -(-length // page)], pos[None, rows].repeat_interleave(rep, 1))
+            parts.append([x[0].unflatten(1, (-1, rep)).transpose(0, 1) for x in some])
+        m, l, y = (torch.cat(x) for x in zip(*parts))
     if prefix:
-        pm, pl, po = _part(q.reshape(Hkv, -1, D), _gather(st.k_pages, st.prefix_table, prefix, page), _gather(st.v_pages, st.prefix_table, prefix, page), None)
-    for b, (n, length) in enumerate(zip(st.rows, st.lens)):
-        r0, r1 = st.starts[b], st.starts[b + 1]
-        keys = torch.arange(length, device=q.device)
-        visible = (keys[None] <= pos[r0:r1].repeat_interleave(rep)[:, None]) if n > 1 else None
-        m, l, y = _part(q[:, r0:r1].reshape(Hkv, -1, D), _gather(st.k_pages, st.block_table[b], length, page),
-                        _gather(st.v_pages, st.block_table[b], length, page), visible)
-        if prefix:
-            at = slice(r0 * rep, r1 * rep)
-            top = torch.maximum(m, pm[:, at])
-            a, c = torch.exp(m - top), torch.exp(pm[:, at] - top)
-            l, y = a * l + c * pl[:, at], a * y + c * po[:, at]
-        o[:, r0:r1] = (y / l).unflatten(1, (n, rep))
-    o = o.permute(1, 0, 2, 3).reshape(-1, H, D)
+        end = torch.full((1, q.shape[0] * rep), prefix - 1, device=q.device)
+        some = _part(st, q[None].transpose(1, 2).flatten(2, 3), st.prefix_table[None], end)
+        pm, pl, py = (x[0].unflatten(1, (-1, rep)).transpose(0, 1) for x in some)
+        top = torch.maximum(m, pm)
+        a, c = torch.exp(m - top), torch.exp(pm - top)
+        l, y = a * l + c * pl, a * y + c * py
+    y = (y / l).flatten(1, 2)
     if case["gate"]:
-        o = o * (_GATE_SCALE * torch.sigmoid(st.gate.float()))[..., None]
-    return o.to(st.q.dtype)
+        y = y * (_GATE_SCALE * torch.sigmoid(st.gate.float()))[..., None]
+    return y.to(st.q.dtype)
 
 
 def run(st):

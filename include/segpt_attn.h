@@ -59,6 +59,7 @@ extern "C" {
 #define SEGPT_E_ALIGN -10      /* a base pointer is not 16-byte aligned                     */
 #define SEGPT_E_ROPE -12       /* rope tables: one NULL, misaligned, or too short for the positions */
 #define SEGPT_E_STAGE -11      /* unknown stage passed to segpt_attn_bwd_stage              */
+#define SEGPT_E_PAGES -14      /* paged cache: page size no power of two from 8 to 65536, no pages, or a table that is too wide */
 #define SEGPT_E_SCRATCH_LIMIT -13 /* segpt_attn_fwd_noalloc: shape needs more than SEGPT_NOALLOC_SCRATCH_BYTES */
 
 /* size of the library-owned device scratch behind segpt_attn_fwd_noalloc (per GPU, held for the process lifetime) */
@@ -274,6 +275,85 @@ typedef struct segpt_linear_rows_params {
 /* Rows of x and of the weights are whole 16-byte pieces at 16-byte aligned addresses (SEGPT_E_ALIGN / SEGPT_E_STRIDE otherwise,
  * nothing launched); the outputs must not overlap x, the weights or each other. */
 int segpt_linear_rows(const segpt_linear_rows_params* p, void* stream);
+
+/* ---- Paged key/value cache.
+ * The rows of a sequence's keys and values lie in pages of page_size rows; block_table[b][j] is the page that holds its keys
+ * j * page_size .. (j + 1) * page_size - 1.  Sequences of unequal lengths share one pool and one call.  The pool holds PREPARED rows:
+ *   k'_j = rot(k_j) * rsqrt(mean_d k_j^2 + eps)      (rotation and normaliser as above, each only if asked for; one rounding)
+ *   v'_j = c1 v_j + c2 v_first_j                     (if vr_coef != NULL)
+ * so that a key is rotated and normalised once, when it is appended, and not again for every token generated after it.  The reference
+ * has no paged cache; its cache is the concatenation attention.py:15-27.
+ *
+ * Rows: T rows of q (k, v), the rows of one sequence side by side: seq_start[b] .. seq_start[b + 1] - 1, or T / B each where
+ * seq_start is NULL.  kv_len[b] counts the keys of sequence b INCLUDING the rows of the call: with n rows, row i stands at position
+ * kv_len[b] - n + i, is appended there, and sees keys 0 .. kv_len[b] - n + i.  Rotary angles are those of rope_pos0 + position.
+ * Lengths, row ranges and tables are read on the device, when the kernels run: a captured call follows them.
+ *
+ * What the host cannot see is checked where it is used, and nothing outside the given tensors is read or written:
+ *   - row ranges are cut off at 0 and T; rows in no sequence are left alone (SEGPT_FLAG_ZERO_REST: segpt_paged_attn sets them to 0);
+ *   - a row that sees no key gives y = 0, lse = -inf;
+ *   - append: a row whose position is negative or max_len or more, or whose page number is not in the pool, is left out;
+ *   - attention: a sequence with kv_len < 0 or above max_len, or with a page number that is not in the pool among
+ *     those of its keys, gives NaN in every row that sees one of these (it may give NaN in its other rows).
+ * Row ranges must not overlap, and two rows of one append must not name one slot: which of them is kept is undefined. */
+#define SEGPT_FLAG_ZERO_REST 32  /* segpt_paged_attn: rows of o that belong to no sequence are set to zero */
+
+/* [T, heads, D] tensor view; the D axis is contiguous. Strides in ELEMENTS. */
+typedef struct segpt_rows {
+  void* ptr;
+  int64_t stride_t, stride_h;
+} segpt_rows;
+
+typedef struct segpt_paged_params {
+  uint32_t struct_bytes; /* = sizeof(segpt_paged_params) */
+  int32_t dtype;         /* SEGPT_DTYPE_*: rows and pool */
+  int32_t T, B, H, Hkv, D;
+  int32_t n_pages, page_size; /* of the pool; page_size a power of two, 8 .. 65536 */
+  int32_t table_width;        /* pages per row of block_table */
+  int32_t max_len;            /* no sequence holds more keys; 0 = table_width * page_size, and never more than that */
+  int32_t prefix_len;         /* segpt_paged_attn: keys of the shared prefix, 0 = none */
+  int32_t gq_numel, gk_numel;
+  int32_t flags; /* SEGPT_FLAG_NO_NORM, SEGPT_FLAG_ZERO_REST */
+  float eps, sm_scale, gate_scale;
+  int32_t rope_len, rope_pos0; /* rope_pos0 + prefix_len + max_len must not exceed rope_len */
+
+  segpt_tensor4 k_pages; /* [n_pages, Hkv, page_size, D]: stride_b from page to page; append: out, attention: in */
+  segpt_tensor4 v_pages;
+  const int32_t* block_table; /* [B, table_width] device */
+  int64_t table_stride;       /* elements between its rows */
+  const int32_t* kv_len;      /* [B] device */
+  const int32_t* seq_start;   /* [B + 1] device, not decreasing, or NULL */
+  const float* rope_cos;      /* [rope_len, D/2] fp32 device, 16 B aligned, or NULL */
+  const float* rope_sin;
+
+  /* append */
+  segpt_rows k, v;      /* [T, Hkv, D] in */
+  segpt_rows v_first;   /* [T, Hkv, D] in, optional */
+  const float* vr_coef; /* [2] fp32 device (c1, c2) or NULL */
+
+  /* attention */
+  segpt_rows q;    /* [T, H, D] in  */
+  segpt_rows o;    /* [T, H, D] out */
+  segpt_rows gate; /* [T, H] logits, in, optional: element (t, h) at t * stride_t + h * stride_h */
+  float* lse;      /* [T, H] fp32 out, natural log, or NULL */
+  const float* g_q; /* [gq_numel] fp32 device */
+  const float* g_k; /* [gk_numel] fp32 device or NULL */
+  const int32_t* prefix_table; /* pages of the shared prefix's keys, device; NULL = none */
+  void* workspace;             /* >= segpt_paged_workspace_bytes(p), 256 B aligned; contents undefined on entry and exit */
+  size_t workspace_bytes;
+} segpt_paged_params;
+
+/* Appends the rows of k and v (mixed with v_first) to the pages of their sequences. */
+int segpt_paged_append(const segpt_paged_params* p, void* stream);
+
+/* Bytes of device scratch segpt_paged_attn needs for these params (sizes only; 0 for invalid ones). */
+size_t segpt_paged_workspace_bytes(const segpt_paged_params* p);
+
+/* Attention of the rows of q over the pages of their sequences.  With prefix_table every row also sees the prefix_len keys of
+ * the prefix's pages, which come before the sequence's own (a sequence's positions then start at prefix_len); they are read once for the
+ * whole batch, not once a sequence.  A row then stands at position prefix_len + kv_len[b] - n + i, with n > kv_len[b] among the
+ * prefix's own keys (as its last token does, in a sequence without keys yet), and sees what is at or before that.  Forward only. */
+int segpt_paged_attn(const segpt_paged_params* p, void* stream);
 
 #ifdef __cplusplus
 }

@@ -20,6 +20,8 @@ SEGPT_FLAG_RUNNING_MAX = 2
 SEGPT_FLAG_DECODE = 4
 SEGPT_FLAG_NO_NORM = 8
 SEGPT_FLAG_F32_SPLIT = 16
+SEGPT_FLAG_ZERO_REST = 32
+SEGPT_E_PAGES = -14
 SEGPT_E_SCRATCH_LIMIT = -13
 SEGPT_NOALLOC_SCRATCH_BYTES = 16 << 20
 SEGPT_WS_KV = 0
@@ -40,6 +42,9 @@ EXPORTED_SYMBOLS = (
     "segpt_attn_fwd_noalloc",
     "segpt_kv_append",
     "segpt_linear_rows",
+    "segpt_paged_append",
+    "segpt_paged_workspace_bytes",
+    "segpt_paged_attn",
 )
 
 
@@ -89,6 +94,36 @@ class LinearRowsParams(C.Structure):
                 ("x", C.c_void_p), ("x_stride", C.c_int64), ("seg", LinearSegment * 4)]
 
 
+class Rows(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("stride_t", C.c_int64), ("stride_h", C.c_int64)]
+
+
+class PagedParams(C.Structure):
+    _fields_ = [
+        ("struct_bytes", C.c_uint32),
+        ("dtype", C.c_int32),
+        ("T", C.c_int32), ("B", C.c_int32), ("H", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32),
+        ("n_pages", C.c_int32), ("page_size", C.c_int32),
+        ("table_width", C.c_int32),
+        ("max_len", C.c_int32),
+        ("prefix_len", C.c_int32),
+        ("gq_numel", C.c_int32), ("gk_numel", C.c_int32),
+        ("flags", C.c_int32),
+        ("eps", C.c_float), ("sm_scale", C.c_float), ("gate_scale", C.c_float),
+        ("rope_len", C.c_int32), ("rope_pos0", C.c_int32),
+        ("k_pages", Tensor4), ("v_pages", Tensor4),
+        ("block_table", C.c_void_p), ("table_stride", C.c_int64),
+        ("kv_len", C.c_void_p), ("seq_start", C.c_void_p),
+        ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p),
+        ("k", Rows), ("v", Rows), ("v_first", Rows), ("vr_coef", C.c_void_p),
+        ("q", Rows), ("o", Rows), ("gate", Rows),
+        ("lse", C.c_void_p),
+        ("g_q", C.c_void_p), ("g_k", C.c_void_p),
+        ("prefix_table", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -133,6 +168,12 @@ def load():
         lib.segpt_kv_append.argtypes = [C.c_int] * 5 + [C.POINTER(Tensor4)] * 4 + [C.c_void_p]
         lib.segpt_linear_rows.restype = C.c_int
         lib.segpt_linear_rows.argtypes = [C.POINTER(LinearRowsParams), C.c_void_p]
+        lib.segpt_paged_append.restype = C.c_int
+        lib.segpt_paged_append.argtypes = [C.POINTER(PagedParams), C.c_void_p]
+        lib.segpt_paged_workspace_bytes.restype = C.c_size_t
+        lib.segpt_paged_workspace_bytes.argtypes = [C.POINTER(PagedParams)]
+        lib.segpt_paged_attn.restype = C.c_int
+        lib.segpt_paged_attn.argtypes = [C.POINTER(PagedParams), C.c_void_p]
         ver = lib.segpt_abi_version()
         if ver != SEGPT_ABI_VERSION:
             raise RuntimeError(f"libsegpt_attn.so ABI version {ver}, binding expects {SEGPT_ABI_VERSION}")

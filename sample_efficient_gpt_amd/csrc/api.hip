@@ -252,6 +252,7 @@ const char* segpt_strerror(int code) {
     case SEGPT_E_ROPE: return "rope tables: both or neither, 16-byte aligned, rope_len >= position + rows";
     case SEGPT_E_STAGE: return "unknown stage (expected SEGPT_FWD_STAGE_* / SEGPT_BWD_STAGE_*)";
     case SEGPT_E_SCRATCH_LIMIT: return "segpt_attn_fwd_noalloc: the key/value scratch this shape needs exceeds SEGPT_NOALLOC_SCRATCH_BYTES";
+    case SEGPT_E_PAGES: return "paged cache: page_size must be a power of two from 8 to 65536, the pool must have pages, and a table's keys must be fewer than 2^31";
     default: return code > 0 ? "HIP runtime error raised by a kernel launch" : "unknown segpt error code";
   }
 }

@@ -14,6 +14,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/FuncTorchTLS.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/autocast_mode.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
@@ -486,6 +487,161 @@ std::optional<std::tuple<Tensor, Tensor, Tensor>> generation_step(const Tensor& 
   return std::make_tuple(out, kbuf.narrow(2, 0, need), vbuf.narrow(2, 0, need));
 }
 
+// ---- the paged cache
+segpt_rows view_rows(const Tensor& t) {
+  if (!t.defined()) return {nullptr, 0, 0};
+  return {t.data_ptr(), t.stride(0), t.stride(1)};
+}
+void no_gradient_asked(const char* what, std::initializer_list<const Tensor*> all) {
+  for (const Tensor* t : all)
+    if (t->defined() && ((at::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined()))
+      throw CheckFailed(std::string(what) + " has no derivative: call it under torch.no_grad() or on detached tensors");
+  if (const auto& transforms = at::functorch::functorchTLSAccessor()) transforms->checkSupportsCppAutogradFunction();
+}
+// What appending and attending have in common: pool, table, lengths, angles.  rows: k or q
+void fill_paged(segpt_paged_params& p, const Tensor& rows, const char* name, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
+                const Tensor& kv_len, const Tensor& seq_start, const Tensor& cos, const Tensor& sin, int64_t pos0, std::optional<int64_t> max_len,
+                double eps, bool qk_norm) {
+  const auto dt = rows.scalar_type();
+  const auto dev = rows.device();
+  if (dt != at::kBFloat16 && dt != at::kFloat) throw BadType(std::string("the paged cache supports bfloat16 and float32 tensors, got ") + c10::toString(dt));
+  check(rows.is_cuda(), "the paged cache works on device tensors");
+  check(rows.dim() == 3, (std::string(name) + " must be [rows, heads, head_dim]").c_str());
+  for (const Tensor* t : {&k_pages, &v_pages}) {
+    if (t->scalar_type() != dt) throw BadType(std::string("the pages have dtype ") + c10::toString(t->scalar_type()) + ", expected " + c10::toString(dt));
+    check(t->device() == dev, "all tensors must be on one device");
+    check(t->dim() == 4 && t->sizes() == k_pages.sizes() && t->size(3) == rows.size(2) && (t->stride(3) == 1 || t->size(3) == 1),
+          "the pages must be [pages, kv heads, page size, head_dim], contiguous in head_dim");
+  }
+  auto indices = [&](const Tensor& t, const char* what) {
+    if (t.scalar_type() != at::kInt) throw BadType(std::string(what) + " must be int32, got " + c10::toString(t.scalar_type()));
+    check(t.device() == dev, "all tensors must be on one device");
+  };
+  indices(table, "block_table");
+  indices(kv_len, "kv_len");
+  check(table.dim() == 2 && (table.size(1) <= 1 || table.stride(1) == 1), "block_table must be [sequences, pages], contiguous in pages");
+  check(kv_len.dim() == 1 && kv_len.size(0) == table.size(0) && kv_len.is_contiguous(), "kv_len must be contiguous, one entry a sequence");
+  if (seq_start.defined()) {
+    indices(seq_start, "seq_start");
+    check(seq_start.dim() == 1 && seq_start.size(0) == table.size(0) + 1 && seq_start.is_contiguous(), "seq_start must be contiguous, one entry a sequence and one more");
+  } else {
+    check(table.size(0) > 0 && rows.size(0) % table.size(0) == 0, "without seq_start every sequence has the same number of rows");
+  }
+  check(rows.size(0) < (int64_t{1} << 30) && table.size(0) <= INT32_MAX && table.size(1) <= INT32_MAX && k_pages.size(0) <= INT32_MAX &&
+        k_pages.size(2) <= INT32_MAX && pos0 >= 0 && pos0 <= INT32_MAX, "a size does not fit 32 bits");
+  check(!max_len.has_value() || *max_len > 0, "max_len must be positive");
+  p.struct_bytes = sizeof(p);
+  p.dtype = dt == at::kFloat ? SEGPT_DTYPE_FP32 : SEGPT_DTYPE_BF16;
+  p.T = (int32_t)rows.size(0); p.B = (int32_t)table.size(0); p.Hkv = (int32_t)k_pages.size(1); p.D = (int32_t)rows.size(2);
+  p.n_pages = (int32_t)k_pages.size(0); p.page_size = (int32_t)k_pages.size(2);
+  p.table_width = (int32_t)table.size(1);
+  p.max_len = max_len.has_value() ? (int32_t)std::min<int64_t>(*max_len, INT32_MAX) : 0;
+  p.flags = qk_norm ? 0 : SEGPT_FLAG_NO_NORM;
+  p.eps = (float)eps;
+  p.k_pages = view4(k_pages, 0); p.v_pages = view4(v_pages, 0);
+  p.block_table = ptr_of<int32_t>(table);
+  p.table_stride = table.stride(0);
+  p.kv_len = ptr_of<int32_t>(kv_len);
+  p.seq_start = ptr_of<int32_t>(seq_start);
+  check(cos.defined() == sin.defined(), "rope_cos and rope_sin go together");
+  if (cos.defined()) {
+    check(cos.dim() == 2 && cos.sizes() == sin.sizes() && cos.size(1) == rows.size(2) / 2 && cos.size(0) <= INT32_MAX, "rope tables must be [len, head_dim // 2]");
+    p.rope_cos = ptr_of<float>(cos); p.rope_sin = ptr_of<float>(sin);
+    p.rope_len = (int32_t)cos.size(0);
+    p.rope_pos0 = (int32_t)pos0;
+  }
+}
+
+void paged_append(const Tensor& k_in, const Tensor& v_in, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& kv_len,
+                  const OptTensor& seq_start, const OptTensor& ov_first, const OptTensor& ocoef, double eps, bool qk_norm, const OptTensor& ocos,
+                  const OptTensor& osin, int64_t pos0, std::optional<int64_t> max_len) {
+  const Tensor first_in = defined_or_none(ov_first), coef = defined_or_none(ocoef);
+  no_gradient_asked("paged_kv_append", {&k_in, &v_in, &k_pages, &v_pages, &first_in, &coef});
+  const auto dev = k_in.device();
+  const Tensor k = last_dim_contiguous(k_in), v = last_dim_contiguous(v_in), v_first = last_dim_contiguous(first_in);
+  const Tensor cos = f32_table(defined_or_none(ocos), dev), sin = f32_table(defined_or_none(osin), dev), c32 = f32_vector(coef, dev);
+  segpt_paged_params p{};
+  fill_paged(p, k, "k", k_pages, v_pages, table, kv_len, defined_or_none(seq_start), cos, sin, pos0, max_len, eps, qk_norm);
+  check(k.size(1) == k_pages.size(1), "k must have the pages' number of kv heads");
+  check(v_first.defined() == coef.defined(), "v_first and vr_coef go together");
+  for (const Tensor* t : {&v, &v_first})
+    if (t->defined()) {
+      if (t->scalar_type() != k.scalar_type()) throw BadType(std::string("v and v_first must have k's dtype, got ") + c10::toString(t->scalar_type()));
+      check(t->device() == dev, "all tensors must be on one device");
+      check(t->sizes() == k.sizes(), "v and v_first must have k's shape");
+    }
+  if (coef.defined()) check(coef.numel() == 2, "vr_coef must have two elements");
+  for (const Tensor* t : {&k_pages, &v_pages})
+    check(!t->is_inference() || c10::InferenceMode::is_enabled(), "pages made in inference mode can be appended to in inference mode only");
+  if (k.numel() == 0) return;
+  p.k = view_rows(k); p.v = view_rows(v); p.v_first = view_rows(v_first);
+  p.vr_coef = ptr_of<float>(c32);
+  const c10::DeviceGuard guard(dev);
+  const int rc = segpt_paged_append(&p, current_stream(dev));
+  if (rc) throw LibraryError(rc, "segpt_paged_append");
+  for (const Tensor* t : {&k_pages, &v_pages})
+    if (!t->is_inference()) torch::autograd::impl::bump_version(*t);
+}
+
+std::pair<Tensor, Tensor> paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& v_pages, const OptTensor& oprefix, int64_t prefix_len,
+                                          const Tensor& table, const Tensor& kv_len, const Tensor& g_q, const OptTensor& og_k, const OptTensor& seq_start,
+                                          const OptTensor& ogate, double gate_scale, double eps, std::optional<double> sm_scale, bool qk_norm,
+                                          const OptTensor& ocos, const OptTensor& osin, int64_t pos0, std::optional<int64_t> max_len,
+                                          const OptTensor& oout, bool with_lse) {
+  const Tensor g_k = defined_or_none(og_k), gate = defined_or_none(ogate), prefix = defined_or_none(oprefix), out = defined_or_none(oout);
+  no_gradient_asked("paged attention", {&q_in, &k_pages, &v_pages, &g_q, &g_k, &gate, &out});
+  const auto dev = q_in.device();
+  const Tensor q = last_dim_contiguous(q_in);
+  const Tensor cos = f32_table(defined_or_none(ocos), dev), sin = f32_table(defined_or_none(osin), dev);
+  const Tensor gq32 = f32_vector(g_q, dev), gk32 = f32_vector(g_k, dev);
+  segpt_paged_params p{};
+  fill_paged(p, q, "q", k_pages, v_pages, table, kv_len, defined_or_none(seq_start), cos, sin, pos0, max_len, eps, qk_norm);
+  check(k_pages.size(1) > 0 && q.size(1) % k_pages.size(1) == 0, "number of query heads must be a multiple of the kv heads");
+  check(gq32.numel() == 1 || gq32.numel() == q.size(2), "gain must have 1 or head_dim elements");
+  check(!gk32.defined() || gk32.numel() == 1 || gk32.numel() == q.size(2), "k_gain must have 1 or head_dim elements");
+  check(prefix_len >= 0 && prefix_len <= INT32_MAX, "prefix_len must not be negative");
+  if (prefix.defined()) {
+    if (prefix.scalar_type() != at::kInt) throw BadType(std::string("prefix_table must be int32, got ") + c10::toString(prefix.scalar_type()));
+    check(prefix.device() == dev, "all tensors must be on one device");
+    const int64_t page = std::max<int64_t>(k_pages.size(2), 1);
+    check(prefix.dim() == 1 && prefix.is_contiguous() && prefix.size(0) >= (prefix_len + page - 1) / page, "prefix_table must name every page of the prefix");
+  }
+  if (gate.defined()) {
+    if (gate.scalar_type() != q.scalar_type()) throw BadType(std::string("gate_logits must have q's dtype, got ") + c10::toString(gate.scalar_type()));
+    check(gate.device() == dev, "all tensors must be on one device");
+    check(gate.dim() == 2 && gate.size(0) == q.size(0) && gate.size(1) == q.size(1), "gate_logits must be [rows, heads]");
+  }
+  if (out.defined()) {
+    if (out.scalar_type() != q.scalar_type()) throw BadType(std::string("out must have q's dtype, got ") + c10::toString(out.scalar_type()));
+    check(out.device() == dev && out.sizes() == q.sizes() && (out.stride(2) == 1 || out.size(2) == 1), "out must have q's shape and device, contiguous in head_dim");
+    check(out.data_ptr() != q.data_ptr() || q.numel() == 0, "out must not be q: a row is read again after others are written");
+    at::assert_no_overlap(out, q);
+    check(!out.is_inference() || c10::InferenceMode::is_enabled(), "out made in inference mode can be written in inference mode only");
+  }
+  const Tensor y = out.defined() ? out : at::empty(q.sizes(), q.options());
+  const Tensor lse = with_lse ? at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat)) : Tensor();
+  if (q.numel() == 0) return {y, lse};
+  p.H = (int32_t)q.size(1);
+  p.prefix_len = prefix.defined() ? (int32_t)prefix_len : 0;
+  p.prefix_table = prefix_len > 0 ? ptr_of<int32_t>(prefix) : nullptr;
+  p.gq_numel = (int32_t)gq32.numel();
+  p.gk_numel = gk32.defined() ? (int32_t)gk32.numel() : 0;
+  p.sm_scale = (float)(sm_scale.has_value() ? *sm_scale : 1.0 / std::sqrt((double)q.size(2)));
+  p.gate_scale = (float)gate_scale;
+  if (!out.defined()) p.flags |= SEGPT_FLAG_ZERO_REST;
+  p.q = view_rows(q); p.o = view_rows(y); p.gate = view_rows(gate);
+  p.lse = ptr_of<float>(lse);
+  p.g_q = ptr_of<float>(gq32); p.g_k = ptr_of<float>(gk32);
+  const size_t bytes = segpt_paged_workspace_bytes(&p);
+  const Tensor ws = at::empty({(int64_t)(bytes < 256 ? 256 : bytes)}, at::TensorOptions().dtype(at::kByte).device(dev));
+  p.workspace = ws.data_ptr(); p.workspace_bytes = (size_t)ws.numel();
+  const c10::DeviceGuard guard(dev);
+  const int rc = segpt_paged_attn(&p, current_stream(dev));
+  if (rc) throw LibraryError(rc, "segpt_paged_attn");
+  if (out.defined() && !out.is_inference()) torch::autograd::impl::bump_version(out);
+  return {y, lse};
+}
+
 // What torch raises (out of memory, an error from a saved-tensor hook) keeps its Python type across the binding
 template <typename R, typename... A>
 auto bound(R (*f)(A...)) {
@@ -525,4 +681,6 @@ PYBIND11_MODULE(_segpt_torch, m) {
   m.def("op_backward", bound(&op_backward));
   m.def("kv_append", bound(&kv_append));
   m.def("generation_step", bound(&generation_step));
+  m.def("paged_append", bound(&paged_append));
+  m.def("paged_attention", bound(&paged_attention));
 }

@@ -11,6 +11,7 @@ from torch.nn.modules import module as _module
 from . import _native
 from .function import QKNormFlashAttnFunc, _call_flags
 from .library_op import _seen_as_operator
+from .paged import PagedKVCache
 
 
 class SelfDotProductAttnQKNorm(nn.Module):
@@ -153,7 +154,8 @@ class MultiHeadSelfAttention(nn.Module):
     the projection output (no ``rearrange(...).contiguous()``), the rotary embedding and the RMS normalisation
     are applied as the rows are loaded, GQA heads are indexed instead of expanded, the value-residual mix is
     folded into the V loads, the per-head gate into the output write, and the output lands in ``b seq (h d)``
-    layout for the output projection.  ``kv_cache`` is this package's ``KVCache`` (raw, un-expanded keys).
+    layout for the output projection.  ``kv_cache`` is this package's ``KVCache`` (raw, un-expanded keys) or, for sequences of
+    unequal lengths and forward only, a ``PagedKVCache`` whose table has been extended for the rows of ``x``.
 
     Differences a caller can see: a layer that is handed ``v1`` returns ``None`` as its second output unless
     ``always_return_values`` is set (the reference's model only ever uses the first layer's, transformer.py:135-136);
@@ -232,10 +234,42 @@ class MultiHeadSelfAttention(nn.Module):
             kv_cache.keys, kv_cache.values = step[1:]
         return step
 
-    def forward(self, x, token_positions=None, v1=None, kv_cache: KVCache | None = None):
+    def _paged_forward(self, x, v1, cache):
+        """`x` is the rows the cache's table was extended for: [b, S, d_model], or [1, rows, d_model] where the sequences have unequal
+        numbers of them.  Values are handed on for these rows only: what earlier ones mixed is in the pages."""
+        b, S, d_model = x.shape
+        H, Hkv = self.n_heads, self.n_kv_heads
+        d = d_model // H
+        rows = self.qkv(x).flatten(0, 1)
+        q, k, v = (t.unflatten(-1, (-1, d)) for t in rows.split([H * d, Hkv * d, Hkv * d], dim=-1))
+        v_first = vr_coef = None
+        v_rows = v if v1 is None or self.always_return_values else None
+        if self.value_residual:
+            v_first = v if v1 is None else v1.permute(0, 2, 1, 3).reshape(v.shape)
+            vr_coef = self._mix_coefficients()
+            if v_rows is not None:
+                v_rows = (vr_coef[0] * v.float() + vr_coef[1] * v_first.float()).to(v.dtype)
+        cache.append(k, v, v_first=v_first, vr_coef=vr_coef, eps=_EPS, qk_norm=self.qknorm, rope_cos=self.rope.cos, rope_sin=self.rope.sin)
+        gate_logits = None
+        if self.gating in ("per-head", "per-head-hd"):
+            gate_logits = self.attn_gate(x if self.gating == "per-head" else x[..., :d]).flatten(0, 1)
+        gain = self.sdpa_qknorm.gain if self.qknorm else self._unit_gain
+        y = cache.attend(q, gain, gate_logits=gate_logits, gate_scale=_GATE_SCALE, eps=_EPS, qk_norm=self.qknorm, rope_cos=self.rope.cos,
+                         rope_sin=self.rope.sin).reshape(b, S, H * d)
+        if self.gating == "elementwise":
+            y = (_GATE_SCALE * self.attn_gate(x).sigmoid()) * y
+        return self.out(y), None if v_rows is None else v_rows.unflatten(0, (b, S)).permute(0, 2, 1, 3)
+
+    def _mix_coefficients(self):
+        n = torch.rsqrt(self.alpha1**2 + self.alpha2**2 + 1e-8)
+        return torch.cat([self.scale * self.alpha1 * n, self.scale * self.alpha2 * n]).float()
+
+    def forward(self, x, token_positions=None, v1=None, kv_cache: KVCache | PagedKVCache | None = None):
         from .function import _canon
         from .library_op import qknorm_attention_op
 
+        if isinstance(kv_cache, PagedKVCache):
+            return self._paged_forward(x, v1, kv_cache)
         b, S, d_model = x.shape
         if S == 1 and kv_cache is not None and x.is_cuda and not torch.compiler.is_compiling():
             step = self._generation_step(x, kv_cache)
@@ -265,8 +299,7 @@ class MultiHeadSelfAttention(nn.Module):
                 v_first = _canon(v1.reshape(Hkv * b, Sk, d), Hkv)
             else:  # the reference's expanded layout: rows of a GQA group are copies, take the first of each
                 v_first = _canon(v1.reshape(H * b, Sk, d), H)[:, :: H // Hkv]
-            n = torch.rsqrt(self.alpha1**2 + self.alpha2**2 + 1e-8)
-            vr_coef = torch.cat([self.scale * self.alpha1 * n, self.scale * self.alpha2 * n]).float()
+            vr_coef = self._mix_coefficients()
             # The returned tensor only (the kernel mixes on its own, in fp32): built when a later layer can take it
             # as v1, with fp32 coefficients like the reference's promotion (attention.py:228), and, during cached
             # generation, for the new rows only.

@@ -1,0 +1,411 @@
+"""The paged cache's operators against their definition in float64 (tests/paged_util.py), on the GPU.
+
+Tolerances.  A rounding to bf16 is off by at most h = 2^-8 of the value, to fp32 by 2^-24.  Append: one rounding of a value that fp32
+arithmetic knows to a few 2^-24 of the row's largest (rotation three, normaliser at most D / 8 + 8 of them).  Attention: the query is rounded
+once, which moves a score by at most h * sum |qhat k'| =: h S and a probability by 2 h S (numerator and sum); a probability is rounded
+once, and the sum is of the rounded ones (2 h); y once: |dy| <= h ((2 S + 2) sum P |v| + |y|), element by element.  That is the worst
+case, with all roundings in one direction; as they are independent, a whole result is far nearer: three of them at h / 2 / sqrt(3) * sqrt(...)
+of y's own size, 3e-3 of its norm, and twice that is asked for.  fp32: the same with 2^-24 times the roundings of a sum of D products, D."""
+
+import math
+
+import pytest
+import torch
+
+from paged_util import EPS, F64, Batch
+from sample_efficient_gpt_amd import (KVCache, MultiHeadSelfAttention, PagedKVCache, PageTable, paged_attention, paged_kv_append,
+                                      shared_prefix_attention)
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+H_BF16, H_F32 = 2.0**-8, 2.0**-24
+
+
+def append(x, **kw):
+    paged_kv_append(x.k, x.v, x.k_pages, x.v_pages, x.block_table, x.kv_len, seq_start=x.seq_start, rope_cos=x.cos, rope_sin=x.sin, eps=EPS, **kw)
+
+
+def attend(x, **kw):
+    kw = dict(dict(seq_start=x.seq_start, rope_cos=x.cos, rope_sin=x.sin, eps=EPS), **kw)
+    if x.prefix:
+        return shared_prefix_attention(x.q, x.k_pages, x.v_pages, x.prefix_table, x.prefix, x.block_table, x.kv_len, x.g_q, **kw)
+    return paged_attention(x.q, x.k_pages, x.v_pages, x.block_table, x.kv_len, x.g_q, **kw)
+
+
+def check_pools(x, kp, vp, mix=False):
+    for got, ref, one_rounding in ((x.k_pages, kp, False), (x.v_pages, vp, not mix)):
+        size = ref.abs().amax(-1, keepdim=True)
+        h = H_BF16 if x.dtype == BF16 else H_F32
+        tol = h * ref.abs() + (x.D / 8 + 16) * H_F32 * size
+        assert ((got.to(F64) - ref).abs() <= tol).all()
+        if one_rounding:
+            assert torch.equal(got.to(F64), ref)  # a copy
+
+
+def check_y(x, y, lse, ref, norm=True):
+    y_ref, lse_ref, bound = ref
+    h = H_BF16 if x.dtype == BF16 else H_F32 * x.D
+    y, none = y.to(F64), lse_ref == -math.inf
+    assert torch.equal(none, lse == -math.inf) and (y[none] == 0).all()
+    far = (y - y_ref).abs()
+    assert (far <= h * bound + 1e-30).all(), (far - h * bound).max()
+    if norm and y_ref.numel() and y_ref.norm() > 0:
+        assert far.norm() / y_ref.norm() <= (6e-3 if x.dtype == BF16 else 5e-6)
+    # bound = (2 S + 2) sum P |v| + |y|, and a score moves by h S: with |v| left out, an upper bound of S is not at hand here
+    assert (lse.to(F64) - lse_ref)[~none].abs().max() <= (0.05 if x.dtype == BF16 else 1e-4) if (~none).any() else True
+
+
+HEADS = [(18, 6, 64, BF16), (16, 4, 128, BF16), (8, 8, 64, BF16), (6, 2, 32, F32), (8, 4, 64, F32), (4, 2, 128, F32)]
+RAGGED = [
+    ([1], [1]), ([1], [33]), ([1, 1, 1], [64, 1, 200]),
+    ([3, 1, 0, 7, 1], [3, 40, 17, 130, 129]),                # a sequence without rows
+    ([33, 1, 70], [33, 500, 100]),
+    ([2, 5], [1, 3]),                                        # rows before the first key
+    ([1] * 70, [1 + 13 * i % 90 for i in range(70)]),        # more sequences than lanes
+]
+
+
+@pytest.mark.parametrize("H,Hkv,D,dtype", HEADS)
+@pytest.mark.parametrize("rows,lens", RAGGED)
+@pytest.mark.parametrize("page", [8, 16, 64])
+def test_append(gpu_device, rows, lens, H, Hkv, D, dtype, page):
+    for i, (qk_norm, mix, rope, layout) in enumerate([(True, False, True, "phsd"), (True, True, True, "pshd"), (False, True, False, "apart")]):
+        x = Batch(rows, lens, H, Hkv, D, page, dtype, gpu_device, seed=i, rope=rope, layout=layout)
+        kp, vp = x.appended(qk_norm, mix, pos0=3 if rope else 0)
+        append(x, qk_norm=qk_norm, v_first=x.v_first if mix else None, vr_coef=x.coef if mix else None, rope_pos0=3 if rope else 0)
+        check_pools(x, kp, vp, mix)
+
+
+@pytest.mark.parametrize("H,Hkv,D,dtype", HEADS)
+@pytest.mark.parametrize("rows,lens", RAGGED)
+@pytest.mark.parametrize("page", [8, 16, 64])
+def test_attention(gpu_device, rows, lens, H, Hkv, D, dtype, page):
+    x = Batch(rows, lens, H, Hkv, D, page, dtype, gpu_device, seed=1)
+    y, lse = attend(x, gate_logits=x.gate, return_lse=True)
+    check_y(x, y, lse, x.attended(gate=True))
+    x = Batch(rows, lens, H, Hkv, D, page, dtype, gpu_device, seed=2, rope=False, layout="pshd")
+    y, lse = attend(x, g_k=x.g_k, qk_norm=False, sm_scale=0.2, return_lse=True)
+    check_y(x, y, lse, x.attended(g_k=x.g_k, qk_norm=False, sm_scale=0.2))
+
+
+@pytest.mark.parametrize("H,Hkv,D,dtype", HEADS + [(32, 2, 128, BF16), (40, 1, 64, BF16)])
+@pytest.mark.parametrize("rows,lens,prefix", [
+    ([1], [1], 1), ([1, 1, 1], [0, 5, 70], 100), ([1] * 40, [i for i in range(40)], 515), ([3, 0, 20, 1], [3, 9, 60, 0], 64), ([150, 130], [150, 260], 333),
+])
+@pytest.mark.parametrize("page", [8, 32])
+def test_shared_prefix(gpu_device, rows, lens, prefix, H, Hkv, D, dtype, page):
+    x = Batch(rows, lens, H, Hkv, D, page, dtype, gpu_device, prefix=prefix, seed=3, uniform=len(set(rows)) == 1, layout="apart")
+    y, lse = attend(x, gate_logits=x.gate, return_lse=True)
+    check_y(x, y, lse, x.attended(gate=True))
+
+
+@pytest.mark.parametrize("H,Hkv,D,dtype", [(18, 6, 64, BF16), (16, 4, 128, BF16), (8, 4, 64, F32), (4, 2, 128, F32)])
+@pytest.mark.parametrize("rows,lens,page", [
+    ([1, 1, 1], [5001, 2, 3000], 16), ([1], [9000], 8), ([300, 1, 1], [2500, 1800, 40], 32), ([2, 2], [4700, 9000], 8), ([700], [700], 64),
+    ([257, 100], [5000, 4500], 8),  # longer than the page numbers a workgroup holds at a time
+])
+def test_long_caches(gpu_device, rows, lens, page, H, Hkv, D, dtype):
+    x = Batch(rows, lens, H, Hkv, D, page, dtype, gpu_device, seed=4, uniform=len(set(rows)) == 1)
+    y, lse = attend(x, return_lse=True)
+    check_y(x, y, lse, x.attended())
+    again, _ = attend(x, return_lse=True)
+    assert torch.equal(y, again)
+
+
+@pytest.mark.parametrize("H,Hkv,D,dtype", [(18, 6, 64, BF16), (16, 4, 128, BF16), (6, 2, 32, F32), (8, 4, 64, F32)])
+def test_only_what_a_row_sees_is_looked_at(gpu_device, H, Hkv, D, dtype):
+    """Slots behind a sequence's end, other pages, and keys and values that later rows of the same call brought are not finite."""
+    rows, lens = [40, 1, 3, 70], [40, 100, 37, 200]
+    x = Batch(rows, lens, H, Hkv, D, 16, dtype, gpu_device, seed=5)
+    clean = attend(x)
+    for bad in (math.nan, math.inf, -math.inf):
+        kp, vp = x.k_pages.clone(), x.v_pages.clone()
+        used = torch.zeros(x.n_pages, x.page, dtype=torch.bool)
+        first = {}
+        for b, L in enumerate(lens):
+            for p in range(L):
+                used[int(x.block_table[b, p // 16]), p % 16] = True
+        free = (~used).to(gpu_device)[:, None, :, None].expand_as(kp)
+        x.k_pages[free] = bad
+        x.v_pages[free] = bad
+        for b, row in ((0, 20), (3, 41)):  # key and value that this row and later ones see
+            p = lens[b] - rows[b] + row
+            x.v_pages[int(x.block_table[b, p // 16]), :, p % 16, 3] = bad
+            x.k_pages[int(x.block_table[b, p // 16]), 0, p % 16, 5] = bad
+            first[b] = x.starts[b] + row
+        y = attend(x)
+        rep = H // Hkv
+        for b in range(4):
+            r0, r1 = x.starts[b], x.starts[b + 1]
+            cut = first.get(b, r1)
+            assert torch.equal(y[r0:cut], clean[r0:cut]), (bad, b)
+            if cut < r1:
+                assert not y[cut:r1, rep:, 3].isfinite().any()                       # the value's column
+                assert y[cut:r1, rep:, 4:].isfinite().all() and y[cut:r1, rep:, :3].isfinite().all()
+                if bad != bad:
+                    assert y[cut:r1, :rep].isnan().all()                              # the key's heads
+        x.k_pages.copy_(kp)
+        x.v_pages.copy_(vp)
+
+
+def test_value_that_is_infinite_is_the_answer_of_the_rows_that_see_it(gpu_device):
+    for H, Hkv, D, dtype in ((6, 2, 64, BF16), (6, 2, 64, F32)):
+        x = Batch([40], [40], H, Hkv, D, 16, dtype, gpu_device, seed=6)
+        x.v_pages[int(x.block_table[0, 1]), :, 4, 7] = math.inf  # key 20
+        y = attend(x)
+        assert (y[20:, :, 7] == math.inf).all() and y[:20].isfinite().all() and y[:, :, 8:].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype,D", [(BF16, 64), (F32, 64)])
+def test_bad_pages_and_lengths(gpu_device, dtype, D):
+    rows, lens = [1, 5, 1, 2, 1], [50, 40, 30, 60, 20]
+    x = Batch(rows, lens, 6, 2, D, 16, dtype, gpu_device, seed=7)
+    clean = attend(x)
+    x.block_table[0, 1] = x.n_pages          # just behind the pool
+    x.block_table[1, 2] = -1                 # holds keys 32 .. 47
+    x.kv_len[2] = -3
+    x.kv_len[3] = x.width * 16 + 1
+    y, lse = attend(x, return_lse=True)
+    s = x.starts
+    assert y[s[0]:s[1]].isnan().all() and y[s[1]:s[2]].isnan().all() and y[s[2]:s[4]].isnan().all() and lse[: s[4]].isnan().all()
+    assert torch.equal(y[s[4]:], clean[s[4]:])
+    before = x.k_pages.clone(), x.v_pages.clone()
+    append(x)  # sequence 0's row lies in page 3, 1's rows 35 .. 39 in the page that is not there, 4's row in its last page;
+    # of 3's two rows, at positions 63 and 64, the second is behind the table
+    changed = (x.k_pages != before[0]).flatten(2).any(-1).any(-1), (x.v_pages != before[1]).flatten(2).any(-1).any(-1)
+    for c in changed:
+        assert sorted(c.nonzero().flatten().tolist()) == sorted(int(x.block_table[b, j]) for b, j in ((0, 3), (3, 3), (4, 1)))
+
+
+def test_rows_behind_the_last_sequence(gpu_device):
+    x = Batch([1, 3, 9], [20, 40, 9], 6, 2, 64, 16, BF16, gpu_device, seed=8)
+    full = attend(x)
+    x.seq_start = torch.tensor([2, 3, 6, 8], dtype=torch.int32, device=gpu_device)  # rows 0, 1 and 8 .. 12 belong to nobody
+    out = torch.full_like(x.q, 7.0)
+    y = attend(x)
+    assert attend(x, out=out) is out
+    rest = [0, 1, 8, 9, 10, 11, 12]
+    assert (y[rest] == 0).all() and (out[rest] == 7).all() and torch.equal(y[2:8], out[2:8]) and y.isfinite().all() and not torch.equal(y, full)
+    before = x.k_pages.clone()
+    append(x)
+    assert int((x.k_pages != before).any(-1).any(1).sum()) == 6  # six slots
+    x.seq_start = torch.tensor([-5, 100, 50, 13], dtype=torch.int32, device=gpu_device)  # cut off at the rows there are; the second has none
+    attend(x)
+    append(x)
+    torch.cuda.synchronize()
+
+
+def test_max_len_limits_a_sequence(gpu_device):
+    x = Batch([1, 1], [40, 41], 6, 2, 64, 16, BF16, gpu_device, seed=9)
+    clean = attend(x)
+    cut = dict(rope_cos=x.cos[:40], rope_sin=x.sin[:40], max_len=40)  # the tables end where the sequences do
+    y = attend(x, **cut)
+    assert torch.equal(y[0], clean[0]) and y[1].isnan().all()
+    before = x.k_pages.clone()
+    paged_kv_append(x.k, x.v, x.k_pages, x.v_pages, x.block_table, x.kv_len, **cut)
+    assert (x.k_pages != before).flatten(2).any(-1).any(-1).nonzero().flatten().tolist() == [int(x.block_table[0, 2])]
+
+
+def test_pool_beyond_32_bits(gpu_device):
+    Hkv, D, page = 2, 64, 64
+    n = (5 << 30) // (Hkv * D * page * 2)  # 5 GiB of keys
+    x = Batch([1, 4], [100, 70], 6, Hkv, D, page, BF16, gpu_device, seed=10)
+    y = attend(x)
+    big_k, big_v = (torch.zeros(n, Hkv, page, D, dtype=BF16, device=gpu_device) for _ in range(2))
+    where = torch.arange(x.n_pages, device=gpu_device) * 2 + n - 2 * x.n_pages - 1
+    big_k[where], big_v[where] = x.k_pages, x.v_pages
+    moved = torch.where(x.block_table >= 0, where.to(torch.int32)[x.block_table.clamp(min=0).long()], x.block_table)
+    x.k_pages, x.v_pages, x.block_table = big_k, big_v, moved
+    assert torch.equal(attend(x), y)
+    kp, vp = (big_k[where].to(F64), big_v[where].to(F64))
+    append(x)
+    assert int((big_k[where].to(F64) != kp).any(-1).any(1).sum()) == 5
+
+
+def test_another_stream_and_a_captured_step(gpu_device):
+    """Appending and attending in a graph whose lengths and tables move on between replays; another stream; two graphs side by side."""
+    x = Batch([1, 1, 1], [30, 200, 65], 18, 6, 64, 16, BF16, gpu_device, seed=11, uniform=True, prefix=0)
+    z = Batch([1, 1], [30, 90], 18, 6, 64, 16, BF16, gpu_device, seed=12, uniform=True, prefix=130)
+
+    def step(t):
+        append(t, rope_pos0=t.prefix)
+        return attend(t, gate_logits=t.gate)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        want = step(x)
+        step(z)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(want, step(x))
+    graphs = []
+    for t in (x, z):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = step(t)
+        graphs.append((g, y, t))
+    for i in range(4):
+        for g, y, t in graphs:
+            t.kv_len.sub_(1 if i % 2 else 2)
+            t.q.copy_(torch.randn_like(t.q))
+            t.k.copy_(torch.randn_like(t.k))
+        for g, y, t in graphs:
+            g.replay()
+        got = [y.clone() for _, y, _ in graphs]
+        torch.cuda.synchronize()
+        for (g, y, t), a in zip(graphs, got):
+            assert torch.equal(a, step(t)), i
+
+
+def test_run_of_steps_against_one_pass(gpu_device):
+    """Ragged prompts, then single tokens, then a mixed step, through the table and the cache: y as the definition has it on the whole history."""
+    H, Hkv, D = 6, 2, 64
+    for dtype in (BF16, F32):
+        g = torch.Generator().manual_seed(13)
+        pages = PageTable(3, 120, 16, device=gpu_device)
+        cache = PagedKVCache(pages, Hkv, D, dtype)
+        hist = [[], [], []]
+        ang = torch.outer(torch.arange(120, dtype=F64), 10_000.0 ** (-2 * torch.arange(D // 2, dtype=F64) / D))
+        cos, sin = ang.cos().float().to(gpu_device), ang.sin().float().to(gpu_device)
+        gain = torch.ones(1, device=gpu_device)
+        for rows in ([17, 40, 5], 1, 1, [1, 30, 0], 2, [60, 1, 1]):
+            pages.extend(rows)
+            each = [rows] * 3 if isinstance(rows, int) else rows
+            T = sum(each)
+            q, k, v = (torch.randn(T, h, D, generator=g).to(dtype).to(gpu_device) for h in (H, Hkv, Hkv))
+            cache.append(k, v, rope_cos=cos, rope_sin=sin)
+            y = cache.attend(q, gain, rope_cos=cos, rope_sin=sin)
+            at = 0
+            for b, n in enumerate(each):
+                for t in range(at, at + n):
+                    hist[b].append((k[t].to(F64), v[t].to(F64)))
+                    K, V = (torch.stack([e[i] for e in hist[b]]) for i in (0, 1))
+                    L = len(K)
+                    turn = lambda x, p: torch.cat([x[..., :32] * cos[p].to(F64)[:, None] - x[..., 32:] * sin[p].to(F64)[:, None],
+                                                   x[..., :32] * sin[p].to(F64)[:, None] + x[..., 32:] * cos[p].to(F64)[:, None]], -1)
+                    unit = lambda x: x * torch.rsqrt(x.square().mean(-1, keepdim=True) + EPS)
+                    K = unit(turn(K, torch.arange(L, device=gpu_device)))
+                    Q = unit(turn(q[t:t + 1].to(F64), torch.tensor([L - 1], device=gpu_device)))[0]
+                    p = torch.softmax(torch.einsum("hd,lhd->hl", Q, K.repeat_interleave(3, 1)) / 8.0, -1)
+                    ref = torch.einsum("hl,lhd->hd", p, V.repeat_interleave(3, 1))
+                    # two roundings of the operands here (query and cached key): h S each
+                    S = torch.einsum("hd,lhd->hl", Q.abs(), K.abs().repeat_interleave(3, 1)).amax(-1, keepdim=True) / 8.0
+                    W = torch.einsum("hl,lhd->hd", p, V.abs().repeat_interleave(3, 1))
+                    h = H_BF16 if dtype == BF16 else H_F32 * D
+                    assert ((y[t].to(F64) - ref).abs() <= h * ((4 * S + 2) * W + ref.abs())).all(), (dtype, rows, b, t)
+                at += n
+        pages.release(1)
+        pages.extend([0, 3, 0])
+        assert pages.kv_len.tolist() == [len(hist[0]), 3, len(hist[2])]
+
+
+@pytest.mark.parametrize("value_residual,gating,qknorm", [(False, "per-head", True), (True, "per-head", True), (True, "elementwise", False), (False, False, True)])
+def test_module_with_a_paged_cache_is_the_module_with_its_cache(gpu_device, value_residual, gating, qknorm):
+    """Two layers, the second handed the first one's values: prompt and steps through pages against the same through ``KVCache``."""
+    torch.manual_seed(14)
+    d, H, Hkv, B = 384, 6, 2, 3
+    layers = [MultiHeadSelfAttention(d, H, Hkv, max_seq_len=100, qknorm=qknorm, value_residual=value_residual, gating=gating, device=gpu_device, dtype=BF16)
+              for _ in range(2)]
+    if value_residual:
+        with torch.no_grad():
+            for m in layers:
+                m.alpha1.fill_(0.8)
+                m.alpha2.fill_(0.5)
+    pages = PageTable(B, 100, 16, device=gpu_device)
+    paged = [PagedKVCache(pages, Hkv, d // H) for _ in layers]
+    dense = [KVCache(), KVCache()]
+    with torch.no_grad():
+        for S in (45, 1, 1, 7, 1):
+            x = torch.randn(B, S, d, device=gpu_device).to(BF16)
+            pages.extend(S)
+            outs = []
+            for caches in (dense, paged):
+                h, v1 = x, None
+                for m, c in zip(layers, caches):
+                    y, v = m(h, v1=v1, kv_cache=c)
+                    v1 = v if v1 is None else v1
+                    h = h + y
+                outs.append((h, y, v1))
+            (a, ya, va), (b, yb, vb) = outs
+            assert yb.shape == ya.shape and (yb.float() - ya.float()).norm() <= 1.5e-2 * ya.float().norm(), S
+            assert vb.shape == (B, Hkv, S, d // H)
+            if not value_residual:
+                assert torch.equal(vb, va[:, :, -S:])
+            else:
+                assert (vb.float() - va[:, :, -S:].float()).norm() <= 1e-2 * va.float().norm()
+        assert type(paged[0]) is PagedKVCache and pages.lengths == [55] * B
+
+
+def test_module_with_a_shared_prefix_and_ragged_rows(gpu_device):
+    """A prompt all sequences share, filled once, then ragged rows of their own, against every sequence by itself with all of its tokens."""
+    torch.manual_seed(15)
+    d, H, Hkv = 384, 6, 2
+    m = MultiHeadSelfAttention(d, H, Hkv, max_seq_len=256, qknorm=True, gating="per-head", device=gpu_device, dtype=BF16)
+    pages = PageTable(3, 60, 16, prefix_len=70, device=gpu_device)
+    cache = PagedKVCache(pages, Hkv, d // H)
+    with torch.no_grad():
+        common = torch.randn(1, 70, d, device=gpu_device).to(BF16)
+        pages.prefix.extend(70)
+        m(common, kv_cache=cache.of(pages.prefix))
+        own = [torch.randn(1, n, d, device=gpu_device).to(BF16) for n in (20, 1, 33)]
+        pages.extend([20, 1, 33])
+        y, _ = m(torch.cat(own, 1), kv_cache=cache)
+        tail = torch.randn(3, 1, d, device=gpu_device).to(BF16)
+        pages.extend(1)
+        y2, _ = m(tail, kv_cache=cache)
+        at = 0
+        for b, x in enumerate(own):
+            ref = m(torch.cat([common, x, tail[b:b + 1]], 1))[0]
+            n = x.shape[1]
+            got = torch.cat([y[:, at:at + n], y2[b:b + 1]], 1)
+            at += n
+            assert (got.float() - ref[:, 70:].float()).norm() <= 1.5e-2 * ref[:, 70:].float().norm()
+
+
+def test_as_operators(gpu_device):
+    """Under torch.compile the calls are nodes of the graph; results are the eager ones bit for bit."""
+    x = Batch([1, 9], [40, 20], 6, 2, 64, 16, BF16, gpu_device, seed=16, prefix=50)
+    eager_k, eager_v = x.k_pages.clone(), x.v_pages.clone()
+    paged_kv_append(x.k, x.v, eager_k, eager_v, x.block_table, x.kv_len, seq_start=x.seq_start, rope_cos=x.cos, rope_sin=x.sin, rope_pos0=50)
+    want = shared_prefix_attention(x.q, eager_k, eager_v, x.prefix_table, 50, x.block_table, x.kv_len, x.g_q, seq_start=x.seq_start, rope_cos=x.cos, rope_sin=x.sin)
+
+    def f(q, k, v, kp, vp):
+        paged_kv_append(k, v, kp, vp, x.block_table, x.kv_len, seq_start=x.seq_start, rope_cos=x.cos, rope_sin=x.sin, rope_pos0=50)
+        return shared_prefix_attention(q * 1, kp, vp, x.prefix_table, 50, x.block_table, x.kv_len, x.g_q, seq_start=x.seq_start, rope_cos=x.cos, rope_sin=x.sin)
+
+    with torch.no_grad():
+        got = torch.compile(f, backend="aot_eager", fullgraph=True)(x.q, x.k, x.v, x.k_pages, x.v_pages)
+    assert torch.equal(got, want) and torch.equal(x.k_pages, eager_k) and torch.equal(x.v_pages, eager_v)
+
+
+def test_refusals(gpu_device):
+    x = Batch([1, 2], [20, 30], 6, 2, 64, 16, BF16, gpu_device, seed=17)
+    from sample_efficient_gpt_amd._lib import SegptError
+
+    with pytest.raises(AssertionError, match="no derivative"):
+        paged_attention(x.q.clone().requires_grad_(), x.k_pages, x.v_pages, x.block_table, x.kv_len, x.g_q, seq_start=x.seq_start)
+    with pytest.raises(TypeError):
+        paged_attention(x.q, x.k_pages, x.v_pages, x.block_table.long(), x.kv_len, x.g_q, seq_start=x.seq_start)
+    with pytest.raises(TypeError):
+        paged_attention(x.q.half(), x.k_pages, x.v_pages, x.block_table, x.kv_len, x.g_q, seq_start=x.seq_start)
+    with pytest.raises(TypeError):
+        paged_attention(x.q.float(), x.k_pages, x.v_pages, x.block_table, x.kv_len, x.g_q, seq_start=x.seq_start)
+    with pytest.raises(AssertionError):
+        paged_attention(x.q, x.k_pages, x.v_pages, x.block_table, x.kv_len, x.g_q)  # three rows of two sequences
+    with pytest.raises(AssertionError):
+        paged_attention(x.q, x.k_pages, x.v_pages, x.block_table, x.kv_len.cpu(), x.g_q, seq_start=x.seq_start)
+    with pytest.raises(AssertionError):
+        paged_attention(x.q, x.k_pages, x.v_pages, x.block_table, x.kv_len, x.g_q, seq_start=x.seq_start, out=x.q)
+    with pytest.raises(AssertionError):
+        shared_prefix_attention(x.q, x.k_pages, x.v_pages, x.block_table[0, :1], 17, x.block_table, x.kv_len, x.g_q, seq_start=x.seq_start)
+    with pytest.raises(SegptError, match="rope"):
+        paged_attention(x.q, x.k_pages, x.v_pages, x.block_table, x.kv_len, x.g_q, seq_start=x.seq_start, rope_cos=x.cos[:20], rope_sin=x.sin[:20])
+    with pytest.raises(SegptError, match="power of two"):
+        paged_attention(x.q, x.k_pages[:, :, :12], x.v_pages[:, :, :12], x.block_table, x.kv_len, x.g_q, seq_start=x.seq_start)
+    with pytest.raises(AssertionError):
+        paged_kv_append(x.k, x.v, x.k_pages, x.v_pages, x.block_table, x.kv_len, seq_start=x.seq_start, v_first=x.v_first)
+    with pytest.raises(SegptError, match="stride"):
+        flat = x.k_pages[:1].expand(4, -1, -1, -1)
+        paged_kv_append(x.k, x.v, flat, flat, x.block_table, x.kv_len, seq_start=x.seq_start)
+    empty = x.q[:0]
+    assert paged_attention(empty, x.k_pages, x.v_pages, x.block_table, x.kv_len, x.g_q, seq_start=x.seq_start * 0).shape == empty.shape

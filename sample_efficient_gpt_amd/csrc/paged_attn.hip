@@ -6,12 +6,14 @@
 // over the prefix's keys and the sequence's keys j <= kv_len - n + i.  The pool's rows are already rotated and normalised, so that what is
 // left per key is a product on either side of the softmax.
 //
-// Work.  The heads of a kv group and the rows of a sequence are the columns n = i * (H / Hkv) + head of one product, in tiles of 32 columns a
-// wave.  An ENTRY is a set of columns that read the same pages: a sequence, or the shared prefix with the rows of the whole batch.  An
-// item of work is (entry, tile, share of its keys, kv head).  Lengths live on the device, so the device deals out the work: the length of
-// a share follows from the sum over all entries such that the items fill the card once, and every workgroup finds its own item in
-// the running sum of the entries' items (one load and a few register moves for up to 64 sequences).  A tile with one share writes y; others
-// leave (reference m, sum l, products O) in fp32, which paged_merge_kernel joins.
+// Work.  The heads of a kv group and the rows of a sequence are the columns n = i * (H / Hkv) + head of one product.  An ENTRY is a set of
+// columns that read the same pages: a sequence, or the shared prefix with the rows of the whole batch.  Entries of up to 32 columns (generated
+// tokens) are FEW: an item of work is one wave with its own buffers, bound by the memory it reads.  The others are MANY: an item is a
+// workgroup of four waves with 32 columns each that share the staged keys, bound by the matrix pipe and the exponentials.  Either way an item
+// is (entry, tile of columns, share of its keys, kv head).  Lengths live on the device, so the device deals out the work: the length of a
+// share follows from the sum over all entries, such that the items fill the card once, and every workgroup finds its own item in the running
+// sum of the entries' items (one load and a few register moves for up to 64 sequences).  A tile with one share writes y; others leave
+// (reference m, sum l, products O) in fp32, which paged_merge_kernel joins.
 //
 // Scores are transposed as in the other forward kernels: lane = query column, S^T = K' . Qhat^T, and the probabilities are already the
 // B operand of O^T = V'^T . P^T.
@@ -27,27 +29,29 @@ struct PagedArgs {
   segpt_paged_params p;
   int32_t entries, shared;        // shared: 1 if entry 0 is the prefix
   int32_t rows_each, log_page, capacity;
-  int32_t target;                 // items that fill the card once
-  int32_t min_share;              // shortest share, in blocks of 32 keys
-  int32_t n_items;                // workgroups: items there may be
-  int32_t n_slots;                // partial results there is room for
-  float* part;                    // [n_slots][tile columns][D]
-  float2* stat;                   // [n_slots][tile columns]
+  int32_t target;                 // workgroups of four waves that fill the card once
+  int32_t min_few, min_many;      // shortest shares, in blocks of 32 keys
+  int32_t n_many, n_few;          // items there may be of either kind
+  int32_t n_joins;                // tiles and kv heads whose partial results there may be to join
+  int32_t n_slots;                // partial results there is room for, 32 columns each
+  float* part;                    // [n_slots][32][D]
+  float2* stat;                   // [n_slots][32]
 };
 
 constexpr int kBlock = 32;          // keys of a score tile
+constexpr int kFew = 32, kMany = 128;  // columns of a tile
 constexpr float kLazy = 8.f;        // the reference is raised where a score exceeds it by 2^8: probabilities stay below 2^8
-constexpr int kTablePages = 512;    // page numbers held in LDS: a longer share takes its keys in windows
 
 // ---- the plan, computed by every wave for itself
 struct Entry {
   int first, n, len;   // rows, keys
   int tiles, blocks;
+  bool many;
   bool broken;         // a length no sequence can have: every row of the entry is NaN
 };
-__device__ __forceinline__ Entry entry_at(const PagedArgs& a, int e, int rep, int tile_cols) {
+__device__ __forceinline__ Entry entry_at(const PagedArgs& a, int e, int rep) {
   const segpt_paged_params& p = a.p;
-  Entry x{0, 0, 0, 0, 0, false};
+  Entry x{0, 0, 0, 0, 0, false, false};
   if (e >= a.entries) return x;
   if (a.shared && e == 0) {
     int f, n;
@@ -61,7 +65,9 @@ __device__ __forceinline__ Entry entry_at(const PagedArgs& a, int e, int rep, in
     x.broken = len < 0 || len > a.capacity;
     x.len = min(max(len, 0), a.capacity);
   }
-  x.tiles = (x.n * rep + tile_cols - 1) / tile_cols;
+  const int cols = x.n * rep;
+  x.many = cols > kFew;
+  x.tiles = x.many ? (cols + kMany - 1) / kMany : cols > 0;
   x.blocks = (x.len + kBlock - 1) / kBlock;
   return x;
 }
@@ -83,48 +89,68 @@ template <typename T>
 __device__ __forceinline__ T lane_value(T v, int lane) {
   return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
-// blocks of a share.  The sum is a float: it may round, but to the same value in every wave of both kernels.
-__device__ __forceinline__ int share_blocks(const PagedArgs& a, int lane, int rep, int tile_cols, Entry* mine) {
-  float work = 0.f;
-  *mine = entry_at(a, lane, rep, tile_cols);
-  work = (float)mine->tiles * (float)mine->blocks;
-  for (int e = 64; e < a.entries; e += 64) {
-    const Entry x = entry_at(a, e + lane, rep, tile_cols);
-    work += (float)x.tiles * (float)x.blocks;
+struct Shares {
+  int few, many;  // blocks of a share
+};
+__device__ __forceinline__ int shares_of(const Entry& x, Shares s) {  // one also of no keys: it writes what such rows get
+  const int len = s.few + (x.many ? s.many - s.few : 0);  // (a choice between the two fields is taken for an indexed access, through memory)
+  return max((x.blocks + len - 1) / len, 1);
+}
+// Blocks of a share, such that the workgroups are resident at once if the tiles alone are not too many for that: the mean first, then longer
+// ones until the begun ones fit too (one workgroup too many is a round of its own).  A block of many columns keeps a workgroup as long as the
+// memory does that of few columns, in a quarter of the workgroup each: a wave's share is a quarter as long.  The sums are
+// floats: they may round, but to the same value in every wave of both kernels.
+__device__ __forceinline__ Shares share_blocks(const PagedArgs& a, int lane, int rep, Entry* mine) {
+  *mine = entry_at(a, lane, rep);
+  auto sum = [&](auto of) {
+    float v = of(*mine);
+    for (int e = 64; e < a.entries; e += 64) v += of(entry_at(a, e + lane, rep));
+    return lane_value(lane_prefix_sum(v), 63) * (float)a.p.Hkv;
+  };
+  const float target = (float)a.target;
+  float len = sum([](const Entry& x) { return (float)x.tiles * (float)x.blocks; }) / target;
+  Shares s;
+  for (int i = 0;; ++i) {
+    s.many = max((int)fminf(ceilf(len), 1e9f), a.min_many);
+    s.few = max((int)fminf(ceilf(0.25f * len), 1e9f), a.min_few);
+    if (i == 3) break;
+    const float groups = sum([&](const Entry& x) { return (float)x.tiles * (float)shares_of(x, s) * (x.many ? 1.f : 0.25f); });
+    if (groups <= target || groups > 2.f * target) break;
+    len *= fmaxf(groups / target, 1.03f);
   }
-  work = lane_value(lane_prefix_sum(work), 63) * (float)a.p.Hkv;
-  return max((int)fminf(ceilf(work / (float)a.target), 1e9f), a.min_share);
+  return s;
 }
 // an entry as the whole wave sees it
 struct Found {
   int entry;          // -1: none
   int first, n, len, blocks;
-  int shares, base;   // shares of its keys; number of its first item
+  int shares, base;   // shares of its keys; number of its first item of its kind (or tile to be joined)
   int slot;           // of its first partial result (entries whose tiles leave any)
-  bool broken;
+  bool many, broken;
 };
-// the first entry, from lane order on, for which hit(entry, number of its first item, its items) holds
-template <typename Hit>
-__device__ __forceinline__ Found find_entry(const PagedArgs& a, int lane, int rep, int tile_cols, int share, const Entry& mine, int from, Hit hit) {
+// The entry of an item of its kind, or of a tile and kv head whose partial results are to be joined, by number; or the first entry
+enum Find { kFindFew, kFindMany, kFindJoin, kFindFirst };
+template <Find F>
+__device__ __forceinline__ Found find_entry(const PagedArgs& a, int lane, int rep, const Shares& share, const Entry& mine, int which) {
   int base = 0, slot = 0;
   for (int e0 = 0; e0 < a.entries; e0 += 64) {
-    const Entry x = e0 == 0 ? mine : entry_at(a, e0 + lane, rep, tile_cols);
-    const int shares = (x.blocks + share - 1) / share, items = x.tiles * shares * a.p.Hkv;
-    const int upto = base + lane_prefix_sum(items);
-    const int slots = a.shared || shares > 1 ? items : 0, slots_upto = slot + lane_prefix_sum(slots);
-    const uint64_t hits = __builtin_amdgcn_ballot_w64(e0 + lane >= from && e0 + lane < a.entries && hit(x, upto - items, items));
+    const Entry x = e0 == 0 ? mine : entry_at(a, e0 + lane, rep);
+    const int shares = shares_of(x, share), items = x.tiles * shares * a.p.Hkv;
+    const bool partial = a.shared || shares > 1;
+    const int slots = partial ? items * (x.many ? kMany / 32 : 1) : 0, slots_upto = slot + lane_prefix_sum(slots);
+    const int mine_n = F == kFindJoin ? (partial && e0 + lane >= a.shared ? x.tiles * a.p.Hkv : 0) : F == kFindFirst ? 0 : x.many == (F == kFindMany) ? items : 0;
+    const int upto = F == kFindFirst ? 0 : base + lane_prefix_sum(mine_n);
+    const uint64_t hits = F == kFindFirst ? 1 : __builtin_amdgcn_ballot_w64(which >= upto - mine_n && which < upto);
     if (hits) {
       const int l = __builtin_ctzll(hits);
       return Found{e0 + l, lane_value(x.first, l), lane_value(x.n, l), lane_value(x.len, l), lane_value(x.blocks, l), lane_value(shares, l),
-                   lane_value(upto - items, l), lane_value(slots_upto - slots, l), lane_value((int)x.broken, l) != 0};
+                   lane_value(upto - mine_n, l), lane_value(slots_upto - slots, l), lane_value((int)x.many, l) != 0, lane_value((int)x.broken, l) != 0};
     }
     base = lane_value(upto, 63);
     slot = lane_value(slots_upto, 63);
   }
-  return Found{-1, 0, 0, 0, 0, 0, 0, 0, false};
+  return Found{-1, 0, 0, 0, 0, 0, 0, 0, false, false};
 }
-// shares are as even as whole blocks allow
-__device__ __forceinline__ int blocks_per_share(const Found& x) { return (x.blocks + x.shares - 1) / x.shares; }
 
 // ---- tiles: BK rows of D elements, filled by direct global->LDS loads of 1 KB; the 16-byte chunk c of row r lies at chunk c ^ f(r)
 template <typename E, int D>
@@ -137,16 +163,19 @@ struct Tile {
     else return (row & 3) | ((row >> 1) & 4) | ((row & 4) << 1);
   }
 };
-
-// NW waves share the keys of a tile; each owns 32 columns.  NW == 1: a wave of its own, nothing to wait for but its own loads.
-template <typename E, int D, int NW>
+template <typename E, int D>
 struct Shape {
-  static constexpr int kBK = NW == 4 && D * sizeof(E) <= 128 ? 64 : 32;  // keys per staged tile
-  static constexpr int kTileBytes = kBK * D * (int)sizeof(E), kStageBytes = 2 * kTileBytes;
-  static constexpr int kStages = kStageBytes >= 32768 ? 2 : 3;
-  static constexpr int kPasses = kTileBytes / 1024 / NW;  // loads of a wave per tensor and tile
-  static constexpr int kCols = 32 * NW;
-  static constexpr int kOcc = D * sizeof(E) <= 128 ? 3 : D * sizeof(E) <= 256 ? 2 : 1;  // waves per SIMD
+  static constexpr int kRB = D * (int)sizeof(E);
+  // MANY: keys per staged tile (16 KB with its values, at fp32 head_dim 128 32) and stages of the ring
+  static constexpr int kBK = kRB <= 128 ? 64 : 32;
+  static constexpr int kTileBytes = kBK * kRB, kStageBytes = 2 * kTileBytes;
+  static constexpr int kStages = kRB <= 256 ? 3 : 2;
+  static constexpr int kManyTable = 256;  // page numbers held in LDS: a longer share takes its keys in windows
+  static constexpr int kManyBytes = kStages * kStageBytes;
+  // FEW: one block of keys and one of values a wave
+  static constexpr int kFewTable = 64;
+  static constexpr int kFewBytes = 2 * kBlock * kRB;
+  static constexpr int kOcc = kRB <= 128 ? 3 : kRB <= 256 ? 2 : 1;  // workgroups of four waves per CU
 };
 
 // query columns in the B operand's layout, scaled by everything that does not depend on the key (gsm: g_q g_k sm_scale log2 e); D / 2 values
@@ -225,460 +254,702 @@ __device__ __forceinline__ float gate_factor(const segpt_paged_params& p, int t,
   return p.gate_scale / (1.0f + __expf(-x));
 }
 
-// Workgroup = NW waves = one item.  LDS holds the page numbers of the item's share and a ring of stages (K' tile, V' tile); tile jt lives
-// in stage jt % kStages.  Per tile: wait for its loads, barrier (also: everyone has left the tile before), request tile jt + kStages - 1
-// over the one before, compute.
-template <typename E, int D, int NW>
-__global__ __launch_bounds__(64 * NW, (Shape<E, D, NW>::kOcc)) void paged_attn_kernel(PagedArgs a) {
-  using S = Shape<E, D, NW>;
+// ---- an item
+struct Item {
+  Found x;
+  int g, part, tile, cols;
+  int k0, nk;        // its keys: k0 .. k0 + nk - 1
+  int past;          // row i of a sequence sees its keys up to past + i; the prefix's all rows see, but for those that stand in it
+  int slot;
+  bool prefix, direct, valid;
+  const int* ids;    // page numbers
+};
+template <bool MANY>
+__device__ __forceinline__ Item locate(const PagedArgs& a, int lane, int rep, const Shares& share, const Entry& mine, int number) {
+  constexpr int COLS = MANY ? kMany : kFew;
+  Item it;
+  it.x = find_entry<MANY ? kFindMany : kFindFew>(a, lane, rep, share, mine, number);
+  const Found& x = it.x;
+  it.valid = x.entry >= 0;
+  if (!it.valid) return it;
+  it.cols = x.n * rep;
+  const int n_tiles = (it.cols + COLS - 1) / COLS, local = number - x.base;
+  it.g = local % a.p.Hkv;
+  it.part = local / a.p.Hkv % x.shares;
+  it.tile = n_tiles - 1 - local / a.p.Hkv / x.shares;  // the last tiles see the most keys: they start first
+  it.prefix = a.shared && x.entry == 0;
+  it.direct = !a.shared && x.shares == 1;
+  it.slot = x.slot + ((it.tile * x.shares + it.part) * a.p.Hkv + it.g) * (COLS / 32);
+  it.valid = it.tile >= 0 && (it.direct || it.slot + COLS / 32 <= a.n_slots);
+  it.past = x.len - x.n;
+  const int per = (x.blocks + x.shares - 1) / x.shares * kBlock;  // shares as even as whole blocks allow
+  const int last_col = min(it.cols, (it.tile + 1) * COLS) - 1, sees = it.prefix ? x.len : min(x.len, it.past + last_col / rep + 1);
+  it.k0 = it.part * per;
+  it.nk = max(min(sees, it.k0 + per) - it.k0, 0);
+  it.ids = it.prefix ? a.p.prefix_table : a.p.block_table + (int64_t)(x.entry - a.shared) * a.p.table_stride;
+  return it;
+}
+// Page numbers of keys w0 .. w0 + wn - 1 into LDS; one that is not in the pool is replaced by page 0: returns whether this wave met one
+__device__ __forceinline__ bool stage_table(const PagedArgs& a, const Item& it, int w0, int wn, int* table, int first, int step) {
+  const int p0 = w0 >> a.log_page, pages = wn ? ((w0 + wn - 1) >> a.log_page) - p0 + 1 : 0;
+  bool bad = false;
+  for (int i = first; i < pages; i += step) {
+    int id = it.ids[p0 + i];
+    if ((uint32_t)id >= (uint32_t)a.p.n_pages) { id = 0; bad = true; }
+    table[i] = id;
+  }
+  return __builtin_amdgcn_ballot_w64(bad) != 0;
+}
+__device__ __forceinline__ float scale_at(const segpt_paged_params& p, int d) {
+  const float v = (p.gq_numel == 1 ? p.g_q[0] : p.g_q[d]) * p.sm_scale * kLog2e;
+  return p.gk_numel == 0 ? v : v * (p.gk_numel == 1 ? p.g_k[0] : p.g_k[d]);
+}
+
+// Requests of tiles of keys w0 .. w0 + wn - 1.  A load covers kRowsPerLoad rows, at most 8, of one page: its address is a scalar base and
+// a lane offset.  LOADS loads a tensor and tile; number ps is load first + ps * step of the tile.
+template <typename E, int D, int BK, int LOADS>
+struct Requests {
   using Z = Tile<E, D>;
-  constexpr bool BF16 = sizeof(E) == 2;
-  constexpr int MB = D / 32, BK = S::kBK, NS = S::kStages, PASSES = S::kPasses;
-  const segpt_paged_params& p = a.p;
-  __shared__ __attribute__((aligned(1024))) char lds[NS * S::kStageBytes];
-  __shared__ __attribute__((aligned(16))) float gsm[D];
-  __shared__ int table[kTablePages + 2];
-  __shared__ int any_bad[NW];
-
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int ln = lane & 31, hh = lane >> 5;
-  const int rep = p.H / p.Hkv;
-  auto sync = [&] {
-    if constexpr (NW == 1) {
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): reads of a tile have returned before it is requested over
-    } else {
-      __syncthreads();
-    }
-  };
-
-  if (p.flags & SEGPT_FLAG_ZERO_REST) {  // rows in no sequence: before the first one and behind the last
-    int head, f, n;
-    sequence_rows(p, a.rows_each, 0, &head, &n);
-    sequence_rows(p, a.rows_each, p.B - 1, &f, &n);
-    const int tail = max(f + n, head);
-    for (int i = blockIdx.x; i < head + p.T - tail; i += gridDim.x) {
-      const int t = i < head ? i : i - head + tail;
-      for (int x = tid; x < p.H * D; x += 64 * NW) row_of<E>(p.o, t, x / D)[x % D] = 0;
-    }
+  const char *kbase, *vbase;
+  int64_t kpage, vpage;
+  uint32_t kstep, vstep;
+  int w0, wn, log_page, first, step, lane;
+  const int* table;
+  __device__ __forceinline__ int first_row(int jt, int ps) const {  // from w0 on; past the last key: the last rows once more
+    return min(jt * BK + (ps * step + first) * Z::kRowsPerLoad, (wn - 1) & ~(Z::kRowsPerLoad - 1));
   }
-
-  Entry mine;
-  const int share = share_blocks(a, lane, rep, S::kCols, &mine);
-  const int item = blockIdx.x;
-  const Found x = find_entry(a, lane, rep, S::kCols, share, mine, 0, [&](const Entry&, int base, int items) { return item >= base && item < base + items; });
-  if (x.entry < 0) return;
-  const int cols = x.n * rep, n_tiles = (cols + S::kCols - 1) / S::kCols;
-  const int local = item - x.base, g = local % p.Hkv, part = local / p.Hkv % x.shares;
-  const int tile = n_tiles - 1 - local / p.Hkv / x.shares;  // the last tiles see the most keys: they start first
-  const bool prefix = a.shared && x.entry == 0, direct = !a.shared && x.shares == 1;
-  const int slot = x.slot + (tile * x.shares + part) * p.Hkv + g;
-  if (tile < 0 || (!direct && slot >= a.n_slots)) return;
-  const int per = blocks_per_share(x) * kBlock;
-
-  // this item's keys: k0 .. k1 - 1, the last ones cut off where no row of the tile sees them
-  const int past = x.len - x.n;  // row i of a sequence sees its keys up to past + i; the prefix's all rows see, but for those that stand in it
-  const int last_col = min(cols, (tile + 1) * S::kCols) - 1;
-  const int k0 = part * per, sees = prefix ? x.len : min(x.len, past + last_col / rep + 1), k1 = min(sees, k0 + per);
-  const int nk = max(k1 - k0, 0);
-
-  // ---- page numbers of a window of the keys into LDS; one that is not in the pool is replaced by page 0 and remembered
-  const int window = kTablePages << a.log_page;
-  const int* const ids = prefix ? p.prefix_table : p.block_table + (int64_t)(x.entry - a.shared) * p.table_stride;
-  bool bad = x.broken;
-  int w0 = k0, wn = min(nk, window);  // first key and keys of the window
-  auto stage_table = [&] {
-    const int p0 = w0 >> a.log_page, pages = wn ? ((w0 + wn - 1) >> a.log_page) - p0 + 1 : 0;
-    bool mine_bad = false;
-    for (int i = tid; i < pages; i += 64 * NW) {
-      int id = ids[p0 + i];
-      if ((uint32_t)id >= (uint32_t)p.n_pages) { id = 0; mine_bad = true; }
-      table[i] = id;
-    }
-    const bool wave_bad = __builtin_amdgcn_ballot_w64(mine_bad) != 0;
-    if (lane == 0) any_bad[wave] = wave_bad;
-  };
-  stage_table();
-  for (int d = tid; d < D; d += 64 * NW) {
-    float v = (p.gq_numel == 1 ? p.g_q[0] : p.g_q[d]) * p.sm_scale * kLog2e;
-    if (p.gk_numel) v *= p.gk_numel == 1 ? p.g_k[0] : p.g_k[d];
-    gsm[d] = v;
+  __device__ __forceinline__ int pages(int jt) const {  // lane ps: the page number of load ps
+    return table[((w0 + first_row(jt, min(lane, LOADS - 1))) >> log_page) - (w0 >> log_page)];
   }
-  sync();
-
-  // ---- tile requests.  A load covers kRowsPerLoad rows, at most 8, of one page: its address is a scalar base and a lane offset
-  const uint32_t lds0 = lds_addr_of(lds);
-  const int lrow = lane / Z::kChunks;
-  const char* const kbase = page_row<E>(p.k_pages, 0, g, 0);
-  const char* const vbase = page_row<E>(p.v_pages, 0, g, 0);
-  const int64_t kpage = p.k_pages.stride_b * (int)sizeof(E), vpage = p.v_pages.stride_b * (int)sizeof(E);
-  const uint32_t kstep = (uint32_t)p.k_pages.stride_s * (int)sizeof(E), vstep = (uint32_t)p.v_pages.stride_s * (int)sizeof(E);
-  auto first_row = [&](int jt, int ps) {  // of load ps, from w0 on; past the last key: the last rows once more
-    return min(jt * BK + (ps * NW + wave) * Z::kRowsPerLoad, (wn - 1) & ~(Z::kRowsPerLoad - 1));
-  };
-  auto page_of = [&](int jt) {  // lane ps: the page number of load ps
-    return table[((w0 + first_row(jt, min(lane, PASSES - 1))) >> a.log_page) - (w0 >> a.log_page)];
-  };
-  auto issue = [&](int jt, int pages) {
-    const uint32_t dst = lds0 + (uint32_t)(jt % NS) * S::kStageBytes + wave * 1024;
+  template <bool VALUES>
+  __device__ __forceinline__ void issue(int jt, int pages, uint32_t dst) const {
+    const int lrow = lane / Z::kChunks;
 #pragma unroll
-    for (int ps = 0; ps < PASSES; ++ps) {
-      const int r0 = first_row(jt, ps), slot_row = (w0 + r0) & ((1 << a.log_page) - 1);
+    for (int ps = 0; ps < LOADS; ++ps) {
+      const int r0 = first_row(jt, ps), slot = (w0 + r0) & ((1 << log_page) - 1);
       const int64_t page = __builtin_amdgcn_readlane(pages, ps);
-      const int r = min(lrow, wn - 1 - r0);
-      const uint32_t col = (uint32_t)((lane % Z::kChunks) ^ Z::f((ps * NW + wave) * Z::kRowsPerLoad + lrow)) << 4;
-      gload_lds16_so(kbase + page * kpage + (int64_t)slot_row * kstep, (uint32_t)r * kstep + col, dst + ps * NW * 1024);
-      gload_lds16_so(vbase + page * vpage + (int64_t)slot_row * vstep, (uint32_t)r * vstep + col, dst + S::kTileBytes + ps * NW * 1024);
+      const uint32_t r = min(lrow, wn - 1 - r0), col = (uint32_t)((lane % Z::kChunks) ^ Z::f((ps * step + first) * Z::kRowsPerLoad + lrow)) << 4;
+      const uint32_t rs = VALUES ? vstep : kstep;
+      gload_lds16_so((VALUES ? vbase + page * vpage : kbase + page * kpage) + (int64_t)slot * rs, r * rs + col, dst + (ps * step + first) * 1024);
     }
-  };
-  auto start_window = [&] {
-#pragma unroll
-    for (int w = 0; w < NW; ++w) bad |= any_bad[w] != 0;
-#pragma unroll
-    for (int t = 0; t < NS - 1; ++t)
-      if (t * BK < wn) issue(t, page_of(t));
-  };
-  start_window();
-
-  // ---- this lane's column
-  const int col = tile * S::kCols + wave * 32 + ln;
-  const bool live = col < cols;
-  const int i = (live ? col : tile * S::kCols) / rep, t_row = x.first + i, h = g * rep + (live ? col : tile * S::kCols) % rep;
-  Query<E, D> q;
-  int own = past + i;  // position among the sequence's own keys: negative where it stands in the prefix
-  {
-    if (prefix) {  // the row's own sequence says where it stands
-      int b = 0, f = 0, n = 0;
-      if (p.seq_start) {
-        for (int lo = 0, hi = p.B - 1; lo <= hi;) {  // last sequence that starts at or before the row
-          const int m = (lo + hi) >> 1;
-          if (p.seq_start[m] <= t_row) { b = m; lo = m + 1; } else hi = m - 1;
-        }
-      } else {
-        b = t_row / a.rows_each;
-      }
-      sequence_rows(p, a.rows_each, b, &f, &n);
-      own = (int)min((int64_t)p.kv_len[b] - n + (t_row - f), (int64_t)a.capacity - 1);
-    }
-    const int64_t pos = max((int64_t)p.prefix_len + own, (int64_t)0);
-    q.load(p, row_of<E>(p.q, t_row, h), (p.rope_pos0 + pos) * (D / 2), live, hh, gsm);
   }
-  // keys from k0 on that the lane's row sees, and what the whole wave sees; a wave without columns computes nothing
-  const int lim = min((prefix ? p.prefix_len : 0) + own - k0, nk - 1);
-  const int wave_col = tile * S::kCols + wave * 32;
-  const bool works = wave_col < cols;
-  const bool cut = prefix && __builtin_amdgcn_ballot_w64(lim < nk - 1) != 0;  // rows that stand in the prefix
-  const int all_see = !works || cut ? -1 : prefix ? nk - 1 : min(past + wave_col / rep - k0, nk - 1);
-  const int any_sees = !works ? -1 : prefix ? nk - 1 : min(past + min(wave_col + 31, cols - 1) / rep - k0, nk - 1);
+};
+template <typename E, int D, int BK, int LOADS>
+__device__ __forceinline__ Requests<E, D, BK, LOADS> requests(const PagedArgs& a, const Item& it, const int* table, int first, int step, int lane) {
+  const segpt_paged_params& p = a.p;
+  return {page_row<E>(p.k_pages, 0, it.g, 0), page_row<E>(p.v_pages, 0, it.g, 0), p.k_pages.stride_b * (int)sizeof(E), p.v_pages.stride_b * (int)sizeof(E),
+          (uint32_t)p.k_pages.stride_s * (int)sizeof(E), (uint32_t)p.v_pages.stride_s * (int)sizeof(E), 0, 0, a.log_page, first, step, lane, table};
+}
 
-  f32x16 oacc[MB];
-#pragma unroll
-  for (int mb = 0; mb < MB; ++mb) oacc[mb] = splat16(0.f);
-  float m_ref = -INFINITY, l_run[2] = {0.f, 0.f};
-
-  auto block = [&](uint32_t stage, int kb, int jb) {  // keys jb .. jb + 31 from k0 on, rows 32 kb .. of the tile
-    const uint32_t kt = stage + kb * 32 * Z::kRB, vt = stage + S::kTileBytes + kb * 32 * Z::kRB;
-    f32x16 s = splat16(0.f);
-    if constexpr (BF16) {
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) s = mfma32(swz_frag_rm<D>(kt + swz_off_rm<D>(lane), 0, ks), q.reg[ks], s);
-    } else {
-      const uint32_t row = kt + ln * Z::kRB;
-      const int fx = Z::f(ln);
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        const f32x4 k4 = lds_read_f4(row + (((2 * c + hh) ^ fx) << 4));
-#pragma unroll
-        for (int t = 0; t < 4; ++t) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k4[t], q.reg[c][t], s, 0, 0, 0);
+// ---- a lane's column, and what it sees of the item's keys (counted from k0 on)
+struct Column {
+  int t, h;      // row and head
+  bool live;
+  int lim;       // last key of the lane's row
+  int all, any;  // last key that all columns of the wave see, that any of them sees
+};
+template <typename E, int D>
+__device__ __forceinline__ Column column_of(const PagedArgs& a, const Item& it, int rep, int wave_col, int lane, Query<E, D>& q, const float* gsm) {
+  const segpt_paged_params& p = a.p;
+  Column c;
+  const bool works = wave_col < it.cols;
+  const int col = wave_col + (lane & 31), safe = min(col, it.cols - 1), i = safe / rep;
+  c.live = col < it.cols;
+  c.t = it.x.first + i;
+  c.h = it.g * rep + safe - i * rep;
+  int own = it.past + i;  // position among the sequence's own keys: negative where it stands in the prefix
+  if (it.prefix) {        // the row's own sequence says where it stands
+    int b = 0, f = 0, n = 0;
+    if (p.seq_start) {
+      for (int lo = 0, hi = p.B - 1; lo <= hi;) {  // last sequence that starts at or before the row
+        const int m = (lo + hi) >> 1;
+        if (p.seq_start[m] <= c.t) { b = m; lo = m + 1; } else hi = m - 1;
       }
+    } else {
+      b = c.t / a.rows_each;
     }
-    const bool masked = jb + 31 > all_see;  // register r holds key jb + 4 hh + c_r, c_r = 8 (r / 4) + r % 4
-    if (masked) {
-      const int t = lim - jb - 4 * hh;
+    sequence_rows(p, a.rows_each, b, &f, &n);
+    own = (int)min((int64_t)p.kv_len[b] - n + (c.t - f), (int64_t)a.capacity - 1);
+  }
+  const int64_t pos = max((int64_t)p.prefix_len + own, (int64_t)0);
+  q.load(p, row_of<E>(p.q, c.t, c.h), (p.rope_pos0 + pos) * (D / 2), c.live, lane >> 5, gsm);
+  c.lim = min((it.prefix ? p.prefix_len : 0) + own - it.k0, it.nk - 1);
+  if (it.prefix) {
+    const bool cut = __builtin_amdgcn_ballot_w64(c.live && c.lim < it.nk - 1) != 0;  // rows that stand in the prefix
+    c.all = !works || cut ? -1 : it.nk - 1;
+    c.any = works ? it.nk - 1 : -1;
+  } else {
+    c.all = works ? min(it.past + wave_col / rep - it.k0, it.nk - 1) : -1;
+    c.any = works ? min(it.past + min(wave_col + 31, it.cols - 1) / rep - it.k0, it.nk - 1) : -1;
+  }
+  return c;
+}
+
+// ---- one block of 32 keys: operands, softmax, products
+// K' rows as the A operand
+template <typename E, int D>
+struct Keys;
+template <int D>
+struct Keys<uint16_t, D> {
+  bf16x8 k[D / 16];
+  __device__ __forceinline__ void read(uint32_t tile, int lane) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (8 * (r >> 2) + (r & 3) > t) s[r] = -INFINITY;
+    for (int ks = 0; ks < D / 16; ++ks) k[ks] = swz_frag_rm<D>(tile + swz_off_rm<D>(lane), 0, ks);
+  }
+  __device__ __forceinline__ f32x16 scores(const Query<uint16_t, D>& q, f32x16 s) const {
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) s = mfma32(k[ks], q.reg[ks], s);
+    return s;
+  }
+};
+template <int D>
+struct Keys<float, D> {
+  f32x4 k[D / 8];
+  __device__ __forceinline__ void read(uint32_t tile, int lane) {
+    const uint32_t row = tile + (lane & 31) * (4 * D);
+    const int fx = Tile<float, D>::f(lane & 31), hh = lane >> 5;
+#pragma unroll
+    for (int c = 0; c < D / 8; ++c) k[c] = lds_read_f4(row + (((2 * c + hh) ^ fx) << 4));
+  }
+  __device__ __forceinline__ f32x16 scores(const Query<float, D>& q, f32x16 s) const {
+#pragma unroll
+    for (int c = 0; c < D / 8; ++c)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[c][t], q.reg[c][t], s, 0, 0, 0);
+    return s;
+  }
+};
+// V' rows as the A operand of O^T.  finite(): replaces what is not a number or infinite by 0, returns whether there was any
+template <typename E, int D>
+struct Values;
+template <int D>
+struct Values<uint16_t, D> {
+  static constexpr int MB = D / 32;
+  bf16x8 v[MB][2];
+  __device__ __forceinline__ void read(uint32_t tile, int lane) {
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) v[mb][s2] = swz_frag_tr<D>(tile + swz_off_tr<D>(lane), mb, s2);
+  }
+  __device__ __forceinline__ bool finite() {
+    bool odd = false;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) {
+        u32x4 w = __builtin_bit_cast(u32x4, v[mb][s2]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool lo = (w[e] & 0x7f80u) == 0x7f80u, hi = (w[e] & 0x7f800000u) == 0x7f800000u;
+          odd |= lo | hi;
+          w[e] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+        }
+        v[mb][s2] = as_bf16x8(w);
+      }
+    return odd;
+  }
+  // adds the probabilities s to the sums l, as they are rounded, and their products with the values to o
+  __device__ __forceinline__ void add(f32x16 s, float (&l)[2], f32x16 (&o)[MB]) const {
+    const bf16x8 pb[2] = {pack_c_half_sum(s, 0, l), pack_c_half_sum(s, 1, l)};
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) o[mb] = mfma32(v[mb][s2], pb[s2], o[mb]);
+  }
+};
+template <int D>
+struct Values<float, D> {
+  static constexpr int MB = D / 32;
+  float v[MB][16];  // step r contracts key c_r = 8 (r / 4) + r % 4 (lower half of the wave) and c_r + 4 (upper half): register r of the scores as it is
+  __device__ __forceinline__ void read(uint32_t tile, int lane) {
+    const int ln = lane & 31, hh = lane >> 5;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int key = 8 * (r >> 2) + (r & 3) + 4 * hh;
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) v[mb][r] = lds_read_f(tile + key * (4 * D) + (((8 * mb + (ln >> 2)) ^ Tile<float, D>::f(key)) << 4) + 4 * (ln & 3));
     }
+  }
+  __device__ __forceinline__ bool finite() {
+    bool odd = false;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const bool no = !(fabsf(v[mb][r]) < INFINITY);
+        odd |= no;
+        if (no) v[mb][r] = 0.f;
+      }
+    return odd;
+  }
+  __device__ __forceinline__ void add(f32x16 s, float (&l)[2], f32x16 (&o)[MB]) const {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) l[r & 1] += s[r];
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) o[mb] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[mb][r], s[r], o[mb], 0, 0, 0);
+  }
+};
+// Values that are not finite, key by key, for the rows that see them: their probability is positive, so the sum is the value, or NaN
+// where signs meet.  (Through the product they would reach the other rows as 0 * inf.)
+template <typename E, int D>
+__device__ __forceinline__ void add_odd_values(uint32_t tile, int seen, int hh, f32x16 (&o)[D / 32]) {
+  for (int key = 0; key < 32; ++key) {
+    const bool visible = key <= seen;
+#pragma unroll
+    for (int mb = 0; mb < D / 32; ++mb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int d = 32 * mb + 8 * (r >> 2) + 4 * hh + (r & 3), byte = d * (int)sizeof(E);
+        const uint32_t at = tile + key * Tile<E, D>::kRB + (((byte >> 4) ^ Tile<E, D>::f(key)) << 4) + (byte & 15);
+        float v;
+        if constexpr (sizeof(E) == 2) v = bf16_to_f32(lds_read_h(at)); else v = lds_read_f(at);
+        if (visible && !(fabsf(v) < INFINITY)) o[mb][r] += v;
+      }
+  }
+}
+template <int MB>
+struct State {
+  f32x16 o[MB];
+  float m, l[2];  // reference (log2 units); sums of this lane's half of the keys
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) o[mb] = splat16(0.f);
+    m = -INFINITY;
+    l[0] = l[1] = 0.f;
+  }
+  // scores to probabilities against the reference, which is raised where a score exceeds it by kLazy
+  __device__ __forceinline__ void exponentials(f32x16& s) {
     float mx = s[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
     mx = half_max(mx);
-    const bool need = mx > m_ref + kLazy;
+    const bool need = mx > m + kLazy;
     if (__builtin_amdgcn_ballot_w64(need) != 0) {
-      const float m_new = need ? mx : m_ref, corr = need ? fast_exp2(m_ref - m_new) : 1.f;
-      m_ref = m_new;
-      l_run[0] *= corr;
-      l_run[1] *= corr;
+      const float m_new = need ? mx : m, corr = need ? fast_exp2(m - m_new) : 1.f;
+      m = m_new;
+      l[0] *= corr;
+      l[1] *= corr;
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) oacc[mb][r] *= corr;
+        for (int r = 0; r < 16; ++r) o[mb][r] *= corr;
     }
-    const float mu = m_ref == -INFINITY ? 0.f : m_ref;  // nothing seen yet: keep exp2 away from inf - inf
+    const float mu = m == -INFINITY ? 0.f : m;  // nothing seen yet: keep exp2 away from inf - inf
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = fast_exp2(s[r] - mu);
-
-    if constexpr (BF16) {
-      const bf16x8 pb[2] = {pack_c_half_sum(s, 0, l_run), pack_c_half_sum(s, 1, l_run)};
-      bf16x8 vT[MB][2];
-      bool odd = false;
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2) vT[mb][s2] = swz_frag_tr<D>(vt + swz_off_tr<D>(lane), mb, s2);
-      if (masked) {  // a value that is not finite must not reach rows that do not see its key through 0 * inf
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-          for (int s2 = 0; s2 < 2; ++s2) {
-            u32x4 w = __builtin_bit_cast(u32x4, vT[mb][s2]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const bool lo = (w[e] & 0x7f80u) == 0x7f80u, hi = (w[e] & 0x7f800000u) == 0x7f800000u;
-              odd |= lo | hi;
-              w[e] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
-            }
-            vT[mb][s2] = as_bf16x8(w);
-          }
-      }
-#pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) oacc[mb] = mfma32(vT[mb][s2], pb[s2], oacc[mb]);
-      if (masked && __builtin_amdgcn_ballot_w64(odd) != 0) {  // rare: those values once more, key by key, for the rows that see them
-        for (int key = 0; key < 32; ++key) {
-          const bool visible = key <= lim - jb;
-#pragma unroll
-          for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int d = 32 * mb + 8 * (r >> 2) + 4 * hh + (r & 3);
-              const float v = bf16_to_f32(lds_read_h(vt + key * Z::kRB + (((d >> 3) ^ Z::f(key)) << 4) + 2 * (d & 7)));
-              if (visible && !(fabsf(v) < INFINITY)) oacc[mb][r] += v;  // its probability is positive: v, or NaN where signs meet
-            }
-        }
-      }
-    } else {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) l_run[r & 1] += s[r];
-      bool odd = false;
-      // step r contracts key c_r (lower half of the wave) and c_r + 4 (upper half): register r of the probabilities as it is
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int key = 8 * (r >> 2) + (r & 3) + 4 * hh;
-        const uint32_t at = vt + key * Z::kRB;
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
-          float v = lds_read_f(at + (((8 * mb + (ln >> 2)) ^ Z::f(key)) << 4) + 4 * (ln & 3));
-          if (masked) {  // as above
-            const bool no_number = !(fabsf(v) < INFINITY);
-            odd |= no_number;
-            if (no_number) v = 0.f;
-          }
-          oacc[mb] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[r], oacc[mb], 0, 0, 0);
-        }
-      }
-      if (masked && __builtin_amdgcn_ballot_w64(odd) != 0) {
-        for (int key = 0; key < 32; ++key) {
-          const bool visible = key <= lim - jb;
-#pragma unroll
-          for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const f32x4 v = lds_read_f4(vt + key * Z::kRB + (((8 * mb + 2 * c + hh) ^ Z::f(key)) << 4));
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (visible && !(fabsf(v[e]) < INFINITY)) oacc[mb][4 * c + e] += v[e];
-            }
-        }
-      }
-    }
-  };
-
-  while (true) {
-    wait_vmcnt<0>();  // the loads below are counted: nothing of the start may be in flight with them
-    const int n_kt = (wn + BK - 1) / BK;
-    int next_pages = n_kt ? page_of(min(NS - 1, n_kt - 1)) : 0;
-    for (int jt = 0; jt < n_kt; ++jt) {
-      if (n_kt - 1 - jt >= NS - 2) wait_vmcnt<(NS - 2) * 2 * PASSES>(); else wait_vmcnt<0>();
-      sync();
-      if (jt + NS - 1 < n_kt) {
-        issue(jt + NS - 1, next_pages);
-        next_pages = page_of(min(jt + NS, n_kt - 1));
-      }
-      const uint32_t stage = lds0 + (uint32_t)(jt % NS) * S::kStageBytes;
-      const int jb = w0 - k0 + jt * BK;
-#pragma unroll
-      for (int kb = 0; kb < BK / 32; ++kb)
-        if (jb + 32 * kb <= any_sees) block(stage, kb, jb + 32 * kb);
-    }
-    w0 += window;
-    if (w0 >= k1) break;
-    wn = min(k1 - w0, window);
-    sync();  // everyone is done with the page numbers and the stages
-    stage_table();
-    sync();
-    start_window();
   }
+};
+__device__ __forceinline__ void hide_unseen(f32x16& s, int seen, int hh) {  // register r holds key 4 hh + c_r, c_r = 8 (r / 4) + r % 4
+  const int t = seen - 4 * hh;
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    if (8 * (r >> 2) + (r & 3) > t) s[r] = -INFINITY;
+}
 
-  // ---- result: row = lane, columns 32 mb + 8 (r / 4) + 4 hh + r % 4
-  float l = half_sum(l_run[0] + l_run[1]);
-  if (bad) { l = __builtin_nanf(""); m_ref = 0.f; }
-  if (!live) return;
-  if (!direct) {
-    const int64_t at = (int64_t)slot * S::kCols + wave * 32 + ln;
+// What an item leaves: y where it is its tile's only one, else a partial result
+template <typename E, int D>
+__device__ __forceinline__ void store_result(const PagedArgs& a, const Item& it, const Column& c, State<D / 32>& st, bool bad, int slot_col, int hh) {
+  const segpt_paged_params& p = a.p;
+  constexpr int MB = D / 32;
+  float l = half_sum(st.l[0] + st.l[1]), m = st.m;
+  if (bad) { l = __builtin_nanf(""); m = 0.f; }
+  if (!c.live) return;
+  if (!it.direct) {
+    const int64_t at = (int64_t)it.slot * 32 + slot_col;
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        *reinterpret_cast<float4*>(a.part + at * D + 32 * mb + 8 * c + 4 * hh) =
-            make_float4(oacc[mb][4 * c], oacc[mb][4 * c + 1], oacc[mb][4 * c + 2], oacc[mb][4 * c + 3]);
-    if (hh == 0) a.stat[at] = make_float2(m_ref, l);
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<float4*>(a.part + at * D + 32 * mb + 8 * q + 4 * hh) =
+            make_float4(st.o[mb][4 * q], st.o[mb][4 * q + 1], st.o[mb][4 * q + 2], st.o[mb][4 * q + 3]);
+    if (hh == 0) a.stat[at] = make_float2(m, l);
     return;
   }
   float f = l == 0.f ? 0.f : 1.0f / l;
-  if (p.lse && hh == 0) p.lse[(int64_t)t_row * p.H + h] = l == 0.f ? -INFINITY : (m_ref + __log2f(l)) * kLn2;
-  if (p.gate.ptr) f *= gate_factor<E, D>(p, t_row, h);
-  E* out = row_of<E>(p.o, t_row, h);
+  if (p.lse && hh == 0) p.lse[(int64_t)c.t * p.H + c.h] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
+  if (p.gate.ptr) f *= gate_factor<E, D>(p, c.t, c.h);
+  E* out = row_of<E>(p.o, c.t, c.h);
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const float y[4] = {oacc[mb][4 * c] * f, oacc[mb][4 * c + 1] * f, oacc[mb][4 * c + 2] * f, oacc[mb][4 * c + 3] * f};
-      E* at = out + 32 * mb + 8 * c + 4 * hh;
-      if constexpr (BF16) *reinterpret_cast<u32x2*>(at) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+    for (int q = 0; q < 4; ++q) {
+      const float y[4] = {st.o[mb][4 * q] * f, st.o[mb][4 * q + 1] * f, st.o[mb][4 * q + 2] * f, st.o[mb][4 * q + 3] * f};
+      E* at = out + 32 * mb + 8 * q + 4 * hh;
+      if constexpr (sizeof(E) == 2) *reinterpret_cast<u32x2*>(at) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
       else store16(at, y);
     }
 }
 
-// Joins the shares of a row: its sequence's own and the prefix's.  WAVES waves a row (one: as many rows as waves), D / 4 lanes side by side,
-// the rest over the shares.  Fixed order: deterministic.
-constexpr int kMergeThreads = 256;
-template <typename E, int D, int WAVES>
-__global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedArgs a, int tile_cols) {
-  const segpt_paged_params& p = a.p;
-  constexpr int LPR = D / 4, G = 64 / LPR, GROUPS = G * WAVES;
-  __shared__ float4 sums[WAVES > 1 ? kMergeThreads : 1];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int rep = p.H / p.Hkv;
-  const int64_t row = WAVES > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (kMergeThreads / 64) + wave;
-  if (row >= (int64_t)p.T * p.H) return;
-  const int t = (int)(row / p.H), h = (int)(row - (int64_t)t * p.H), g = h / rep;
-  Entry mine;
-  const int share = share_blocks(a, lane, rep, tile_cols, &mine);
-  const Found own = find_entry(a, lane, rep, tile_cols, share, mine, a.shared, [&](const Entry& x, int, int) { return t >= x.first && t < x.first + x.n; });
-  if (own.entry < 0) return;  // in no sequence
-  if (!a.shared && own.shares == 1) return;  // written by its only share
-  Found pre{-1, 0, 0, 0, 0, 0, 0, 0, false};
-  if (a.shared) pre = find_entry(a, lane, rep, tile_cols, share, mine, 0, [&](const Entry&, int, int) { return true; });
-  const int n = pre.shares + own.shares;
-  auto slot = [&](int s) {  // of share s: the prefix's first
-    const bool in_prefix = s < pre.shares;
-    const Found& x = in_prefix ? pre : own;
-    const int col = (t - x.first) * rep + h - g * rep, tile = col / tile_cols;
-    const int64_t at = x.slot + ((int64_t)tile * x.shares + (in_prefix ? s : s - pre.shares)) * p.Hkv + g;
-    return at < a.n_slots ? at * tile_cols + (col - tile * tile_cols) : (int64_t)-1;
-  };
-  auto stat_of = [&](int64_t at) { return at < 0 ? make_float2(0.f, __builtin_nanf("")) : a.stat[at]; };
+// this wave's LDS reads have returned (before what they came from is requested over), its LDS writes are there
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0) only
+}
 
-  float m = -INFINITY;
-  for (int s = lane; s < n; s += 64) {
-    const float2 x = stat_of(slot(s));
-    m = fmaxf(m, x.x);
+// ---- FEW: one wave, up to 32 columns.  One buffer for the keys of a block and one for its values, each requested again as soon as its
+// reader has it in registers: the next keys are in flight during the softmax and the product with the values, the next values
+// during the next scores.
+template <typename E, int D>
+__device__ __forceinline__ void few_columns(const PagedArgs& a, const Item& it, int rep, int lane, uint32_t lds, int* table, float* gsm) {
+  using S = Shape<E, D>;
+  constexpr int LOADS = kBlock * S::kRB / 1024;
+  const int hh = lane >> 5, window = S::kFewTable << a.log_page;
+  const uint32_t kt = lds, vt = lds + kBlock * S::kRB;
+  auto rq = requests<E, D, kBlock, LOADS>(a, it, table, 0, 1, lane);
+  rq.w0 = it.k0;
+  rq.wn = min(it.nk, window);
+  bool bad = it.x.broken | stage_table(a, it, rq.w0, rq.wn, table, lane, 64);
+  for (int d = lane; d < D; d += 64) gsm[d] = scale_at(a.p, d);
+  wave_sync();
+  int pages = rq.wn ? rq.pages(0) : 0;
+  if (rq.wn) {
+    rq.template issue<false>(0, pages, kt);
+    rq.template issue<true>(0, pages, vt);
   }
+  Query<E, D> q;
+  const Column c = column_of<E, D>(a, it, rep, it.tile * kFew, lane, q, gsm);
+  State<D / 32> st;
+  st.clear();
+  while (true) {
+    const int n_kt = (rq.wn + kBlock - 1) / kBlock;
+    wait_vmcnt<0>();  // the loads below are counted: nothing of the start may be in flight with them
+    if (n_kt > 1) pages = rq.pages(1);
+    for (int jt = 0; jt < n_kt; ++jt) {
+      const bool more = jt + 1 < n_kt;
+      const int seen = c.lim - (rq.w0 - it.k0) - jt * kBlock;
+      const bool masked = rq.w0 - it.k0 + jt * kBlock + kBlock - 1 > c.all;
+      wait_vmcnt<LOADS>();  // the keys are there, the values younger
+      wave_sync();
+      Keys<E, D> k;
+      k.read(kt, lane);
+      wave_sync();
+      if (more) rq.template issue<false>(jt + 1, pages, kt);
+      f32x16 s = k.scores(q, splat16(0.f));
+      if (masked) hide_unseen(s, seen, hh);
+      st.exponentials(s);
+      if (more) wait_vmcnt<LOADS>(); else wait_vmcnt<0>();  // the values; the next keys are younger
+      wave_sync();
+      Values<E, D> v;
+      v.read(vt, lane);
+      if (masked && __builtin_amdgcn_ballot_w64(v.finite()) != 0) add_odd_values<E, D>(vt, seen, hh, st.o);
+      wave_sync();
+      if (more) {
+        rq.template issue<true>(jt + 1, pages, vt);
+        pages = rq.pages(min(jt + 2, n_kt - 1));
+      }
+      v.add(s, st.l, st.o);
+    }
+    rq.w0 += window;
+    if (rq.w0 >= it.k0 + it.nk) break;
+    rq.wn = min(it.k0 + it.nk - rq.w0, window);
+    bad |= stage_table(a, it, rq.w0, rq.wn, table, lane, 64);
+    wave_sync();
+    pages = rq.pages(0);
+    rq.template issue<false>(0, pages, kt);
+    rq.template issue<true>(0, pages, vt);
+  }
+  store_result<E, D>(a, it, c, st, bad, lane & 31, hh);
+}
+
+// ---- MANY: four waves of 32 columns around a ring of stages (K' tile, V' tile); tile jt lives in stage jt % kStages.  Per tile: wait for its
+// loads, barrier (also: everyone has left the tile before), request tile jt + kStages - 1 over the one before, compute.
+template <typename E, int D>
+__device__ __forceinline__ void many_columns(const PagedArgs& a, const Item& it, int rep, int tid, uint32_t lds, int* table, float* gsm, int* any_bad) {
+  using S = Shape<E, D>;
+  constexpr int BK = S::kBK, NS = S::kStages, LOADS = S::kTileBytes / 1024 / 4;
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, window = S::kManyTable << a.log_page;
+  auto rq = requests<E, D, BK, LOADS>(a, it, table, wave, 4, lane);
+  rq.w0 = it.k0;
+  rq.wn = min(it.nk, window);
+  bool bad = it.x.broken;
+  auto stage = [&] {
+    const bool mine = stage_table(a, it, rq.w0, rq.wn, table, tid, 256);
+    if (lane == 0) any_bad[wave] = mine;
+  };
+  auto request = [&](int jt, int pages) {
+    const uint32_t dst = lds + (uint32_t)(jt % NS) * S::kStageBytes;
+    rq.template issue<false>(jt, pages, dst);
+    rq.template issue<true>(jt, pages, dst + S::kTileBytes);
+  };
+  auto start_window = [&] {
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  const float mu = m == -INFINITY ? 0.f : m;
-  const int gi = lane / LPR + (WAVES > 1 ? wave * G : 0), c = lane % LPR;
-  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-  for (int s = gi; s < n; s += GROUPS) {
-    const int64_t at = slot(s);
-    const float2 x = stat_of(at);
-    if (x.y == 0.f) continue;  // saw no key
-    const float w = fast_exp2(x.x - mu);
-    l += w * x.y;
-    if (at < 0) continue;
-    const float4 o = *reinterpret_cast<const float4*>(a.part + at * D + 4 * c);
-    y.x += w * o.x; y.y += w * o.y; y.z += w * o.z; y.w += w * o.w;
-  }
+    for (int w = 0; w < 4; ++w) bad |= any_bad[w] != 0;
 #pragma unroll
-  for (int o = LPR; o < 64; o <<= 1) {
-    l += __shfl_xor(l, o, 64);
-    y.x += __shfl_xor(y.x, o, 64); y.y += __shfl_xor(y.y, o, 64); y.z += __shfl_xor(y.z, o, 64); y.w += __shfl_xor(y.w, o, 64);
-  }
-  if constexpr (WAVES > 1) {
-    __shared__ float ls[WAVES];
-    sums[tid] = y;
-    if (lane == 0) ls[wave] = l;
+    for (int t = 0; t < NS - 1; ++t)
+      if (t * BK < rq.wn) request(t, rq.pages(t));
+  };
+  stage();
+  if (tid < D) gsm[tid] = scale_at(a.p, tid);
+  __syncthreads();
+  start_window();
+  Query<E, D> q;
+  const Column c = column_of<E, D>(a, it, rep, it.tile * kMany + wave * 32, lane, q, gsm);
+  State<D / 32> st;
+  st.clear();
+  auto block = [&](auto masked_c, uint32_t kt, int jb) {
+    constexpr bool MASKED = decltype(masked_c)::value != 0;
+    const uint32_t vt = kt + S::kTileBytes;
+    Keys<E, D> k;
+    k.read(kt, lane);
+    f32x16 s = k.scores(q, splat16(0.f));
+    if (MASKED) hide_unseen(s, c.lim - jb, hh);
+    st.exponentials(s);
+    Values<E, D> v;
+    v.read(vt, lane);
+    if (MASKED && __builtin_amdgcn_ballot_w64(v.finite()) != 0) add_odd_values<E, D>(vt, c.lim - jb, hh, st.o);
+    v.add(s, st.l, st.o);
+  };
+  while (true) {
+    wait_vmcnt<0>();  // the loads below are counted: nothing of the start may be in flight with them
+    const int n_kt = (rq.wn + BK - 1) / BK, off = rq.w0 - it.k0;
+    int next_pages = n_kt ? rq.pages(min(NS - 1, n_kt - 1)) : 0;
+    auto turn = [&](int jt) {
+      if (n_kt - 1 - jt >= NS - 2) wait_vmcnt<(NS - 2) * 2 * LOADS>(); else wait_vmcnt<0>();
+      __syncthreads();
+      if (jt + NS - 1 < n_kt) {
+        request(jt + NS - 1, next_pages);
+        next_pages = rq.pages(min(jt + NS, n_kt - 1));
+      }
+    };
+    // tiles every column of the wave sees whole, then the others: two loops, each with one form of the block
+    int jt = 0;
+    const int n_whole = max(min((c.all + 1 - off) / BK, n_kt), 0);
+    for (; jt < n_whole; ++jt) {
+      turn(jt);
+#pragma unroll
+      for (int kb = 0; kb < BK / 32; ++kb) block(IC<0>{}, lds + (uint32_t)(jt % NS) * S::kStageBytes + kb * 32 * S::kRB, off + jt * BK + 32 * kb);
+    }
+    for (; jt < n_kt; ++jt) {
+      turn(jt);
+#pragma unroll
+      for (int kb = 0; kb < BK / 32; ++kb)
+        if (off + jt * BK + 32 * kb <= c.any) block(IC<1>{}, lds + (uint32_t)(jt % NS) * S::kStageBytes + kb * 32 * S::kRB, off + jt * BK + 32 * kb);
+    }
+    rq.w0 += window;
+    if (rq.w0 >= it.k0 + it.nk) break;
+    rq.wn = min(it.k0 + it.nk - rq.w0, window);
+    __syncthreads();  // everyone is done with the page numbers and the stages
+    stage();
     __syncthreads();
-    if (wave) return;
-    l = 0.f;
-    y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      const float4 o = sums[w * 64 + lane];
-      l += ls[w];
-      y.x += o.x; y.y += o.y; y.z += o.z; y.w += o.w;
+    start_window();
+  }
+  store_result<E, D>(a, it, c, st, bad, wave * 32 + (lane & 31), hh);
+}
+
+__device__ __forceinline__ void clear_rest(const PagedArgs& a, int tid, int threads, int elem, int D) {
+  const segpt_paged_params& p = a.p;
+  int head, f, n;
+  sequence_rows(p, a.rows_each, 0, &head, &n);
+  sequence_rows(p, a.rows_each, p.B - 1, &f, &n);
+  const int tail = max(f + n, head);
+  for (int i = blockIdx.x; i < head + p.T - tail; i += gridDim.x) {  // rows before the first sequence and behind the last
+    const int t = i < head ? i : i - head + tail;
+    for (int x = tid; x < p.H * D; x += threads) {
+      if (elem == 2) row_of<uint16_t>(p.o, t, x / D)[x % D] = 0;
+      else row_of<float>(p.o, t, x / D)[x % D] = 0.f;
     }
   }
-  if (own.broken) l = __builtin_nanf("");
-  if (lane >= LPR) return;
-  float f = l == 0.f ? 0.f : 1.0f / l;
-  if (p.lse && c == 0) p.lse[(int64_t)t * p.H + h] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
-  if (p.gate.ptr) f *= gate_factor<E, D>(p, t, h);
-  E* out = row_of<E>(p.o, t, h) + 4 * c;
-  const float v[4] = {y.x * f, y.y * f, y.z * f, y.w * f};
-  if constexpr (sizeof(E) == 2) *reinterpret_cast<u32x2*>(out) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-  else store16(out, v);
+}
+
+// Launches whose entries are all FEW: a workgroup is one wave
+template <typename E, int D>
+__global__ __launch_bounds__(64, (Shape<E, D>::kOcc)) void paged_few_kernel(PagedArgs a) {
+  using S = Shape<E, D>;
+  __shared__ __attribute__((aligned(1024))) char lds[S::kFewBytes];
+  __shared__ __attribute__((aligned(16))) float gsm[D];
+  __shared__ int table[S::kFewTable + 2];
+  const int lane = threadIdx.x, rep = a.p.H / a.p.Hkv;
+  if (a.p.flags & SEGPT_FLAG_ZERO_REST) clear_rest(a, lane, 64, sizeof(E), D);
+  Entry mine;
+  const Shares share = share_blocks(a, lane, rep, &mine);
+  const Item it = locate<false>(a, lane, rep, share, mine, blockIdx.x);
+  if (it.valid) few_columns<E, D>(a, it, rep, lane, lds_addr_of(lds), table, gsm);
+}
+
+// Any launch: a workgroup is an item of many columns, or four of few
+template <typename E, int D>
+__global__ __launch_bounds__(256, (Shape<E, D>::kOcc)) void paged_any_kernel(PagedArgs a) {
+  using S = Shape<E, D>;
+  constexpr int kLds = S::kManyBytes > 4 * S::kFewBytes ? S::kManyBytes : 4 * S::kFewBytes;
+  __shared__ __attribute__((aligned(1024))) char lds[kLds];
+  __shared__ __attribute__((aligned(16))) float gsm[4][D];
+  __shared__ int table[S::kManyTable + 8];
+  __shared__ int any_bad[4];
+  static_assert(4 * (S::kFewTable + 2) <= S::kManyTable + 8, "four waves' page numbers");
+  const int tid = threadIdx.x, lane = tid & 63, rep = a.p.H / a.p.Hkv;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if (a.p.flags & SEGPT_FLAG_ZERO_REST) clear_rest(a, tid, 256, sizeof(E), D);
+  Entry mine;
+  const Shares share = share_blocks(a, lane, rep, &mine);
+  if ((int)blockIdx.x < a.n_many) {
+    const Item it = locate<true>(a, lane, rep, share, mine, blockIdx.x);
+    if (it.valid) many_columns<E, D>(a, it, rep, tid, lds_addr_of(lds), table, gsm[0], any_bad);
+  } else {
+    const Item it = locate<false>(a, lane, rep, share, mine, ((int)blockIdx.x - a.n_many) * 4 + wave);
+    if (it.valid) few_columns<E, D>(a, it, rep, lane, lds_addr_of(lds) + wave * S::kFewBytes, table + wave * (S::kFewTable + 2), gsm[wave]);
+  }
+}
+
+// Joins the partial results of a tile's columns: its sequence's shares and, behind them, the prefix's.  A unit of D / 4 lanes holds a row; a
+// workgroup takes `step` columns at a time, with its other units side by side over the shares (kBatch of them requested together).  The
+// units' sums meet in LDS.  Fixed order: deterministic.
+constexpr int kMergeThreads = 256;
+template <typename E, int D>
+__global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedArgs a, int subs, int per_sub, int step) {
+  const segpt_paged_params& p = a.p;
+  constexpr int LPR = D / 4, kUnits = kMergeThreads / LPR, kBatch = 4;
+  __shared__ float4 sums[kMergeThreads];
+  __shared__ float2 stats[kUnits];
+  const int tid = threadIdx.x, lane = tid & 63, unit = tid / LPR, c = tid % LPR;
+  const int rep = p.H / p.Hkv;
+  Entry mine;
+  const Shares share = share_blocks(a, lane, rep, &mine);
+  const int which = blockIdx.x / subs, sub = blockIdx.x - which * subs;
+  const Found own = find_entry<kFindJoin>(a, lane, rep, share, mine, which);
+  if (own.entry < 0) return;
+  const int g = (which - own.base) % p.Hkv, tile = (which - own.base) / p.Hkv, cols = own.n * rep, tile_cols = own.many ? kMany : kFew;
+  Found pre{-1, 0, 0, 0, 0, 0, 0, 0, false, false};
+  if (a.shared) pre = find_entry<kFindFirst>(a, lane, rep, share, mine, 0);
+  const int pre_cols = pre.many ? kMany : kFew;
+  const int n = own.shares + pre.shares, wide = kUnits / step;  // units of a column
+  for (int c0 = sub * per_sub; c0 < min((sub + 1) * per_sub, tile_cols); c0 += step) {  // the same for all threads
+    if (tile * tile_cols + c0 >= cols) return;
+    const int col = tile * tile_cols + min(c0 + unit % step, tile_cols - 1);
+    const bool live = col < cols && c0 + unit % step < min((sub + 1) * per_sub, tile_cols);
+    const int i = min(col, cols - 1) / rep, t = own.first + i, h = g * rep + (min(col, cols - 1) - i * rep);
+    const int pcol = (t - pre.first) * rep + h - g * rep, ptile = pcol / pre_cols;
+    auto place = [&](int s) {  // row of share s among all partial results; none: there is no room for it
+      const bool is_own = s < own.shares;
+      const Found& x = is_own ? own : pre;
+      const int slot = x.slot + (((is_own ? tile : ptile) * x.shares + (is_own ? s : s - own.shares)) * p.Hkv + g) * (x.many ? kMany / 32 : 1);
+      return slot < a.n_slots - (x.many ? kMany / 32 - 1 : 0) ? (int64_t)slot * 32 + (is_own ? col - tile * tile_cols : pcol - ptile * pre_cols) : (int64_t)-1;
+    };
+    float m = -INFINITY, l = 0.f;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (live)
+      for (int s0 = unit / step; s0 < n; s0 += kBatch * wide) {
+        float2 x[kBatch];
+        float4 o[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int64_t at = place(min(s0 + u * wide, n - 1));
+          x[u] = at < 0 ? make_float2(0.f, __builtin_nanf("")) : a.stat[at];
+          o[u] = *reinterpret_cast<const float4*>(a.part + max(at, (int64_t)0) * D + 4 * c);
+          if (s0 + u * wide >= n) x[u] = make_float2(-INFINITY, 0.f);
+        }
+        float top = m;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) top = fmaxf(top, x[u].x);
+        const float ref = top == -INFINITY ? 0.f : top, w0 = fast_exp2(m - ref);
+        m = top;
+        l *= w0;
+        y.x *= w0; y.y *= w0; y.z *= w0; y.w *= w0;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          if (x[u].y == 0.f) continue;  // saw no key
+          const float w = fast_exp2(x[u].x - ref);
+          l += w * x[u].y;
+          y.x += w * o[u].x; y.y += w * o[u].y; y.z += w * o[u].z; y.w += w * o[u].w;
+        }
+      }
+    if (wide > 1) {
+      __syncthreads();  // the round before has been read
+      sums[tid] = y;
+      if (c == 0) stats[unit] = make_float2(m, l);
+      __syncthreads();
+      if (unit >= step) continue;
+      float top = m;
+      for (int w = 1; w < wide; ++w) top = fmaxf(top, stats[w * step + unit].x);
+      const float ref = top == -INFINITY ? 0.f : top, w0 = fast_exp2(m - ref);
+      m = top;
+      l *= w0;
+      y.x *= w0; y.y *= w0; y.z *= w0; y.w *= w0;
+      for (int w = 1; w < wide; ++w) {
+        const float2 x = stats[w * step + unit];
+        const float4 o = sums[w * step * LPR + tid];
+        const float f = fast_exp2(x.x - ref);
+        l += f * x.y;
+        y.x += f * o.x; y.y += f * o.y; y.z += f * o.z; y.w += f * o.w;
+      }
+    }
+    if (!live) continue;
+    if (own.broken) l = __builtin_nanf("");
+    float f = l == 0.f ? 0.f : 1.0f / l;
+    if (p.lse && c == 0) p.lse[(int64_t)t * p.H + h] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
+    if (p.gate.ptr) f *= gate_factor<E, D>(p, t, h);
+    E* out = row_of<E>(p.o, t, h) + 4 * c;
+    const float v[4] = {y.x * f, y.y * f, y.z * f, y.w * f};
+    if constexpr (sizeof(E) == 2) *reinterpret_cast<u32x2*>(out) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    else store16(out, v);
+  }
 }
 
 // ---- host side
-int waves_of(const segpt_paged_params& p) {
-  if (p.dtype == SEGPT_DTYPE_FP32 && p.D == 128) return 4;
-  return p.prefix_table || (int64_t)p.H / p.Hkv * p.T > 32ll * p.B ? 4 : 1;
+bool all_few(const segpt_paged_params& p) {  // known on the host
+  return !p.prefix_table && !p.seq_start && (int64_t)p.H / p.Hkv * (p.T / p.B) <= kFew;
 }
 
 // fills the plan; returns the scratch bytes of the partials
 size_t plan(const segpt_paged_params& p, PagedArgs& a) {
-  const int nw = waves_of(p), cols = 32 * nw, elem = p.dtype == SEGPT_DTYPE_FP32 ? 4 : 2;
+  const int row_bytes = p.D * (p.dtype == SEGPT_DTYPE_FP32 ? 4 : 2), rep = p.H / p.Hkv;
   a.shared = p.prefix_table ? 1 : 0;
   a.entries = p.B + a.shared;
   a.rows_each = p.seq_start ? 0 : p.T / p.B;
   a.log_page = __builtin_ctz((unsigned)p.page_size);
   a.capacity = paged_capacity(p);
-  const int row_bytes = p.D * elem;
-  a.target = nw == 4 ? 256 * (row_bytes <= 128 ? 3 : row_bytes <= 256 ? 2 : 1) : 256 * (row_bytes <= 128 ? 6 : row_bytes <= 256 ? 3 : 2);
-  a.min_share = nw == 4 ? 4 : 2;
-  // every entry's tiles: whole ones of the rows there are, and one begun; every tile's shares: its part of the target, and one begun
-  const int64_t all_cols = (int64_t)p.T * (p.H / p.Hkv);
-  int64_t tiles = all_cols / cols + p.B;
-  if (!p.seq_start) tiles = (all_cols / p.B + cols - 1) / cols * p.B;
-  if (a.shared) tiles += (all_cols + cols - 1) / cols;
-  const int64_t items = tiles * p.Hkv + a.target + 64;  // the sum that gives the length of a share is rounded
-  a.n_items = (int32_t)std::min<int64_t>(items, INT32_MAX);
+  a.target = 256 * (row_bytes <= 128 ? 3 : row_bytes <= 256 ? 2 : 1);
+  a.min_few = 2;
+  a.min_many = 4;
+  // Tiles: whole ones of the columns there are, and one begun an entry.  Items: a tile's part of what the target stands for, and one begun.
+  const int64_t cols = (int64_t)p.T * rep;
+  int64_t many = cols / kMany + std::min<int64_t>(p.B, cols / (kFew + 1)), few = std::min<int64_t>(p.B, p.T);
+  if (!p.seq_start) {
+    const int64_t each = cols / p.B;
+    many = each > kFew ? (each + kMany - 1) / kMany * p.B : 0;
+    few = each > kFew ? 0 : p.B;
+  }
+  const int64_t own = many + few;
+  if (a.shared && cols > kFew) many += (cols + kMany - 1) / kMany;
+  else if (a.shared) few += 1;
+  const int64_t slack = 64;  // the sum that gives the length of a share is rounded
+  const int64_t n_many = many ? many * p.Hkv + a.target + slack : 0, n_few = few ? few * p.Hkv + 4 * a.target + slack : 0;
+  a.n_many = (int32_t)std::min<int64_t>(n_many, INT32_MAX);
+  a.n_few = (int32_t)std::min<int64_t>(n_few, INT32_MAX);
   // a tile that leaves partial results has two shares or more, i.e. at most twice its part of the target; beside a prefix all leave them
-  a.n_slots = a.shared ? a.n_items : (int32_t)std::min<int64_t>(items, 2 * a.target + 64);
-  return items > INT32_MAX ? SIZE_MAX : (size_t)a.n_slots * cols * (p.D + 2) * sizeof(float);
+  const int64_t most = 2 * ((int64_t)a.target + slack);
+  const int64_t slots = kMany / 32 * (a.shared ? n_many : std::min(n_many, most)) + (a.shared ? n_few : std::min(n_few, 4 * most));
+  a.n_slots = (int32_t)std::min<int64_t>(slots, INT32_MAX / 32);
+  a.n_joins = (int32_t)std::min<int64_t>(own * p.Hkv, a.shared ? INT32_MAX : 5 * most);
+  return n_many + n_few > INT32_MAX / 2 || slots > INT32_MAX / 32 ? SIZE_MAX : (size_t)a.n_slots * 32 * (p.D + 2) * sizeof(float);
 }
 
-template <typename E, int D, int NW>
+template <typename E, int D>
 int launch(const PagedArgs& a, hipStream_t st) {
   const segpt_paged_params& p = a.p;
-  hipLaunchKernelGGL((paged_attn_kernel<E, D, NW>), dim3((unsigned)a.n_items), dim3(64 * NW), 0, st, a);
+  if (all_few(p)) hipLaunchKernelGGL((paged_few_kernel<E, D>), dim3((unsigned)a.n_few), dim3(64), 0, st, a);
+  else hipLaunchKernelGGL((paged_any_kernel<E, D>), dim3((unsigned)(a.n_many + (a.n_few + 3) / 4)), dim3(256), 0, st, a);
   const int rc = (int)hipGetLastError();
   if (rc) return rc;
-  const int64_t rows = (int64_t)p.T * p.H;
-  if (rows <= 4096) hipLaunchKernelGGL((paged_merge_kernel<E, D, 4>), dim3((unsigned)rows), dim3(kMergeThreads), 0, st, a, 32 * NW);
-  else hipLaunchKernelGGL((paged_merge_kernel<E, D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(kMergeThreads), 0, st, a, 32 * NW);
+  // columns at a time and workgroups a tile: as many units over the shares as leave each a batch
+  constexpr int kUnits = kMergeThreads / (D / 4);
+  const int64_t all = (int64_t)p.T * (p.H / p.Hkv);
+  const int most = a.n_many - (a.shared && all > kFew) > 0 ? kMany : kFew, cols = p.seq_start ? most : (int)std::min<int64_t>(most, all / p.B);
+  int64_t shares = 4 * a.target / std::max<int64_t>(1, a.n_joins) + 1;
+  if (a.shared) {  // the prefix's own: its length is known, the sequences' are not
+    const int64_t blocks = (p.prefix_len + kBlock - 1) / kBlock, tiles = (all + kMany - 1) / kMany * p.Hkv;
+    shares = std::max(shares, blocks / std::max<int64_t>(a.min_many, tiles * blocks / a.target));
+  }
+  int step = kUnits;
+  while (step > 1 && kUnits / step * 4 < shares) step /= 2;
+  int per_sub = step;
+  while ((int64_t)a.n_joins * ((cols + per_sub - 1) / per_sub) > 8192 && per_sub < kMany) per_sub *= 2;
+  const int subs = (cols + per_sub - 1) / per_sub;
+  hipLaunchKernelGGL((paged_merge_kernel<E, D>), dim3((unsigned)(a.n_joins * subs)), dim3(kMergeThreads), 0, st, a, subs, per_sub, step);
   return (int)hipGetLastError();
-}
-template <typename E, int D>
-int launch_waves(const PagedArgs& a, int nw, hipStream_t st) {
-  if constexpr (D * sizeof(E) > 256) return launch<E, D, 4>(a, st);
-  else return nw == 4 ? launch<E, D, 4>(a, st) : launch<E, D, 1>(a, st);
 }
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -708,11 +979,10 @@ int segpt_paged_attn(const segpt_paged_params* p, void* stream) {
   if (!p->workspace || p->workspace_bytes < up256(need)) return SEGPT_E_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(p->workspace) & 255u) return SEGPT_E_ALIGN;
   a.part = reinterpret_cast<float*>(p->workspace);
-  a.stat = reinterpret_cast<float2*>(a.part + (size_t)a.n_slots * 32 * waves_of(*p) * p->D);
+  a.stat = reinterpret_cast<float2*>(a.part + (size_t)a.n_slots * 32 * p->D);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const int nw = waves_of(*p);
-  if (p->dtype == SEGPT_DTYPE_BF16) return p->D == 64 ? launch_waves<uint16_t, 64>(a, nw, st) : launch_waves<uint16_t, 128>(a, nw, st);
-  return p->D == 32 ? launch_waves<float, 32>(a, nw, st) : p->D == 64 ? launch_waves<float, 64>(a, nw, st) : launch_waves<float, 128>(a, nw, st);
+  if (p->dtype == SEGPT_DTYPE_BF16) return p->D == 64 ? launch<uint16_t, 64>(a, st) : launch<uint16_t, 128>(a, st);
+  return p->D == 32 ? launch<float, 32>(a, st) : p->D == 64 ? launch<float, 64>(a, st) : launch<float, 128>(a, st);
 }
 
 }  // extern "C"

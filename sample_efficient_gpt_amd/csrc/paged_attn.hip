@@ -175,7 +175,7 @@ struct Shape {
   // FEW: one block of keys and one of values a wave
   static constexpr int kFewTable = 64;
   static constexpr int kFewBytes = 2 * kBlock * kRB;
-  static constexpr int kOcc = kRB <= 128 ? 3 : kRB <= 256 ? 2 : 1;  // workgroups of four waves per CU
+  static constexpr int kOcc = kRB > 256 ? 1 : kRB > 128 || sizeof(E) == 4 ? 2 : 3;  // workgroups of four waves per CU
 };
 
 // query columns in the B operand's layout, scaled by everything that does not depend on the key (gsm: g_q g_k sm_scale log2 e); D / 2 values
@@ -244,7 +244,6 @@ struct Query<float, D> {
 };
 
 __device__ __forceinline__ float lds_read_f(uint32_t addr) { return *(const __attribute__((address_space(3))) float*)addr; }
-__device__ __forceinline__ uint16_t lds_read_h(uint32_t addr) { return *(const __attribute__((address_space(3))) uint16_t*)addr; }
 
 template <typename E, int D>
 __device__ __forceinline__ float gate_factor(const segpt_paged_params& p, int t, int h) {
@@ -306,7 +305,11 @@ __device__ __forceinline__ float scale_at(const segpt_paged_params& p, int d) {
 }
 
 // Requests of tiles of keys w0 .. w0 + wn - 1.  A load covers kRowsPerLoad rows, at most 8, of one page: its address is a scalar base and
-// a lane offset.  LOADS loads a tensor and tile; number ps is load first + ps * step of the tile.
+// a lane offset.  LOADS loads a tensor and tile; number ps is load first + ps * step of the tile.  Where the rows of a load begin is worked out
+// side by side, by lane ps for load ps, one tile ahead; what a lane adds is the same for every whole tile.
+struct Places {
+  int64_t k, v;  // byte offsets from the head's first row, lane ps: of load ps
+};
 template <typename E, int D, int BK, int LOADS>
 struct Requests {
   using Z = Tile<E, D>;
@@ -315,30 +318,48 @@ struct Requests {
   uint32_t kstep, vstep;
   int w0, wn, log_page, first, step, lane;
   const int* table;
+  uint32_t klane[LOADS], vlane[LOADS];
   __device__ __forceinline__ int first_row(int jt, int ps) const {  // from w0 on; past the last key: the last rows once more
     return min(jt * BK + (ps * step + first) * Z::kRowsPerLoad, (wn - 1) & ~(Z::kRowsPerLoad - 1));
   }
-  __device__ __forceinline__ int pages(int jt) const {  // lane ps: the page number of load ps
-    return table[((w0 + first_row(jt, min(lane, LOADS - 1))) >> log_page) - (w0 >> log_page)];
+  __device__ __forceinline__ uint32_t chunk(int ps) const {
+    return (uint32_t)((lane % Z::kChunks) ^ Z::f((ps * step + first) * Z::kRowsPerLoad + lane / Z::kChunks)) << 4;
+  }
+  __device__ __forceinline__ Places places(int jt) const {
+    const int key = w0 + first_row(jt, min(lane, LOADS - 1)), page = table[(key >> log_page) - (w0 >> log_page)];
+    const uint32_t slot = (uint32_t)(key & ((1 << log_page) - 1));
+    return {page * kpage + (int64_t)((uint64_t)slot * kstep), page * vpage + (int64_t)((uint64_t)slot * vstep)};
+  }
+  static __device__ __forceinline__ const char* at(const char* base, int64_t off, int ps) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)off, ps), hi = __builtin_amdgcn_readlane((int)(off >> 32), ps);
+    return base + (int64_t)((uint64_t)hi << 32 | lo);
   }
   template <bool VALUES>
-  __device__ __forceinline__ void issue(int jt, int pages, uint32_t dst) const {
-    const int lrow = lane / Z::kChunks;
+  __device__ __forceinline__ void issue(int jt, const Places& places, uint32_t dst) const {
+    if (wn - jt * BK >= BK) {
 #pragma unroll
-    for (int ps = 0; ps < LOADS; ++ps) {
-      const int r0 = first_row(jt, ps), slot = (w0 + r0) & ((1 << log_page) - 1);
-      const int64_t page = __builtin_amdgcn_readlane(pages, ps);
-      const uint32_t r = min(lrow, wn - 1 - r0), col = (uint32_t)((lane % Z::kChunks) ^ Z::f((ps * step + first) * Z::kRowsPerLoad + lrow)) << 4;
-      const uint32_t rs = VALUES ? vstep : kstep;
-      gload_lds16_so((VALUES ? vbase + page * vpage : kbase + page * kpage) + (int64_t)slot * rs, r * rs + col, dst + (ps * step + first) * 1024);
+      for (int ps = 0; ps < LOADS; ++ps)
+        gload_lds16_so(VALUES ? at(vbase, places.v, ps) : at(kbase, places.k, ps), VALUES ? vlane[ps] : klane[ps], dst + (ps * step + first) * 1024);
+    } else {
+#pragma unroll
+      for (int ps = 0; ps < LOADS; ++ps) {
+        const uint32_t r = min(lane / Z::kChunks, wn - 1 - first_row(jt, ps));
+        gload_lds16_so(VALUES ? at(vbase, places.v, ps) : at(kbase, places.k, ps), r * (VALUES ? vstep : kstep) + chunk(ps), dst + (ps * step + first) * 1024);
+      }
     }
   }
 };
 template <typename E, int D, int BK, int LOADS>
 __device__ __forceinline__ Requests<E, D, BK, LOADS> requests(const PagedArgs& a, const Item& it, const int* table, int first, int step, int lane) {
   const segpt_paged_params& p = a.p;
-  return {page_row<E>(p.k_pages, 0, it.g, 0), page_row<E>(p.v_pages, 0, it.g, 0), p.k_pages.stride_b * (int)sizeof(E), p.v_pages.stride_b * (int)sizeof(E),
-          (uint32_t)p.k_pages.stride_s * (int)sizeof(E), (uint32_t)p.v_pages.stride_s * (int)sizeof(E), 0, 0, a.log_page, first, step, lane, table};
+  Requests<E, D, BK, LOADS> r{page_row<E>(p.k_pages, 0, it.g, 0), page_row<E>(p.v_pages, 0, it.g, 0), p.k_pages.stride_b * (int)sizeof(E), p.v_pages.stride_b * (int)sizeof(E),
+          (uint32_t)p.k_pages.stride_s * (int)sizeof(E), (uint32_t)p.v_pages.stride_s * (int)sizeof(E), it.k0, 0, a.log_page, first, step, lane, table};
+#pragma unroll
+  for (int ps = 0; ps < LOADS; ++ps) {
+    r.klane[ps] = (uint32_t)(lane / Tile<E, D>::kChunks) * r.kstep + r.chunk(ps);
+    r.vlane[ps] = (uint32_t)(lane / Tile<E, D>::kChunks) * r.vstep + r.chunk(ps);
+  }
+  return r;
 }
 
 // ---- a lane's column, and what it sees of the item's keys (counted from k0 on)
@@ -419,35 +440,36 @@ struct Keys<float, D> {
     return s;
   }
 };
-// V' rows as the A operand of O^T.  finite(): replaces what is not a number or infinite by 0, returns whether there was any
+// V' rows as the A operand of O^T.  A value that is not finite must reach the rows that see its key, and not the others as 0 * inf: in a block
+// that not all rows see, clear() makes those 0 and says whether there were any; add_odd_values() puts them back behind the loop.
 template <typename E, int D>
 struct Values;
 template <int D>
 struct Values<uint16_t, D> {
   static constexpr int MB = D / 32;
-  bf16x8 v[MB][2];
+  u32x4 v[MB][2];
   __device__ __forceinline__ void read(uint32_t tile, int lane) {
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2) v[mb][s2] = swz_frag_tr<D>(tile + swz_off_tr<D>(lane), mb, s2);
+      for (int s2 = 0; s2 < 2; ++s2) v[mb][s2] = __builtin_bit_cast(u32x4, swz_frag_tr<D>(tile + swz_off_tr<D>(lane), mb, s2));
   }
-  __device__ __forceinline__ bool finite() {
-    bool odd = false;
+  __device__ __forceinline__ bool clear() {
+    typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+    uint32_t all = ~0u;
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
-        u32x4 w = __builtin_bit_cast(u32x4, v[mb][s2]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool lo = (w[e] & 0x7f80u) == 0x7f80u, hi = (w[e] & 0x7f800000u) == 0x7f800000u;
-          odd |= lo | hi;
-          w[e] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+        for (int e = 0; e < 4; ++e) {  // sign of |x| - inf: all ones where x is finite
+          const uint32_t finite = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(i16x2, v[mb][s2][e] & 0x7fff7fffu) - (int16_t)0x7f80) >> 15);
+          v[mb][s2][e] &= finite;
+          all &= finite;
         }
-        v[mb][s2] = as_bf16x8(w);
+        asm volatile("" : "+v"(v[mb][s2]));  // whole registers again: as bf16 vectors they would be taken apart, element by element
       }
-    return odd;
+    return all != ~0u;
   }
   // adds the probabilities s to the sums l, as they are rounded, and their products with the values to o
   __device__ __forceinline__ void add(f32x16 s, float (&l)[2], f32x16 (&o)[MB]) const {
@@ -455,7 +477,7 @@ struct Values<uint16_t, D> {
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb) o[mb] = mfma32(v[mb][s2], pb[s2], o[mb]);
+      for (int mb = 0; mb < MB; ++mb) o[mb] = mfma32(as_bf16x8(v[mb][s2]), pb[s2], o[mb]);
   }
 };
 template <int D>
@@ -471,7 +493,7 @@ struct Values<float, D> {
       for (int mb = 0; mb < MB; ++mb) v[mb][r] = lds_read_f(tile + key * (4 * D) + (((8 * mb + (ln >> 2)) ^ Tile<float, D>::f(key)) << 4) + 4 * (ln & 3));
     }
   }
-  __device__ __forceinline__ bool finite() {
+  __device__ __forceinline__ bool clear() {
     bool odd = false;
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
@@ -492,54 +514,54 @@ struct Values<float, D> {
       for (int mb = 0; mb < MB; ++mb) o[mb] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[mb][r], s[r], o[mb], 0, 0, 0);
   }
 };
-// Values that are not finite, key by key, for the rows that see them: their probability is positive, so the sum is the value, or NaN
-// where signs meet.  (Through the product they would reach the other rows as 0 * inf.)
-template <typename E, int D>
-__device__ __forceinline__ void add_odd_values(uint32_t tile, int seen, int hh, f32x16 (&o)[D / 32]) {
-  for (int key = 0; key < 32; ++key) {
-    const bool visible = key <= seen;
-#pragma unroll
-    for (int mb = 0; mb < D / 32; ++mb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int d = 32 * mb + 8 * (r >> 2) + 4 * hh + (r & 3), byte = d * (int)sizeof(E);
-        const uint32_t at = tile + key * Tile<E, D>::kRB + (((byte >> 4) ^ Tile<E, D>::f(key)) << 4) + (byte & 15);
-        float v;
-        if constexpr (sizeof(E) == 2) v = bf16_to_f32(lds_read_h(at)); else v = lds_read_f(at);
-        if (visible && !(fabsf(v) < INFINITY)) o[mb][r] += v;
-      }
-  }
-}
+// Sums of a column.  Scores come out of the product less the reference already: it is the C operand of their first instruction.
 template <int MB>
 struct State {
-  f32x16 o[MB];
-  float m, l[2];  // reference (log2 units); sums of this lane's half of the keys
+  f32x16 o[MB], less;  // less: the reference's negative, in every register
+  float m, limit;      // reference (log2 units); a score may exceed it by `limit` before it is raised: -inf as long as no key has been seen
+  float l[2];          // of this lane's half of the keys
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) o[mb] = splat16(0.f);
-    m = -INFINITY;
+    less = splat16(0.f);
+    m = 0.f;
+    limit = -INFINITY;
     l[0] = l[1] = 0.f;
   }
-  // scores to probabilities against the reference, which is raised where a score exceeds it by kLazy
-  __device__ __forceinline__ void exponentials(f32x16& s) {
-    float mx = s[0];
+  __device__ __forceinline__ float reference() const { return limit == -INFINITY ? -INFINITY : m; }
+  // scores of N blocks to probabilities
+  template <int N>
+  __device__ __forceinline__ void exponentials(f32x16 (&s)[N]) {
+    float mx[N];
 #pragma unroll
-    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-    mx = half_max(mx);
-    const bool need = mx > m + kLazy;
-    if (__builtin_amdgcn_ballot_w64(need) != 0) {
-      const float m_new = need ? mx : m, corr = need ? fast_exp2(m - m_new) : 1.f;
-      m = m_new;
+    for (int n = 0; n < N; ++n) {
+      mx[n] = s[n][0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) mx[n] = fmaxf(mx[n], s[n][r]);
+    }
+#pragma unroll
+    for (int n = 1; n < N; ++n) mx[0] = fmaxf(mx[0], mx[n]);
+    const float top = half_max(mx[0]);
+    if (__builtin_amdgcn_ballot_w64(top > limit) != 0) {
+      const float up = top > limit ? top : 0.f, corr = limit == -INFINITY ? 1.f : fast_exp2(-up);  // nothing to scale before the first key
+      m += up;
+      if (top > limit) limit = kLazy;
+      less = splat16(-m);
       l[0] *= corr;
       l[1] *= corr;
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[mb][r] *= corr;
-    }
-    const float mu = m == -INFINITY ? 0.f : m;  // nothing seen yet: keep exp2 away from inf - inf
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = fast_exp2(s[r] - mu);
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[n][r] -= up;
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[n][r] = fast_exp2(s[n][r]);
   }
 };
 __device__ __forceinline__ void hide_unseen(f32x16& s, int seen, int hh) {  // register r holds key 4 hh + c_r, c_r = 8 (r / 4) + r % 4
@@ -549,12 +571,32 @@ __device__ __forceinline__ void hide_unseen(f32x16& s, int seen, int hh) {  // r
     if (8 * (r >> 2) + (r & 3) > t) s[r] = -INFINITY;
 }
 
+// The values that Values::clear() left out of the product, key by key, for the rows that see them: their probability is positive, so a sum
+// with one is that value, or NaN where signs meet.
+template <typename E, int D, int BK>
+__device__ __forceinline__ void add_odd_values(const PagedArgs& a, const Item& it, const Column& c, int hh, f32x16 (&o)[D / 32]) {
+  for (int j = (max(c.all, -1) + 1) & ~(BK - 1); j <= c.any; ++j) {  // tiles that not all rows see whole
+    const int key = it.k0 + j, page = it.ids[key >> a.log_page];
+    if ((uint32_t)page >= (uint32_t)a.p.n_pages) continue;  // the rows are NaN as a whole
+    const E* row = reinterpret_cast<const E*>(page_row<E>(a.p.v_pages, page, it.g, key & ((1 << a.log_page) - 1)));
+#pragma unroll
+    for (int mb = 0; mb < D / 32; ++mb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const E e = row[32 * mb + 8 * (r >> 2) + 4 * hh + (r & 3)];
+        float v;
+        if constexpr (sizeof(E) == 2) v = bf16_to_f32(e); else v = e;
+        if (j <= c.lim && !(fabsf(v) < INFINITY)) o[mb][r] += v;
+      }
+  }
+}
+
 // What an item leaves: y where it is its tile's only one, else a partial result
 template <typename E, int D>
 __device__ __forceinline__ void store_result(const PagedArgs& a, const Item& it, const Column& c, State<D / 32>& st, bool bad, int slot_col, int hh) {
   const segpt_paged_params& p = a.p;
   constexpr int MB = D / 32;
-  float l = half_sum(st.l[0] + st.l[1]), m = st.m;
+  float l = half_sum(st.l[0] + st.l[1]), m = st.reference();
   if (bad) { l = __builtin_nanf(""); m = 0.f; }
   if (!c.live) return;
   if (!it.direct) {
@@ -605,19 +647,21 @@ __device__ __forceinline__ void few_columns(const PagedArgs& a, const Item& it, 
   bool bad = it.x.broken | stage_table(a, it, rq.w0, rq.wn, table, lane, 64);
   for (int d = lane; d < D; d += 64) gsm[d] = scale_at(a.p, d);
   wave_sync();
-  int pages = rq.wn ? rq.pages(0) : 0;
+  Places at{0, 0};
   if (rq.wn) {
-    rq.template issue<false>(0, pages, kt);
-    rq.template issue<true>(0, pages, vt);
+    at = rq.places(0);
+    rq.template issue<false>(0, at, kt);
+    rq.template issue<true>(0, at, vt);
   }
   Query<E, D> q;
   const Column c = column_of<E, D>(a, it, rep, it.tile * kFew, lane, q, gsm);
   State<D / 32> st;
   st.clear();
+  bool odd = false;
   while (true) {
     const int n_kt = (rq.wn + kBlock - 1) / kBlock;
     wait_vmcnt<0>();  // the loads below are counted: nothing of the start may be in flight with them
-    if (n_kt > 1) pages = rq.pages(1);
+    if (n_kt > 1) at = rq.places(1);
     for (int jt = 0; jt < n_kt; ++jt) {
       const bool more = jt + 1 < n_kt;
       const int seen = c.lim - (rq.w0 - it.k0) - jt * kBlock;
@@ -627,31 +671,32 @@ __device__ __forceinline__ void few_columns(const PagedArgs& a, const Item& it, 
       Keys<E, D> k;
       k.read(kt, lane);
       wave_sync();
-      if (more) rq.template issue<false>(jt + 1, pages, kt);
-      f32x16 s = k.scores(q, splat16(0.f));
-      if (masked) hide_unseen(s, seen, hh);
+      if (more) rq.template issue<false>(jt + 1, at, kt);
+      f32x16 s[1] = {k.scores(q, st.less)};
+      if (masked) hide_unseen(s[0], seen, hh);
       st.exponentials(s);
       if (more) wait_vmcnt<LOADS>(); else wait_vmcnt<0>();  // the values; the next keys are younger
       wave_sync();
       Values<E, D> v;
       v.read(vt, lane);
-      if (masked && __builtin_amdgcn_ballot_w64(v.finite()) != 0) add_odd_values<E, D>(vt, seen, hh, st.o);
+      if (masked) odd |= v.clear();
       wave_sync();
       if (more) {
-        rq.template issue<true>(jt + 1, pages, vt);
-        pages = rq.pages(min(jt + 2, n_kt - 1));
+        rq.template issue<true>(jt + 1, at, vt);
+        at = rq.places(min(jt + 2, n_kt - 1));
       }
-      v.add(s, st.l, st.o);
+      v.add(s[0], st.l, st.o);
     }
     rq.w0 += window;
     if (rq.w0 >= it.k0 + it.nk) break;
     rq.wn = min(it.k0 + it.nk - rq.w0, window);
     bad |= stage_table(a, it, rq.w0, rq.wn, table, lane, 64);
     wave_sync();
-    pages = rq.pages(0);
-    rq.template issue<false>(0, pages, kt);
-    rq.template issue<true>(0, pages, vt);
+    at = rq.places(0);
+    rq.template issue<false>(0, at, kt);
+    rq.template issue<true>(0, at, vt);
   }
+  if (__builtin_amdgcn_ballot_w64(odd) != 0) add_odd_values<E, D, kBlock>(a, it, c, hh, st.o);
   store_result<E, D>(a, it, c, st, bad, lane & 31, hh);
 }
 
@@ -666,23 +711,22 @@ __device__ __forceinline__ void many_columns(const PagedArgs& a, const Item& it,
   rq.w0 = it.k0;
   rq.wn = min(it.nk, window);
   bool bad = it.x.broken;
-  auto stage = [&] {
+  auto stage_pages = [&] {
     const bool mine = stage_table(a, it, rq.w0, rq.wn, table, tid, 256);
     if (lane == 0) any_bad[wave] = mine;
   };
-  auto request = [&](int jt, int pages) {
-    const uint32_t dst = lds + (uint32_t)(jt % NS) * S::kStageBytes;
-    rq.template issue<false>(jt, pages, dst);
-    rq.template issue<true>(jt, pages, dst + S::kTileBytes);
+  auto request = [&](int jt, const Places& at, uint32_t stage) {
+    rq.template issue<false>(jt, at, lds + stage);
+    rq.template issue<true>(jt, at, lds + stage + S::kTileBytes);
   };
   auto start_window = [&] {
 #pragma unroll
     for (int w = 0; w < 4; ++w) bad |= any_bad[w] != 0;
 #pragma unroll
     for (int t = 0; t < NS - 1; ++t)
-      if (t * BK < rq.wn) request(t, rq.pages(t));
+      if (t * BK < rq.wn) request(t, rq.places(t), t * S::kStageBytes);
   };
-  stage();
+  stage_pages();
   if (tid < D) gsm[tid] = scale_at(a.p, tid);
   __syncthreads();
   start_window();
@@ -690,53 +734,70 @@ __device__ __forceinline__ void many_columns(const PagedArgs& a, const Item& it,
   const Column c = column_of<E, D>(a, it, rep, it.tile * kMany + wave * 32, lane, q, gsm);
   State<D / 32> st;
   st.clear();
-  auto block = [&](auto masked_c, uint32_t kt, int jb) {
+  bool odd = false;
+  // N blocks of 32 keys, jb .. from k0 on
+  auto blocks = [&](auto n_c, auto masked_c, uint32_t kt, int jb) {
+    constexpr int N = decltype(n_c)::value;
     constexpr bool MASKED = decltype(masked_c)::value != 0;
-    const uint32_t vt = kt + S::kTileBytes;
-    Keys<E, D> k;
-    k.read(kt, lane);
-    f32x16 s = k.scores(q, splat16(0.f));
-    if (MASKED) hide_unseen(s, c.lim - jb, hh);
+    f32x16 s[N];
+    {
+      Keys<E, D> k[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) k[n].read(kt + n * 32 * S::kRB, lane);
+#pragma unroll
+      for (int n = 0; n < N; ++n) s[n] = k[n].scores(q, st.less);
+    }
+    Values<E, D> v[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n].read(kt + S::kTileBytes + n * 32 * S::kRB, lane);
+    if (MASKED) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) hide_unseen(s[n], c.lim - jb - 32 * n, hh);
+    }
     st.exponentials(s);
-    Values<E, D> v;
-    v.read(vt, lane);
-    if (MASKED && __builtin_amdgcn_ballot_w64(v.finite()) != 0) add_odd_values<E, D>(vt, c.lim - jb, hh, st.o);
-    v.add(s, st.l, st.o);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      if (MASKED) odd |= v[n].clear();
+      v[n].add(s[n], st.l, st.o);
+    }
   };
   while (true) {
     wait_vmcnt<0>();  // the loads below are counted: nothing of the start may be in flight with them
     const int n_kt = (rq.wn + BK - 1) / BK, off = rq.w0 - it.k0;
-    int next_pages = n_kt ? rq.pages(min(NS - 1, n_kt - 1)) : 0;
+    Places next{0, 0};
+    if (n_kt) next = rq.places(min(NS - 1, n_kt - 1));
+    uint32_t stage = 0;  // of tile jt; the tile before it lay in the one before
     auto turn = [&](int jt) {
       if (n_kt - 1 - jt >= NS - 2) wait_vmcnt<(NS - 2) * 2 * LOADS>(); else wait_vmcnt<0>();
       __syncthreads();
       if (jt + NS - 1 < n_kt) {
-        request(jt + NS - 1, next_pages);
-        next_pages = rq.pages(min(jt + NS, n_kt - 1));
+        request(jt + NS - 1, next, stage == 0 ? (NS - 1) * S::kStageBytes : stage - S::kStageBytes);
+        next = rq.places(min(jt + NS, n_kt - 1));
       }
     };
+    auto advance = [&] { stage = stage == (NS - 1) * S::kStageBytes ? 0 : stage + S::kStageBytes; };
     // tiles every column of the wave sees whole, then the others: two loops, each with one form of the block
     int jt = 0;
     const int n_whole = max(min((c.all + 1 - off) / BK, n_kt), 0);
-    for (; jt < n_whole; ++jt) {
+    for (; jt < n_whole; ++jt, advance()) {
       turn(jt);
-#pragma unroll
-      for (int kb = 0; kb < BK / 32; ++kb) block(IC<0>{}, lds + (uint32_t)(jt % NS) * S::kStageBytes + kb * 32 * S::kRB, off + jt * BK + 32 * kb);
+      blocks(IC<BK / 32>{}, IC<0>{}, lds + stage, off + jt * BK);
     }
-    for (; jt < n_kt; ++jt) {
+    for (; jt < n_kt; ++jt, advance()) {
       turn(jt);
 #pragma unroll
       for (int kb = 0; kb < BK / 32; ++kb)
-        if (off + jt * BK + 32 * kb <= c.any) block(IC<1>{}, lds + (uint32_t)(jt % NS) * S::kStageBytes + kb * 32 * S::kRB, off + jt * BK + 32 * kb);
+        if (off + jt * BK + 32 * kb <= c.any) blocks(IC<1>{}, IC<1>{}, lds + stage + kb * 32 * S::kRB, off + jt * BK + 32 * kb);
     }
     rq.w0 += window;
     if (rq.w0 >= it.k0 + it.nk) break;
     rq.wn = min(it.k0 + it.nk - rq.w0, window);
     __syncthreads();  // everyone is done with the page numbers and the stages
-    stage();
+    stage_pages();
     __syncthreads();
     start_window();
   }
+  if (__builtin_amdgcn_ballot_w64(odd) != 0) add_odd_values<E, D, BK>(a, it, c, hh, st.o);
   store_result<E, D>(a, it, c, st, bad, wave * 32 + (lane & 31), hh);
 }
 

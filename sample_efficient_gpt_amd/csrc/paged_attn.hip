@@ -25,8 +25,34 @@
 namespace segpt {
 namespace {
 
+// Division by a number the host knows, for 0 <= n < 2^31: a product's upper half (the quotient's own sequence takes 25 dependent instructions,
+// and an item's place in the work takes seven of them)
+struct Divisor {
+  int32_t d;
+  uint32_t mul, shift;
+  __host__ void set(int32_t by) {
+    int bits = 1;
+    while ((int64_t{1} << bits) < by) ++bits;
+    d = by;
+    mul = (uint32_t)((uint64_t{1} << (31 + bits)) / (uint32_t)by + 1);
+    shift = (uint32_t)bits - 1;
+  }
+  __device__ __forceinline__ int of(int n) const { return d == 1 ? n : (int)(__umulhi((uint32_t)n, mul) >> shift); }
+};
+// the same by a number of the device's own, that all lanes have
+struct DeviceDivisor {
+  int32_t d;
+  double inverse;
+  __device__ __forceinline__ explicit DeviceDivisor(int by) : d(by) {
+    const double x = by, r = __builtin_amdgcn_rcp(x), r1 = fma(fma(-x, r, 1.0), r, r);
+    inverse = fma(fma(-x, r1, 1.0), r1, r1);
+  }
+  __device__ __forceinline__ int of(int n) const { return (int)((n + 0.5) * inverse); }  // exact: the half keeps the quotient off the whole numbers
+};
+
 struct PagedArgs {
   segpt_paged_params p;
+  Divisor rep, hkv;               // H / Hkv, Hkv
   int32_t entries, shared;        // shared: 1 if entry 0 is the prefix
   int32_t rows_each, log_page, capacity;
   int32_t target;                 // workgroups of four waves that fill the card once
@@ -49,28 +75,38 @@ struct Entry {
   bool many;
   bool broken;         // a length no sequence can have: every row of the entry is NaN
 };
-__device__ __forceinline__ Entry entry_at(const PagedArgs& a, int e, int rep) {
+// what an entry's numbers are made of: loads alone, so that several entries' are on their way together
+struct Raw {
+  int r0, r1, len;
+};
+__device__ __forceinline__ Raw raw_at(const PagedArgs& a, int e) {
   const segpt_paged_params& p = a.p;
-  Entry x{0, 0, 0, 0, 0, false, false};
-  if (e >= a.entries) return x;
-  if (a.shared && e == 0) {
-    int f, n;
-    sequence_rows(p, a.rows_each, 0, &x.first, &n);
-    sequence_rows(p, a.rows_each, p.B - 1, &f, &n);
-    x.n = max(f + n - x.first, 0);
-    x.len = p.prefix_len;
-  } else {
-    sequence_rows(p, a.rows_each, e - a.shared, &x.first, &x.n);
-    const int len = p.kv_len[e - a.shared];
-    x.broken = len < 0 || len > a.capacity;
-    x.len = min(max(len, 0), a.capacity);
+  const int b = min(max(e - a.shared, 0), p.B - 1);
+  if (p.seq_start) return {p.seq_start[b], p.seq_start[b + 1], p.kv_len[b]};
+  return {b * a.rows_each, (b + 1) * a.rows_each, p.kv_len[b]};
+}
+__device__ __forceinline__ Entry entry_of(const PagedArgs& a, int e, int rep, const Raw& raw) {
+  const segpt_paged_params& p = a.p;
+  int r0 = min(max(raw.r0, 0), p.T), r1 = min(max(raw.r1, 0), p.T), len = min(max(raw.len, 0), a.capacity);
+  bool broken = raw.len < 0 || raw.len > a.capacity;
+  if (a.shared && e == 0) {  // the prefix, with the rows of the whole batch
+    r0 = p.seq_start ? min(max(p.seq_start[0], 0), p.T) : 0;
+    r1 = p.seq_start ? min(max(p.seq_start[p.B], 0), p.T) : p.T;
+    len = p.prefix_len;
+    broken = false;
   }
+  Entry x;
+  x.first = r0;
+  x.n = e < a.entries ? max(r1 - r0, 0) : 0;
+  x.len = len;
   const int cols = x.n * rep;
   x.many = cols > kFew;
   x.tiles = x.many ? (cols + kMany - 1) / kMany : cols > 0;
   x.blocks = (x.len + kBlock - 1) / kBlock;
+  x.broken = broken;
   return x;
 }
+__device__ __forceinline__ Entry entry_at(const PagedArgs& a, int e, int rep) { return entry_of(a, e, rep, raw_at(a, e)); }
 // inclusive running sum over the lanes of a wave
 template <typename T>
 __device__ __forceinline__ T lane_prefix_sum(T v) {
@@ -91,20 +127,42 @@ __device__ __forceinline__ T lane_value(T v, int lane) {
 }
 struct Shares {
   int few, many;  // blocks of a share
+  double per_few, per_many;  // 1 / that
 };
-__device__ __forceinline__ int shares_of(const Entry& x, Shares s) {  // one also of no keys: it writes what such rows get
-  const int len = s.few + (x.many ? s.many - s.few : 0);  // (a choice between the two fields is taken for an indexed access, through memory)
-  return max((x.blocks + len - 1) / len, 1);
+// Shares of an entry, its blocks over the share's, rounded up; one also of no keys: it writes what such rows get.  A division by a number
+// that all lanes have: in fp64 it is exact (blocks < 2^26; the half keeps the quotient off the whole numbers) and a tenth of the instructions.
+__device__ __forceinline__ int shares_of(const Entry& x, Shares s) {
+  const int few = max((int)(((double)x.blocks + (s.few - 0.5)) * s.per_few), 1), many = max((int)(((double)x.blocks + (s.many - 0.5)) * s.per_many), 1);
+  return x.many ? many : few;
+}
+// The first entries, a lane each, kept in registers (all of them loaded at once: one after the other, 129 entries cost a launch of 47 us
+// 8); more than kKept * 64 are read again where they are needed.
+constexpr int kKept = 4;
+struct Entries {
+  Entry e[kKept];
+};
+__device__ __forceinline__ Entries load_entries(const PagedArgs& a, int lane, int rep) {
+  Raw raw[kKept] = {};
+#pragma unroll
+  for (int u = 0; u < kKept; ++u)
+    if (64 * u < a.entries) raw[u] = raw_at(a, 64 * u + lane);
+  Entries x = {};
+#pragma unroll
+  for (int u = 0; u < kKept; ++u)
+    if (64 * u < a.entries) x.e[u] = entry_of(a, 64 * u + lane, rep, raw[u]);
+  return x;
 }
 // Blocks of a share, such that the workgroups are resident at once if the tiles alone are not too many for that: the mean first, then longer
 // ones until the begun ones fit too (one workgroup too many is a round of its own).  A block of many columns keeps a workgroup as long as the
 // memory does that of few columns, in a quarter of the workgroup each: a wave's share is a quarter as long.  The sums are
 // floats: they may round, but to the same value in every wave of both kernels.
-__device__ __forceinline__ Shares share_blocks(const PagedArgs& a, int lane, int rep, Entry* mine) {
-  *mine = entry_at(a, lane, rep);
+__device__ __forceinline__ Shares share_blocks(const PagedArgs& a, int lane, int rep, const Entries& kept) {
   auto sum = [&](auto of) {
-    float v = of(*mine);
-    for (int e = 64; e < a.entries; e += 64) v += of(entry_at(a, e + lane, rep));
+    float v = 0.f;
+#pragma unroll
+    for (int u = 0; u < kKept; ++u)
+      if (64 * u < a.entries) v += of(kept.e[u]);
+    for (int e = 64 * kKept; e < a.entries; e += 64) v += of(entry_at(a, e + lane, rep));
     return lane_value(lane_prefix_sum(v), 63) * (float)a.p.Hkv;
   };
   const float target = (float)a.target;
@@ -113,6 +171,8 @@ __device__ __forceinline__ Shares share_blocks(const PagedArgs& a, int lane, int
   for (int i = 0;; ++i) {
     s.many = max((int)fminf(ceilf(len), 1e9f), a.min_many);
     s.few = max((int)fminf(ceilf(0.25f * len), 1e9f), a.min_few);
+    s.per_many = DeviceDivisor(s.many).inverse;
+    s.per_few = DeviceDivisor(s.few).inverse;
     if (i == 3) break;
     const float groups = sum([&](const Entry& x) { return (float)x.tiles * (float)shares_of(x, s) * (x.many ? 1.f : 0.25f); });
     if (groups <= target || groups > 2.f * target) break;
@@ -131,10 +191,10 @@ struct Found {
 // The entry of an item of its kind, or of a tile and kv head whose partial results are to be joined, by number; or the first entry
 enum Find { kFindFew, kFindMany, kFindJoin, kFindFirst };
 template <Find F>
-__device__ __forceinline__ Found find_entry(const PagedArgs& a, int lane, int rep, const Shares& share, const Entry& mine, int which) {
+__device__ __forceinline__ Found find_entry(const PagedArgs& a, int lane, int rep, const Shares& share, const Entries& kept, int which) {
   int base = 0, slot = 0;
-  for (int e0 = 0; e0 < a.entries; e0 += 64) {
-    const Entry x = e0 == 0 ? mine : entry_at(a, e0 + lane, rep);
+  Found found{-1, 0, 0, 0, 0, 0, 0, 0, false, false};
+  auto look = [&](int e0, const Entry& x) {  // true: it is among these 64
     const int shares = shares_of(x, share), items = x.tiles * shares * a.p.Hkv;
     const bool partial = a.shared || shares > 1;
     const int slots = partial ? items * (x.many ? kMany / 32 : 1) : 0, slots_upto = slot + lane_prefix_sum(slots);
@@ -143,13 +203,20 @@ __device__ __forceinline__ Found find_entry(const PagedArgs& a, int lane, int re
     const uint64_t hits = F == kFindFirst ? 1 : __builtin_amdgcn_ballot_w64(which >= upto - mine_n && which < upto);
     if (hits) {
       const int l = __builtin_ctzll(hits);
-      return Found{e0 + l, lane_value(x.first, l), lane_value(x.n, l), lane_value(x.len, l), lane_value(x.blocks, l), lane_value(shares, l),
-                   lane_value(upto - mine_n, l), lane_value(slots_upto - slots, l), lane_value((int)x.many, l) != 0, lane_value((int)x.broken, l) != 0};
+      found = Found{e0 + l, lane_value(x.first, l), lane_value(x.n, l), lane_value(x.len, l), lane_value(x.blocks, l), lane_value(shares, l),
+                    lane_value(upto - mine_n, l), lane_value(slots_upto - slots, l), lane_value((int)x.many, l) != 0, lane_value((int)x.broken, l) != 0};
+      return true;
     }
     base = lane_value(upto, 63);
     slot = lane_value(slots_upto, 63);
-  }
-  return Found{-1, 0, 0, 0, 0, 0, 0, 0, false, false};
+    return false;
+  };
+#pragma unroll
+  for (int u = 0; u < kKept; ++u)
+    if (64 * u < a.entries && look(64 * u, kept.e[u])) return found;
+  for (int e0 = 64 * kKept; e0 < a.entries; e0 += 64)
+    if (look(e0, entry_at(a, e0 + lane, rep))) return found;
+  return found;
 }
 
 // ---- tiles: BK rows of D elements, filled by direct global->LDS loads of 1 KB; the 16-byte chunk c of row r lies at chunk c ^ f(r)
@@ -264,7 +331,7 @@ struct Item {
   const int* ids;    // page numbers
 };
 template <bool MANY>
-__device__ __forceinline__ Item locate(const PagedArgs& a, int lane, int rep, const Shares& share, const Entry& mine, int number) {
+__device__ __forceinline__ Item locate(const PagedArgs& a, int lane, int rep, const Shares& share, const Entries& mine, int number) {
   constexpr int COLS = MANY ? kMany : kFew;
   Item it;
   it.x = find_entry<MANY ? kFindMany : kFindFew>(a, lane, rep, share, mine, number);
@@ -273,16 +340,18 @@ __device__ __forceinline__ Item locate(const PagedArgs& a, int lane, int rep, co
   if (!it.valid) return it;
   it.cols = x.n * rep;
   const int n_tiles = (it.cols + COLS - 1) / COLS, local = number - x.base;
-  it.g = local % a.p.Hkv;
-  it.part = local / a.p.Hkv % x.shares;
-  it.tile = n_tiles - 1 - local / a.p.Hkv / x.shares;  // the last tiles see the most keys: they start first
+  const DeviceDivisor shares(x.shares);
+  const int per_head = a.hkv.of(local), from_last = shares.of(per_head);
+  it.g = local - per_head * a.p.Hkv;
+  it.part = per_head - from_last * x.shares;
+  it.tile = n_tiles - 1 - from_last;  // the last tiles see the most keys: they start first
   it.prefix = a.shared && x.entry == 0;
   it.direct = !a.shared && x.shares == 1;
   it.slot = x.slot + ((it.tile * x.shares + it.part) * a.p.Hkv + it.g) * (COLS / 32);
   it.valid = it.tile >= 0 && (it.direct || it.slot + COLS / 32 <= a.n_slots);
   it.past = x.len - x.n;
-  const int per = (x.blocks + x.shares - 1) / x.shares * kBlock;  // shares as even as whole blocks allow
-  const int last_col = min(it.cols, (it.tile + 1) * COLS) - 1, sees = it.prefix ? x.len : min(x.len, it.past + last_col / rep + 1);
+  const int per = shares.of(x.blocks + x.shares - 1) * kBlock;  // shares as even as whole blocks allow
+  const int last_col = min(it.cols, (it.tile + 1) * COLS) - 1, sees = it.prefix ? x.len : min(x.len, it.past + a.rep.of(last_col) + 1);
   it.k0 = it.part * per;
   it.nk = max(min(sees, it.k0 + per) - it.k0, 0);
   it.ids = it.prefix ? a.p.prefix_table : a.p.block_table + (int64_t)(x.entry - a.shared) * a.p.table_stride;
@@ -374,7 +443,7 @@ __device__ __forceinline__ Column column_of(const PagedArgs& a, const Item& it, 
   const segpt_paged_params& p = a.p;
   Column c;
   const bool works = wave_col < it.cols;
-  const int col = wave_col + (lane & 31), safe = min(col, it.cols - 1), i = safe / rep;
+  const int col = wave_col + (lane & 31), safe = min(col, it.cols - 1), i = a.rep.of(safe);
   c.live = col < it.cols;
   c.t = it.x.first + i;
   c.h = it.g * rep + safe - i * rep;
@@ -400,8 +469,8 @@ __device__ __forceinline__ Column column_of(const PagedArgs& a, const Item& it, 
     c.all = !works || cut ? -1 : it.nk - 1;
     c.any = works ? it.nk - 1 : -1;
   } else {
-    c.all = works ? min(it.past + wave_col / rep - it.k0, it.nk - 1) : -1;
-    c.any = works ? min(it.past + min(wave_col + 31, it.cols - 1) / rep - it.k0, it.nk - 1) : -1;
+    c.all = works ? min(it.past + a.rep.of(wave_col) - it.k0, it.nk - 1) : -1;
+    c.any = works ? min(it.past + a.rep.of(min(wave_col + 31, it.cols - 1)) - it.k0, it.nk - 1) : -1;
   }
   return c;
 }
@@ -823,10 +892,10 @@ __global__ __launch_bounds__(64, (Shape<E, D>::kOcc)) void paged_few_kernel(Page
   __shared__ __attribute__((aligned(1024))) char lds[S::kFewBytes];
   __shared__ __attribute__((aligned(16))) float gsm[D];
   __shared__ int table[S::kFewTable + 2];
-  const int lane = threadIdx.x, rep = a.p.H / a.p.Hkv;
+  const int lane = threadIdx.x, rep = a.rep.d;
   if (a.p.flags & SEGPT_FLAG_ZERO_REST) clear_rest(a, lane, 64, sizeof(E), D);
-  Entry mine;
-  const Shares share = share_blocks(a, lane, rep, &mine);
+  const Entries mine = load_entries(a, lane, rep);
+  const Shares share = share_blocks(a, lane, rep, mine);
   const Item it = locate<false>(a, lane, rep, share, mine, blockIdx.x);
   if (it.valid) few_columns<E, D>(a, it, rep, lane, lds_addr_of(lds), table, gsm);
 }
@@ -841,11 +910,11 @@ __global__ __launch_bounds__(256, (Shape<E, D>::kOcc)) void paged_any_kernel(Pag
   __shared__ int table[S::kManyTable + 8];
   __shared__ int any_bad[4];
   static_assert(4 * (S::kFewTable + 2) <= S::kManyTable + 8, "four waves' page numbers");
-  const int tid = threadIdx.x, lane = tid & 63, rep = a.p.H / a.p.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63, rep = a.rep.d;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (a.p.flags & SEGPT_FLAG_ZERO_REST) clear_rest(a, tid, 256, sizeof(E), D);
-  Entry mine;
-  const Shares share = share_blocks(a, lane, rep, &mine);
+  const Entries mine = load_entries(a, lane, rep);
+  const Shares share = share_blocks(a, lane, rep, mine);
   if ((int)blockIdx.x < a.n_many) {
     const Item it = locate<true>(a, lane, rep, share, mine, blockIdx.x);
     if (it.valid) many_columns<E, D>(a, it, rep, tid, lds_addr_of(lds), table, gsm[0], any_bad);
@@ -855,33 +924,36 @@ __global__ __launch_bounds__(256, (Shape<E, D>::kOcc)) void paged_any_kernel(Pag
   }
 }
 
-// Joins the partial results of a tile's columns: its sequence's shares and, behind them, the prefix's.  A unit of D / 4 lanes holds a row; a
-// workgroup takes `step` columns at a time, with its other units side by side over the shares (kBatch of them requested together).  The
-// units' sums meet in LDS.  Fixed order: deterministic.
+// Joins the partial results of `per_sub` columns of a tile: its sequence's shares and, behind them, the prefix's.  A unit of D / 4 lanes holds a
+// row; as many units stand side by side over the shares of a column as leave each one batch of kBatch that is requested together, and
+// their sums meet in LDS.  Fixed order: deterministic.
 constexpr int kMergeThreads = 256;
 template <typename E, int D>
-__global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedArgs a, int subs, int per_sub, int step) {
+__global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedArgs a, int subs, int per_sub) {
   const segpt_paged_params& p = a.p;
   constexpr int LPR = D / 4, kUnits = kMergeThreads / LPR, kBatch = 4;
   __shared__ float4 sums[kMergeThreads];
   __shared__ float2 stats[kUnits];
   const int tid = threadIdx.x, lane = tid & 63, unit = tid / LPR, c = tid % LPR;
-  const int rep = p.H / p.Hkv;
-  Entry mine;
-  const Shares share = share_blocks(a, lane, rep, &mine);
+  const int rep = a.rep.d;
+  const Entries mine = load_entries(a, lane, rep);
+  const Shares share = share_blocks(a, lane, rep, mine);
   const int which = blockIdx.x / subs, sub = blockIdx.x - which * subs;
   const Found own = find_entry<kFindJoin>(a, lane, rep, share, mine, which);
   if (own.entry < 0) return;
-  const int g = (which - own.base) % p.Hkv, tile = (which - own.base) / p.Hkv, cols = own.n * rep, tile_cols = own.many ? kMany : kFew;
+  const int tile = a.hkv.of(which - own.base), g = which - own.base - tile * p.Hkv, cols = own.n * rep, tile_cols = own.many ? kMany : kFew;
   Found pre{-1, 0, 0, 0, 0, 0, 0, 0, false, false};
   if (a.shared) pre = find_entry<kFindFirst>(a, lane, rep, share, mine, 0);
   const int pre_cols = pre.many ? kMany : kFew;
-  const int n = own.shares + pre.shares, wide = kUnits / step;  // units of a column
+  const int n = own.shares + pre.shares;
+  int step = min(per_sub, kUnits);  // columns at a time
+  while (step > 1 && kUnits / step * kBatch < n) step >>= 1;
+  const int wide = kUnits / step;  // units of a column
   for (int c0 = sub * per_sub; c0 < min((sub + 1) * per_sub, tile_cols); c0 += step) {  // the same for all threads
     if (tile * tile_cols + c0 >= cols) return;
     const int col = tile * tile_cols + min(c0 + unit % step, tile_cols - 1);
     const bool live = col < cols && c0 + unit % step < min((sub + 1) * per_sub, tile_cols);
-    const int i = min(col, cols - 1) / rep, t = own.first + i, h = g * rep + (min(col, cols - 1) - i * rep);
+    const int i = a.rep.of(min(col, cols - 1)), t = own.first + i, h = g * rep + (min(col, cols - 1) - i * rep);
     const int pcol = (t - pre.first) * rep + h - g * rep, ptile = pcol / pre_cols;
     auto place = [&](int s) {  // row of share s among all partial results; none: there is no room for it
       const bool is_own = s < own.shares;
@@ -957,6 +1029,8 @@ bool all_few(const segpt_paged_params& p) {  // known on the host
 // fills the plan; returns the scratch bytes of the partials
 size_t plan(const segpt_paged_params& p, PagedArgs& a) {
   const int row_bytes = p.D * (p.dtype == SEGPT_DTYPE_FP32 ? 4 : 2), rep = p.H / p.Hkv;
+  a.rep.set(rep);
+  a.hkv.set(p.Hkv);
   a.shared = p.prefix_table ? 1 : 0;
   a.entries = p.B + a.shared;
   a.rows_each = p.seq_start ? 0 : p.T / p.B;
@@ -973,7 +1047,7 @@ size_t plan(const segpt_paged_params& p, PagedArgs& a) {
     many = each > kFew ? (each + kMany - 1) / kMany * p.B : 0;
     few = each > kFew ? 0 : p.B;
   }
-  const int64_t own = many + few;
+  const int64_t own = many + few, own_many = many;
   if (a.shared && cols > kFew) many += (cols + kMany - 1) / kMany;
   else if (a.shared) few += 1;
   const int64_t slack = 64;  // the sum that gives the length of a share is rounded
@@ -981,10 +1055,11 @@ size_t plan(const segpt_paged_params& p, PagedArgs& a) {
   a.n_many = (int32_t)std::min<int64_t>(n_many, INT32_MAX);
   a.n_few = (int32_t)std::min<int64_t>(n_few, INT32_MAX);
   // a tile that leaves partial results has two shares or more, i.e. at most twice its part of the target; beside a prefix all leave them
-  const int64_t most = 2 * ((int64_t)a.target + slack);
-  const int64_t slots = kMany / 32 * (a.shared ? n_many : std::min(n_many, most)) + (a.shared ? n_few : std::min(n_few, 4 * most));
+  const int64_t most = (int64_t)a.target + slack;
+  const int64_t slots = kMany / 32 * (a.shared ? n_many : std::min(n_many, 2 * most)) + (a.shared ? n_few : std::min(n_few, 8 * most));
   a.n_slots = (int32_t)std::min<int64_t>(slots, INT32_MAX / 32);
-  a.n_joins = (int32_t)std::min<int64_t>(own * p.Hkv, a.shared ? INT32_MAX : 5 * most);
+  const int64_t joins = a.shared ? own * p.Hkv : std::min(own_many * p.Hkv, most) + std::min((own - own_many) * p.Hkv, 4 * most);
+  a.n_joins = (int32_t)std::min<int64_t>(joins, INT32_MAX);
   return n_many + n_few > INT32_MAX / 2 || slots > INT32_MAX / 32 ? SIZE_MAX : (size_t)a.n_slots * 32 * (p.D + 2) * sizeof(float);
 }
 
@@ -995,21 +1070,14 @@ int launch(const PagedArgs& a, hipStream_t st) {
   else hipLaunchKernelGGL((paged_any_kernel<E, D>), dim3((unsigned)(a.n_many + (a.n_few + 3) / 4)), dim3(256), 0, st, a);
   const int rc = (int)hipGetLastError();
   if (rc) return rc;
-  // columns at a time and workgroups a tile: as many units over the shares as leave each a batch
-  constexpr int kUnits = kMergeThreads / (D / 4);
+  // a column a workgroup, or so many that there are not more workgroups than the card holds a few times over
   const int64_t all = (int64_t)p.T * (p.H / p.Hkv);
-  const int most = a.n_many - (a.shared && all > kFew) > 0 ? kMany : kFew, cols = p.seq_start ? most : (int)std::min<int64_t>(most, all / p.B);
-  int64_t shares = 4 * a.target / std::max<int64_t>(1, a.n_joins) + 1;
-  if (a.shared) {  // the prefix's own: its length is known, the sequences' are not
-    const int64_t blocks = (p.prefix_len + kBlock - 1) / kBlock, tiles = (all + kMany - 1) / kMany * p.Hkv;
-    shares = std::max(shares, blocks / std::max<int64_t>(a.min_many, tiles * blocks / a.target));
-  }
-  int step = kUnits;
-  while (step > 1 && kUnits / step * 4 < shares) step /= 2;
-  int per_sub = step;
-  while ((int64_t)a.n_joins * ((cols + per_sub - 1) / per_sub) > 8192 && per_sub < kMany) per_sub *= 2;
+  const bool any_many = p.seq_start ? all > kFew : all / p.B > kFew;
+  const int most = any_many ? kMany : kFew, cols = p.seq_start ? most : (int)std::min<int64_t>(most, all / p.B);
+  int per_sub = 1;
+  while (per_sub < kMany && (int64_t)a.n_joins * ((cols + per_sub - 1) / per_sub) > 4096) per_sub *= 2;
   const int subs = (cols + per_sub - 1) / per_sub;
-  hipLaunchKernelGGL((paged_merge_kernel<E, D>), dim3((unsigned)(a.n_joins * subs)), dim3(kMergeThreads), 0, st, a, subs, per_sub, step);
+  hipLaunchKernelGGL((paged_merge_kernel<E, D>), dim3((unsigned)(a.n_joins * subs)), dim3(kMergeThreads), 0, st, a, subs, per_sub);
   return (int)hipGetLastError();
 }
 

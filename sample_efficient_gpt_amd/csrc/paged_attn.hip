@@ -236,13 +236,14 @@ struct Shape {
   // MANY: keys per staged tile (16 KB with its values, at fp32 head_dim 128 32) and stages of the ring
   static constexpr int kBK = kRB <= 128 ? 64 : 32;
   static constexpr int kTileBytes = kBK * kRB, kStageBytes = 2 * kTileBytes;
-  static constexpr int kStages = kRB <= 256 ? 3 : 2;
+  static constexpr int kStages = kRB <= 256 ? 4 : 3;
   static constexpr int kManyTable = 256;  // page numbers held in LDS: a longer share takes its keys in windows
   static constexpr int kManyBytes = kStages * kStageBytes;
   // FEW: one block of keys and one of values a wave
   static constexpr int kFewTable = 64;
-  static constexpr int kFewBytes = 2 * kBlock * kRB;
-  static constexpr int kOcc = kRB > 256 ? 1 : kRB > 128 || sizeof(E) == 4 ? 2 : 3;  // workgroups of four waves per CU
+  static constexpr int kDepth = kRB <= 128 ? 2 : 1;
+  static constexpr int kFewBytes = kDepth * 2 * kBlock * kRB;
+  static constexpr int kOcc = kRB > 256 ? 1 : 2;  // workgroups of four waves per CU
 };
 
 // query columns in the B operand's layout, scaled by everything that does not depend on the key (gsm: g_q g_k sm_scale log2 e); D / 2 values
@@ -375,10 +376,8 @@ __device__ __forceinline__ float scale_at(const segpt_paged_params& p, int d) {
 
 // Requests of tiles of keys w0 .. w0 + wn - 1.  A load covers kRowsPerLoad rows, at most 8, of one page: its address is a scalar base and
 // a lane offset.  LOADS loads a tensor and tile; number ps is load first + ps * step of the tile.  Where the rows of a load begin is worked out
-// side by side, by lane ps for load ps, one tile ahead; what a lane adds is the same for every whole tile.
-struct Places {
-  int64_t k, v;  // byte offsets from the head's first row, lane ps: of load ps
-};
+// side by side, a lane a load, for as many tiles as there are lanes (27 of 72 vector instructions a block of MANY, one tile at a time);
+// what a lane adds is the same for every whole tile.
 template <typename E, int D, int BK, int LOADS>
 struct Requests {
   using Z = Tile<E, D>;
@@ -388,32 +387,38 @@ struct Requests {
   int w0, wn, log_page, first, step, lane;
   const int* table;
   uint32_t klane[LOADS], vlane[LOADS];
+  static constexpr int kAhead = 64 / LOADS;  // tiles worked out at a time
+  int64_t kplace, vplace;                    // byte offsets from the head's first row, lane t * LOADS + ps: of load ps of the t-th of these tiles
   __device__ __forceinline__ int first_row(int jt, int ps) const {  // from w0 on; past the last key: the last rows once more
     return min(jt * BK + (ps * step + first) * Z::kRowsPerLoad, (wn - 1) & ~(Z::kRowsPerLoad - 1));
   }
   __device__ __forceinline__ uint32_t chunk(int ps) const {
     return (uint32_t)((lane % Z::kChunks) ^ Z::f((ps * step + first) * Z::kRowsPerLoad + lane / Z::kChunks)) << 4;
   }
-  __device__ __forceinline__ Places places(int jt) const {
-    const int key = w0 + first_row(jt, min(lane, LOADS - 1)), page = table[(key >> log_page) - (w0 >> log_page)];
+  __device__ __forceinline__ void work_out(int jt) {  // tiles jt .. jt + kAhead - 1
+    const int key = w0 + first_row(jt + lane / LOADS, lane % LOADS), page = table[(key >> log_page) - (w0 >> log_page)];
     const uint32_t slot = (uint32_t)(key & ((1 << log_page) - 1));
-    return {page * kpage + (int64_t)((uint64_t)slot * kstep), page * vpage + (int64_t)((uint64_t)slot * vstep)};
+    kplace = page * kpage + (int64_t)((uint64_t)slot * kstep);
+    vplace = page * vpage + (int64_t)((uint64_t)slot * vstep);
   }
-  static __device__ __forceinline__ const char* at(const char* base, int64_t off, int ps) {
-    const uint32_t lo = __builtin_amdgcn_readlane((int)off, ps), hi = __builtin_amdgcn_readlane((int)(off >> 32), ps);
+  static __device__ __forceinline__ const char* at(const char* base, int64_t off, int l) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)off, l), hi = __builtin_amdgcn_readlane((int)(off >> 32), l);
     return base + (int64_t)((uint64_t)hi << 32 | lo);
   }
+  // the keys or values of tile jt; the first tile of every kAhead is asked for its keys first
   template <bool VALUES>
-  __device__ __forceinline__ void issue(int jt, const Places& places, uint32_t dst) const {
+  __device__ __forceinline__ void issue(int jt, uint32_t dst) {
+    const int l = jt % kAhead * LOADS;
+    if (!VALUES && l == 0) work_out(jt);
     if (wn - jt * BK >= BK) {
 #pragma unroll
       for (int ps = 0; ps < LOADS; ++ps)
-        gload_lds16_so(VALUES ? at(vbase, places.v, ps) : at(kbase, places.k, ps), VALUES ? vlane[ps] : klane[ps], dst + (ps * step + first) * 1024);
+        gload_lds16_so(VALUES ? at(vbase, vplace, l + ps) : at(kbase, kplace, l + ps), VALUES ? vlane[ps] : klane[ps], dst + (ps * step + first) * 1024);
     } else {
 #pragma unroll
       for (int ps = 0; ps < LOADS; ++ps) {
         const uint32_t r = min(lane / Z::kChunks, wn - 1 - first_row(jt, ps));
-        gload_lds16_so(VALUES ? at(vbase, places.v, ps) : at(kbase, places.k, ps), r * (VALUES ? vstep : kstep) + chunk(ps), dst + (ps * step + first) * 1024);
+        gload_lds16_so(VALUES ? at(vbase, vplace, l + ps) : at(kbase, kplace, l + ps), r * (VALUES ? vstep : kstep) + chunk(ps), dst + (ps * step + first) * 1024);
       }
     }
   }
@@ -598,9 +603,9 @@ struct State {
     l[0] = l[1] = 0.f;
   }
   __device__ __forceinline__ float reference() const { return limit == -INFINITY ? -INFINITY : m; }
-  // scores of N blocks to probabilities
+  // raises the reference where scores of N blocks exceed it
   template <int N>
-  __device__ __forceinline__ void exponentials(f32x16 (&s)[N]) {
+  __device__ __forceinline__ void raise(f32x16 (&s)[N]) {
     float mx[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -627,6 +632,9 @@ struct State {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[n][r] -= up;
     }
+  }
+  template <int N>
+  static __device__ __forceinline__ void exponentials(f32x16 (&s)[N]) {
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
@@ -644,7 +652,7 @@ __device__ __forceinline__ void hide_unseen(f32x16& s, int seen, int hh) {  // r
 // with one is that value, or NaN where signs meet.
 template <typename E, int D, int BK>
 __device__ __forceinline__ void add_odd_values(const PagedArgs& a, const Item& it, const Column& c, int hh, f32x16 (&o)[D / 32]) {
-  for (int j = (max(c.all, -1) + 1) & ~(BK - 1); j <= c.any; ++j) {  // tiles that not all rows see whole
+  for (int j = (max(c.all, -1) + 1) / BK * BK; j <= c.any; ++j) {  // tiles that not all rows see whole
     const int key = it.k0 + j, page = it.ids[key >> a.log_page];
     if ((uint32_t)page >= (uint32_t)a.p.n_pages) continue;  // the rows are NaN as a whole
     const E* row = reinterpret_cast<const E*>(page_row<E>(a.p.v_pages, page, it.g, key & ((1 << a.log_page) - 1)));
@@ -701,76 +709,85 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0) only
 }
 
-// ---- FEW: one wave, up to 32 columns.  One buffer for the keys of a block and one for its values, each requested again as soon as its
-// reader has it in registers: the next keys are in flight during the softmax and the product with the values, the next values
-// during the next scores.
+// ---- FEW: one wave, up to 32 columns.  kDepth buffers for the keys of a block and as many for its values, each requested again as soon
+// as its reader has it in registers.  Order of the requests: keys, values of blocks 0 .. kDepth - 1, then keys, values of each further block.
 template <typename E, int D>
 __device__ __forceinline__ void few_columns(const PagedArgs& a, const Item& it, int rep, int lane, uint32_t lds, int* table, float* gsm) {
   using S = Shape<E, D>;
   constexpr int LOADS = kBlock * S::kRB / 1024;
   const int hh = lane >> 5, window = S::kFewTable << a.log_page;
-  const uint32_t kt = lds, vt = lds + kBlock * S::kRB;
+  constexpr int DEPTH = S::kDepth;
+  constexpr uint32_t kBuffer = kBlock * S::kRB;
   auto rq = requests<E, D, kBlock, LOADS>(a, it, table, 0, 1, lane);
-  rq.w0 = it.k0;
   rq.wn = min(it.nk, window);
   bool bad = it.x.broken | stage_table(a, it, rq.w0, rq.wn, table, lane, 64);
   for (int d = lane; d < D; d += 64) gsm[d] = scale_at(a.p, d);
   wave_sync();
-  Places at{0, 0};
-  if (rq.wn) {
-    at = rq.places(0);
-    rq.template issue<false>(0, at, kt);
-    rq.template issue<true>(0, at, vt);
-  }
+  auto start_window = [&] {
+#pragma unroll
+    for (int t = 0; t < DEPTH; ++t)
+      if (t * kBlock < rq.wn) {
+        rq.template issue<false>(t, lds + 2 * t * kBuffer);
+        rq.template issue<true>(t, lds + (2 * t + 1) * kBuffer);
+      }
+  };
+  // leaves the loads of the n youngest tiles (keys or values) in flight
+  auto wait_but = [&](int n) {
+    if (n == 0) wait_vmcnt<0>();
+    else if (n == 1) wait_vmcnt<LOADS>();
+    else if (n == 2) wait_vmcnt<2 * LOADS>();
+    else wait_vmcnt<3 * LOADS>();
+  };
+  start_window();
   Query<E, D> q;
   const Column c = column_of<E, D>(a, it, rep, it.tile * kFew, lane, q, gsm);
   State<D / 32> st;
   st.clear();
   bool odd = false;
   while (true) {
-    const int n_kt = (rq.wn + kBlock - 1) / kBlock;
+    const int n_kt = (rq.wn + kBlock - 1) / kBlock, off = rq.w0 - it.k0;
     wait_vmcnt<0>();  // the loads below are counted: nothing of the start may be in flight with them
-    if (n_kt > 1) at = rq.places(1);
+    uint32_t buffer = 0;
     for (int jt = 0; jt < n_kt; ++jt) {
-      const bool more = jt + 1 < n_kt;
-      const int seen = c.lim - (rq.w0 - it.k0) - jt * kBlock;
-      const bool masked = rq.w0 - it.k0 + jt * kBlock + kBlock - 1 > c.all;
-      wait_vmcnt<LOADS>();  // the keys are there, the values younger
+      const int left = n_kt - 1 - jt;
+      const uint32_t kt = lds + 2 * buffer * kBuffer, vt = kt + kBuffer;
+      const int seen = c.lim - off - jt * kBlock;
+      const bool masked = off + jt * kBlock + kBlock - 1 > c.all;
+      wait_but(1 + 2 * min(left, DEPTH - 1));  // the keys are there; its values and the other buffers' tiles are younger
       wave_sync();
       Keys<E, D> k;
       k.read(kt, lane);
       wave_sync();
-      if (more) rq.template issue<false>(jt + 1, at, kt);
+      if (left >= DEPTH) rq.template issue<false>(jt + DEPTH, kt);
       f32x16 s[1] = {k.scores(q, st.less)};
       if (masked) hide_unseen(s[0], seen, hh);
+      st.raise(s);
       st.exponentials(s);
-      if (more) wait_vmcnt<LOADS>(); else wait_vmcnt<0>();  // the values; the next keys are younger
+      wait_but(2 * min(left, DEPTH - 1) + (left >= DEPTH));  // the values; the other buffers' tiles and the keys just requested are younger
       wave_sync();
       Values<E, D> v;
       v.read(vt, lane);
       if (masked) odd |= v.clear();
       wave_sync();
-      if (more) {
-        rq.template issue<true>(jt + 1, at, vt);
-        at = rq.places(min(jt + 2, n_kt - 1));
-      }
+      if (left >= DEPTH) rq.template issue<true>(jt + DEPTH, vt);
       v.add(s[0], st.l, st.o);
+      buffer = buffer == DEPTH - 1 ? 0 : buffer + 1;
     }
     rq.w0 += window;
     if (rq.w0 >= it.k0 + it.nk) break;
     rq.wn = min(it.k0 + it.nk - rq.w0, window);
     bad |= stage_table(a, it, rq.w0, rq.wn, table, lane, 64);
     wave_sync();
-    at = rq.places(0);
-    rq.template issue<false>(0, at, kt);
-    rq.template issue<true>(0, at, vt);
+    start_window();
   }
   if (__builtin_amdgcn_ballot_w64(odd) != 0) add_odd_values<E, D, kBlock>(a, it, c, hh, st.o);
   store_result<E, D>(a, it, c, st, bad, lane & 31, hh);
 }
 
-// ---- MANY: four waves of 32 columns around a ring of stages (K' tile, V' tile); tile jt lives in stage jt % kStages.  Per tile: wait for its
-// loads, barrier (also: everyone has left the tile before), request tile jt + kStages - 1 over the one before, compute.
+// ---- MANY: four waves of 32 columns around a ring of stages (K' tile, V' tile); tile jt lives in stage jt % kStages.  A turn computes the
+// scores of tile jt + 1 beside the exponentials of tile jt and its product with the values, so that the matrix pipe has work while
+// the exponentials are formed.  Per turn: wait for tile jt + 1, barrier (also: everyone has left tile jt - 1), request tile jt + kStages - 1 over
+// that one, compute.
 template <typename E, int D>
 __device__ __forceinline__ void many_columns(const PagedArgs& a, const Item& it, int rep, int tid, uint32_t lds, int* table, float* gsm, int* any_bad) {
   using S = Shape<E, D>;
@@ -784,16 +801,16 @@ __device__ __forceinline__ void many_columns(const PagedArgs& a, const Item& it,
     const bool mine = stage_table(a, it, rq.w0, rq.wn, table, tid, 256);
     if (lane == 0) any_bad[wave] = mine;
   };
-  auto request = [&](int jt, const Places& at, uint32_t stage) {
-    rq.template issue<false>(jt, at, lds + stage);
-    rq.template issue<true>(jt, at, lds + stage + S::kTileBytes);
+  auto request = [&](int jt, uint32_t stage) {
+    rq.template issue<false>(jt, lds + stage);
+    rq.template issue<true>(jt, lds + stage + S::kTileBytes);
   };
   auto start_window = [&] {
 #pragma unroll
     for (int w = 0; w < 4; ++w) bad |= any_bad[w] != 0;
 #pragma unroll
     for (int t = 0; t < NS - 1; ++t)
-      if (t * BK < rq.wn) request(t, rq.places(t), t * S::kStageBytes);
+      if (t * BK < rq.wn) request(t, t * S::kStageBytes);
   };
   stage_pages();
   if (tid < D) gsm[tid] = scale_at(a.p, tid);
@@ -804,59 +821,90 @@ __device__ __forceinline__ void many_columns(const PagedArgs& a, const Item& it,
   State<D / 32> st;
   st.clear();
   bool odd = false;
-  // N blocks of 32 keys, jb .. from k0 on
-  auto blocks = [&](auto n_c, auto masked_c, uint32_t kt, int jb) {
-    constexpr int N = decltype(n_c)::value;
-    constexpr bool MASKED = decltype(masked_c)::value != 0;
-    f32x16 s[N];
-    {
-      Keys<E, D> k[N];
+  constexpr int N = BK / 32;  // blocks of a tile
+  typedef f32x16 Scores[N];
+  auto read_keys = [&](Keys<E, D> (&k)[N], uint32_t stage) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) k[n].read(kt + n * 32 * S::kRB, lane);
+    for (int n = 0; n < N; ++n) k[n].read(lds + stage + n * 32 * S::kRB, lane);
+  };
+  auto read_values = [&](Values<E, D> (&v)[N], uint32_t stage) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) s[n] = k[n].scores(q, st.less);
-    }
-    Values<E, D> v[N];
+    for (int n = 0; n < N; ++n) v[n].read(lds + stage + S::kTileBytes + n * 32 * S::kRB, lane);
+  };
+  auto scores = [&](auto masked_c, const Keys<E, D> (&k)[N], Scores& s, int jb) {  // of the tile whose keys begin at jb, from k0 on
 #pragma unroll
-    for (int n = 0; n < N; ++n) v[n].read(kt + S::kTileBytes + n * 32 * S::kRB, lane);
-    if (MASKED) {
+    for (int n = 0; n < N; ++n) s[n] = k[n].scores(q, st.less);
+    if (decltype(masked_c)::value != 0) {
 #pragma unroll
       for (int n = 0; n < N; ++n) hide_unseen(s[n], c.lim - jb - 32 * n, hh);
     }
-    st.exponentials(s);
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      if (MASKED) odd |= v[n].clear();
-      v[n].add(s[n], st.l, st.o);
-    }
   };
   while (true) {
-    wait_vmcnt<0>();  // the loads below are counted: nothing of the start may be in flight with them
     const int n_kt = (rq.wn + BK - 1) / BK, off = rq.w0 - it.k0;
-    Places next{0, 0};
-    if (n_kt) next = rq.places(min(NS - 1, n_kt - 1));
-    uint32_t stage = 0;  // of tile jt; the tile before it lay in the one before
-    auto turn = [&](int jt) {
-      if (n_kt - 1 - jt >= NS - 2) wait_vmcnt<(NS - 2) * 2 * LOADS>(); else wait_vmcnt<0>();
-      __syncthreads();
-      if (jt + NS - 1 < n_kt) {
-        request(jt + NS - 1, next, stage == 0 ? (NS - 1) * S::kStageBytes : stage - S::kStageBytes);
-        next = rq.places(min(jt + NS, n_kt - 1));
-      }
+    wait_vmcnt<0>();  // the loads below are counted: nothing of the start may be in flight with them
+    __syncthreads();
+    uint32_t stage = 0;  // of tile jt
+    auto stage_from = [&](int steps) {  // of tile jt + steps
+      const uint32_t x = stage + steps * S::kStageBytes;
+      return x >= NS * S::kStageBytes ? x - NS * S::kStageBytes : x;
     };
-    auto advance = [&] { stage = stage == (NS - 1) * S::kStageBytes ? 0 : stage + S::kStageBytes; };
-    // tiles every column of the wave sees whole, then the others: two loops, each with one form of the block
-    int jt = 0;
-    const int n_whole = max(min((c.all + 1 - off) / BK, n_kt), 0);
-    for (; jt < n_whole; ++jt, advance()) {
-      turn(jt);
-      blocks(IC<BK / 32>{}, IC<0>{}, lds + stage, off + jt * BK);
+    auto turn = [&](int jt) {
+      if (n_kt - 2 - jt >= NS - 3) wait_vmcnt<(NS - 3) * 2 * LOADS>(); else wait_vmcnt<0>();
+      __syncthreads();
+      if (jt + NS - 1 < n_kt) request(jt + NS - 1, stage_from(NS - 1));
+    };
+    auto active = [&](int jt) { return jt < n_kt && off + jt * BK <= c.any; };  // some column of the wave sees a key of the tile
+    const int n_whole = max(min((c.all + 1 - off) / BK, n_kt), 0);  // tiles that all columns of the wave see whole
+    Scores s0, s1;
+    if (active(0)) {
+      Keys<E, D> k[N];
+      read_keys(k, 0);
+      scores(IC<1>{}, k, s0, off);
+      st.raise(s0);
     }
-    for (; jt < n_kt; ++jt, advance()) {
+    auto both_whole = [&](int jt, Scores& s, Scores& ahead) {  // neither tile jt nor the next needs a mask
       turn(jt);
+      Keys<E, D> k[N];
+      Values<E, D> v[N];
+      read_keys(k, stage_from(1));
+      read_values(v, stage);
+      scores(IC<0>{}, k, ahead, 0);
+      st.exponentials(s);
 #pragma unroll
-      for (int kb = 0; kb < BK / 32; ++kb)
-        if (off + jt * BK + 32 * kb <= c.any) blocks(IC<1>{}, IC<1>{}, lds + stage + kb * 32 * S::kRB, off + jt * BK + 32 * kb);
+      for (int n = 0; n < N; ++n) v[n].add(s[n], st.l, st.o);
+      st.raise(ahead);
+      stage = stage_from(1);
+    };
+    auto any_tiles = [&](int jt, Scores& s, Scores& ahead) {
+      turn(jt);
+      if (active(jt)) {
+        Values<E, D> v[N];
+        read_values(v, stage);
+        if (jt >= n_whole) {
+#pragma unroll
+          for (int n = 0; n < N; ++n) odd |= v[n].clear();
+        }
+        st.exponentials(s);
+#pragma unroll
+        for (int n = 0; n < N; ++n) v[n].add(s[n], st.l, st.o);
+      }
+      if (active(jt + 1)) {
+        Keys<E, D> k[N];
+        read_keys(k, stage_from(1));
+        scores(IC<1>{}, k, ahead, off + (jt + 1) * BK);
+        st.raise(ahead);
+      }
+      stage = stage_from(1);
+    };
+    // two turns a round, so that the scores change places without being copied
+    int jt = 0;
+    for (; jt + 2 < n_whole; jt += 2) {
+      both_whole(jt, s0, s1);
+      both_whole(jt + 1, s1, s0);
+    }
+    for (; jt < n_kt; jt += 2) {
+      any_tiles(jt, s0, s1);
+      if (jt + 1 < n_kt) any_tiles(jt + 1, s1, s0);
     }
     rq.w0 += window;
     if (rq.w0 >= it.k0 + it.nk) break;
@@ -1036,7 +1084,7 @@ size_t plan(const segpt_paged_params& p, PagedArgs& a) {
   a.rows_each = p.seq_start ? 0 : p.T / p.B;
   a.log_page = __builtin_ctz((unsigned)p.page_size);
   a.capacity = paged_capacity(p);
-  a.target = 256 * (row_bytes <= 128 ? 3 : row_bytes <= 256 ? 2 : 1);
+  a.target = 256 * (row_bytes <= 256 ? 2 : 1);
   a.min_few = 2;
   a.min_many = 4;
   // Tiles: whole ones of the columns there are, and one begun an entry.  Items: a tile's part of what the target stands for, and one begun.

@@ -52,7 +52,7 @@ struct DeviceDivisor {
 
 struct PagedArgs {
   segpt_paged_params p;
-  Divisor rep, hkv;               // H / Hkv, Hkv
+  Divisor rep, hkv, each;         // H / Hkv, Hkv, rows_each
   int32_t entries, shared;        // shared: 1 if entry 0 is the prefix
   int32_t rows_each, log_page, capacity;
   int32_t target;                 // workgroups of four waves that fill the card once
@@ -60,6 +60,7 @@ struct PagedArgs {
   int32_t n_many, n_few;          // items there may be of either kind
   int32_t n_joins;                // tiles and kv heads whose partial results there may be to join
   int32_t n_slots;                // partial results there is room for, 32 columns each
+  int32_t* lens;                  // blocks of a share (few, many), left for the merge by workgroup 0
   float* part;                    // [n_slots][32][D]
   float2* stat;                   // [n_slots][32]
 };
@@ -152,10 +153,11 @@ __device__ __forceinline__ Entries load_entries(const PagedArgs& a, int lane, in
     if (64 * u < a.entries) x.e[u] = entry_of(a, 64 * u + lane, rep, raw[u]);
   return x;
 }
+__device__ __forceinline__ Shares shares_from(int few, int many) { return {few, many, DeviceDivisor(few).inverse, DeviceDivisor(many).inverse}; }
 // Blocks of a share, such that the workgroups are resident at once if the tiles alone are not too many for that: the mean first, then longer
 // ones until the begun ones fit too (one workgroup too many is a round of its own).  A block of many columns keeps a workgroup as long as the
 // memory does that of few columns, in a quarter of the workgroup each: a wave's share is a quarter as long.  The sums are
-// floats: they may round, but to the same value in every wave of both kernels.
+// floats: they may round, but to the same value in every wave.
 __device__ __forceinline__ Shares share_blocks(const PagedArgs& a, int lane, int rep, const Entries& kept) {
   auto sum = [&](auto of) {
     float v = 0.f;
@@ -165,20 +167,17 @@ __device__ __forceinline__ Shares share_blocks(const PagedArgs& a, int lane, int
     for (int e = 64 * kKept; e < a.entries; e += 64) v += of(entry_at(a, e + lane, rep));
     return lane_value(lane_prefix_sum(v), 63) * (float)a.p.Hkv;
   };
-  const float target = (float)a.target;
-  float len = sum([](const Entry& x) { return (float)x.tiles * (float)x.blocks; }) / target;
-  Shares s;
+  auto room = [](const Entry& x) { return (float)x.tiles * (x.many ? 1.f : 0.25f); };  // workgroups of a share of each tile
+  const float target = (float)a.target, per = __builtin_amdgcn_rcpf(target);
+  float len = sum([](const Entry& x) { return (float)x.tiles * (float)x.blocks; }) * per;
+  const bool fits = sum(room) < target;
   for (int i = 0;; ++i) {
-    s.many = max((int)fminf(ceilf(len), 1e9f), a.min_many);
-    s.few = max((int)fminf(ceilf(0.25f * len), 1e9f), a.min_few);
-    s.per_many = DeviceDivisor(s.many).inverse;
-    s.per_few = DeviceDivisor(s.few).inverse;
-    if (i == 3) break;
-    const float groups = sum([&](const Entry& x) { return (float)x.tiles * (float)shares_of(x, s) * (x.many ? 1.f : 0.25f); });
-    if (groups <= target || groups > 2.f * target) break;
-    len *= fmaxf(groups / target, 1.03f);
+    const Shares s = shares_from(max((int)fminf(ceilf(0.25f * len), 1e9f), a.min_few), max((int)fminf(ceilf(len), 1e9f), a.min_many));
+    if (!fits || i == 2) return s;
+    const float groups = sum([&](const Entry& x) { return room(x) * (float)shares_of(x, s); });
+    if (groups <= target) return s;
+    len *= fmaxf(groups * per, 1.03f);
   }
-  return s;
 }
 // an entry as the whole wave sees it
 struct Found {
@@ -241,68 +240,90 @@ struct Shape {
   static constexpr int kManyBytes = kStages * kStageBytes;
   // FEW: one block of keys and one of values a wave
   static constexpr int kFewTable = 64;
-  static constexpr int kDepth = kRB <= 128 ? 2 : 1;
-  static constexpr int kFewBytes = kDepth * 2 * kBlock * kRB;
+  static constexpr int kDepth = kRB <= 128 ? 2 : 1;  // buffers
+  static constexpr int kFewBytes = 2 * kBlock * kRB;  // of a buffer
   static constexpr int kOcc = kRB > 256 ? 1 : 2;  // workgroups of four waves per CU
 };
 
-// query columns in the B operand's layout, scaled by everything that does not depend on the key (gsm: g_q g_k sm_scale log2 e); D / 2 values
-// a lane.  bf16: element 16 ks + 8 hh + t; fp32: chunk 2 c + hh of four.
+// Query columns in the B operand's layout, scaled by everything that does not depend on the key (gsm: g_q g_k sm_scale log2 e); D / 2 values
+// a lane.  bf16: element 16 ks + 8 hh + t; fp32: chunk 2 c + hh of four.  fetch() asks for the row and its angles, no branch between (without
+// a rotation the row's own bytes stand in for the angles and are not used), so that they are on their way with the page numbers; finish()
+// makes the operand of them.  (Fetched where they are needed they took 7500 of an item's 25000 cycles: two round trips behind the tiles.)
 template <typename E, int D>
 struct Query;
 template <int D>
 struct Query<uint16_t, D> {
-  bf16x8 reg[D / 16];
-  __device__ __forceinline__ void load(const segpt_paged_params& p, const uint16_t* row, int64_t angle, bool live, int hh, const float* gsm) {
-    constexpr int KS = D / 16;
-    u32x4 raw[KS];
+  static constexpr int KS = D / 16;
+  bf16x8 reg[KS];
+  u32x4 raw[KS];
+  f32x4 cs[KS], sn[KS];
+  __device__ __forceinline__ void fetch(const segpt_paged_params& p, const uint16_t* row, int64_t angle, int hh) {
+    const float* c = (p.rope_cos ? p.rope_cos + angle : reinterpret_cast<const float*>(row)) + 8 * hh;
+    const float* s = (p.rope_cos ? p.rope_sin + angle : reinterpret_cast<const float*>(row)) + 8 * hh;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) raw[ks] = *reinterpret_cast<const u32x4*>(row + 16 * ks + 8 * hh);
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {  // floats 16 (i / 2) + 8 hh + 4 (i % 2) ..
+      cs[i] = *reinterpret_cast<const f32x4*>(c + 16 * (i / 2) + 4 * (i % 2));
+      sn[i] = *reinterpret_cast<const f32x4*>(s + 16 * (i / 2) + 4 * (i % 2));
+    }
+  }
+  __device__ __forceinline__ void finish(const segpt_paged_params& p, bool live, int hh, const float* gsm) {
     float x[KS][8];
     unpack_b_layout<KS>(raw, x);
-    if (p.rope_cos) rope_b_layout<KS>(x, p.rope_cos + angle, p.rope_sin + angle, hh);
-    float ss = 0.f;
+    if (p.rope_cos) {
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) rope_pair(x[i / 2][4 * (i % 2) + t], x[i / 2 + KS / 2][4 * (i % 2) + t], cs[i][t], sn[i][t]);
+    }
+    float sq[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int t = 0; t < 8; ++t) ss += x[ks][t] * x[ks][t];
-    ss = half_sum(ss);
-    const float alpha = !live ? 0.f : (p.flags & SEGPT_FLAG_NO_NORM) ? 1.f : __builtin_amdgcn_rsqf(ss * (1.0f / D) + p.eps);
+      for (int t = 0; t < 8; ++t) sq[t % 4] += x[ks][t] * x[ks][t];
+    const float ss = half_sum((sq[0] + sq[1]) + (sq[2] + sq[3]));
+    const float alpha = (p.flags & SEGPT_FLAG_NO_NORM) ? 1.f : __builtin_amdgcn_rsqf(ss * (1.0f / D) + p.eps);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
+      const float4 ga = *reinterpret_cast<const float4*>(gsm + 16 * ks + 8 * hh), gb = *reinterpret_cast<const float4*>(gsm + 16 * ks + 8 * hh + 4);
+      const float g[8] = {ga.x, ga.y, ga.z, ga.w, gb.x, gb.y, gb.z, gb.w};
       u32x4 w;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float* g = gsm + 16 * ks + 8 * hh + 2 * i;
-        w[i] = live ? pack_bf16x2(x[ks][2 * i] * alpha * g[0], x[ks][2 * i + 1] * alpha * g[1]) : 0u;
-      }
+      for (int i = 0; i < 4; ++i) w[i] = live ? pack_bf16x2(x[ks][2 * i] * alpha * g[2 * i], x[ks][2 * i + 1] * alpha * g[2 * i + 1]) : 0u;
       reg[ks] = as_bf16x8(w);
     }
   }
 };
 template <int D>
 struct Query<float, D> {
-  float reg[D / 8][4];
-  __device__ __forceinline__ void load(const segpt_paged_params& p, const float* row, int64_t angle, bool live, int hh, const float* gsm) {
-    constexpr int C = D / 8;
+  static constexpr int C = D / 8;
+  float reg[C][4];
+  f32x4 cs[C / 2], sn[C / 2];
+  __device__ __forceinline__ void fetch(const segpt_paged_params& p, const float* row, int64_t angle, int hh) {
+    const float* c = (p.rope_cos ? p.rope_cos + angle : row) + 4 * hh;
+    const float* s = (p.rope_cos ? p.rope_sin + angle : row) + 4 * hh;
 #pragma unroll
-    for (int c = 0; c < C; ++c) load16(row + 8 * c + 4 * hh, reg[c]);
+    for (int i = 0; i < C; ++i) load16(row + 8 * i + 4 * hh, reg[i]);
+#pragma unroll
+    for (int i = 0; i < C / 2; ++i) {
+      cs[i] = *reinterpret_cast<const f32x4*>(c + 8 * i);
+      sn[i] = *reinterpret_cast<const f32x4*>(s + 8 * i);
+    }
+  }
+  __device__ __forceinline__ void finish(const segpt_paged_params& p, bool live, int hh, const float* gsm) {
     if (p.rope_cos) {
 #pragma unroll
-      for (int c = 0; c < C / 2; ++c) {
-        float cs[4], sn[4];
-        load16(p.rope_cos + angle + 8 * c + 4 * hh, cs);
-        load16(p.rope_sin + angle + 8 * c + 4 * hh, sn);
+      for (int c = 0; c < C / 2; ++c)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) rope_pair(reg[c][t], reg[c + C / 2][t], cs[t], sn[t]);
-      }
+        for (int t = 0; t < 4; ++t) rope_pair(reg[c][t], reg[c + C / 2][t], cs[c][t], sn[c][t]);
     }
-    float ss = 0.f;
+    float sq[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) ss += reg[c][t] * reg[c][t];
-    ss = half_sum(ss);
+      for (int t = 0; t < 4; ++t) sq[t] += reg[c][t] * reg[c][t];
+    const float ss = half_sum((sq[0] + sq[1]) + (sq[2] + sq[3]));
     const float alpha = (p.flags & SEGPT_FLAG_NO_NORM) ? 1.f : 1.0f / sqrtf(ss * (1.0f / D) + p.eps);
 #pragma unroll
     for (int c = 0; c < C; ++c)
@@ -369,10 +390,15 @@ __device__ __forceinline__ bool stage_table(const PagedArgs& a, const Item& it, 
   }
   return __builtin_amdgcn_ballot_w64(bad) != 0;
 }
-__device__ __forceinline__ float scale_at(const segpt_paged_params& p, int d) {
-  const float v = (p.gq_numel == 1 ? p.g_q[0] : p.g_q[d]) * p.sm_scale * kLog2e;
-  return p.gk_numel == 0 ? v : v * (p.gk_numel == 1 ? p.g_k[0] : p.g_k[d]);
+// what scales component d of every query: asked for, and worked out
+struct Gain {
+  float q, k;
+};
+__device__ __forceinline__ Gain fetch_gain(const segpt_paged_params& p, int d) {
+  const float* gk = p.g_k ? p.g_k : p.g_q;
+  return {p.g_q[p.gq_numel == 1 ? 0 : d], gk[p.gk_numel > 1 ? d : 0]};
 }
+__device__ __forceinline__ float scale_of(const segpt_paged_params& p, const Gain& g) { return g.q * (p.g_k ? g.k : 1.f) * p.sm_scale * kLog2e; }
 
 // Requests of tiles of keys w0 .. w0 + wn - 1.  A load covers kRowsPerLoad rows, at most 8, of one page: its address is a scalar base and
 // a lane offset.  LOADS loads a tensor and tile; number ps is load first + ps * step of the tile.  Where the rows of a load begin is worked out
@@ -444,7 +470,7 @@ struct Column {
   int all, any;  // last key that all columns of the wave see, that any of them sees
 };
 template <typename E, int D>
-__device__ __forceinline__ Column column_of(const PagedArgs& a, const Item& it, int rep, int wave_col, int lane, Query<E, D>& q, const float* gsm) {
+__device__ __forceinline__ Column column_of(const PagedArgs& a, const Item& it, int rep, int wave_col, int lane, Query<E, D>& q) {
   const segpt_paged_params& p = a.p;
   Column c;
   const bool works = wave_col < it.cols;
@@ -461,13 +487,13 @@ __device__ __forceinline__ Column column_of(const PagedArgs& a, const Item& it, 
         if (p.seq_start[m] <= c.t) { b = m; lo = m + 1; } else hi = m - 1;
       }
     } else {
-      b = c.t / a.rows_each;
+      b = a.each.of(c.t);
     }
     sequence_rows(p, a.rows_each, b, &f, &n);
     own = (int)min((int64_t)p.kv_len[b] - n + (c.t - f), (int64_t)a.capacity - 1);
   }
   const int64_t pos = max((int64_t)p.prefix_len + own, (int64_t)0);
-  q.load(p, row_of<E>(p.q, c.t, c.h), (p.rope_pos0 + pos) * (D / 2), c.live, lane >> 5, gsm);
+  q.fetch(p, row_of<E>(p.q, c.t, c.h), (p.rope_pos0 + pos) * (D / 2), lane >> 5);
   c.lim = min((it.prefix ? p.prefix_len : 0) + own - it.k0, it.nk - 1);
   if (it.prefix) {
     const bool cut = __builtin_amdgcn_ballot_w64(c.live && c.lim < it.nk - 1) != 0;  // rows that stand in the prefix
@@ -717,11 +743,19 @@ __device__ __forceinline__ void few_columns(const PagedArgs& a, const Item& it, 
   constexpr int LOADS = kBlock * S::kRB / 1024;
   const int hh = lane >> 5, window = S::kFewTable << a.log_page;
   constexpr int DEPTH = S::kDepth;
-  constexpr uint32_t kBuffer = kBlock * S::kRB;
+  constexpr uint32_t kBuffer = S::kFewBytes / 2;
   auto rq = requests<E, D, kBlock, LOADS>(a, it, table, 0, 1, lane);
   rq.wn = min(it.nk, window);
+  // one round trip: gain, query row and angles, page numbers
+  Gain gain[(D + 63) / 64];
+#pragma unroll
+  for (int i = 0; i < (D + 63) / 64; ++i) gain[i] = fetch_gain(a.p, (64 * i + lane) % D);
+  Query<E, D> q;
+  const Column c = column_of<E, D>(a, it, rep, it.tile * kFew, lane, q);
   bool bad = it.x.broken | stage_table(a, it, rq.w0, rq.wn, table, lane, 64);
-  for (int d = lane; d < D; d += 64) gsm[d] = scale_at(a.p, d);
+#pragma unroll
+  for (int i = 0; i < (D + 63) / 64; ++i)
+    if (64 * i + lane < D) gsm[64 * i + lane] = scale_of(a.p, gain[i]);
   wave_sync();
   auto start_window = [&] {
 #pragma unroll
@@ -739,8 +773,7 @@ __device__ __forceinline__ void few_columns(const PagedArgs& a, const Item& it, 
     else wait_vmcnt<3 * LOADS>();
   };
   start_window();
-  Query<E, D> q;
-  const Column c = column_of<E, D>(a, it, rep, it.tile * kFew, lane, q, gsm);
+  q.finish(a.p, c.live, hh, gsm);
   State<D / 32> st;
   st.clear();
   bool odd = false;
@@ -812,12 +845,15 @@ __device__ __forceinline__ void many_columns(const PagedArgs& a, const Item& it,
     for (int t = 0; t < NS - 1; ++t)
       if (t * BK < rq.wn) request(t, t * S::kStageBytes);
   };
+  // one round trip: gain, query row and angles, page numbers
+  const Gain gain = fetch_gain(a.p, tid % D);
+  Query<E, D> q;
+  const Column c = column_of<E, D>(a, it, rep, it.tile * kMany + wave * 32, lane, q);
   stage_pages();
-  if (tid < D) gsm[tid] = scale_at(a.p, tid);
+  if (tid < D) gsm[tid] = scale_of(a.p, gain);
   __syncthreads();
   start_window();
-  Query<E, D> q;
-  const Column c = column_of<E, D>(a, it, rep, it.tile * kMany + wave * 32, lane, q, gsm);
+  q.finish(a.p, c.live, hh, gsm);
   State<D / 32> st;
   st.clear();
   bool odd = false;
@@ -918,18 +954,20 @@ __device__ __forceinline__ void many_columns(const PagedArgs& a, const Item& it,
   store_result<E, D>(a, it, c, st, bad, wave * 32 + (lane & 31), hh);
 }
 
-__device__ __forceinline__ void clear_rest(const PagedArgs& a, int tid, int threads, int elem, int D) {
+// Rows before the first sequence and behind the last, by the last workgroups of the launch, which mostly have no item
+template <typename E>
+__device__ __forceinline__ void clear_rest(const PagedArgs& a, int tid, int threads, int D) {
+  constexpr int kBy = 64;
   const segpt_paged_params& p = a.p;
+  const int by = min(kBy, (int)gridDim.x), from = (int)blockIdx.x - ((int)gridDim.x - by);
+  if (!p.seq_start || !(p.flags & SEGPT_FLAG_ZERO_REST) || from < 0) return;
   int head, f, n;
-  sequence_rows(p, a.rows_each, 0, &head, &n);
-  sequence_rows(p, a.rows_each, p.B - 1, &f, &n);
+  sequence_rows(p, 0, 0, &head, &n);
+  sequence_rows(p, 0, p.B - 1, &f, &n);
   const int tail = max(f + n, head);
-  for (int i = blockIdx.x; i < head + p.T - tail; i += gridDim.x) {  // rows before the first sequence and behind the last
+  for (int i = from; i < head + p.T - tail; i += by) {
     const int t = i < head ? i : i - head + tail;
-    for (int x = tid; x < p.H * D; x += threads) {
-      if (elem == 2) row_of<uint16_t>(p.o, t, x / D)[x % D] = 0;
-      else row_of<float>(p.o, t, x / D)[x % D] = 0.f;
-    }
+    for (int x = tid; x < p.H * D; x += threads) row_of<E>(p.o, t, x / D)[x % D] = 0;
   }
 }
 
@@ -937,13 +975,14 @@ __device__ __forceinline__ void clear_rest(const PagedArgs& a, int tid, int thre
 template <typename E, int D>
 __global__ __launch_bounds__(64, (Shape<E, D>::kOcc)) void paged_few_kernel(PagedArgs a) {
   using S = Shape<E, D>;
-  __shared__ __attribute__((aligned(1024))) char lds[S::kFewBytes];
+  __shared__ __attribute__((aligned(1024))) char lds[S::kDepth * S::kFewBytes];
   __shared__ __attribute__((aligned(16))) float gsm[D];
   __shared__ int table[S::kFewTable + 2];
   const int lane = threadIdx.x, rep = a.rep.d;
-  if (a.p.flags & SEGPT_FLAG_ZERO_REST) clear_rest(a, lane, 64, sizeof(E), D);
+  clear_rest<E>(a, lane, 64, D);
   const Entries mine = load_entries(a, lane, rep);
   const Shares share = share_blocks(a, lane, rep, mine);
+  if (blockIdx.x == 0 && threadIdx.x == 0) { a.lens[0] = share.few; a.lens[1] = share.many; }
   const Item it = locate<false>(a, lane, rep, share, mine, blockIdx.x);
   if (it.valid) few_columns<E, D>(a, it, rep, lane, lds_addr_of(lds), table, gsm);
 }
@@ -952,7 +991,7 @@ __global__ __launch_bounds__(64, (Shape<E, D>::kOcc)) void paged_few_kernel(Page
 template <typename E, int D>
 __global__ __launch_bounds__(256, (Shape<E, D>::kOcc)) void paged_any_kernel(PagedArgs a) {
   using S = Shape<E, D>;
-  constexpr int kLds = S::kManyBytes > 4 * S::kFewBytes ? S::kManyBytes : 4 * S::kFewBytes;
+  constexpr int kLds = std::max(S::kManyBytes, 4 * S::kDepth * S::kFewBytes);
   __shared__ __attribute__((aligned(1024))) char lds[kLds];
   __shared__ __attribute__((aligned(16))) float gsm[4][D];
   __shared__ int table[S::kManyTable + 8];
@@ -960,15 +999,16 @@ __global__ __launch_bounds__(256, (Shape<E, D>::kOcc)) void paged_any_kernel(Pag
   static_assert(4 * (S::kFewTable + 2) <= S::kManyTable + 8, "four waves' page numbers");
   const int tid = threadIdx.x, lane = tid & 63, rep = a.rep.d;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  if (a.p.flags & SEGPT_FLAG_ZERO_REST) clear_rest(a, tid, 256, sizeof(E), D);
+  clear_rest<E>(a, tid, 256, D);
   const Entries mine = load_entries(a, lane, rep);
   const Shares share = share_blocks(a, lane, rep, mine);
+  if (blockIdx.x == 0 && threadIdx.x == 0) { a.lens[0] = share.few; a.lens[1] = share.many; }
   if ((int)blockIdx.x < a.n_many) {
     const Item it = locate<true>(a, lane, rep, share, mine, blockIdx.x);
     if (it.valid) many_columns<E, D>(a, it, rep, tid, lds_addr_of(lds), table, gsm[0], any_bad);
   } else {
     const Item it = locate<false>(a, lane, rep, share, mine, ((int)blockIdx.x - a.n_many) * 4 + wave);
-    if (it.valid) few_columns<E, D>(a, it, rep, lane, lds_addr_of(lds) + wave * S::kFewBytes, table + wave * (S::kFewTable + 2), gsm[wave]);
+    if (it.valid) few_columns<E, D>(a, it, rep, lane, lds_addr_of(lds) + wave * S::kDepth * S::kFewBytes, table + wave * (S::kFewTable + 2), gsm[wave]);
   }
 }
 
@@ -984,8 +1024,9 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedArgs a,
   __shared__ float2 stats[kUnits];
   const int tid = threadIdx.x, lane = tid & 63, unit = tid / LPR, c = tid % LPR;
   const int rep = a.rep.d;
+  const int few = a.lens[0], many = a.lens[1];
   const Entries mine = load_entries(a, lane, rep);
-  const Shares share = share_blocks(a, lane, rep, mine);
+  const Shares share = shares_from(few, many);
   const int which = blockIdx.x / subs, sub = blockIdx.x - which * subs;
   const Found own = find_entry<kFindJoin>(a, lane, rep, share, mine, which);
   if (own.entry < 0) return;
@@ -1037,25 +1078,25 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedArgs a,
           y.x += w * o[u].x; y.y += w * o[u].y; y.z += w * o[u].z; y.w += w * o[u].w;
         }
       }
+    auto take_in = [&](float2 x, float4 o) {  // another unit's sums of the column
+      const float top = fmaxf(m, x.x), ref = top == -INFINITY ? 0.f : top, w0 = fast_exp2(m - ref), w1 = fast_exp2(x.x - ref);
+      m = top;
+      l = l * w0 + x.y * w1;
+      y.x = y.x * w0 + o.x * w1; y.y = y.y * w0 + o.y * w1; y.z = y.z * w0 + o.z * w1; y.w = y.w * w0 + o.w * w1;
+    };
+    // the units of a wave first, then the waves
+    for (int o = step * LPR; o < 64; o <<= 1)
+      take_in(make_float2(__shfl_xor(m, o, 64), __shfl_xor(l, o, 64)), make_float4(__shfl_xor(y.x, o, 64), __shfl_xor(y.y, o, 64), __shfl_xor(y.z, o, 64), __shfl_xor(y.w, o, 64)));
     if (wide > 1) {
       __syncthreads();  // the round before has been read
       sums[tid] = y;
       if (c == 0) stats[unit] = make_float2(m, l);
       __syncthreads();
       if (unit >= step) continue;
-      float top = m;
-      for (int w = 1; w < wide; ++w) top = fmaxf(top, stats[w * step + unit].x);
-      const float ref = top == -INFINITY ? 0.f : top, w0 = fast_exp2(m - ref);
-      m = top;
-      l *= w0;
-      y.x *= w0; y.y *= w0; y.z *= w0; y.w *= w0;
-      for (int w = 1; w < wide; ++w) {
-        const float2 x = stats[w * step + unit];
-        const float4 o = sums[w * step * LPR + tid];
-        const float f = fast_exp2(x.x - ref);
-        l += f * x.y;
-        y.x += f * o.x; y.y += f * o.y; y.z += f * o.z; y.w += f * o.w;
-      }
+      const int far = max(step, 64 / LPR);  // units from one wave's sums to the next one's
+#pragma unroll
+      for (int w = 1; w < 4; ++w)
+        if (unit + w * far < kUnits) take_in(stats[unit + w * far], sums[w * far * LPR + tid]);
     }
     if (!live) continue;
     if (own.broken) l = __builtin_nanf("");
@@ -1082,6 +1123,7 @@ size_t plan(const segpt_paged_params& p, PagedArgs& a) {
   a.shared = p.prefix_table ? 1 : 0;
   a.entries = p.B + a.shared;
   a.rows_each = p.seq_start ? 0 : p.T / p.B;
+  a.each.set(p.seq_start ? 1 : a.rows_each);
   a.log_page = __builtin_ctz((unsigned)p.page_size);
   a.capacity = paged_capacity(p);
   a.target = 256 * (row_bytes <= 256 ? 2 : 1);
@@ -1108,7 +1150,7 @@ size_t plan(const segpt_paged_params& p, PagedArgs& a) {
   a.n_slots = (int32_t)std::min<int64_t>(slots, INT32_MAX / 32);
   const int64_t joins = a.shared ? own * p.Hkv : std::min(own_many * p.Hkv, most) + std::min((own - own_many) * p.Hkv, 4 * most);
   a.n_joins = (int32_t)std::min<int64_t>(joins, INT32_MAX);
-  return n_many + n_few > INT32_MAX / 2 || slots > INT32_MAX / 32 ? SIZE_MAX : (size_t)a.n_slots * 32 * (p.D + 2) * sizeof(float);
+  return n_many + n_few > INT32_MAX / 2 || slots > INT32_MAX / 32 ? SIZE_MAX : 256 + (size_t)a.n_slots * 32 * (p.D + 2) * sizeof(float);
 }
 
 template <typename E, int D>
@@ -1155,7 +1197,8 @@ int segpt_paged_attn(const segpt_paged_params* p, void* stream) {
   if (need > SIZE_MAX - 256) return SEGPT_E_SHAPE;
   if (!p->workspace || p->workspace_bytes < up256(need)) return SEGPT_E_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(p->workspace) & 255u) return SEGPT_E_ALIGN;
-  a.part = reinterpret_cast<float*>(p->workspace);
+  a.lens = reinterpret_cast<int32_t*>(p->workspace);
+  a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(p->workspace) + 256);
   a.stat = reinterpret_cast<float2*>(a.part + (size_t)a.n_slots * 32 * p->D);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (p->dtype == SEGPT_DTYPE_BF16) return p->D == 64 ? launch<uint16_t, 64>(a, st) : launch<uint16_t, 128>(a, st);

@@ -628,8 +628,7 @@ struct State {
     limit = -INFINITY;
     l[0] = l[1] = 0.f;
   }
-  // no score can exceed `bound`: the reference stays 0
-  __device__ __forceinline__ void bounded_by(float bound) { limit = bound; }
+  __device__ __forceinline__ float reference() const { return limit == -INFINITY ? -INFINITY : m; }
   // raises the reference where scores of N blocks exceed it
   template <int N>
   __device__ __forceinline__ void raise(f32x16 (&s)[N]) {
@@ -700,7 +699,7 @@ template <typename E, int D>
 __device__ __forceinline__ void store_result(const PagedArgs& a, const Item& it, const Column& c, State<D / 32>& st, bool bad, int slot_col, int hh) {
   const segpt_paged_params& p = a.p;
   constexpr int MB = D / 32;
-  float l = half_sum(st.l[0] + st.l[1]), m = l == 0.f ? -INFINITY : st.m;  // nothing seen: no part in the join's reference
+  float l = half_sum(st.l[0] + st.l[1]), m = st.reference();
   if (bad) { l = __builtin_nanf(""); m = 0.f; }
   if (!c.live) return;
   if (!it.direct) {
@@ -857,12 +856,6 @@ __device__ __forceinline__ void many_columns(const PagedArgs& a, const Item& it,
   q.finish(a.p, c.live, hh, gsm);
   State<D / 32> st;
   st.clear();
-  // Normalised on both sides, a score is at most sm_scale D max |g| (in log2 units): where that is small the softmax needs no maximum, which
-  // is a sixth of a turn's vector work (one prompt of 8192 tokens, 18 / 6 heads of 64: BOUNDED_US).  The keys' side holds because the pool's rows are what
-  // paged_kv_append normalised.
-  const float most = logit_bound<D>(gsm, lane);
-  const bool bounded = !(a.p.flags & SEGPT_FLAG_NO_NORM) && most <= kNoMaxBound;
-  if (bounded) st.bounded_by(kNoMaxBound);
   bool odd = false;
   constexpr int N = BK / 32;  // blocks of a tile
   typedef f32x16 Scores[N];
@@ -903,6 +896,7 @@ __device__ __forceinline__ void many_columns(const PagedArgs& a, const Item& it,
       Keys<E, D> k[N];
       read_keys(k, 0);
       scores(IC<1>{}, k, s0, off);
+      st.raise(s0);
     }
     auto both_whole = [&](int jt, Scores& s, Scores& ahead) {  // neither tile jt nor the next needs a mask
       turn(jt);
@@ -910,11 +904,11 @@ __device__ __forceinline__ void many_columns(const PagedArgs& a, const Item& it,
       Values<E, D> v[N];
       read_keys(k, stage_from(1));
       read_values(v, stage);
-      if (!bounded) st.raise(s);  // while the fragments arrive (two loops instead of a branch in one: 300 spilled registers)
       scores(IC<0>{}, k, ahead, 0);
       st.exponentials(s);
 #pragma unroll
       for (int n = 0; n < N; ++n) v[n].add(s[n], st.l, st.o);
+      st.raise(ahead);
       stage = stage_from(1);
     };
     auto any_tiles = [&](int jt, Scores& s, Scores& ahead) {
@@ -926,7 +920,6 @@ __device__ __forceinline__ void many_columns(const PagedArgs& a, const Item& it,
 #pragma unroll
           for (int n = 0; n < N; ++n) odd |= v[n].clear();
         }
-        st.raise(s);
         st.exponentials(s);
 #pragma unroll
         for (int n = 0; n < N; ++n) v[n].add(s[n], st.l, st.o);
@@ -935,6 +928,7 @@ __device__ __forceinline__ void many_columns(const PagedArgs& a, const Item& it,
         Keys<E, D> k[N];
         read_keys(k, stage_from(1));
         scores(IC<1>{}, k, ahead, off + (jt + 1) * BK);
+        st.raise(ahead);
       }
       stage = stage_from(1);
     };

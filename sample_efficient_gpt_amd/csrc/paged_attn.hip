@@ -968,6 +968,7 @@ __device__ __forceinline__ void clear_rest(const PagedArgs& a, int tid, int thre
   for (int i = from; i < head + p.T - tail; i += by) {
     const int t = i < head ? i : i - head + tail;
     for (int x = tid; x < p.H * D; x += threads) row_of<E>(p.o, t, x / D)[x % D] = 0;
+    for (int h = tid; p.lse && h < p.H; h += threads) p.lse[(int64_t)t * p.H + h] = -INFINITY;
   }
 }
 

@@ -571,6 +571,7 @@ void paged_append(const Tensor& k_in, const Tensor& v_in, const Tensor& k_pages,
       check(t->sizes() == k.sizes(), "v and v_first must have k's shape");
     }
   if (coef.defined()) check(coef.numel() == 2, "vr_coef must have two elements");
+  if (at::has_internal_overlap(k_pages) != at::MemOverlap::Yes) at::assert_no_overlap(k_pages, v_pages);  // the entry refuses the other kind
   for (const Tensor* t : {&k_pages, &v_pages})
     check(!t->is_inference() || c10::InferenceMode::is_enabled(), "pages made in inference mode can be appended to in inference mode only");
   if (k.numel() == 0) return;
@@ -600,6 +601,7 @@ std::pair<Tensor, Tensor> paged_attention(const Tensor& q_in, const Tensor& k_pa
   check(gq32.numel() == 1 || gq32.numel() == q.size(2), "gain must have 1 or head_dim elements");
   check(!gk32.defined() || gk32.numel() == 1 || gk32.numel() == q.size(2), "k_gain must have 1 or head_dim elements");
   check(prefix_len >= 0 && prefix_len <= INT32_MAX, "prefix_len must not be negative");
+  check(prefix.defined() || prefix_len == 0, "a shared prefix needs its prefix_table");
   if (prefix.defined()) {
     if (prefix.scalar_type() != at::kInt) throw BadType(std::string("prefix_table must be int32, got ") + c10::toString(prefix.scalar_type()));
     check(prefix.device() == dev, "all tensors must be on one device");
@@ -615,11 +617,13 @@ std::pair<Tensor, Tensor> paged_attention(const Tensor& q_in, const Tensor& k_pa
     if (out.scalar_type() != q.scalar_type()) throw BadType(std::string("out must have q's dtype, got ") + c10::toString(out.scalar_type()));
     check(out.device() == dev && out.sizes() == q.sizes() && (out.stride(2) == 1 || out.size(2) == 1), "out must have q's shape and device, contiguous in head_dim");
     check(out.data_ptr() != q.data_ptr() || q.numel() == 0, "out must not be q: a row is read again after others are written");
-    at::assert_no_overlap(out, q);
+    for (const Tensor* t : {&q, &k_pages, &v_pages}) at::assert_no_overlap(out, *t);
+    if (gate.defined()) at::assert_no_overlap(out, gate);
     check(!out.is_inference() || c10::InferenceMode::is_enabled(), "out made in inference mode can be written in inference mode only");
   }
   const Tensor y = out.defined() ? out : at::empty(q.sizes(), q.options());
-  const Tensor lse = with_lse ? at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat)) : Tensor();
+  const auto lse_options = q.options().dtype(at::kFloat);
+  const Tensor lse = !with_lse ? Tensor() : out.defined() ? at::full({q.size(0), q.size(1)}, -INFINITY, lse_options) : at::empty({q.size(0), q.size(1)}, lse_options);
   if (q.numel() == 0) return {y, lse};
   p.H = (int32_t)q.size(1);
   p.prefix_len = prefix.defined() ? (int32_t)prefix_len : 0;

@@ -409,3 +409,141 @@ def test_refusals(gpu_device):
         paged_kv_append(x.k, x.v, flat, flat, x.block_table, x.kv_len, seq_start=x.seq_start)
     empty = x.q[:0]
     assert paged_attention(empty, x.k_pages, x.v_pages, x.block_table, x.kv_len, x.g_q, seq_start=x.seq_start * 0).shape == empty.shape
+
+
+@pytest.mark.parametrize("rows,lens,prefix", [
+    ([1] * 300, [1 + 29 * i % 150 for i in range(300)], 0),                      # every sequence one token, more than a wave keeps in registers
+    ([(0, 1, 1, 3, 12)[i % 5] for i in range(300)], [30 + 17 * i % 90 for i in range(300)], 0),
+    ([1] * 300, [i % 40 for i in range(300)], 140),
+    ([(1, 0, 14)[i % 3] for i in range(270)], [15 + i % 40 for i in range(270)], 33),
+])
+@pytest.mark.parametrize("uniform", [False, True])
+def test_many_sequences(gpu_device, rows, lens, prefix, uniform):
+    for H, Hkv, D, dtype in ((6, 2, 64, BF16), (6, 2, 32, F32)):
+        x = Batch(rows, lens, H, Hkv, D, 16, dtype, gpu_device, seed=18, prefix=prefix, uniform=uniform and len(set(rows)) == 1)
+        y, lse = attend(x, return_lse=True)
+        check_y(x, y, lse, x.attended())
+        kp, vp = x.appended(pos0=prefix)
+        append(x, rope_pos0=prefix)
+        check_pools(x, kp, vp)
+
+
+@pytest.mark.parametrize("H,Hkv,D,dtype", [(16, 8, 64, BF16), (16, 8, 32, F32), (16, 8, 128, BF16)])
+def test_a_wave_holds_part_of_its_page_numbers(gpu_device, H, Hkv, D, dtype):
+    """Tokens whose shares are longer than 64 pages, beside slots that are not finite behind every sequence's end."""
+    lens = [4000 + 37 * i for i in range(64)]
+    x = Batch([1] * 64, lens, H, Hkv, D, 8, dtype, gpu_device, seed=19, uniform=True)
+    for b, L in enumerate(lens):
+        if L % 8:
+            x.k_pages[int(x.block_table[b, L // 8]), :, L % 8:] = math.nan
+            x.v_pages[int(x.block_table[b, L // 8]), :, L % 8:] = math.inf
+    y, lse = attend(x, return_lse=True)
+    some = [0, 31, 63]
+    ref = Batch([1] * 3, [lens[b] for b in some], H, Hkv, D, 8, dtype, gpu_device, seed=19)
+    ref.block_table, ref.k_pages, ref.v_pages, ref.q, ref.cos, ref.sin, ref.g_q = x.block_table[some], x.k_pages, x.v_pages, x.q[some], x.cos, x.sin, x.g_q
+    check_y(x, y[some], lse[some], ref.attended())
+    alone = attend(ref)  # other shares, other sums
+    assert (alone.double() - y[some].double()).norm() <= (6e-3 if dtype == BF16 else 1e-5) * alone.double().norm()
+    assert y.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,lens", [([1, 1], [700, 90]), ([200, 1], [900, 300])])
+@pytest.mark.parametrize("order", ["rising", "falling", "spike"])
+def test_scores_far_apart(gpu_device, dtype, rows, lens, order):
+    """Keys along the queries, so that the scores of a row run over several hundred: upwards (every tile has a new maximum), downwards (all but
+    the first underflow), or with one key above all others."""
+    for H, Hkv, D in ((6, 2, 64), (4, 2, 128)):
+        x = Batch(rows, lens, H, Hkv, D, 16, dtype, gpu_device, seed=20, rope=False)
+        x.q.copy_(1.0 + 0.05 * torch.randn(x.q.shape, device=gpu_device))
+        x.g_q = torch.ones(1, device=gpu_device)
+        for b, L in enumerate(lens):
+            for p in range(L):
+                size = {"rising": p / L, "falling": 1 - p / L, "spike": float(p == L // 2)}[order] * 2 - 1
+                x.k_pages[int(x.block_table[b, p // 16]), :, p % 16] = 4.0 * size
+        y, lse = attend(x, qk_norm=False, return_lse=True, sm_scale=1.0)
+        y_ref, lse_ref, bound = x.attended(qk_norm=False, sm_scale=1.0)
+        # scores up to 4 D: their roundings (2^-8 or D 2^-24 of that) move the sums by more than their size at bf16; y stays among the values
+        assert y.isfinite().all() and lse.isfinite().all()
+        h = H_BF16 if dtype == BF16 else H_F32 * D
+        assert ((y.to(F64) - y_ref).abs() <= h * bound).all()
+        assert ((lse.to(F64) - lse_ref).abs() <= h * (4.5 * D + 16)).all()
+
+
+def test_strided_rows_gate_and_out(gpu_device):
+    for H, Hkv, D, dtype in ((6, 2, 64, BF16), (4, 2, 128, BF16), (6, 2, 32, F32)):
+        for rows, lens in (([1, 1, 1], [40, 9, 200]), ([60, 1, 5], [60, 100, 30])):
+            x = Batch(rows, lens, H, Hkv, D, 16, dtype, gpu_device, seed=21)
+            T = sum(rows)
+            x.gate = torch.randn(T, H, 3, device=gpu_device).to(dtype)[..., 1]
+            x.q = x.q.transpose(0, 1).contiguous().transpose(0, 1)  # heads outermost
+            want, lse = attend(x, gate_logits=x.gate, return_lse=True)
+            check_y(x, want, lse, x.attended(gate=True))
+            wide = torch.full((H, T + 2, D + 8), 5.0, dtype=dtype, device=gpu_device)
+            out = wide[:, 1:-1, :D].transpose(0, 1)
+            y, lse2 = attend(x, gate_logits=x.gate, return_lse=True, out=out)
+            assert y is out and torch.equal(out, want) and torch.equal(lse, lse2)
+            assert (wide[:, [0, -1]] == 5).all() and (wide[..., D:] == 5).all()
+
+
+def test_lse_of_rows_in_no_sequence(gpu_device):
+    x = Batch([1, 3, 9], [20, 40, 9], 6, 2, 64, 16, BF16, gpu_device, seed=22)
+    x.seq_start = torch.tensor([2, 3, 6, 8], dtype=torch.int32, device=gpu_device)
+    rest = [0, 1, 8, 9, 10, 11, 12]
+    for kw in (dict(), dict(out=torch.zeros_like(x.q))):
+        _, lse = attend(x, return_lse=True, **kw)
+        assert (lse[rest] == -math.inf).all() and lse[2:8].isfinite().all()
+
+
+def test_two_calls_at_once(gpu_device):
+    """Calls on two streams, each with work of its own, give what they give alone."""
+    xs = [Batch([1] * 8, [3000 + i for i in range(8)], 18, 6, 64, 16, BF16, gpu_device, seed=23, uniform=True),
+          Batch([200, 1, 90], [900, 4000, 300], 18, 6, 64, 32, BF16, gpu_device, seed=24),
+          Batch([1] * 20, [i for i in range(20)], 18, 6, 64, 32, BF16, gpu_device, seed=25, prefix=700)]
+    want = [attend(x) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[] for _ in xs]
+    for _ in range(6):
+        for x, s, g in zip(xs, streams, got):
+            with torch.cuda.stream(s):
+                g.append(attend(x))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(w, y) for y in g)
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_batches_drawn_at_random(gpu_device, seed):
+    import random
+    r = random.Random(100 + seed)
+    H, Hkv, D, dtype = r.choice(HEADS + [(24, 1, 64, BF16), (5, 5, 128, BF16), (33, 11, 64, F32)])
+    page, prefix = r.choice([8, 16, 32, 64, 128]), r.choice([0, 0, 1, 31, 32, 100, 257])
+    B = r.choice([1, 2, 5, 17, 65])
+    rows = [r.choice([0, 1, 1, 2, 5, 11, 33, 64, 129]) for _ in range(B)] if r.random() < 0.7 else [r.choice([1, 4, 12])] * B
+    if sum(rows) == 0:
+        rows[0] = 1
+    lens = [max(n + r.choice([0, 0, 1, 7, 64, 500]) - (r.random() < 0.2), 0) for n in rows]
+    x = Batch(rows, lens, H, Hkv, D, page, dtype, gpu_device, seed=seed, prefix=prefix, uniform=len(set(rows)) == 1, rope=r.random() < 0.7,
+              layout=r.choice(["phsd", "pshd", "apart"]))
+    gate, norm = r.random() < 0.5, r.random() < 0.7
+    kp, vp = x.appended(norm, True, pos0=prefix if x.cos is not None else 0)
+    append(x, qk_norm=norm, v_first=x.v_first, vr_coef=x.coef, rope_pos0=prefix if x.cos is not None else 0)
+    check_pools(x, kp, vp, True)
+    y, lse = attend(x, qk_norm=norm, gate_logits=x.gate if gate else None, g_k=x.g_k, sm_scale=0.1, return_lse=True)
+    check_y(x, y, lse, x.attended(qk_norm=norm, gate=gate, g_k=x.g_k, sm_scale=0.1))
+
+
+def test_further_refusals(gpu_device):
+    x = Batch([1, 2], [20, 30], 6, 2, 64, 16, BF16, gpu_device, seed=26)
+    kw = dict(seq_start=x.seq_start)
+    with pytest.raises(AssertionError, match="prefix_table"):
+        shared_prefix_attention(x.q, x.k_pages, x.v_pages, None, 16, x.block_table, x.kv_len, x.g_q, **kw)
+    with pytest.raises(RuntimeError, match="overlap|single memory location"):
+        attend(x, out=x.k_pages.flatten()[: x.q.numel()].view(x.q.shape))
+    with pytest.raises(RuntimeError, match="overlap|single memory location"):
+        paged_kv_append(x.k, x.v, x.k_pages, x.k_pages, x.block_table, x.kv_len, **kw)
+    both = torch.stack([x.k_pages, x.v_pages], 1)  # keys and values of a page side by side are no overlap
+    paged_kv_append(x.k, x.v, both[:, 0], both[:, 1], x.block_table, x.kv_len, **kw)
+    paged_kv_append(x.k, x.v, x.k_pages, x.v_pages, x.block_table, x.kv_len, **kw)
+    assert torch.equal(both[:, 0], x.k_pages) and torch.equal(both[:, 1], x.v_pages)

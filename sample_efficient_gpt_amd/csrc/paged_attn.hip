@@ -55,7 +55,7 @@ struct PagedArgs {
   Divisor rep, hkv, each;         // H / Hkv, Hkv, rows_each
   int32_t entries, shared;        // shared: 1 if entry 0 is the prefix
   int32_t rows_each, log_page, capacity;
-  int32_t target;                 // workgroups of four waves that fill the card once
+  int32_t target;                 // workgroups of four waves there are to be
   int32_t min_few, min_many;      // shortest shares, in blocks of 32 keys
   int32_t n_many, n_few;          // items there may be of either kind
   int32_t n_joins;                // tiles and kv heads whose partial results there may be to join
@@ -183,7 +183,7 @@ __device__ __forceinline__ Shares share_blocks(const PagedArgs& a, int lane, int
 struct Found {
   int entry;          // -1: none
   int first, n, len, blocks;
-  int shares, base;   // shares of its keys; number of its first item of its kind (or tile to be joined)
+  int shares, base;   // shares of its keys; number of its first item of its kind (or tile to be joined); none: how many there are
   int slot;           // of its first partial result (entries whose tiles leave any)
   bool many, broken;
 };
@@ -215,6 +215,7 @@ __device__ __forceinline__ Found find_entry(const PagedArgs& a, int lane, int re
     if (64 * u < a.entries && look(64 * u, kept.e[u])) return found;
   for (int e0 = 64 * kKept; e0 < a.entries; e0 += 64)
     if (look(e0, entry_at(a, e0 + lane, rep))) return found;
+  found.base = base;
   return found;
 }
 
@@ -988,7 +989,9 @@ __global__ __launch_bounds__(64, (Shape<E, D>::kOcc)) void paged_few_kernel(Page
   if (it.valid) few_columns<E, D>(a, it, rep, lane, lds_addr_of(lds), table, gsm);
 }
 
-// Any launch: a workgroup is an item of many columns, or four of few
+// Any launch: the first workgroups are items of many columns, the next four items each of few, the rest have none.  (With a fixed number
+// of workgroups for the first kind those without an item kept the second kind
+// waiting: 128 rows beside 15 tokens 45.9 us, now 40.4.)
 template <typename E, int D>
 __global__ __launch_bounds__(256, (Shape<E, D>::kOcc)) void paged_any_kernel(PagedArgs a) {
   using S = Shape<E, D>;
@@ -1004,12 +1007,12 @@ __global__ __launch_bounds__(256, (Shape<E, D>::kOcc)) void paged_any_kernel(Pag
   const Entries mine = load_entries(a, lane, rep);
   const Shares share = share_blocks(a, lane, rep, mine);
   if (blockIdx.x == 0 && threadIdx.x == 0) { a.lens[0] = share.few; a.lens[1] = share.many; }
-  if ((int)blockIdx.x < a.n_many) {
-    const Item it = locate<true>(a, lane, rep, share, mine, blockIdx.x);
+  const Item it = locate<true>(a, lane, rep, share, mine, blockIdx.x);
+  if (it.x.entry >= 0) {
     if (it.valid) many_columns<E, D>(a, it, rep, tid, lds_addr_of(lds), table, gsm[0], any_bad);
   } else {
-    const Item it = locate<false>(a, lane, rep, share, mine, ((int)blockIdx.x - a.n_many) * 4 + wave);
-    if (it.valid) few_columns<E, D>(a, it, rep, lane, lds_addr_of(lds) + wave * S::kDepth * S::kFewBytes, table + wave * (S::kFewTable + 2), gsm[wave]);
+    const Item it4 = locate<false>(a, lane, rep, share, mine, ((int)blockIdx.x - it.x.base) * 4 + wave);
+    if (it4.valid) few_columns<E, D>(a, it4, rep, lane, lds_addr_of(lds) + wave * S::kDepth * S::kFewBytes, table + wave * (S::kFewTable + 2), gsm[wave]);
   }
 }
 
@@ -1127,7 +1130,12 @@ size_t plan(const segpt_paged_params& p, PagedArgs& a) {
   a.each.set(p.seq_start ? 1 : a.rows_each);
   a.log_page = __builtin_ctz((unsigned)p.page_size);
   a.capacity = paged_capacity(p);
-  a.target = 256 * (row_bytes <= 256 ? 2 : 1);
+  // Two workgroups a CU are resident.  Where the host sees that the work is of many columns (a prefix, prompts of equal length) three on two
+  // CUs: longer shares leave a quarter less to be joined, which is more than what the idle places would have done (us, 512 and 384: 128 tokens
+  // behind a prefix of 16001, 16 / 4 heads of 128, 50.1, 47.6; 32 behind 8192, 18 / 6 of 64, 23.3, 21.7; a prompt of 1024 tokens 32.0, 29.7, of
+  // 2048 42.0, 39.6).  Tokens want all of them (a chunk of 512 rows beside 63 tokens: 123, 143).
+  const bool wide = a.shared || (!p.seq_start && (int64_t)rep * a.rows_each > kFew);
+  a.target = row_bytes > 256 ? 256 : wide ? 384 : 512;
   a.min_few = 2;
   a.min_many = 4;
   // Tiles: whole ones of the columns there are, and one begun an entry.  Items: a tile's part of what the target stands for, and one begun.

@@ -250,12 +250,16 @@ struct Shape {
 // a lane.  bf16: element 16 ks + 8 hh + t; fp32: chunk 2 c + hh of four.  fetch() asks for the row and its angles, no branch between (without
 // a rotation the row's own bytes stand in for the angles and are not used), so that they are on their way with the page numbers; finish()
 // makes the operand of them.  (Fetched where they are needed they took 7500 of an item's 25000 cycles: two round trips behind the tiles.)
-template <typename E, int D>
+// FINE: bf16 with a second operand, what the first one's rounding left, so that scores are as good as the pool's keys.  FEW has it: its matrix
+// pipe is idle (a block's products are 400 cycles of the 4400 that its bytes take), and its error against 64 bits goes down from 2.8e-3 to
+// 2.3e-3 of y, of which 1.7e-3 is y's own rounding.  In MANY the further products would be a quarter of the loop; there the query is rounded once,
+// as in the other forward kernels.
+template <typename E, int D, bool FINE>
 struct Query;
-template <int D>
-struct Query<uint16_t, D> {
+template <int D, bool FINE>
+struct Query<uint16_t, D, FINE> {
   static constexpr int KS = D / 16;
-  bf16x8 reg[KS];
+  bf16x8 reg[KS], rest[FINE ? KS : 1];
   u32x4 raw[KS];
   f32x4 cs[KS], sn[KS];
   __device__ __forceinline__ void fetch(const segpt_paged_params& p, const uint16_t* row, int64_t angle, int hh) {
@@ -289,15 +293,20 @@ struct Query<uint16_t, D> {
     for (int ks = 0; ks < KS; ++ks) {
       const float4 ga = *reinterpret_cast<const float4*>(gsm + 16 * ks + 8 * hh), gb = *reinterpret_cast<const float4*>(gsm + 16 * ks + 8 * hh + 4);
       const float g[8] = {ga.x, ga.y, ga.z, ga.w, gb.x, gb.y, gb.z, gb.w};
-      u32x4 w;
+      u32x4 w, r;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = live ? pack_bf16x2(x[ks][2 * i] * alpha * g[2 * i], x[ks][2 * i + 1] * alpha * g[2 * i + 1]) : 0u;
+      for (int i = 0; i < 4; ++i) {
+        const float a = x[ks][2 * i] * alpha * g[2 * i], b = x[ks][2 * i + 1] * alpha * g[2 * i + 1];
+        w[i] = live ? pack_bf16x2(a, b) : 0u;
+        if constexpr (FINE) r[i] = live ? pack_bf16x2(a - bf16lo(w[i]), b - bf16hi(w[i])) : 0u;
+      }
       reg[ks] = as_bf16x8(w);
+      if constexpr (FINE) rest[ks] = as_bf16x8(r);
     }
   }
 };
-template <int D>
-struct Query<float, D> {
+template <int D, bool FINE>
+struct Query<float, D, FINE> {
   static constexpr int C = D / 8;
   float reg[C][4];
   f32x4 cs[C / 2], sn[C / 2];
@@ -470,8 +479,8 @@ struct Column {
   int lim;       // last key of the lane's row
   int all, any;  // last key that all columns of the wave see, that any of them sees
 };
-template <typename E, int D>
-__device__ __forceinline__ Column column_of(const PagedArgs& a, const Item& it, int rep, int wave_col, int lane, Query<E, D>& q) {
+template <typename E, int D, bool FINE>
+__device__ __forceinline__ Column column_of(const PagedArgs& a, const Item& it, int rep, int wave_col, int lane, Query<E, D, FINE>& q) {
   const segpt_paged_params& p = a.p;
   Column c;
   const bool works = wave_col < it.cols;
@@ -518,7 +527,12 @@ struct Keys<uint16_t, D> {
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) k[ks] = swz_frag_rm<D>(tile + swz_off_rm<D>(lane), 0, ks);
   }
-  __device__ __forceinline__ f32x16 scores(const Query<uint16_t, D>& q, f32x16 s) const {
+  template <bool FINE>
+  __device__ __forceinline__ f32x16 scores(const Query<uint16_t, D, FINE>& q, f32x16 s) const {
+    if constexpr (FINE) {
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) s = mfma32(k[ks], q.rest[ks], s);
+    }
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) s = mfma32(k[ks], q.reg[ks], s);
     return s;
@@ -533,7 +547,8 @@ struct Keys<float, D> {
 #pragma unroll
     for (int c = 0; c < D / 8; ++c) k[c] = lds_read_f4(row + (((2 * c + hh) ^ fx) << 4));
   }
-  __device__ __forceinline__ f32x16 scores(const Query<float, D>& q, f32x16 s) const {
+  template <bool FINE>
+  __device__ __forceinline__ f32x16 scores(const Query<float, D, FINE>& q, f32x16 s) const {
 #pragma unroll
     for (int c = 0; c < D / 8; ++c)
 #pragma unroll
@@ -751,8 +766,8 @@ __device__ __forceinline__ void few_columns(const PagedArgs& a, const Item& it, 
   Gain gain[(D + 63) / 64];
 #pragma unroll
   for (int i = 0; i < (D + 63) / 64; ++i) gain[i] = fetch_gain(a.p, (64 * i + lane) % D);
-  Query<E, D> q;
-  const Column c = column_of<E, D>(a, it, rep, it.tile * kFew, lane, q);
+  Query<E, D, true> q;
+  const Column c = column_of(a, it, rep, it.tile * kFew, lane, q);
   bool bad = it.x.broken | stage_table(a, it, rq.w0, rq.wn, table, lane, 64);
 #pragma unroll
   for (int i = 0; i < (D + 63) / 64; ++i)
@@ -848,8 +863,8 @@ __device__ __forceinline__ void many_columns(const PagedArgs& a, const Item& it,
   };
   // one round trip: gain, query row and angles, page numbers
   const Gain gain = fetch_gain(a.p, tid % D);
-  Query<E, D> q;
-  const Column c = column_of<E, D>(a, it, rep, it.tile * kMany + wave * 32, lane, q);
+  Query<E, D, false> q;
+  const Column c = column_of(a, it, rep, it.tile * kMany + wave * 32, lane, q);
   stage_pages();
   if (tid < D) gsm[tid] = scale_of(a.p, gain);
   __syncthreads();

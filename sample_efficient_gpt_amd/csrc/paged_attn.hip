@@ -837,6 +837,8 @@ __device__ __forceinline__ void few_columns(const PagedArgs& a, const Item& it, 
 // scores of tile jt + 1 beside the exponentials of tile jt and its product with the values, so that the matrix pipe has work while
 // the exponentials are formed.  Per turn: wait for tile jt + 1, barrier (also: everyone has left tile jt - 1), request tile jt + kStages - 1 over
 // that one, compute.
+// Bound by the vector port beside the matrix pipe (12 vector instructions a matrix instruction): a prompt of 8192 tokens, 18 / 6 heads of 64,
+// 195 us (790 TFLOP/s); short shares by their start, about 10 us until the first products.
 template <typename E, int D>
 __device__ __forceinline__ void many_columns(const PagedArgs& a, const Item& it, int rep, int tid, uint32_t lds, int* table, float* gsm, int* any_bad) {
   using S = Shape<E, D>;
@@ -988,7 +990,9 @@ __device__ __forceinline__ void clear_rest(const PagedArgs& a, int tid, int thre
   }
 }
 
-// Launches whose entries are all FEW: a workgroup is one wave
+// Launches whose entries are all FEW: a workgroup is one wave, eight a CU (twelve: the same work in more shares, 49.6 -> 52.5 us).  Bound by HBM:
+// 32 tokens, 200 .. 8192 keys, 18 / 6 heads of 64: 213 MB in 44 us (4.8 TB/s); 48 tokens, 255 .. 16000 keys, 16 / 4 heads of 128: 803 MB in 147 us
+// (5.4 TB/s).  A single token's 4096 keys take 8.7 us: launch and three dependent round trips (lengths, page numbers, keys); the plan's arithmetic is 0.3.
 template <typename E, int D>
 __global__ __launch_bounds__(64, (Shape<E, D>::kOcc)) void paged_few_kernel(PagedArgs a) {
   using S = Shape<E, D>;
@@ -1033,7 +1037,8 @@ __global__ __launch_bounds__(256, (Shape<E, D>::kOcc)) void paged_any_kernel(Pag
 
 // Joins the partial results of `per_sub` columns of a tile: its sequence's shares and, behind them, the prefix's.  A unit of D / 4 lanes holds a
 // row; as many units stand side by side over the shares of a column as leave each one batch of kBatch that is requested together, and
-// their sums meet in LDS.  Fixed order: deterministic.
+// their sums meet in LDS.  Fixed order: deterministic.  4.6 us for one token of 18 heads (launch and two round trips), 5.8 for 32 of them, 12 for
+// 128 tokens of 16 heads of 128 behind a prefix (25 MB).
 constexpr int kMergeThreads = 256;
 template <typename E, int D>
 __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedArgs a, int subs, int per_sub) {

@@ -245,6 +245,8 @@ class MultiHeadSelfAttention(nn.Module):
         v_first = vr_coef = None
         v_rows = v if v1 is None or self.always_return_values else None
         if self.value_residual:
+            if v1 is not None and v1.shape != (b, Hkv, S, d):
+                raise ValueError(f"with a paged cache v1 is what the first layer handed on for these rows, {(b, Hkv, S, d)}, got {tuple(v1.shape)}")
             v_first = v if v1 is None else v1.permute(0, 2, 1, 3).reshape(v.shape)
             vr_coef = self._mix_coefficients()
             if v_rows is not None:

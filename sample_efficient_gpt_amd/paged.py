@@ -56,6 +56,21 @@ def _(q, k_pages, v_pages, prefix_table, prefix_len, block_table, kv_len, g_q, g
     return [q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)]
 
 
+@torch.library.custom_op("segpt::paged_attention_out", mutates_args=("out",))
+def _attend_out_op(out: Tensor, q: Tensor, k_pages: Tensor, v_pages: Tensor, prefix_table: Optional[Tensor], prefix_len: int, block_table: Tensor,
+                   kv_len: Tensor, g_q: Tensor, g_k: Optional[Tensor], seq_start: Optional[Tensor], gate_logits: Optional[Tensor], gate_scale: float,
+                   eps: float, sm_scale: float, qk_norm: bool, rope_cos: Optional[Tensor], rope_sin: Optional[Tensor], rope_pos0: int,
+                   max_len: Optional[int]) -> Tensor:
+    return _native.load().paged_attention(q, k_pages, v_pages, prefix_table, prefix_len, block_table, kv_len, g_q, g_k, seq_start, gate_logits,
+                                          gate_scale, eps, sm_scale, qk_norm, rope_cos, rope_sin, rope_pos0, max_len, out, True)[1]
+
+
+@_attend_out_op.register_fake
+def _(out, q, k_pages, v_pages, prefix_table, prefix_len, block_table, kv_len, g_q, g_k, seq_start, gate_logits, gate_scale, eps, sm_scale, qk_norm,
+      rope_cos, rope_sin, rope_pos0, max_len):
+    return q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
 def paged_kv_append(k, v, k_pages, v_pages, block_table, kv_len, *, seq_start=None, v_first=None, vr_coef=None, eps=1e-6, qk_norm=True,
                     rope_cos=None, rope_sin=None, rope_pos0=0, max_len=None):
     """Writes the rows k, v ``[T, Hkv, D]`` (any strides, last dim contiguous, rows 16 B aligned) into the pages of their sequences.
@@ -86,11 +101,12 @@ def _attend(q, k_pages, v_pages, prefix_table, prefix_len, block_table, kv_len, 
         y, lse = _native.load().paged_attention(q, k_pages, v_pages, prefix_table, prefix_len, block_table, kv_len, g_q, g_k, seq_start, gate_logits,
                                                 gate_scale, eps, sm_scale, qk_norm, rope_cos, rope_sin, rope_pos0, max_len, out, return_lse)
         return (y, lse) if return_lse else y
-    y, lse = torch.ops.segpt.paged_attention(q, k_pages, v_pages, prefix_table, int(prefix_len), block_table, kv_len, g_q, g_k, seq_start, gate_logits,
-                                             float(gate_scale), float(eps), float(1.0 / math.sqrt(q.shape[-1]) if sm_scale is None else sm_scale),
-                                             bool(qk_norm), rope_cos, rope_sin, int(rope_pos0), max_len)
-    if out is not None:
-        y = out.copy_(y)
+    args = (q, k_pages, v_pages, prefix_table, int(prefix_len), block_table, kv_len, g_q, g_k, seq_start, gate_logits, float(gate_scale), float(eps),
+            float(1.0 / math.sqrt(q.shape[-1]) if sm_scale is None else sm_scale), bool(qk_norm), rope_cos, rope_sin, int(rope_pos0), max_len)
+    if out is None:
+        y, lse = torch.ops.segpt.paged_attention(*args)
+    else:  # rows in no sequence are left as they are
+        y, lse = out, torch.ops.segpt.paged_attention_out(out, *args)
     return (y, lse) if return_lse else y
 
 

@@ -547,3 +547,55 @@ def test_further_refusals(gpu_device):
     paged_kv_append(x.k, x.v, both[:, 0], both[:, 1], x.block_table, x.kv_len, **kw)
     paged_kv_append(x.k, x.v, x.k_pages, x.v_pages, x.block_table, x.kv_len, **kw)
     assert torch.equal(both[:, 0], x.k_pages) and torch.equal(both[:, 1], x.v_pages)
+
+
+def test_as_an_operator_with_out(gpu_device):
+    """Rows in no sequence keep what they held, also where the call is a node of a graph."""
+    x = Batch([1, 9, 3], [40, 20, 30], 6, 2, 64, 16, BF16, gpu_device, seed=27)
+    x.seq_start = torch.tensor([1, 2, 11, 12], dtype=torch.int32, device=gpu_device)
+
+    def f(q, out):
+        y, lse = paged_attention(q * 1, x.k_pages, x.v_pages, x.block_table, x.kv_len, x.g_q, seq_start=x.seq_start, rope_cos=x.cos, rope_sin=x.sin,
+                                 out=out, return_lse=True)
+        return y * 2, lse
+
+    eager, traced = torch.full_like(x.q, 7.0), torch.full_like(x.q, 7.0)
+    with torch.no_grad():
+        want = f(x.q, eager)
+        got = torch.compile(f, backend="aot_eager", fullgraph=True)(x.q, traced)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(traced, eager)
+    assert (traced[[0, 12]] == 7).all() and not (traced[1:12] == 7).all()
+
+
+def test_module_refuses_other_values(gpu_device):
+    m = MultiHeadSelfAttention(384, 6, 2, max_seq_len=64, qknorm=True, value_residual=True, device=gpu_device, dtype=BF16)
+    pages = PageTable(2, 64, 16, device=gpu_device)
+    cache = PagedKVCache(pages, 2, 64)
+    x = torch.randn(2, 5, 384, device=gpu_device).to(BF16)
+    pages.extend(5)
+    with torch.no_grad(), pytest.raises(ValueError, match="v1"):
+        m(x, v1=torch.zeros(2, 6, 5, 64, device=gpu_device, dtype=BF16), kv_cache=cache)
+
+
+def test_a_very_long_sequence(gpu_device):
+    x = Batch([1, 2], [400_003, 5], 4, 2, 64, 64, BF16, gpu_device, seed=28)
+    y, lse = attend(x, return_lse=True)
+    check_y(x, y, lse, x.attended())
+    z = Batch([1, 40], [3, 50], 4, 2, 64, 64, BF16, gpu_device, seed=29, prefix=200_001)
+    y, lse = attend(z, return_lse=True)
+    check_y(z, y, lse, z.attended())
+
+
+@pytest.mark.parametrize("H,Hkv,D,dtype", [(6, 2, 64, BF16), (4, 2, 128, BF16), (4, 2, 64, F32)])
+def test_a_long_prompt_is_the_contiguous_attention(gpu_device, H, Hkv, D, dtype):
+    """10007 rows, appended and attended in pages, against the attention over contiguous keys (its own roundings: as many again)."""
+    from sample_efficient_gpt_amd import qknorm_attention
+
+    n = 10_007
+    x = Batch([n], [n], H, Hkv, D, 32, dtype, gpu_device, seed=30)
+    append(x)
+    y = attend(x)
+    with torch.no_grad():
+        dense = qknorm_attention(*(t.transpose(0, 1)[None] for t in (x.q, x.k, x.v)), x.g_q, eps=EPS, rope_cos=x.cos, rope_sin=x.sin)
+    dense = dense[0].transpose(0, 1).double()
+    assert (y.double() - dense).norm() <= (1.2e-2 if dtype == BF16 else 1e-5) * dense.norm()

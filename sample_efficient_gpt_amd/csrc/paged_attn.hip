@@ -500,7 +500,7 @@ __device__ __forceinline__ Column column_of(const PagedArgs& a, const Item& it, 
       b = a.each.of(c.t);
     }
     sequence_rows(p, a.rows_each, b, &f, &n);
-    own = (int)min((int64_t)p.kv_len[b] - n + (c.t - f), (int64_t)a.capacity - 1);
+    own = (int)max(min((int64_t)p.kv_len[b] - n + (c.t - f), (int64_t)a.capacity - 1), -1 - (int64_t)p.prefix_len);  // whatever the length says
   }
   const int64_t pos = max((int64_t)p.prefix_len + own, (int64_t)0);
   q.fetch(p, row_of<E>(p.q, c.t, c.h), (p.rope_pos0 + pos) * (D / 2), lane >> 5);

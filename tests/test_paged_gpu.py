@@ -599,3 +599,17 @@ def test_a_long_prompt_is_the_contiguous_attention(gpu_device, H, Hkv, D, dtype)
         dense = qknorm_attention(*(t.transpose(0, 1)[None] for t in (x.q, x.k, x.v)), x.g_q, eps=EPS, rope_cos=x.cos, rope_sin=x.sin)
     dense = dense[0].transpose(0, 1).double()
     assert (y.double() - dense).norm() <= (1.2e-2 if dtype == BF16 else 1e-5) * dense.norm()
+
+
+@pytest.mark.parametrize("prefix", [0, 70])
+@pytest.mark.parametrize("uniform", [False, True])
+def test_lengths_at_the_ends_of_32_bits(gpu_device, prefix, uniform):
+    """A length that is no length at all: NaN in that sequence's rows, nothing elsewhere, and nothing outside the tensors is read."""
+    x = Batch([2, 2, 2, 2], [9, 40, 30, 2], 6, 2, 64, 16, BF16, gpu_device, seed=31, prefix=prefix, uniform=uniform)
+    clean = attend(x)
+    x.kv_len[1], x.kv_len[2] = -(2**31), 2**31 - 1
+    y = attend(x)
+    assert y[2:6].isnan().all() and torch.equal(y[:2], clean[:2]) and torch.equal(y[6:], clean[6:])
+    before = x.k_pages.clone()
+    append(x, rope_pos0=prefix)
+    assert int((x.k_pages != before).any(-1).any(1).sum()) == 4  # slots of the two sequences that have a length

@@ -1150,12 +1150,15 @@ size_t plan(const segpt_paged_params& p, PagedArgs& a) {
   a.each.set(p.seq_start ? 1 : a.rows_each);
   a.log_page = __builtin_ctz((unsigned)p.page_size);
   a.capacity = paged_capacity(p);
-  // Two workgroups a CU are resident.  Where the host sees that the work is of many columns (a prefix, prompts of equal length) three on two
-  // CUs: longer shares leave a quarter less to be joined, which is more than what the idle places would have done (us, 512 and 384: 128 tokens
-  // behind a prefix of 16001, 16 / 4 heads of 128, 50.1, 47.6; 32 behind 8192, 18 / 6 of 64, 23.3, 21.7; a prompt of 1024 tokens 32.0, 29.7, of
-  // 2048 42.0, 39.6).  Tokens want all of them (a chunk of 512 rows beside 63 tokens: 123, 143).
+  // 512 workgroups are resident, two a CU.  The shares' length is found in three steps and may leave a few more than asked for, and one that has to wait
+  // for a place is a round of its own: 480 are asked for, 496 where all are single waves (us, asked for 512 and now: 512 rows beside 31 tokens
+  // 79.5, 64; beside 63 126, 105; beside 15 52.7, 52.4; 128 rows beside 15 39.6, 42.5; eight fp32 tokens 20.0, 18.1; 128 of bf16 179, 175).  Where the host sees that the work
+  // is of many columns (a prefix, prompts of equal length) three on two CUs: longer shares leave a quarter less to be joined, which is more than
+  // the idle places would have done (480 and 384: 128 tokens behind a prefix of 16001, 16 / 4 heads of 128, 51.5, 48.7; 32 behind 8192,
+  // 18 / 6 of 64, 23.6, 22.0; 512 and 384: a prompt of 1024 tokens 32.0, 29.7, of 2048 42.0, 39.6).  fp32 rows of 512 bytes: one a CU, all of them
+  // (fewer: 32 tokens 77, 80; 100 118, 129).
   const bool wide = a.shared || (!p.seq_start && (int64_t)rep * a.rows_each > kFew);
-  a.target = row_bytes > 256 ? 256 : wide ? 384 : 512;
+  a.target = row_bytes > 256 ? 256 : wide ? 384 : p.seq_start ? 480 : 496;
   a.min_few = 2;
   a.min_many = 4;
   // Tiles: whole ones of the columns there are, and one begun an entry.  Items: a tile's part of what the target stands for, and one begun.

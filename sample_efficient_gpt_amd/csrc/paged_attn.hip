@@ -60,7 +60,7 @@ struct PagedArgs {
   int32_t n_many, n_few;          // items there may be of either kind
   int32_t n_joins;                // tiles and kv heads whose partial results there may be to join
   int32_t n_slots;                // partial results there is room for, 32 columns each
-  int32_t* lens;                  // blocks of a share (few, many), left for the merge by workgroup 0
+  int32_t* lens;                  // blocks of a share (few, many) and tiles and kv heads to join, left for the merge
   float* part;                    // [n_slots][32][D]
   float2* stat;                   // [n_slots][32]
 };
@@ -990,6 +990,13 @@ __device__ __forceinline__ void clear_rest(const PagedArgs& a, int tid, int thre
   }
 }
 
+// What the merge goes by, from the last workgroup, which mostly has no item
+__device__ __forceinline__ void leave_plan(const PagedArgs& a, int lane, int rep, const Shares& share, const Entries& mine) {
+  if (blockIdx.x != gridDim.x - 1) return;
+  const int joins = find_entry<kFindJoin>(a, lane, rep, share, mine, INT32_MAX).base;
+  if (threadIdx.x == 0) { a.lens[0] = share.few; a.lens[1] = share.many; a.lens[2] = joins; }
+}
+
 // Launches whose entries are all FEW: a workgroup is one wave, eight a CU (twelve: the same work in more shares, 49.6 -> 52.5 us).  Bound by HBM:
 // 32 tokens, 200 .. 8192 keys, 18 / 6 heads of 64: 213 MB in 44 us (4.8 TB/s); 48 tokens, 255 .. 16000 keys, 16 / 4 heads of 128: 803 MB in 147 us
 // (5.4 TB/s).  A single token's 4096 keys take 8.7 us: launch and three dependent round trips (lengths, page numbers, keys); the plan's arithmetic is 0.3.
@@ -1003,7 +1010,7 @@ __global__ __launch_bounds__(64, (Shape<E, D>::kOcc)) void paged_few_kernel(Page
   clear_rest<E>(a, lane, 64, D);
   const Entries mine = load_entries(a, lane, rep);
   const Shares share = share_blocks(a, lane, rep, mine);
-  if (blockIdx.x == 0 && threadIdx.x == 0) { a.lens[0] = share.few; a.lens[1] = share.many; }
+  leave_plan(a, lane, rep, share, mine);
   const Item it = locate<false>(a, lane, rep, share, mine, blockIdx.x);
   if (it.valid) few_columns<E, D>(a, it, rep, lane, lds_addr_of(lds), table, gsm);
 }
@@ -1025,7 +1032,7 @@ __global__ __launch_bounds__(256, (Shape<E, D>::kOcc)) void paged_any_kernel(Pag
   clear_rest<E>(a, tid, 256, D);
   const Entries mine = load_entries(a, lane, rep);
   const Shares share = share_blocks(a, lane, rep, mine);
-  if (blockIdx.x == 0 && threadIdx.x == 0) { a.lens[0] = share.few; a.lens[1] = share.many; }
+  leave_plan(a, lane, rep, share, mine);
   const Item it = locate<true>(a, lane, rep, share, mine, blockIdx.x);
   if (it.x.entry >= 0) {
     if (it.valid) many_columns<E, D>(a, it, rep, tid, lds_addr_of(lds), table, gsm[0], any_bad);
@@ -1048,10 +1055,11 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedArgs a,
   __shared__ float2 stats[kUnits];
   const int tid = threadIdx.x, lane = tid & 63, unit = tid / LPR, c = tid % LPR;
   const int rep = a.rep.d;
-  const int few = a.lens[0], many = a.lens[1];
+  const int few = a.lens[0], many = a.lens[1], joins = a.lens[2];
   const Entries mine = load_entries(a, lane, rep);
-  const Shares share = shares_from(few, many);
   const int which = blockIdx.x / subs, sub = blockIdx.x - which * subs;
+  if (which >= joins) return;
+  const Shares share = shares_from(few, many);
   const Found own = find_entry<kFindJoin>(a, lane, rep, share, mine, which);
   if (own.entry < 0) return;
   const int tile = a.hkv.of(which - own.base), g = which - own.base - tile * p.Hkv, cols = own.n * rep, tile_cols = own.many ? kMany : kFew;

@@ -246,20 +246,32 @@ struct Shape {
   static constexpr int kOcc = kRB > 256 ? 1 : 2;  // workgroups of four waves per CU
 };
 
+// A pair of values in two bf16 parts each.  The first is cut off, a little below the value in size and never the value itself, so that the second has
+// the same sign and is not zero: the products of both with an infinity are that infinity, not NaN.  The second is at most 2^-7 + 2^-9 of the
+// value and exact in fp32; what its rounding leaves out is less than 2^-14 of the value.
+__device__ __forceinline__ void two_parts(float a, float b, uint32_t& first, uint32_t& second) {
+  constexpr float kBelow = 1.f - 0x1p-9f;
+  const uint32_t x = __float_as_uint(a * kBelow) & 0xffff0000u, y = __float_as_uint(b * kBelow) & 0xffff0000u;
+  first = x >> 16 | y;
+  second = pack_bf16x2(a - __uint_as_float(x), b - __uint_as_float(y));
+}
+
 // Query columns in the B operand's layout, scaled by everything that does not depend on the key (gsm: g_q g_k sm_scale log2 e); D / 2 values
 // a lane.  bf16: element 16 ks + 8 hh + t; fp32: chunk 2 c + hh of four.  fetch() asks for the row and its angles, no branch between (without
 // a rotation the row's own bytes stand in for the angles and are not used), so that they are on their way with the page numbers; finish()
 // makes the operand of them.  (Fetched where they are needed they took 7500 of an item's 25000 cycles: two round trips behind the tiles.)
-// FINE: bf16 with a second operand, what the first one's rounding left, so that scores are as good as the pool's keys.  FEW has it: its matrix
-// pipe is idle (a block's products are 400 cycles of the 4400 that its bytes take), and its error against 64 bits goes down from 2.8e-3 to
-// 2.3e-3 of y, of which 1.7e-3 is y's own rounding.  In MANY the further products cost what they are (six prompts of 333 .. 4096 tokens, 18 / 6 heads
-// of 64: 148 us, with them 168): there the query is rounded once, as in the other forward kernels.
-template <typename E, int D, bool FINE>
+// bf16 has a second operand, what the first one's rounding left, so that scores are as good as the pool's keys.  With one operand, and probabilities
+// rounded once, the error against 64 bits is 2.9e-3 of y, of which 1.7e-3 is y's own rounding: more than one and a half times what it has to be.
+// In FEW the further products are hidden (a block's products are 400 cycles of the 4400 that its bytes take).  In MANY they cost what they are: six
+// prompts of 333 .. 4096 tokens, 18 / 6 heads of 64, 148 -> 171 us (2.5e-3 -> 2.1e-3), with 16 / 4 of 128 213 -> 266; 512 rows beside 15 tokens 56 -> 62
+// (2.9e-3 -> 2.3e-3); 128 tokens behind 16001 keys, 16 / 4 heads of 128, 50 -> 58 (2.9e-3 -> 2.3e-3); 32 behind 8192 20.6 -> 21.1.  The probabilities in
+// two parts instead: 188, 268, 67, 54 and 21.4, the same errors.
+template <typename E, int D>
 struct Query;
-template <int D, bool FINE>
-struct Query<uint16_t, D, FINE> {
+template <int D>
+struct Query<uint16_t, D> {
   static constexpr int KS = D / 16;
-  bf16x8 reg[KS], rest[FINE ? KS : 1];
+  bf16x8 reg[KS], rest[KS];
   u32x4 raw[KS];
   f32x4 cs[KS], sn[KS];
   __device__ __forceinline__ void fetch(const segpt_paged_params& p, const uint16_t* row, int64_t angle, int hh) {
@@ -296,17 +308,18 @@ struct Query<uint16_t, D, FINE> {
       u32x4 w, r;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float a = x[ks][2 * i] * alpha * g[2 * i], b = x[ks][2 * i + 1] * alpha * g[2 * i + 1];
-        w[i] = live ? pack_bf16x2(a, b) : 0u;
-        if constexpr (FINE) r[i] = live ? pack_bf16x2(a - bf16lo(w[i]), b - bf16hi(w[i])) : 0u;
+        uint32_t first, second;
+        two_parts(x[ks][2 * i] * alpha * g[2 * i], x[ks][2 * i + 1] * alpha * g[2 * i + 1], first, second);
+        w[i] = live ? first : 0u;
+        r[i] = live ? second : 0u;
       }
       reg[ks] = as_bf16x8(w);
-      if constexpr (FINE) rest[ks] = as_bf16x8(r);
+      rest[ks] = as_bf16x8(r);
     }
   }
 };
-template <int D, bool FINE>
-struct Query<float, D, FINE> {
+template <int D>
+struct Query<float, D> {
   static constexpr int C = D / 8;
   float reg[C][4];
   f32x4 cs[C / 2], sn[C / 2];
@@ -479,8 +492,8 @@ struct Column {
   int lim;       // last key of the lane's row
   int all, any;  // last key that all columns of the wave see, that any of them sees
 };
-template <typename E, int D, bool FINE>
-__device__ __forceinline__ Column column_of(const PagedArgs& a, const Item& it, int rep, int wave_col, int lane, Query<E, D, FINE>& q) {
+template <typename E, int D>
+__device__ __forceinline__ Column column_of(const PagedArgs& a, const Item& it, int rep, int wave_col, int lane, Query<E, D>& q) {
   const segpt_paged_params& p = a.p;
   Column c;
   const bool works = wave_col < it.cols;
@@ -527,12 +540,9 @@ struct Keys<uint16_t, D> {
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) k[ks] = swz_frag_rm<D>(tile + swz_off_rm<D>(lane), 0, ks);
   }
-  template <bool FINE>
-  __device__ __forceinline__ f32x16 scores(const Query<uint16_t, D, FINE>& q, f32x16 s) const {
-    if constexpr (FINE) {
+  __device__ __forceinline__ f32x16 scores(const Query<uint16_t, D>& q, f32x16 s) const {
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) s = mfma32(k[ks], q.rest[ks], s);
-    }
+    for (int ks = 0; ks < D / 16; ++ks) s = mfma32(k[ks], q.rest[ks], s);
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) s = mfma32(k[ks], q.reg[ks], s);
     return s;
@@ -547,8 +557,7 @@ struct Keys<float, D> {
 #pragma unroll
     for (int c = 0; c < D / 8; ++c) k[c] = lds_read_f4(row + (((2 * c + hh) ^ fx) << 4));
   }
-  template <bool FINE>
-  __device__ __forceinline__ f32x16 scores(const Query<float, D, FINE>& q, f32x16 s) const {
+  __device__ __forceinline__ f32x16 scores(const Query<float, D>& q, f32x16 s) const {
 #pragma unroll
     for (int c = 0; c < D / 8; ++c)
 #pragma unroll
@@ -587,13 +596,40 @@ struct Values<uint16_t, D> {
       }
     return all != ~0u;
   }
-  // adds the probabilities s to the sums l, as they are rounded, and their products with the values to o
+  // Adds the probabilities s to the sums l and their products with the values to o.  FINE: in two bf16 parts, so that y's own rounding is all its error
+  // (2.3e-3 of y -> 1.65e-3).  FEW has it beside its loads (32 tokens of 200 .. 8192 keys 44.3 -> 44.7 us, 48 of 255 .. 16000 153 -> 155); in MANY,
+  // where the vector port is what is short, the prompts above would take 214 us instead of 169: there they are rounded once and summed as rounded.
+  template <bool FINE>
   __device__ __forceinline__ void add(f32x16 s, float (&l)[2], f32x16 (&o)[MB]) const {
-    const bf16x8 pb[2] = {pack_c_half_sum(s, 0, l), pack_c_half_sum(s, 1, l)};
+    bf16x8 pb[2], rest[2];
+    if constexpr (FINE) {
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) {
+        u32x4 w, r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float a = s[8 * s2 + 2 * i], b = s[8 * s2 + 2 * i + 1];
+          uint32_t first, second;
+          two_parts(a, b, first, second);
+          w[i] = first;
+          r[i] = second;
+          l[0] += a;
+          l[1] += b;
+        }
+        pb[s2] = as_bf16x8(w);
+        rest[s2] = as_bf16x8(r);
+      }
+    } else {
+      pb[0] = pack_c_half_sum(s, 0, l);
+      pb[1] = pack_c_half_sum(s, 1, l);
+    }
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb) o[mb] = mfma32(as_bf16x8(v[mb][s2]), pb[s2], o[mb]);
+      for (int mb = 0; mb < MB; ++mb) {
+        if constexpr (FINE) o[mb] = mfma32(as_bf16x8(v[mb][s2]), rest[s2], o[mb]);
+        o[mb] = mfma32(as_bf16x8(v[mb][s2]), pb[s2], o[mb]);
+      }
   }
 };
 template <int D>
@@ -621,6 +657,7 @@ struct Values<float, D> {
       }
     return odd;
   }
+  template <bool FINE>
   __device__ __forceinline__ void add(f32x16 s, float (&l)[2], f32x16 (&o)[MB]) const {
 #pragma unroll
     for (int r = 0; r < 16; ++r) l[r & 1] += s[r];
@@ -766,7 +803,7 @@ __device__ __forceinline__ void few_columns(const PagedArgs& a, const Item& it, 
   Gain gain[(D + 63) / 64];
 #pragma unroll
   for (int i = 0; i < (D + 63) / 64; ++i) gain[i] = fetch_gain(a.p, (64 * i + lane) % D);
-  Query<E, D, true> q;
+  Query<E, D> q;
   const Column c = column_of(a, it, rep, it.tile * kFew, lane, q);
   bool bad = it.x.broken | stage_table(a, it, rq.w0, rq.wn, table, lane, 64);
 #pragma unroll
@@ -819,7 +856,7 @@ __device__ __forceinline__ void few_columns(const PagedArgs& a, const Item& it, 
       if (masked) odd |= v.clear();
       wave_sync();
       if (left >= DEPTH) rq.template issue<true>(jt + DEPTH, vt);
-      v.add(s[0], st.l, st.o);
+      v.template add<true>(s[0], st.l, st.o);
       buffer = buffer == DEPTH - 1 ? 0 : buffer + 1;
     }
     rq.w0 += window;
@@ -865,7 +902,7 @@ __device__ __forceinline__ void many_columns(const PagedArgs& a, const Item& it,
   };
   // one round trip: gain, query row and angles, page numbers
   const Gain gain = fetch_gain(a.p, tid % D);
-  Query<E, D, false> q;
+  Query<E, D> q;
   const Column c = column_of(a, it, rep, it.tile * kMany + wave * 32, lane, q);
   stage_pages();
   if (tid < D) gsm[tid] = scale_of(a.p, gain);
@@ -925,7 +962,7 @@ __device__ __forceinline__ void many_columns(const PagedArgs& a, const Item& it,
       scores(IC<0>{}, k, ahead, 0);
       st.exponentials(s);
 #pragma unroll
-      for (int n = 0; n < N; ++n) v[n].add(s[n], st.l, st.o);
+      for (int n = 0; n < N; ++n) v[n].template add<false>(s[n], st.l, st.o);
       st.raise(ahead);
       stage = stage_from(1);
     };
@@ -940,7 +977,7 @@ __device__ __forceinline__ void many_columns(const PagedArgs& a, const Item& it,
         }
         st.exponentials(s);
 #pragma unroll
-        for (int n = 0; n < N; ++n) v[n].add(s[n], st.l, st.o);
+        for (int n = 0; n < N; ++n) v[n].template add<false>(s[n], st.l, st.o);
       }
       if (active(jt + 1)) {
         Keys<E, D> k[N];

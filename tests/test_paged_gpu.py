@@ -613,3 +613,18 @@ def test_lengths_at_the_ends_of_32_bits(gpu_device, prefix, uniform):
     before = x.k_pages.clone()
     append(x, rope_pos0=prefix)
     assert int((x.k_pages != before).any(-1).any(1).sum()) == 4  # slots of the two sequences that have a length
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(18, 6, 64), (16, 4, 128)])
+@pytest.mark.parametrize("rows,lens,prefix,most", [
+    ([1] * 32, [200 + 61 * i for i in range(32)], 0, 1.1), ([1, 1], [3000, 500], 0, 1.1),                       # generated tokens
+    ([1] * 32, [5 + i for i in range(32)], 1500, 1.5), ([200, 1, 1, 1], [1500, 900, 40, 1200], 0, 1.5), ([700, 300], [700, 900], 0, 1.5),
+])
+def test_error_of_bf16_is_that_of_its_outputs(gpu_device, rows, lens, prefix, most, H, Hkv, D):
+    """Against 64 bits, in units of what rounding the exact y to bf16 costs (r, in norm).  Single tokens of up to 32 heads a kv group: query and
+    probabilities are in two parts, what they leave is 2^-14 of a score and of a probability, nothing beside r.  More columns: the probabilities are rounded
+    once, an independent error of the size of y's own: sqrt(2) r.  A second such rounding, of the query, would make it sqrt(3) r."""
+    x = Batch(rows, lens, H, Hkv, D, 16, BF16, gpu_device, seed=32, prefix=prefix, uniform=len(set(rows)) == 1)
+    y_ref = x.attended()[0]
+    r = (y_ref.to(BF16).to(F64) - y_ref).norm()
+    assert (attend(x).to(F64) - y_ref).norm() <= most * r

@@ -121,8 +121,9 @@ def paged_attention(q, k_pages, v_pages, block_table, kv_len, g_q, g_k=None, *, 
 
     A row that sees no key gives y = 0 and lse = -inf.  Rows in no sequence (behind ``seq_start[-1]``) are zero in a y that is allocated
     here, and left as they are in ``out``; their lse is -inf.  A sequence whose length is negative or above max_len, or whose
-    table has a page number that is not in the pool, gives NaN.  A key that is not finite gives NaN in the rows that see it, a value in
-    their component; neither shows in other rows."""
+    table has a page number that is not in the pool, gives NaN.  A key or value that is not finite takes part in the rows that see it as the formula
+    has it, and shows in no other: a key with a NaN gives NaN, one with an infinity NaN or, where its score is -inf, no weight; a value
+    that is not finite is what its component of y becomes."""
     return _attend(q, k_pages, v_pages, None, 0, block_table, kv_len, g_q, g_k, seq_start, gate_logits, gate_scale, eps, sm_scale, qk_norm,
                    rope_cos, rope_sin, rope_pos0, max_len, out, return_lse)
 

@@ -628,3 +628,28 @@ def test_error_of_bf16_is_that_of_its_outputs(gpu_device, rows, lens, prefix, mo
     y_ref = x.attended()[0]
     r = (y_ref.to(BF16).to(F64) - y_ref).norm()
     assert (attend(x).to(F64) - y_ref).norm() <= most * r
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("H,Hkv,D,dtype", [(6, 2, 64, BF16), (4, 2, 128, BF16), (6, 2, 64, F32)])
+def test_infinities_are_what_the_formula_makes_of_them(gpu_device, rows, H, Hkv, D, dtype):
+    """An infinite value is the answer of the rows that see it, whichever items they are part of.  An infinite component of a key makes the score an
+    infinity of the sign that the query's component gives it: NaN where that is positive, no weight where it is negative."""
+    x = Batch([rows, rows], [600, 40], H, Hkv, D, 16, dtype, gpu_device, seed=33, uniform=True, rope=False)
+    where = 600 - rows  # all rows of the first sequence see this key
+    page, slot = int(x.block_table[0, where // 16]), where % 16
+    clean = attend(x)
+    v = x.v_pages[page, :, slot, 7].clone()
+    for sign in (math.inf, -math.inf):
+        x.v_pages[page, :, slot, 7] = sign
+        y = attend(x)
+        assert (y[:rows, :, 7] == sign).all() and torch.equal(y[rows:], clean[rows:])
+        assert torch.equal(y[:rows, :, 8:], clean[:rows, :, 8:]) and torch.equal(y[:rows, :, :7], clean[:rows, :, :7])
+    x.v_pages[page, :, slot, 7] = v
+    x.q[..., 5] = torch.where(x.q[..., 5].abs() < 0.01, torch.ones_like(x.q[..., 5]), x.q[..., 5])
+    x.k_pages[page, :, slot, 5] = math.inf
+    y = attend(x, qk_norm=False)
+    up = x.q[:rows, :, 5] > 0
+    assert y[:rows][up].isnan().all() and y[:rows][~up].isfinite().all() and up.any() and (~up).any()
+    x.k_pages[page, :, slot, 5] = 30.0 * 2.0**100  # finite, and as far down for the rows whose component is negative
+    assert torch.equal(y[:rows][~up], attend(x, qk_norm=False)[:rows][~up])

@@ -346,7 +346,8 @@ typedef struct segpt_paged_params {
 /* Appends the rows of k and v (mixed with v_first) to the pages of their sequences. */
 int segpt_paged_append(const segpt_paged_params* p, void* stream);
 
-/* Bytes of device scratch segpt_paged_attn needs for these params (sizes only; 0 for invalid ones). */
+/* Bytes of device scratch segpt_paged_attn needs for these params; 0 for invalid ones.  Of the pointers only seq_start and prefix_table
+ * count, and only whether they are NULL: as they will be in the call. */
 size_t segpt_paged_workspace_bytes(const segpt_paged_params* p);
 
 /* Attention of the rows of q over the pages of their sequences.  With prefix_table every row also sees the prefix_len keys of

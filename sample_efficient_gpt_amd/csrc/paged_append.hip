@@ -165,7 +165,8 @@ int check_rows(const segpt_rows& r, const segpt_paged_params& p, int heads, bool
 
 }  // namespace
 
-int check_paged(const segpt_paged_params* p, bool append) {
+// what can be said of the sizes alone, without an address being looked at
+int check_paged_sizes(const segpt_paged_params* p, bool append) {
   if (!p) return SEGPT_E_NULL;
   if (p->struct_bytes != sizeof(segpt_paged_params)) return SEGPT_E_STRUCT;
   if (p->dtype != SEGPT_DTYPE_BF16 && p->dtype != SEGPT_DTYPE_FP32) return SEGPT_E_DTYPE;
@@ -173,13 +174,19 @@ int check_paged(const segpt_paged_params* p, bool append) {
   if (p->Hkv > 65535 || (!append && p->H > 65535) || p->B > (1 << 24)) return SEGPT_E_SHAPE;
   if ((int64_t)p->T * (append ? p->Hkv : p->H) > (1 << 30) || (!p->seq_start && p->T % p->B)) return SEGPT_E_SHAPE;
   if (p->D != 64 && p->D != 128 && !(p->D == 32 && p->dtype == SEGPT_DTYPE_FP32)) return SEGPT_E_HEAD_DIM;
-  if (p->n_pages <= 0 || p->page_size < 8 || p->page_size > 65536 || (p->page_size & (p->page_size - 1)) || p->table_width <= 0) return SEGPT_E_PAGES;
+  if (p->page_size < 8 || p->page_size > 65536 || (p->page_size & (p->page_size - 1)) || p->table_width <= 0) return SEGPT_E_PAGES;
   if (p->prefix_len < 0 || p->max_len < 0 || (int64_t)p->table_width * p->page_size + p->prefix_len > INT32_MAX - (1 << 20)) return SEGPT_E_PAGES;
+  return SEGPT_OK;
+}
+
+int check_paged(const segpt_paged_params* p, bool append) {
+  int rc = check_paged_sizes(p, append);
+  if (rc) return rc;
+  if (p->n_pages <= 0) return SEGPT_E_PAGES;
   const int64_t positions = (int64_t)paged_capacity(*p) + (append ? 0 : p->prefix_len);
   if (!p->block_table || !p->kv_len) return SEGPT_E_NULL;
   if (p->table_stride < 0) return SEGPT_E_STRIDE;
   if (!aligned(p->block_table, 4) || !aligned(p->kv_len, 4) || !aligned(p->seq_start, 4)) return SEGPT_E_ALIGN;
-  int rc;
   if ((rc = check_pool(p->k_pages, *p, append))) return rc;
   if ((rc = check_pool(p->v_pages, *p, append))) return rc;
   if (p->rope_cos || p->rope_sin) {

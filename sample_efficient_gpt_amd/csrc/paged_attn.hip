@@ -1257,8 +1257,7 @@ extern "C" {
 
 size_t segpt_paged_workspace_bytes(const segpt_paged_params* p) {
   using namespace segpt;
-  if (!p || p->struct_bytes != sizeof(segpt_paged_params) || (p->dtype != SEGPT_DTYPE_BF16 && p->dtype != SEGPT_DTYPE_FP32)) return 0;
-  if (p->T <= 0 || p->B <= 0 || p->H <= 0 || p->Hkv <= 0 || p->H % p->Hkv || p->D <= 0 || p->page_size < 8 || p->table_width <= 0 || p->prefix_len < 0) return 0;
+  if (check_paged_sizes(p, false) != SEGPT_OK) return 0;
   PagedArgs a{};
   const size_t n = plan(*p, a);
   return n > SIZE_MAX - 256 ? 0 : up256(n);

@@ -5,6 +5,7 @@
 
 namespace segpt {
 
+int check_paged_sizes(const segpt_paged_params* p, bool append);
 int check_paged(const segpt_paged_params* p, bool append);
 // keys a sequence may hold (checked: fits an int)
 __host__ __device__ inline int paged_capacity(const segpt_paged_params& p) {

@@ -181,3 +181,17 @@ def test_cache_shapes():
         c.append(torch.zeros(3, 2, 64), torch.zeros(3, 2, 64))
     with pytest.raises(AssertionError, match="holds 0 of its 20"):
         c.attend(torch.zeros(2, 2, 64), torch.ones(1))
+
+
+def test_workspace_bytes_of_sizes_that_no_call_has(lib):
+    """Without seq_start the rows are the same number for every sequence: fewer rows than sequences, or no multiple, is no shape."""
+    for change in (dict(seq_start=None, T=1, B=2), dict(seq_start=None, T=7), dict(D=48), dict(page_size=12), dict(max_len=-1), dict(T=1 << 30, B=1),
+                   dict(B=(1 << 24) + 1), dict(table_width=1 << 28), dict(prefix_table=0x20000, prefix_len=-1)):
+        p = _params()
+        for key, value in change.items():
+            setattr(p, key, value)
+        assert lib.segpt_paged_workspace_bytes(p) == 0, change
+        assert lib.segpt_paged_attn(p, None) < 0, change
+    p = _params()
+    p.seq_start = p.k_pages.ptr = p.block_table = None  # addresses do not matter
+    assert lib.segpt_paged_workspace_bytes(p) > 0

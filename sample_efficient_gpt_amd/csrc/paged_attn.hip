@@ -12,8 +12,9 @@
 // workgroup of four waves with 32 columns each that share the staged keys, bound by the matrix pipe and the exponentials.  Either way an item
 // is (entry, tile of columns, share of its keys, kv head).  Lengths live on the device, so the device deals out the work: the length of a
 // share follows from the sum over all entries, such that the items fill the card once, and every workgroup finds its own item in the running
-// sum of the entries' items (one load and a few register moves for up to 64 sequences).  A tile with one share writes y; others leave
-// (reference m, sum l, products O) in fp32, which paged_merge_kernel joins.
+// sum of the entries' items (one load and a few register moves for up to 64 sequences).  Up to 256 entries every wave forms the sums for itself;
+// more are summed once, by paged_plan_kernel, and searched.  A tile with one share writes y; others leave (reference m, sum l, products O) in
+// fp32, which paged_merge_kernel joins.
 //
 // Scores are transposed as in the other forward kernels: lane = query column, S^T = K' . Qhat^T, and the probabilities are already the
 // B operand of O^T = V'^T . P^T.
@@ -60,7 +61,9 @@ struct PagedArgs {
   int32_t n_many, n_few;          // items there may be of either kind
   int32_t n_joins;                // tiles and kv heads whose partial results there may be to join
   int32_t n_slots;                // partial results there is room for, 32 columns each
+  size_t planned_bytes;           // of upto
   int32_t* lens;                  // blocks of a share (few, many) and tiles and kv heads to join, left for the merge
+  int32_t* upto;                  // more than kKept * 64 entries: their running sums, [4][entries] in the order of Counts; else NULL
   float* part;                    // [n_slots][32][D]
   float2* stat;                   // [n_slots][32]
 };
@@ -69,7 +72,7 @@ constexpr int kBlock = 32;          // keys of a score tile
 constexpr int kFew = 32, kMany = 128;  // columns of a tile
 constexpr float kLazy = 8.f;        // the reference is raised where a score exceeds it by 2^8: probabilities stay below 2^8
 
-// ---- the plan, computed by every wave for itself
+// ---- the plan, computed by every wave for itself or, for many entries, by paged_plan_kernel
 struct Entry {
   int first, n, len;   // rows, keys
   int tiles, blocks;
@@ -136,37 +139,35 @@ __device__ __forceinline__ int shares_of(const Entry& x, Shares s) {
   const int few = max((int)(((double)x.blocks + (s.few - 0.5)) * s.per_few), 1), many = max((int)(((double)x.blocks + (s.many - 0.5)) * s.per_many), 1);
   return x.many ? many : few;
 }
-// The first entries, a lane each, kept in registers (all of them loaded at once: one after the other, 129 entries cost a launch of 47 us
-// 8); more than kKept * 64 are read again where they are needed.
+// The entries a wave (the plan's kernel: its workgroup) keeps in registers, one a lane and turn, all of them loaded at once (one after the other,
+// 129 entries cost a launch of 47 us 8).
 constexpr int kKept = 4;
 struct Entries {
   Entry e[kKept];
 };
+template <int LANES>
 __device__ __forceinline__ Entries load_entries(const PagedArgs& a, int lane, int rep) {
   Raw raw[kKept] = {};
 #pragma unroll
   for (int u = 0; u < kKept; ++u)
-    if (64 * u < a.entries) raw[u] = raw_at(a, 64 * u + lane);
+    if (LANES * u < a.entries) raw[u] = raw_at(a, LANES * u + lane);
   Entries x = {};
 #pragma unroll
   for (int u = 0; u < kKept; ++u)
-    if (64 * u < a.entries) x.e[u] = entry_of(a, 64 * u + lane, rep, raw[u]);
+    if (LANES * u < a.entries) x.e[u] = entry_of(a, LANES * u + lane, rep, raw[u]);
   return x;
+}
+__device__ __forceinline__ Entries kept_entries(const PagedArgs& a, int lane, int rep) {
+  if (a.upto) return {};
+  return load_entries<64>(a, lane, rep);
 }
 __device__ __forceinline__ Shares shares_from(int few, int many) { return {few, many, DeviceDivisor(few).inverse, DeviceDivisor(many).inverse}; }
 // Blocks of a share, such that the workgroups are resident at once if the tiles alone are not too many for that: the mean first, then longer
 // ones until the begun ones fit too (one workgroup too many is a round of its own).  A block of many columns keeps a workgroup as long as the
-// memory does that of few columns, in a quarter of the workgroup each: a wave's share is a quarter as long.  The sums are
-// floats: they may round, but to the same value in every wave.
-__device__ __forceinline__ Shares share_blocks(const PagedArgs& a, int lane, int rep, const Entries& kept) {
-  auto sum = [&](auto of) {
-    float v = 0.f;
-#pragma unroll
-    for (int u = 0; u < kKept; ++u)
-      if (64 * u < a.entries) v += of(kept.e[u]);
-    for (int e = 64 * kKept; e < a.entries; e += 64) v += of(entry_at(a, e + lane, rep));
-    return lane_value(lane_prefix_sum(v), 63) * (float)a.p.Hkv;
-  };
+// memory does that of few columns, in a quarter of the workgroup each: a wave's share is a quarter as long.  sum(of): of() over all entries
+// and kv heads, in floats: it may round, but to the same value in every wave.
+template <typename F>
+__device__ __forceinline__ Shares share_blocks(const PagedArgs& a, F sum) {
   auto room = [](const Entry& x) { return (float)x.tiles * (x.many ? 1.f : 0.25f); };  // workgroups of a share of each tile
   const float target = (float)a.target, per = __builtin_amdgcn_rcpf(target);
   float len = sum([](const Entry& x) { return (float)x.tiles * (float)x.blocks; }) * per;
@@ -179,6 +180,27 @@ __device__ __forceinline__ Shares share_blocks(const PagedArgs& a, int lane, int
     len *= fmaxf(groups * per, 1.03f);
   }
 }
+__device__ __forceinline__ Shares share_blocks(const PagedArgs& a, const Entries& kept) {
+  if (a.upto) return shares_from(a.lens[0], a.lens[1]);
+  return share_blocks(a, [&](auto of) {
+    float v = 0.f;
+#pragma unroll
+    for (int u = 0; u < kKept; ++u)
+      if (64 * u < a.entries) v += of(kept.e[u]);
+    return lane_value(lane_prefix_sum(v), 63) * (float)a.p.Hkv;
+  });
+}
+// What an entry adds to the running sums: items of either kind, tiles and kv heads whose partial results are to be joined, partial results
+enum Find { kFindFew, kFindMany, kFindJoin, kSlots, kFindFirst };
+struct Counts {
+  int of[4];  // by Find
+  int shares;
+};
+__device__ __forceinline__ Counts counts_of(const PagedArgs& a, int e, const Entry& x, const Shares& share) {
+  const int shares = shares_of(x, share), items = x.tiles * shares * a.p.Hkv;
+  const bool partial = a.shared || shares > 1;
+  return {{x.many ? 0 : items, x.many ? items : 0, partial && e >= a.shared ? x.tiles * a.p.Hkv : 0, partial ? items * (x.many ? kMany / 32 : 1) : 0}, shares};
+}
 // an entry as the whole wave sees it
 struct Found {
   int entry;          // -1: none
@@ -187,22 +209,48 @@ struct Found {
   int slot;           // of its first partial result (entries whose tiles leave any)
   bool many, broken;
 };
-// The entry of an item of its kind, or of a tile and kv head whose partial results are to be joined, by number; or the first entry
-enum Find { kFindFew, kFindMany, kFindJoin, kFindFirst };
+// The entry of an item of its kind, or of a tile and kv head whose partial results are to be joined, by number; or the first entry.  With the sums of
+// paged_plan_kernel: 64 of them are looked at a time (three loads one after the other for 2^18 entries).
+template <Find F>
+__device__ __forceinline__ Found search_entry(const PagedArgs& a, int lane, int rep, const Shares& share, int which) {
+  Found found{-1, 0, 0, 0, 0, 0, 0, 0, false, false};
+  const int32_t* upto = a.upto + (int64_t)(F == kFindFirst ? kSlots : F) * a.entries;
+  int e = 0;
+  if (F != kFindFirst) {
+    const int all = upto[a.entries - 1];
+    if (which >= all) {
+      found.base = all;
+      return found;
+    }
+    for (int n = a.entries, step = n; step > 1;) {  // the first of e .. e + n - 1 whose sum is above `which`
+      step = (n + 63) >> 6;
+      const uint64_t above = __builtin_amdgcn_ballot_w64(upto[e + min((lane + 1) * step, n) - 1] > which);
+      if (!above) return found;  // row ranges that overlap, their sum beyond 32 bits
+      const int l = __builtin_ctzll(above);
+      e += l * step;
+      n = min(step, n - l * step);
+    }
+  }
+  const Entry x = entry_at(a, e, rep);
+  const Counts c = counts_of(a, e, x, share);
+  const int base = F == kFindFirst || e == 0 ? 0 : upto[e - 1];
+  if (F != kFindFirst && (uint32_t)(which - base) >= (uint32_t)c.of[F]) return found;
+  return {e, x.first, x.n, x.len, x.blocks, c.shares, base, e == 0 ? 0 : a.upto[(int64_t)kSlots * a.entries + e - 1], x.many, x.broken};
+}
 template <Find F>
 __device__ __forceinline__ Found find_entry(const PagedArgs& a, int lane, int rep, const Shares& share, const Entries& kept, int which) {
+  if (a.upto) return search_entry<F>(a, lane, rep, share, which);
   int base = 0, slot = 0;
   Found found{-1, 0, 0, 0, 0, 0, 0, 0, false, false};
   auto look = [&](int e0, const Entry& x) {  // true: it is among these 64
-    const int shares = shares_of(x, share), items = x.tiles * shares * a.p.Hkv;
-    const bool partial = a.shared || shares > 1;
-    const int slots = partial ? items * (x.many ? kMany / 32 : 1) : 0, slots_upto = slot + lane_prefix_sum(slots);
-    const int mine_n = F == kFindJoin ? (partial && e0 + lane >= a.shared ? x.tiles * a.p.Hkv : 0) : F == kFindFirst ? 0 : x.many == (F == kFindMany) ? items : 0;
+    const Counts c = counts_of(a, e0 + lane, x, share);
+    const int slots = c.of[kSlots], slots_upto = slot + lane_prefix_sum(slots);
+    const int mine_n = F == kFindFirst ? 0 : c.of[F == kFindFirst ? 0 : F];
     const int upto = F == kFindFirst ? 0 : base + lane_prefix_sum(mine_n);
     const uint64_t hits = F == kFindFirst ? 1 : __builtin_amdgcn_ballot_w64(which >= upto - mine_n && which < upto);
     if (hits) {
       const int l = __builtin_ctzll(hits);
-      found = Found{e0 + l, lane_value(x.first, l), lane_value(x.n, l), lane_value(x.len, l), lane_value(x.blocks, l), lane_value(shares, l),
+      found = Found{e0 + l, lane_value(x.first, l), lane_value(x.n, l), lane_value(x.len, l), lane_value(x.blocks, l), lane_value(c.shares, l),
                     lane_value(upto - mine_n, l), lane_value(slots_upto - slots, l), lane_value((int)x.many, l) != 0, lane_value((int)x.broken, l) != 0};
       return true;
     }
@@ -213,10 +261,62 @@ __device__ __forceinline__ Found find_entry(const PagedArgs& a, int lane, int re
 #pragma unroll
   for (int u = 0; u < kKept; ++u)
     if (64 * u < a.entries && look(64 * u, kept.e[u])) return found;
-  for (int e0 = 64 * kKept; e0 < a.entries; e0 += 64)
-    if (look(e0, entry_at(a, e0 + lane, rep))) return found;
   found.base = base;
   return found;
+}
+// The plan of more than kKept * 64 entries, by one workgroup: lengths of the shares and running sums.  Formed by every wave for itself, an entry's
+// numbers are read by all of them, several times over, and the time grows with the square of the entries.  Single tokens, 18 / 6 heads of 64, us, by
+// every wave and here: 300 sequences 132, 134; 1000 200, 197; 4000 590, 247.
+constexpr int kPlanThreads = 1024;
+__global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a) {
+  constexpr int kWaves = kPlanThreads / 64;
+  __shared__ float sums[kWaves];
+  __shared__ int counts[4][kWaves];
+  const int tid = threadIdx.x, wave = tid >> 6, rep = a.rep.d;
+  const Entries kept = load_entries<kPlanThreads>(a, tid, rep);
+  const Shares share = share_blocks(a, [&](auto of) {
+    float v = 0.f;
+#pragma unroll
+    for (int u = 0; u < kKept; ++u)
+      if (kPlanThreads * u < a.entries) v += of(kept.e[u]);
+    for (int e = kPlanThreads * kKept; e < a.entries; e += kPlanThreads) v += of(entry_at(a, e + tid, rep));
+    v = lane_prefix_sum(v);
+    __syncthreads();  // the sums before have been read
+    if ((tid & 63) == 63) sums[wave] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) v += sums[w];
+    return v * (float)a.p.Hkv;
+  });
+  int before[4] = {0, 0, 0, 0};
+  auto add = [&](int e, const Entry& x) {
+    const Counts c = counts_of(a, e, x, share);
+    int own[4];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      own[k] = lane_prefix_sum(c.of[k]);
+      if ((tid & 63) == 63) counts[k][wave] = own[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      int upto = before[k] + own[k];
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const int n = counts[k][w];
+        before[k] += n;
+        upto += w < wave ? n : 0;
+      }
+      if (e < a.entries) a.upto[(int64_t)k * a.entries + e] = upto;
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < kKept; ++u)
+    if (kPlanThreads * u < a.entries) add(kPlanThreads * u + tid, kept.e[u]);
+  for (int e = kPlanThreads * kKept; e < a.entries; e += kPlanThreads) add(e + tid, entry_at(a, e + tid, rep));
+  if (tid == 0) { a.lens[0] = share.few; a.lens[1] = share.many; a.lens[2] = before[kFindJoin]; }
 }
 
 // ---- tiles: BK rows of D elements, filled by direct global->LDS loads of 1 KB; the 16-byte chunk c of row r lies at chunk c ^ f(r)
@@ -1027,9 +1127,9 @@ __device__ __forceinline__ void clear_rest(const PagedArgs& a, int tid, int thre
   }
 }
 
-// What the merge goes by, from the last workgroup, which mostly has no item
+// What the merge goes by, from the last workgroup, which mostly has no item, where no plan was made before
 __device__ __forceinline__ void leave_plan(const PagedArgs& a, int lane, int rep, const Shares& share, const Entries& mine) {
-  if (blockIdx.x != gridDim.x - 1) return;
+  if (a.upto || blockIdx.x != gridDim.x - 1) return;
   const int joins = find_entry<kFindJoin>(a, lane, rep, share, mine, INT32_MAX).base;
   if (threadIdx.x == 0) { a.lens[0] = share.few; a.lens[1] = share.many; a.lens[2] = joins; }
 }
@@ -1045,8 +1145,8 @@ __global__ __launch_bounds__(64, (Shape<E, D>::kOcc)) void paged_few_kernel(Page
   __shared__ int table[S::kFewTable + 2];
   const int lane = threadIdx.x, rep = a.rep.d;
   clear_rest<E>(a, lane, 64, D);
-  const Entries mine = load_entries(a, lane, rep);
-  const Shares share = share_blocks(a, lane, rep, mine);
+  const Entries mine = kept_entries(a, lane, rep);
+  const Shares share = share_blocks(a, mine);
   leave_plan(a, lane, rep, share, mine);
   const Item it = locate<false>(a, lane, rep, share, mine, blockIdx.x);
   if (it.valid) few_columns<E, D>(a, it, rep, lane, lds_addr_of(lds), table, gsm);
@@ -1067,8 +1167,8 @@ __global__ __launch_bounds__(256, (Shape<E, D>::kOcc)) void paged_any_kernel(Pag
   const int tid = threadIdx.x, lane = tid & 63, rep = a.rep.d;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   clear_rest<E>(a, tid, 256, D);
-  const Entries mine = load_entries(a, lane, rep);
-  const Shares share = share_blocks(a, lane, rep, mine);
+  const Entries mine = kept_entries(a, lane, rep);
+  const Shares share = share_blocks(a, mine);
   leave_plan(a, lane, rep, share, mine);
   const Item it = locate<true>(a, lane, rep, share, mine, blockIdx.x);
   if (it.x.entry >= 0) {
@@ -1093,7 +1193,7 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedArgs a,
   const int tid = threadIdx.x, lane = tid & 63, unit = tid / LPR, c = tid % LPR;
   const int rep = a.rep.d;
   const int few = a.lens[0], many = a.lens[1], joins = a.lens[2];
-  const Entries mine = load_entries(a, lane, rep);
+  const Entries mine = kept_entries(a, lane, rep);
   const int which = blockIdx.x / subs, sub = blockIdx.x - which * subs;
   if (which >= joins) return;
   const Shares share = shares_from(few, many);
@@ -1184,7 +1284,9 @@ bool all_few(const segpt_paged_params& p) {  // known on the host
   return !p.prefix_table && !p.seq_start && (int64_t)p.H / p.Hkv * (p.T / p.B) <= kFew;
 }
 
-// fills the plan; returns the scratch bytes of the partials
+size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// fills the plan; returns the scratch bytes
 size_t plan(const segpt_paged_params& p, PagedArgs& a) {
   const int row_bytes = p.D * (p.dtype == SEGPT_DTYPE_FP32 ? 4 : 2), rep = p.H / p.Hkv;
   a.rep.set(rep);
@@ -1227,12 +1329,18 @@ size_t plan(const segpt_paged_params& p, PagedArgs& a) {
   a.n_slots = (int32_t)std::min<int64_t>(slots, INT32_MAX / 32);
   const int64_t joins = a.shared ? own * p.Hkv : std::min(own_many * p.Hkv, most) + std::min((own - own_many) * p.Hkv, 4 * most);
   a.n_joins = (int32_t)std::min<int64_t>(joins, INT32_MAX);
-  return n_many + n_few > INT32_MAX / 2 || slots > INT32_MAX / 32 ? SIZE_MAX : 256 + (size_t)a.n_slots * 32 * (p.D + 2) * sizeof(float);
+  a.planned_bytes = a.entries > kKept * 64 ? (size_t)4 * a.entries * sizeof(int32_t) : 0;
+  return n_many + n_few > INT32_MAX / 2 || slots > INT32_MAX / 32 ? SIZE_MAX : 256 + up256(a.planned_bytes) + (size_t)a.n_slots * 32 * (p.D + 2) * sizeof(float);
 }
 
 template <typename E, int D>
 int launch(const PagedArgs& a, hipStream_t st) {
   const segpt_paged_params& p = a.p;
+  if (a.upto) {
+    hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a);
+    const int rc = (int)hipGetLastError();
+    if (rc) return rc;
+  }
   if (all_few(p)) hipLaunchKernelGGL((paged_few_kernel<E, D>), dim3((unsigned)a.n_few), dim3(64), 0, st, a);
   else hipLaunchKernelGGL((paged_any_kernel<E, D>), dim3((unsigned)(a.n_many + (a.n_few + 3) / 4)), dim3(256), 0, st, a);
   const int rc = (int)hipGetLastError();
@@ -1247,8 +1355,6 @@ int launch(const PagedArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((paged_merge_kernel<E, D>), dim3((unsigned)(a.n_joins * subs)), dim3(kMergeThreads), 0, st, a, subs, per_sub);
   return (int)hipGetLastError();
 }
-
-size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 }  // namespace
 }  // namespace segpt
@@ -1274,7 +1380,8 @@ int segpt_paged_attn(const segpt_paged_params* p, void* stream) {
   if (!p->workspace || p->workspace_bytes < up256(need)) return SEGPT_E_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(p->workspace) & 255u) return SEGPT_E_ALIGN;
   a.lens = reinterpret_cast<int32_t*>(p->workspace);
-  a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(p->workspace) + 256);
+  if (a.planned_bytes) a.upto = a.lens + 256 / sizeof(int32_t);
+  a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(p->workspace) + 256 + up256(a.planned_bytes));
   a.stat = reinterpret_cast<float2*>(a.part + (size_t)a.n_slots * 32 * p->D);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (p->dtype == SEGPT_DTYPE_BF16) return p->D == 64 ? launch<uint16_t, 64>(a, st) : launch<uint16_t, 128>(a, st);

@@ -653,3 +653,54 @@ def test_infinities_are_what_the_formula_makes_of_them(gpu_device, rows, H, Hkv,
     assert y[:rows][up].isnan().all() and y[:rows][~up].isfinite().all() and up.any() and (~up).any()
     x.k_pages[page, :, slot, 5] = 30.0 * 2.0**100  # finite, and as far down for the rows whose component is negative
     assert torch.equal(y[:rows][~up], attend(x, qk_norm=False)[:rows][~up])
+
+
+@pytest.mark.parametrize("H,Hkv,D,dtype", [(6, 2, 64, BF16), (6, 2, 32, F32)])
+@pytest.mark.parametrize("rows,lens,prefix", [
+    (lambda i: 1, lambda i: 1 + 29 * i % 90, 0), (lambda i: (1, 0, 2, 14)[i % 4], lambda i: 14 + 17 * i % 60, 0), (lambda i: (1, 0, 3)[i % 3], lambda i: 3 + i % 40, 45),
+    (lambda i: 3000 * (i == 255), lambda i: 3000 * (i == 255), 0),  # one prompt among sequences without rows
+])
+@pytest.mark.parametrize("B", [256, 257, 5000])
+def test_thousands_of_sequences(gpu_device, B, rows, lens, prefix, H, Hkv, D, dtype):
+    """As many as waves plan for by themselves, one more, and more than the plan's workgroup keeps in registers: some of them against the definition, the others against the same call in pieces."""
+    rows, lens = [rows(i) for i in range(B)], [lens(i) for i in range(B)]
+    x = Batch(rows, lens, H, Hkv, D, 16, dtype, gpu_device, seed=34, prefix=prefix, uniform=len(set(rows)) == 1)
+    y, lse = attend(x, return_lse=True)
+    assert torch.equal(attend(x), y)
+    some = sorted(b for b in {0, 1, 2, 3, 255, 256, 257, 1022, 1023, 1024, 4095, 4096, 4097, B - 2, B - 1} if b < B)
+    take = lambda bs: torch.cat([torch.arange(x.starts[b], x.starts[b + 1]) for b in bs]).to(gpu_device)
+
+    def part(bs):
+        p = Batch([rows[b] for b in bs], [lens[b] for b in bs], H, Hkv, D, 16, dtype, gpu_device, seed=34, prefix=prefix)
+        p.block_table, p.kv_len, p.k_pages, p.v_pages, p.prefix_table = x.block_table[bs], x.kv_len[bs], x.k_pages, x.v_pages, x.prefix_table
+        p.q, p.cos, p.sin, p.g_q = x.q[take(bs)], x.cos, x.sin, x.g_q
+        return p
+
+    few = part(some)
+    if sum(lens) > 3000:
+        check_y(few, y[take(some)], lse[take(some)], few.attended())
+    for b0 in range(0, B, 200):
+        bs = list(range(b0, min(b0 + 200, B)))
+        if sum(rows[b] for b in bs):
+            z = attend(part(bs))
+            assert (z.to(F64) - y[take(bs)].to(F64)).norm() <= (6e-3 if dtype == BF16 else 1e-5) * z.to(F64).norm()
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+def test_two_hundred_thousand_sequences(gpu_device, ragged):
+    """Sequences of one to eight keys, in pages that many of them share: the time a call takes grows with the sequences, not with their square."""
+    B, H, Hkv, D = 200_000, 4, 2, 64
+    g = torch.Generator(device=gpu_device).manual_seed(35)
+    n = lambda *s: torch.randn(*s, generator=g, device=gpu_device)
+    kp, vp, q = n(64, Hkv, 8, D).to(BF16), n(64, Hkv, 8, D).to(BF16), n(B, H, D).to(BF16)
+    table = torch.randint(0, 64, (B, 1), generator=g, device=gpu_device, dtype=torch.int32)
+    lens = torch.randint(1, 9, (B,), generator=g, device=gpu_device, dtype=torch.int32)
+    starts = torch.arange(B + 1, device=gpu_device, dtype=torch.int32) if ragged else None
+    y = paged_attention(q, kp, vp, table, lens, torch.ones(1, device=gpu_device), seq_start=starts, qk_norm=False)
+    r = H // Hkv
+    K, V = (p[table[:, 0].long()].float().repeat_interleave(r, 1) for p in (kp, vp))
+    s = (q.float()[:, :, None] * K).sum(-1) / 8.0
+    s = s.masked_fill(torch.arange(8, device=gpu_device) >= lens[:, None, None], -math.inf)
+    want = (torch.softmax(s, -1)[..., None] * V).sum(2)
+    assert (y.float() - want).norm() <= 3e-3 * want.norm()  # y's rounding 1.7e-3, and in fp32 sums nothing beside it
+    assert ((y.float() - want).abs() <= H_BF16 * (want.abs() + 0.1)).all()

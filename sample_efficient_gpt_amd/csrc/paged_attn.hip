@@ -493,7 +493,8 @@ __device__ __forceinline__ Item locate(const PagedArgs& a, int lane, int rep, co
   it.prefix = a.shared && x.entry == 0;
   it.direct = !a.shared && x.shares == 1;
   it.slot = x.slot + ((it.tile * x.shares + it.part) * a.p.Hkv + it.g) * (COLS / 32);
-  it.valid = it.tile >= 0 && (it.direct || it.slot + COLS / 32 <= a.n_slots);
+  // row ranges that overlap may add up to more than 32 bits hold: nothing is written outside the scratch
+  it.valid = it.tile >= 0 && (it.direct || (it.slot >= 0 && it.slot <= a.n_slots - COLS / 32));
   it.past = x.len - x.n;
   const int per = shares.of(x.blocks + x.shares - 1) * kBlock;  // shares as even as whole blocks allow
   const int last_col = min(it.cols, (it.tile + 1) * COLS) - 1, sees = it.prefix ? x.len : min(x.len, it.past + a.rep.of(last_col) + 1);

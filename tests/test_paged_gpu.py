@@ -704,3 +704,23 @@ def test_two_hundred_thousand_sequences(gpu_device, ragged):
     want = (torch.softmax(s, -1)[..., None] * V).sum(2)
     assert (y.float() - want).norm() <= 3e-3 * want.norm()  # y's rounding 1.7e-3, and in fp32 sums nothing beside it
     assert ((y.float() - want).abs() <= H_BF16 * (want.abs() + 0.1)).all()
+
+
+def test_row_ranges_that_overlap_beyond_32_bits(gpu_device):
+    """No call is meant to have them, and their rows are undefined: but the partial results of 2^15 sequences of 2^13 rows, counted before those of the last
+    sequence, come to 2^31, and nothing may be written there."""
+    T, H, D, B = 1 << 13, 256, 64, (1 << 16) + 1
+    q = torch.randn(T, H, D, device=gpu_device).to(BF16)
+    kp, vp = torch.randn(2, 2, H, 8, D, device=gpu_device).to(BF16)
+    table = torch.zeros(B, 1, dtype=torch.int32, device=gpu_device)
+    lens = torch.full((B,), 8, dtype=torch.int32, device=gpu_device)
+    starts = torch.zeros(B + 1, dtype=torch.int32, device=gpu_device)
+    starts[1:-1:2] = T
+    starts[-1] = 1
+    gain = torch.ones(1, device=gpu_device)
+    call = lambda s, n: shared_prefix_attention(q, kp, vp, table[0], 8, table[:n], lens[:n], gain, seq_start=s, qk_norm=False)
+    one = torch.tensor([0, T], dtype=torch.int32, device=gpu_device)
+    clean = call(one, 1)
+    call(starts, B)
+    torch.cuda.synchronize()
+    assert torch.equal(call(one, 1), clean)

@@ -109,7 +109,9 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(segpt_paged_para
 template <typename E, int D>
 int launch(const segpt_paged_params& p, hipStream_t st) {
   constexpr int kRows = kThreads / 64 * (64 / (D / 2 / (16 / (int)sizeof(E))));
-  const dim3 grid((unsigned)(((int64_t)p.T * p.Hkv + kRows - 1) / kRows));
+  const int64_t groups = ((int64_t)p.T * p.Hkv + kRows - 1) / kRows;
+  if (groups > UINT32_MAX / kThreads) return SEGPT_E_SHAPE;  // a launch has fewer than 2^32 threads: rows of 128 GiB and more
+  const dim3 grid((unsigned)groups);
   const int log_page = __builtin_ctz((unsigned)p.page_size), each = p.seq_start ? 0 : p.T / p.B;
   const bool mix = p.v_first.ptr != nullptr;
   if (p.rope_cos) {

@@ -1331,7 +1331,9 @@ size_t plan(const segpt_paged_params& p, PagedArgs& a) {
   const int64_t joins = a.shared ? own * p.Hkv : std::min(own_many * p.Hkv, most) + std::min((own - own_many) * p.Hkv, 4 * most);
   a.n_joins = (int32_t)std::min<int64_t>(joins, INT32_MAX);
   a.planned_bytes = a.entries > kKept * 64 ? (size_t)4 * a.entries * sizeof(int32_t) : 0;
-  return n_many + n_few > INT32_MAX / 2 || slots > INT32_MAX / 32 ? SIZE_MAX : 256 + up256(a.planned_bytes) + (size_t)a.n_slots * 32 * (p.D + 2) * sizeof(float);
+  // a launch has fewer than 2^32 threads (the merge: a workgroup a join at least)
+  const int64_t most_groups = UINT32_MAX / 256;
+  return n_many + (n_few + 3) / 4 > most_groups || joins > most_groups || slots > INT32_MAX / 32 ? SIZE_MAX : 256 + up256(a.planned_bytes) + (size_t)a.n_slots * 32 * (p.D + 2) * sizeof(float);
 }
 
 template <typename E, int D>

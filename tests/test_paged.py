@@ -195,3 +195,24 @@ def test_workspace_bytes_of_sizes_that_no_call_has(lib):
     p = _params()
     p.seq_start = p.k_pages.ptr = p.block_table = None  # addresses do not matter
     assert lib.segpt_paged_workspace_bytes(p) > 0
+
+
+def test_launches_of_more_threads_than_one_may_have(lib):
+    """2^32 and more: refused before anything is launched."""
+    def change(**kw):
+        p = _params()
+        for key, value in kw.items():
+            setattr(p, key, value)
+        return p
+
+    huge = dict(T=1 << 24, B=1 << 24, H=4, Hkv=4, workspace_bytes=(1 << 63) - 1)
+    for kw in (huge, dict(huge, H=1, Hkv=1, prefix_table=0x20000, prefix_len=8), dict(huge, seq_start=None), dict(T=1 << 28, B=1, H=4, Hkv=4, prefix_table=0x20000, prefix_len=8)):
+        p = change(**kw)
+        p.q = p.o = _lib.Rows(0x10000, p.H * 64, 64)
+        assert lib.segpt_paged_workspace_bytes(p) == 0 and lib.segpt_paged_attn(p, None) == -4, kw
+    p = change(T=1 << 24, B=1 << 22, H=1, Hkv=1)
+    assert lib.segpt_paged_workspace_bytes(p) > 0
+    p = change(T=1 << 28, B=1, Hkv=4, D=128)
+    p.k_pages = p.v_pages = _lib.Tensor4(0x10000, 4 * 16 * 128, 16 * 128, 128)
+    p.k = p.v = _lib.Rows(0x10000, 4 * 128, 128)
+    assert lib.segpt_paged_append(p, None) == -4

@@ -295,7 +295,8 @@ int segpt_linear_rows(const segpt_linear_rows_params* p, void* stream);
  *   - append: a row whose position is negative or max_len or more, or whose page number is not in the pool, is left out;
  *   - attention: a sequence with kv_len < 0 or above max_len, or with a page number that is not in the pool among
  *     those of its keys, gives NaN in every row that sees one of these (it may give NaN in its other rows).
- * Row ranges must not overlap, and two rows of one append must not name one slot: which of them is kept is undefined. */
+ * Row ranges must not overlap, and two rows of one append must not name one slot: which of them is kept is undefined.  No output (o, lse; the pools
+ * of an append) may overlap an input or another output: rows are read again after others are written. */
 #define SEGPT_FLAG_ZERO_REST 32  /* segpt_paged_attn: rows of o that belong to no sequence are set to zero, their lse to -inf */
 
 /* [T, heads, D] tensor view; the D axis is contiguous. Strides in ELEMENTS. */

@@ -24,6 +24,7 @@
 #include <string>
 #include <tuple>
 
+#include "footprint.hpp"
 #include "segpt_attn.h"
 
 namespace {
@@ -492,6 +493,13 @@ segpt_rows view_rows(const Tensor& t) {
   if (!t.defined()) return {nullptr, 0, 0};
   return {t.data_ptr(), t.stride(0), t.stride(1)};
 }
+using segpt::Footprint, segpt::apart;
+void check_apart(const Tensor& a, const char* a_name, const Tensor& b, const char* b_name) {
+  if (!a.defined() || !b.defined() || a.numel() == 0 || b.numel() == 0) return;
+  const auto at = [](const Tensor& t) { return reinterpret_cast<intptr_t>(t.data_ptr()); };
+  const auto where = [](const Tensor& t) { return Footprint(t.dim(), t.sizes().data(), t.strides().data(), t.element_size()); };
+  TORCH_CHECK(apart(where(a), 0, where(b), 0, at(b) - at(a)), a_name, " must not overlap ", b_name);
+}
 void no_gradient_asked(const char* what, std::initializer_list<const Tensor*> all) {
   for (const Tensor* t : all)
     if (t->defined() && ((at::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined()))
@@ -571,7 +579,9 @@ void paged_append(const Tensor& k_in, const Tensor& v_in, const Tensor& k_pages,
       check(t->sizes() == k.sizes(), "v and v_first must have k's shape");
     }
   if (coef.defined()) check(coef.numel() == 2, "vr_coef must have two elements");
-  if (at::has_internal_overlap(k_pages) != at::MemOverlap::Yes) at::assert_no_overlap(k_pages, v_pages);  // the entry refuses the other kind
+  if (at::has_internal_overlap(k_pages) != at::MemOverlap::Yes) check_apart(k_pages, "k_pages", v_pages, "v_pages");  // the entry refuses the other kind
+  for (const Tensor* t : {&k, &v, &v_first})
+    for (const Tensor* pool : {&k_pages, &v_pages}) check_apart(*pool, "the pages", *t, "k, v or v_first");
   for (const Tensor* t : {&k_pages, &v_pages})
     check(!t->is_inference() || c10::InferenceMode::is_enabled(), "pages made in inference mode can be appended to in inference mode only");
   if (k.numel() == 0) return;
@@ -617,8 +627,8 @@ std::pair<Tensor, Tensor> paged_attention(const Tensor& q_in, const Tensor& k_pa
     if (out.scalar_type() != q.scalar_type()) throw BadType(std::string("out must have q's dtype, got ") + c10::toString(out.scalar_type()));
     check(out.device() == dev && out.sizes() == q.sizes() && (out.stride(2) == 1 || out.size(2) == 1), "out must have q's shape and device, contiguous in head_dim");
     check(out.data_ptr() != q.data_ptr() || q.numel() == 0, "out must not be q: a row is read again after others are written");
-    for (const Tensor* t : {&q, &k_pages, &v_pages}) at::assert_no_overlap(out, *t);
-    if (gate.defined()) at::assert_no_overlap(out, gate);
+    const Tensor starts = defined_or_none(seq_start);
+    for (const Tensor* t : {&q, &k_pages, &v_pages, &gate, &table, &kv_len, &starts, &prefix, &gq32, &gk32, &cos, &sin}) check_apart(out, "out", *t, "an input");
     check(!out.is_inference() || c10::InferenceMode::is_enabled(), "out made in inference mode can be written in inference mode only");
   }
   const Tensor y = out.defined() ? out : at::empty(q.sizes(), q.options());

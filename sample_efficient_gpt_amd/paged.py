@@ -85,7 +85,7 @@ def paged_kv_append(k, v, k_pages, v_pages, block_table, kv_len, *, seq_start=No
 
     max_len: no sequence holds more keys (default: what its table row can).  Lengths and tables are read on the device: a row whose position
     is negative or not below max_len, or whose page number is not in the pool, is left out.  Two rows of one call must not have one
-    slot: sequences must not append into a page they share."""
+    slot: sequences must not append into a page they share.  The rows must not lie in the pools (RuntimeError)."""
     if k.is_cuda and not _seen_as_operator(k, v, k_pages, v_pages, block_table, kv_len, seq_start, v_first, vr_coef, rope_cos, rope_sin):
         _native.load().paged_append(k, v, k_pages, v_pages, block_table, kv_len, seq_start, v_first, vr_coef, eps, qk_norm, rope_cos, rope_sin,
                                     rope_pos0, max_len)
@@ -120,7 +120,7 @@ def paged_attention(q, k_pages, v_pages, block_table, kv_len, g_q, g_k=None, *, 
     ``1/sqrt(D)``: as in ``qknorm_attention``.  Returns y ``[T, H, D]`` (and the natural log-sum-exp ``[T, H]``, fp32).
 
     A row that sees no key gives y = 0 and lse = -inf.  Rows in no sequence (behind ``seq_start[-1]``) are zero in a y that is allocated
-    here, and left as they are in ``out``; their lse is -inf.  A sequence whose length is negative or above max_len, or whose
+    here, and left as they are in ``out``, which must not overlap an input (RuntimeError); their lse is -inf.  A sequence whose length is negative or above max_len, or whose
     table has a page number that is not in the pool, gives NaN.  A key or value that is not finite takes part in the rows that see it as the formula
     has it, and shows in no other: a key with a NaN gives NaN, one with an infinity NaN or, where its score is -inf, no weight; a value
     that is not finite is what its component of y becomes."""

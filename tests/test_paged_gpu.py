@@ -724,3 +724,35 @@ def test_row_ranges_that_overlap_beyond_32_bits(gpu_device):
     call(starts, B)
     torch.cuda.synchronize()
     assert torch.equal(call(one, 1), clean)
+
+
+def test_outputs_that_overlap_inputs_are_refused(gpu_device):
+    """Rows are read again after others are written.  Views of one buffer that lie side by side in every row are no overlap."""
+    rows, lens, H, Hkv, D = [1, 70], [20, 90], 6, 2, 64
+    x = Batch(rows, lens, H, Hkv, D, 16, BF16, gpu_device, seed=36)
+    want = attend(x, gate_logits=x.gate)
+    T = sum(rows)
+    wide = torch.zeros(T, 2 * H * D + 64, dtype=BF16, device=gpu_device)
+    q, beside = (wide[:, i * H * D:(i + 1) * H * D].unflatten(-1, (H, D)) for i in range(2))
+    shifted = wide[:, 3 * D:(H + 3) * D].unflatten(-1, (H, D))
+    gate = wide[:, 2 * H * D:2 * H * D + H]
+    q.copy_(x.q)
+    gate.copy_(x.gate)
+    x.q = q
+    with pytest.raises(RuntimeError, match="overlap"):
+        attend(x, out=shifted)
+    with pytest.raises(RuntimeError, match="overlap"):
+        attend(x, gate_logits=beside[:, :, 0], out=beside)
+    pools = torch.zeros(2, x.n_pages, Hkv, 16, D + 8, dtype=BF16, device=gpu_device)[..., :D]  # rows apart
+    pools[0], pools[1] = x.k_pages, x.v_pages
+    x.k_pages, x.v_pages = pools[0], pools[1]
+    inside = pools.as_strided((T, H, D), (H * (D + 8), D + 8, 1))
+    with pytest.raises(RuntimeError, match="overlap"):
+        attend(x, out=inside)
+    assert torch.equal(attend(x, gate_logits=gate, out=beside), want) and torch.equal(x.q, q)
+    k = x.k_pages[:3].flatten(0, 1).transpose(0, 1)[:, :Hkv]  # rows of the pool itself
+    starts = torch.tensor([0, 1, k.shape[0]], dtype=torch.int32, device=gpu_device)
+    fresh = torch.zeros_like(k)
+    for a, b, first in ((k, fresh, None), (fresh, k, None), (fresh, fresh, k)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            paged_kv_append(a, b, x.k_pages, x.v_pages, x.block_table, x.kv_len, seq_start=starts, v_first=first, vr_coef=None if first is None else x.coef)

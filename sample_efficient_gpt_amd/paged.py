@@ -144,7 +144,8 @@ class PageTable:
     """Which pages of a pool hold the keys of which sequence, for a batch of sequences and all layers of a model.
 
     ``extend(n)`` before a step makes room for its rows: n more for every sequence, or a list with a number for each.  The device
-    tensors ``block_table``, ``kv_len`` and ``seq_start`` are updated in place, so that a captured step sees them; only an extension
+    tensors ``block_table``, ``kv_len`` and ``seq_start`` are updated in place, so that a captured step sees them: one that was captured with a
+    ``seq_start`` serves any step of no more rows, one without (the same number for every sequence) those of that number.  Only an extension
     that begins a new page copies a table from the host.  ``release(b)`` ends sequence b: its pages go back, and it starts again at length 0.
 
     max_len: keys a sequence may hold.  n_pages: pages of the pool (default: as many as a full batch and the prefix need).
@@ -165,7 +166,7 @@ class PageTable:
         self._host = torch.zeros(batch, width, dtype=torch.int32)
         self.block_table = torch.zeros(batch, width, dtype=torch.int32, device=device)
         self.kv_len = torch.zeros(batch, dtype=torch.int32, device=device)
-        self._starts = torch.zeros(batch + 1, dtype=torch.int32, device=device)
+        self._starts = None  # handed out as seq_start by the first step of unequal numbers; kept up to date from then on
         self.seq_start, self.rows = None, 0  # of the step that was last made room for: None means rows / batch each
         self.prefix = self.prefix_table = None
         if prefix_len:
@@ -198,10 +199,15 @@ class PageTable:
         if len(set(each)) == 1:
             self.seq_start = None
             self.kv_len.add_(each[0])
+            if self._starts is not None:
+                torch.mul(self._numbers, each[0], out=self._starts)
         else:
             starts = [0]
             for x in each:
                 starts.append(starts[-1] + x)
+            if self._starts is None:
+                self._numbers = torch.arange(self.batch + 1, dtype=torch.int32, device=self.kv_len.device)
+                self._starts = torch.empty_like(self._numbers)
             self._starts.copy_(torch.tensor(starts, dtype=torch.int32))
             self.kv_len.copy_(torch.tensor(after, dtype=torch.int32))
             self.seq_start = self._starts

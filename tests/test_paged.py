@@ -216,3 +216,19 @@ def test_launches_of_more_threads_than_one_may_have(lib):
     p.k_pages = p.v_pages = _lib.Tensor4(0x10000, 4 * 16 * 128, 16 * 128, 128)
     p.k = p.v = _lib.Rows(0x10000, 4 * 128, 128)
     assert lib.segpt_paged_append(p, None) == -4
+
+
+def test_page_table_keeps_the_row_ranges_that_it_handed_out():
+    """A captured step holds on to ``seq_start``: it has to follow steps with one number for all sequences as well."""
+    t = PageTable(3, 100, 16, device="cpu")
+    t.extend(2)
+    assert t.seq_start is None
+    t.extend([2, 0, 1])
+    held = t.seq_start
+    assert held.tolist() == [0, 2, 2, 3]
+    t.extend(1)
+    assert t.seq_start is None and held.tolist() == [0, 1, 2, 3]
+    t.extend([0, 0, 5])
+    assert t.seq_start is held and held.tolist() == [0, 0, 0, 5]
+    t.extend(0)
+    assert held.tolist() == [0, 0, 0, 0] and t.kv_len.tolist() == [5, 3, 9] == t.lengths

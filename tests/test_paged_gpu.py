@@ -756,3 +756,29 @@ def test_outputs_that_overlap_inputs_are_refused(gpu_device):
     for a, b, first in ((k, fresh, None), (fresh, k, None), (fresh, fresh, k)):
         with pytest.raises(RuntimeError, match="overlap"):
             paged_kv_append(a, b, x.k_pages, x.v_pages, x.block_table, x.kv_len, seq_start=starts, v_first=first, vr_coef=None if first is None else x.coef)
+
+
+def test_a_captured_step_of_unequal_numbers_serves_equal_ones(gpu_device):
+    H, Hkv, D = 6, 2, 64
+    pages = PageTable(3, 100, 16, device=gpu_device)
+    cache = PagedKVCache(pages, Hkv, D)
+    gain = torch.ones(1, device=gpu_device)
+    q, k, v = (torch.randn(6, h, D, device=gpu_device).to(BF16) for h in (H, Hkv, Hkv))
+
+    def step(n=6):
+        cache.append(k[:n], v[:n])
+        return cache.attend(q[:n], gain)
+
+    pages.extend([3, 1, 2])
+    step()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = step()
+    for rows in (1, [2, 0, 4], 2, [1, 0, 0], 1):
+        pages.extend(rows)
+        for t in (q, k, v):
+            t.copy_(torch.randn_like(t))
+        g.replay()
+        n = pages.rows
+        got = y.clone()
+        assert torch.equal(got[:n], step(n)) and (got[n:] == 0).all(), rows

@@ -71,6 +71,12 @@ def _(out, q, k_pages, v_pages, prefix_table, prefix_len, block_table, kv_len, g
     return q.new_empty(q.shape[:2], dtype=torch.float32)
 
 
+def _no_gradient_asked(what, *operands):
+    """The registered operators run below autograd and cannot see that a gradient is asked for."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands):
+        raise AssertionError(f"{what} has no derivative: call it under torch.no_grad() or on detached tensors")
+
+
 def paged_kv_append(k, v, k_pages, v_pages, block_table, kv_len, *, seq_start=None, v_first=None, vr_coef=None, eps=1e-6, qk_norm=True,
                     rope_cos=None, rope_sin=None, rope_pos0=0, max_len=None):
     """Writes the rows k, v ``[T, Hkv, D]`` (any strides, last dim contiguous, rows 16 B aligned) into the pages of their sequences.
@@ -90,6 +96,7 @@ def paged_kv_append(k, v, k_pages, v_pages, block_table, kv_len, *, seq_start=No
         _native.load().paged_append(k, v, k_pages, v_pages, block_table, kv_len, seq_start, v_first, vr_coef, eps, qk_norm, rope_cos, rope_sin,
                                     rope_pos0, max_len)
     else:
+        _no_gradient_asked("paged_kv_append", k, v, k_pages, v_pages, v_first, vr_coef)
         torch.ops.segpt.paged_kv_append(k, v, k_pages, v_pages, block_table, kv_len, seq_start, v_first, vr_coef, float(eps), bool(qk_norm),
                                         rope_cos, rope_sin, int(rope_pos0), max_len)
 
@@ -101,6 +108,7 @@ def _attend(q, k_pages, v_pages, prefix_table, prefix_len, block_table, kv_len, 
         y, lse = _native.load().paged_attention(q, k_pages, v_pages, prefix_table, prefix_len, block_table, kv_len, g_q, g_k, seq_start, gate_logits,
                                                 gate_scale, eps, sm_scale, qk_norm, rope_cos, rope_sin, rope_pos0, max_len, out, return_lse)
         return (y, lse) if return_lse else y
+    _no_gradient_asked("paged attention", q, k_pages, v_pages, g_q, g_k, gate_logits, out)
     args = (q, k_pages, v_pages, prefix_table, int(prefix_len), block_table, kv_len, g_q, g_k, seq_start, gate_logits, float(gate_scale), float(eps),
             float(1.0 / math.sqrt(q.shape[-1]) if sm_scale is None else sm_scale), bool(qk_norm), rope_cos, rope_sin, int(rope_pos0), max_len)
     if out is None:

@@ -232,3 +232,18 @@ def test_page_table_keeps_the_row_ranges_that_it_handed_out():
     assert t.seq_start is held and held.tolist() == [0, 0, 0, 5]
     t.extend(0)
     assert held.tolist() == [0, 0, 0, 0] and t.kv_len.tolist() == [5, 3, 9] == t.lengths
+
+
+def test_a_gradient_is_refused_before_anything_else():
+    """Also where the call is made as a registered operator, which runs below autograd: an append would drop the gradient without a word."""
+    pages = torch.zeros(3, 2, 16, 64, dtype=torch.bfloat16)
+    table, lens = torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    z, g = (torch.zeros(2, 2, 64, dtype=torch.bfloat16) for _ in range(2))
+    g.requires_grad_()
+    calls = [lambda: paged_kv_append(g, z, pages, pages, table, lens), lambda: paged_kv_append(z, z, pages, pages, table, lens, v_first=g, vr_coef=torch.ones(2)),
+             lambda: paged_attention(g, pages, pages, table, lens, torch.ones(1)), lambda: paged_attention(z, pages, pages, table, lens, torch.ones(1, requires_grad=True))]
+    for call in calls:
+        with pytest.raises(AssertionError, match="no derivative"):
+            call()
+        with torch.no_grad(), pytest.raises(AssertionError, match="device tensors"):
+            call()

@@ -782,3 +782,20 @@ def test_a_captured_step_of_unequal_numbers_serves_equal_ones(gpu_device):
         n = pages.rows
         got = y.clone()
         assert torch.equal(got[:n], step(n)) and (got[n:] == 0).all(), rows
+
+
+def test_an_append_of_rows_with_a_gradient_is_refused_under_compilation(gpu_device):
+    x = Batch([1, 9], [40, 20], 6, 2, 64, 16, BF16, gpu_device, seed=37)
+    k = x.k.clone().requires_grad_()
+    before = x.k_pages.clone()
+
+    def f(k):
+        paged_kv_append(k, x.v, x.k_pages, x.v_pages, x.block_table, x.kv_len, seq_start=x.seq_start)
+        return x.k_pages * 1
+
+    with pytest.raises(Exception, match="no derivative"):
+        torch.compile(f, backend="aot_eager", fullgraph=True)(k)
+    assert torch.equal(x.k_pages, before)
+    with torch.no_grad():
+        torch.compile(f, backend="aot_eager", fullgraph=True)(k)
+    assert not torch.equal(x.k_pages, before)

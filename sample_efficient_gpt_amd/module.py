@@ -238,6 +238,10 @@ class MultiHeadSelfAttention(nn.Module):
         """`x` is the rows the cache's table was extended for: [b, S, d_model], or [1, rows, d_model] where the sequences have unequal
         numbers of them.  Values are handed on for these rows only: what earlier ones mixed is in the pages."""
         b, S, d_model = x.shape
+        pages = cache.pages
+        if b != 1 and (pages.seq_start is not None or b != pages.batch):
+            raise ValueError(f"x must be [1, {pages.rows}, {d_model}]" + ("" if pages.seq_start is not None else f" or [{pages.batch}, {pages.rows // pages.batch}, {d_model}]")
+                             + f" for the rows the cache's table was extended for, got {tuple(x.shape)}")
         H, Hkv = self.n_heads, self.n_kv_heads
         d = d_model // H
         rows = self.qkv(x).flatten(0, 1)

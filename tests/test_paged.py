@@ -247,3 +247,21 @@ def test_a_gradient_is_refused_before_anything_else():
             call()
         with torch.no_grad(), pytest.raises(AssertionError, match="device tensors"):
             call()
+
+
+def test_module_refuses_rows_in_another_order():
+    """Rows of a step with unequal numbers are packed; [B, S, d] is for S rows of every sequence."""
+    from sample_efficient_gpt_amd import MultiHeadSelfAttention
+
+    m = MultiHeadSelfAttention(128, 2, 2, max_seq_len=64, qknorm=True)
+    t = PageTable(3, 64, 16, device="cpu")
+    c = PagedKVCache(t, 2, 64)
+    with torch.no_grad():
+        t.extend([4, 1, 1])
+        for shape in ((3, 2), (2, 3), (6, 1)):
+            with pytest.raises(ValueError, match="1, 6, 128"):
+                m(torch.zeros(*shape, 128), kv_cache=c)
+        t.extend(2)
+        for shape in ((2, 3), (6, 1)):
+            with pytest.raises(ValueError, match="3, 2, 128"):
+                m(torch.zeros(*shape, 128), kv_cache=c)

@@ -57,7 +57,11 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(segpt_paged_para
   int b, r0, n;
   if (p.seq_start) {
     b = sequence_of_row(p, (int)(first / p.Hkv), lane);
-    while (b + 1 < p.B && p.seq_start[b + 1] <= t) ++b;
+    // a later row of the wave: mostly the next sequence, but any number without rows may lie between
+    int step = 1;
+    for (; b + step < p.B && p.seq_start[b + step] <= t; step *= 2) b += step;
+    while (step >>= 1)
+      if (b + step < p.B && p.seq_start[b + step] <= t) b += step;
   } else {
     b = t / rows_each;
   }

@@ -799,3 +799,37 @@ def test_an_append_of_rows_with_a_gradient_is_refused_under_compilation(gpu_devi
     with torch.no_grad():
         torch.compile(f, backend="aot_eager", fullgraph=True)(k)
     assert not torch.equal(x.k_pages, before)
+
+
+@pytest.mark.parametrize("gaps", [[0, 0, 0], [1, 2, 3, 4, 5, 6, 7, 8, 9], [1 << 20, 5, 0, 1 << 19, 63, 64, 65]])
+def test_an_append_behind_sequences_without_rows(gpu_device, gaps):
+    """Rows of neighbouring sequences with that many in between that bring none: a row finds its own in a few loads, not in one for each of those (2^20
+    of them one after the other took 100 ms)."""
+    page, Hkv, D = 8, 2, 64
+    has = [0]
+    for n in gaps:
+        has.append(has[-1] + n + 1)
+    B, T = has[-1] + 1, len(has)
+    rows = torch.zeros(B, dtype=torch.int32)
+    rows[has] = 1
+    starts = torch.cat([torch.zeros(1, dtype=torch.int32), rows.cumsum(0).int()]).to(gpu_device)
+    lens = torch.randint(0, 8, (B,), dtype=torch.int32)
+    lens[has] = torch.arange(1, T + 1, dtype=torch.int32) % 8 + 1
+    table = torch.zeros(B, 1, dtype=torch.int32)
+    table[has, 0] = torch.arange(T, dtype=torch.int32)
+    k, v = (torch.randn(T, Hkv, D, device=gpu_device).to(BF16) for _ in range(2))
+    kp, vp = torch.zeros(2, T, Hkv, page, D, dtype=BF16, device=gpu_device)
+    want = kp.clone(), vp.clone()
+    for t, b in enumerate(has):
+        for w, x in zip(want, (k, v)):
+            w[t, :, int(lens[b]) - 1] = x[t]
+    table, lens = table.to(gpu_device), lens.to(gpu_device)
+    call = lambda: paged_kv_append(k, v, kp, vp, table, lens, seq_start=starts, qk_norm=False)
+    call()
+    a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    a.record()
+    call()
+    b.record()
+    torch.cuda.synchronize()
+    assert torch.equal(kp, want[0]) and torch.equal(vp, want[1])
+    assert a.elapsed_time(b) < 20

@@ -266,7 +266,7 @@ __device__ __forceinline__ Found find_entry(const PagedArgs& a, int lane, int re
 }
 // The plan of more than kKept * 64 entries, by one workgroup: lengths of the shares and running sums.  Formed by every wave for itself, an entry's
 // numbers are read by all of them, several times over, and the time grows with the square of the entries.  Single tokens, 18 / 6 heads of 64, us, by
-// every wave and here: 300 sequences 132, 134; 1000 200, 197; 4000 590, 247.
+// every wave and here: 300 sequences 132, 134; 1000 200, 197; 4000 586, 244.
 constexpr int kPlanThreads = 1024;
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a) {
   constexpr int kWaves = kPlanThreads / 64;
@@ -363,8 +363,8 @@ __device__ __forceinline__ void two_parts(float a, float b, uint32_t& first, uin
 // bf16 has a second operand, what the first one's rounding left, so that scores are as good as the pool's keys.  With one operand, and probabilities
 // rounded once, the error against 64 bits is 2.9e-3 of y, of which 1.7e-3 is y's own rounding: more than one and a half times what it has to be.
 // In FEW the further products are hidden (a block's products are 400 cycles of the 4400 that its bytes take).  In MANY they cost what they are: six
-// prompts of 333 .. 4096 tokens, 18 / 6 heads of 64, 148 -> 171 us (2.5e-3 -> 2.1e-3), with 16 / 4 of 128 213 -> 266; 512 rows beside 15 tokens 56 -> 62
-// (2.9e-3 -> 2.3e-3); 128 tokens behind 16001 keys, 16 / 4 heads of 128, 50 -> 58 (2.9e-3 -> 2.3e-3); 32 behind 8192 20.6 -> 21.1.  The probabilities in
+// prompts of 333 .. 4096 tokens, 18 / 6 heads of 64, 148 -> 169 us (2.5e-3 -> 2.1e-3), with 16 / 4 of 128 208 -> 257; 512 rows beside 15 tokens 56 -> 62
+// (2.9e-3 -> 2.3e-3); 128 tokens behind 16001 keys, 16 / 4 heads of 128, 49 -> 55 (2.9e-3 -> 2.3e-3); 32 behind 8192 20.6 -> 21.0.  The probabilities in
 // two parts instead: 188, 268, 67, 54 and 21.4, the same errors.
 template <typename E, int D>
 struct Query;
@@ -699,7 +699,7 @@ struct Values<uint16_t, D> {
   }
   // Adds the probabilities s to the sums l and their products with the values to o.  FINE: in two bf16 parts, so that y's own rounding is all its error
   // (2.3e-3 of y -> 1.65e-3).  FEW has it beside its loads (32 tokens of 200 .. 8192 keys 44.3 -> 44.7 us, 48 of 255 .. 16000 153 -> 155); in MANY,
-  // where the vector port is what is short, the prompts above would take 214 us instead of 169: there they are rounded once and summed as rounded.
+  // the prompts above would take 214 us instead of 169: there they are rounded once and summed as rounded.
   template <bool FINE>
   __device__ __forceinline__ void add(f32x16 s, float (&l)[2], f32x16 (&o)[MB]) const {
     bf16x8 pb[2], rest[2];
@@ -975,8 +975,10 @@ __device__ __forceinline__ void few_columns(const PagedArgs& a, const Item& it, 
 // scores of tile jt + 1 beside the exponentials of tile jt and its product with the values, so that the matrix pipe has work while
 // the exponentials are formed.  Per turn: wait for tile jt + 1, barrier (also: everyone has left tile jt - 1), request tile jt + kStages - 1 over
 // that one, compute.
-// Bound by the vector port beside the matrix pipe (12 vector instructions a matrix instruction): a prompt of 8192 tokens, 18 / 6 heads of 64,
-// 195 us (790 TFLOP/s); short shares by their start, about 10 us until the first products.
+// Six prompts of 333 .. 4096 tokens, 18 / 6 heads of 64: the matrix pipe is busy for 41 % of the time (a third of it with the query's second part), the
+// vector port for 52 %, 8 vector instructions a matrix instruction; with two waves a SIMD neither is full.  A third of the cycles of the LDS are
+// bank conflicts at 128-byte rows.  A prompt of 8192 tokens takes 232 us (666 TFLOP/s without the second part's products); short shares are bound
+// by their start, about 10 us until the first products.
 template <typename E, int D>
 __device__ __forceinline__ void many_columns(const PagedArgs& a, const Item& it, int rep, int tid, uint32_t lds, int* table, float* gsm, int* any_bad) {
   using S = Shape<E, D>;
@@ -1136,7 +1138,7 @@ __device__ __forceinline__ void leave_plan(const PagedArgs& a, int lane, int rep
 }
 
 // Launches whose entries are all FEW: a workgroup is one wave, eight a CU (twelve: the same work in more shares, 49.6 -> 52.5 us).  Bound by HBM:
-// 32 tokens, 200 .. 8192 keys, 18 / 6 heads of 64: 213 MB in 44 us (4.8 TB/s); 48 tokens, 255 .. 16000 keys, 16 / 4 heads of 128: 803 MB in 147 us
+// 32 tokens, 200 .. 8192 keys, 18 / 6 heads of 64: 213 MB in 45 us (4.7 TB/s); 48 tokens, 255 .. 16000 keys, 16 / 4 heads of 128: 803 MB in 149 us
 // (5.4 TB/s).  A single token's 4096 keys take 8.7 us: launch and three dependent round trips (lengths, page numbers, keys); the plan's arithmetic is 0.3.
 template <typename E, int D>
 __global__ __launch_bounds__(64, (Shape<E, D>::kOcc)) void paged_few_kernel(PagedArgs a) {
@@ -1153,9 +1155,9 @@ __global__ __launch_bounds__(64, (Shape<E, D>::kOcc)) void paged_few_kernel(Page
   if (it.valid) few_columns<E, D>(a, it, rep, lane, lds_addr_of(lds), table, gsm);
 }
 
-// Any launch: the first workgroups are items of many columns, the next four items each of few, the rest have none.  (With a fixed number
-// of workgroups for the first kind those without an item kept the second kind
-// waiting: 128 rows beside 15 tokens 45.9 us, now 40.4.)
+// Any launch: the first workgroups are items of many columns, the next four items each of few, the rest have none.  (With a fixed number of
+// workgroups for the first kind those without an item, which still go through the plan, kept the second kind waiting: 128 rows beside 15 tokens 45.9
+// instead of 40.4 us.)
 template <typename E, int D>
 __global__ __launch_bounds__(256, (Shape<E, D>::kOcc)) void paged_any_kernel(PagedArgs a) {
   using S = Shape<E, D>;
@@ -1182,7 +1184,7 @@ __global__ __launch_bounds__(256, (Shape<E, D>::kOcc)) void paged_any_kernel(Pag
 
 // Joins the partial results of `per_sub` columns of a tile: its sequence's shares and, behind them, the prefix's.  A unit of D / 4 lanes holds a
 // row; as many units stand side by side over the shares of a column as leave each one batch of kBatch that is requested together, and
-// their sums meet in LDS.  Fixed order: deterministic.  4.6 us for one token of 18 heads (launch and two round trips), 5.8 for 32 of them, 12 for
+// their sums meet in LDS.  Fixed order: deterministic.  4.9 us for one token of 18 heads (launch and two round trips), 5.9 for 32 of them, 12 for
 // 128 tokens of 16 heads of 128 behind a prefix (25 MB).
 constexpr int kMergeThreads = 256;
 template <typename E, int D>
@@ -1299,12 +1301,12 @@ size_t plan(const segpt_paged_params& p, PagedArgs& a) {
   a.log_page = __builtin_ctz((unsigned)p.page_size);
   a.capacity = paged_capacity(p);
   // 512 workgroups are resident, two a CU.  The shares' length is found in three steps and may leave a few more than asked for, and one that has to wait
-  // for a place is a round of its own: 480 are asked for, 496 where all are single waves (us, asked for 512 and now: 512 rows beside 31 tokens
-  // 79.5, 64; beside 63 126, 105; beside 15 52.7, 52.4; 128 rows beside 15 39.6, 42.5; eight fp32 tokens 20.0, 18.1; 128 of bf16 179, 175).  Where the host sees that the work
-  // is of many columns (a prefix, prompts of equal length) three on two CUs: longer shares leave a quarter less to be joined, which is more than
-  // the idle places would have done (480 and 384: 128 tokens behind a prefix of 16001, 16 / 4 heads of 128, 51.5, 48.7; 32 behind 8192,
-  // 18 / 6 of 64, 23.6, 22.0; 512 and 384: a prompt of 1024 tokens 32.0, 29.7, of 2048 42.0, 39.6).  fp32 rows of 512 bytes: one a CU, all of them
-  // (fewer: 32 tokens 77, 80; 100 118, 129).
+  // for a place is a round of its own: 480 are asked for, 496 where all are single waves (us, asked for 512 and now; 18 / 6 heads of 64, up to 8192 keys:
+  // 512 rows beside 31 tokens 78, 73; beside 63 132, 111; beside 15 66, 66; 128 rows beside 15 40.7, 45.2; eight fp32 tokens 19.9, 17.8; 128 of bf16
+  // 102, 103).  Where the host sees that the work is of many columns (a prefix, prompts of equal length) three on two CUs: longer shares leave a
+  // quarter less to be joined, which is more than the idle places would have done (512 and 384: a prompt of 1024 tokens 33.6, 31.0, of 2048 46.2, 42.8,
+  // of 8192 237, 237, four of 512 34.8, 21.3; 32 tokens behind 8192 keys 23.3, 21.8; 128 behind 16001, 16 / 4 heads of 128, 57 .. 60 either way).  fp32 rows
+  // of 512 bytes: one a CU, all of them (256 and 224: 32 tokens of 16 / 4 heads 48.5, 53.6; 100 122, 134; of 4 / 2 heads 80, 66).
   const bool wide = a.shared || (!p.seq_start && (int64_t)rep * a.rows_each > kFew);
   a.target = row_bytes > 256 ? 256 : wide ? 384 : p.seq_start ? 480 : 496;
   a.min_few = 2;

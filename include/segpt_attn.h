@@ -357,6 +357,38 @@ size_t segpt_paged_workspace_bytes(const segpt_paged_params* p);
  * prefix's own keys (as its last token does, in a sequence without keys yet), and sees what is at or before that.  Forward only. */
 int segpt_paged_attn(const segpt_paged_params* p, void* stream);
 
+/* ---- Paged key/value cache of 8 or 4 bits.
+ * A stored row is the prepared row above (k', v') in blocks of SEGPT_SCALE_BLOCK components, each with one scale, a power of two:
+ *   e = the smallest number from -110 on with max |x| <= 2^e top,    component i = code(x_i / 2^e), the nearest code, ties to the even one
+ * SEGPT_POOL_E4M3: one byte a component, four bits of exponent (bias 7) and three of mantissa, top = 448.
+ * SEGPT_POOL_E2M1: half a byte, the first component of a pair in the low half: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives, top = 6.
+ * The scale is held as the byte e + 127.  Rows are prepared in 64 bits, so that the codes are those of the exact value.  A block with a
+ * component that is not finite, or beyond top 2^119 (E2M1: top 2^125), has the scale 255 and is NaN as a whole, when it is read and
+ * in the attention; everything else that is stored is finite, and exact in bf16.  The reference has no such cache.
+ *
+ * The calls below are those above with such pools: segpt_paged_params as there, dtype that of the rows, head_dim 64 or 128, and
+ * k_pages, v_pages [n_pages, Hkv, page_size, D (E2M1: D / 2)] of bytes, strides in BYTES, rows 16-byte aligned. */
+#define SEGPT_SCALE_BLOCK 32
+#define SEGPT_POOL_E4M3 1
+#define SEGPT_POOL_E2M1 2
+
+typedef struct segpt_paged_quant {
+  uint32_t struct_bytes; /* = sizeof(segpt_paged_quant) */
+  int32_t format;        /* SEGPT_POOL_* */
+  segpt_tensor4 k_scales; /* [n_pages, Hkv, page_size, D / 32] bytes, strides in BYTES; rows aligned to D / 32 bytes */
+  segpt_tensor4 v_scales;
+} segpt_paged_quant;
+
+int segpt_paged_append_quant(const segpt_paged_params* p, const segpt_paged_quant* q, void* stream);
+size_t segpt_paged_quant_workspace_bytes(const segpt_paged_params* p, const segpt_paged_quant* q);
+int segpt_paged_attn_quant(const segpt_paged_params* p, const segpt_paged_quant* q, void* stream);
+
+/* Stored rows back as rows: row i of n of sequence b of k and v, [T, Hkv, D], both written here, is what the pages hold for key
+ * kv_len[b] - n + i.  q == NULL: a pool of the rows' dtype (any head_dim of the calls above).  A row before the first key is 0; every row of
+ * a sequence whose length is negative or above max_len, and a row whose page number is not in the pool, is NaN; rows in no sequence are left
+ * alone (SEGPT_FLAG_ZERO_REST: set to 0).  k and v must not overlap each other or the pools.  H, angles and what belongs to the attention are not looked at. */
+int segpt_paged_read(const segpt_paged_params* p, const segpt_paged_quant* q, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

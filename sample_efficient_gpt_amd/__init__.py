@@ -10,7 +10,7 @@ through the C ABI of ``libsegpt_attn.so``; there is no fallback path.
 from .function import FlashAttnFunc, QKNormFlashAttnFunc, TritonFlashAttnQKNormFunc, qknorm_attention  # noqa: F401
 from .module import KVCache, MultiHeadSelfAttention, SelfDotProductAttnQKNorm  # noqa: F401
 from .library_op import qknorm_attention_op  # noqa: F401  (registers torch.ops.segpt.qknorm_attention)
-from .paged import PagedKVCache, PageTable, paged_attention, paged_kv_append, shared_prefix_attention  # noqa: F401
+from .paged import PagedKVCache, PageTable, paged_attention, paged_kv_append, paged_kv_read, shared_prefix_attention  # noqa: F401
 from .inputs import CONFIGS, AttnConfig, make_inputs  # noqa: F401
 
 # the reference's class names, so `from ... import TritonFlashAttnFunc` call sites keep working

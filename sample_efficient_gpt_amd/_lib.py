@@ -21,6 +21,9 @@ SEGPT_FLAG_DECODE = 4
 SEGPT_FLAG_NO_NORM = 8
 SEGPT_FLAG_F32_SPLIT = 16
 SEGPT_FLAG_ZERO_REST = 32
+SEGPT_SCALE_BLOCK = 32
+SEGPT_POOL_E4M3 = 1
+SEGPT_POOL_E2M1 = 2
 SEGPT_E_PAGES = -14
 SEGPT_E_SCRATCH_LIMIT = -13
 SEGPT_NOALLOC_SCRATCH_BYTES = 16 << 20
@@ -45,6 +48,10 @@ EXPORTED_SYMBOLS = (
     "segpt_paged_append",
     "segpt_paged_workspace_bytes",
     "segpt_paged_attn",
+    "segpt_paged_append_quant",
+    "segpt_paged_quant_workspace_bytes",
+    "segpt_paged_attn_quant",
+    "segpt_paged_read",
 )
 
 
@@ -124,6 +131,10 @@ class PagedParams(C.Structure):
     ]
 
 
+class PagedQuant(C.Structure):
+    _fields_ = [("struct_bytes", C.c_uint32), ("format", C.c_int32), ("k_scales", Tensor4), ("v_scales", Tensor4)]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -174,6 +185,11 @@ def load():
         lib.segpt_paged_workspace_bytes.argtypes = [C.POINTER(PagedParams)]
         lib.segpt_paged_attn.restype = C.c_int
         lib.segpt_paged_attn.argtypes = [C.POINTER(PagedParams), C.c_void_p]
+        for name in ("segpt_paged_append_quant", "segpt_paged_attn_quant", "segpt_paged_read"):
+            getattr(lib, name).restype = C.c_int
+            getattr(lib, name).argtypes = [C.POINTER(PagedParams), C.POINTER(PagedQuant), C.c_void_p]
+        lib.segpt_paged_quant_workspace_bytes.restype = C.c_size_t
+        lib.segpt_paged_quant_workspace_bytes.argtypes = [C.POINTER(PagedParams), C.POINTER(PagedQuant)]
         ver = lib.segpt_abi_version()
         if ver != SEGPT_ABI_VERSION:
             raise RuntimeError(f"libsegpt_attn.so ABI version {ver}, binding expects {SEGPT_ABI_VERSION}")

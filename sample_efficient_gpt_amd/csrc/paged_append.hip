@@ -19,20 +19,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Sequence of row t, for a whole wave: the number of the last sequence that starts at or before it.  64 starts are looked at a time, so
-// that a batch of up to 64 sequences is one load, of up to 4096 two one after the other.
-__device__ __forceinline__ int sequence_of_row(const segpt_paged_params& p, int t, int lane) {
-  int lo = 0, n = p.B;
-  while (true) {
-    const int step = (n + 63) / 64, i = lane * step;
-    const bool before = i < n && p.seq_start[lo + i] <= t;
-    const int k = __popcll(__builtin_amdgcn_ballot_w64(before));
-    if (k > 0) lo += (k - 1) * step;
-    if (step == 1) return lo;
-    n = min(step, p.B - lo);
-  }
-}
-
 template <typename E, int D, bool ROPE, bool MIX>
 __global__ __launch_bounds__(kThreads) void paged_append_kernel(segpt_paged_params p, int log_page, int rows_each, int capacity) {
   constexpr int VEC = 16 / sizeof(E), LPR = D / 2 / VEC, kRowsPerWave = 64 / LPR;
@@ -54,17 +40,8 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(segpt_paged_para
   load(p.v, v);
   if constexpr (MIX) load(p.v_first, f);
 
-  int b, r0, n;
-  if (p.seq_start) {
-    b = sequence_of_row(p, (int)(first / p.Hkv), lane);
-    // a later row of the wave: mostly the next sequence, but any number without rows may lie between
-    int step = 1;
-    for (; b + step < p.B && p.seq_start[b + step] <= t; step *= 2) b += step;
-    while (step >>= 1)
-      if (b + step < p.B && p.seq_start[b + step] <= t) b += step;
-  } else {
-    b = t / rows_each;
-  }
+  int r0, n;
+  const int b = lane_sequence(p, rows_each, (int)(first / p.Hkv), t, lane);
   sequence_rows(p, rows_each, b, &r0, &n);
   const int64_t pos = (int64_t)p.kv_len[b] - n + (t - r0);
   const bool placed = live && t >= r0 && t < r0 + n && pos >= 0 && pos < capacity;
@@ -131,8 +108,10 @@ int launch(const segpt_paged_params& p, hipStream_t st) {
 int64_t elem_bytes(const segpt_paged_params& p) { return p.dtype == SEGPT_DTYPE_FP32 ? 4 : 2; }
 bool aligned(const void* ptr, uintptr_t n) { return (reinterpret_cast<uintptr_t>(ptr) & (n - 1)) == 0; }
 
+}  // namespace
+
 // extents sorted by stride: each stride has to step over everything below it
-bool overlaps_itself(int64_t (&st)[3], int64_t (&ex)[3], int D) {
+static bool overlaps_itself(int64_t (&st)[3], int64_t (&ex)[3], int64_t D) {
   for (int i = 0; i < 3; ++i)
     for (int j = i + 1; j < 3; ++j)
       if (st[j] < st[i]) {
@@ -149,16 +128,18 @@ bool overlaps_itself(int64_t (&st)[3], int64_t (&ex)[3], int D) {
   return false;
 }
 
-int check_pool(const segpt_tensor4& t, const segpt_paged_params& p, bool out) {
+// row, whole: elements of a row and what pieces of `bytes` bytes a row is read in
+int check_pool(const segpt_tensor4& t, const segpt_paged_params& p, int64_t row, int64_t whole, int bytes, bool out) {
   if (!t.ptr) return SEGPT_E_NULL;
-  if (!aligned(t.ptr, 16)) return SEGPT_E_ALIGN;
-  const int64_t per16 = 16 / elem_bytes(p);
-  if (t.stride_b < 0 || t.stride_h < 0 || t.stride_s < p.D) return SEGPT_E_STRIDE;
-  if (t.stride_b % per16 || t.stride_h % per16 || t.stride_s % per16) return SEGPT_E_STRIDE;
+  if (!aligned(t.ptr, bytes)) return SEGPT_E_ALIGN;
+  if (t.stride_b < 0 || t.stride_h < 0 || t.stride_s < row) return SEGPT_E_STRIDE;
+  if (t.stride_b % whole || t.stride_h % whole || t.stride_s % whole) return SEGPT_E_STRIDE;
   if (t.stride_s > (int64_t)(UINT32_MAX / (16 * 4))) return SEGPT_E_STRIDE;  // rows of a wave-wide load: 32-bit offsets
   int64_t st[3] = {t.stride_b, t.stride_h, t.stride_s}, ex[3] = {p.n_pages, p.Hkv, p.page_size};
-  return out && overlaps_itself(st, ex, p.D) ? SEGPT_E_STRIDE : SEGPT_OK;
+  return out && overlaps_itself(st, ex, row) ? SEGPT_E_STRIDE : SEGPT_OK;
 }
+
+namespace {
 
 int check_rows(const segpt_rows& r, const segpt_paged_params& p, int heads, bool out) {
   if (!r.ptr) return SEGPT_E_NULL;
@@ -172,7 +153,8 @@ int check_rows(const segpt_rows& r, const segpt_paged_params& p, int heads, bool
 }  // namespace
 
 // what can be said of the sizes alone, without an address being looked at
-int check_paged_sizes(const segpt_paged_params* p, bool append) {
+int check_paged_sizes(const segpt_paged_params* p, PagedCall call) {
+  const bool append = call != PagedCall::kAttend;  // no query heads
   if (!p) return SEGPT_E_NULL;
   if (p->struct_bytes != sizeof(segpt_paged_params)) return SEGPT_E_STRUCT;
   if (p->dtype != SEGPT_DTYPE_BF16 && p->dtype != SEGPT_DTYPE_FP32) return SEGPT_E_DTYPE;
@@ -185,16 +167,22 @@ int check_paged_sizes(const segpt_paged_params* p, bool append) {
   return SEGPT_OK;
 }
 
-int check_paged(const segpt_paged_params* p, bool append) {
-  int rc = check_paged_sizes(p, append);
+int check_paged(const segpt_paged_params* p, PagedCall call, int64_t row, int64_t whole) {
+  const bool append = call == PagedCall::kAppend, read = call == PagedCall::kRead;
+  int rc = check_paged_sizes(p, call);
   if (rc) return rc;
+  if (!row) {
+    row = p->D;
+    whole = 16 / elem_bytes(*p);
+  }
   if (p->n_pages <= 0) return SEGPT_E_PAGES;
-  const int64_t positions = (int64_t)paged_capacity(*p) + (append ? 0 : p->prefix_len);
+  const int64_t positions = (int64_t)paged_capacity(*p) + (append || read ? 0 : p->prefix_len);
   if (!p->block_table || !p->kv_len) return SEGPT_E_NULL;
   if (p->table_stride < 0) return SEGPT_E_STRIDE;
   if (!aligned(p->block_table, 4) || !aligned(p->kv_len, 4) || !aligned(p->seq_start, 4)) return SEGPT_E_ALIGN;
-  if ((rc = check_pool(p->k_pages, *p, append))) return rc;
-  if ((rc = check_pool(p->v_pages, *p, append))) return rc;
+  if ((rc = check_pool(p->k_pages, *p, row, whole, 16, append))) return rc;
+  if ((rc = check_pool(p->v_pages, *p, row, whole, 16, append))) return rc;
+  if (read) return (rc = check_rows(p->k, *p, p->Hkv, true)) ? rc : check_rows(p->v, *p, p->Hkv, true);
   if (p->rope_cos || p->rope_sin) {
     if (!p->rope_cos || !p->rope_sin || !aligned(p->rope_cos, 16) || !aligned(p->rope_sin, 16)) return SEGPT_E_ROPE;
     if (p->rope_pos0 < 0 || p->rope_pos0 + positions > p->rope_len) return SEGPT_E_ROPE;
@@ -221,7 +209,7 @@ int check_paged(const segpt_paged_params* p, bool append) {
 
 extern "C" int segpt_paged_append(const segpt_paged_params* p, void* stream) {
   using namespace segpt;
-  const int rc = check_paged(p, true);
+  const int rc = check_paged(p, PagedCall::kAppend);
   if (rc) return rc;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (p->dtype == SEGPT_DTYPE_BF16) return p->D == 64 ? launch<uint16_t, 64>(*p, st) : launch<uint16_t, 128>(*p, st);

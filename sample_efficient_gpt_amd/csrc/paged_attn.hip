@@ -689,7 +689,7 @@ extern "C" {
 
 size_t segpt_paged_workspace_bytes(const segpt_paged_params* p) {
   using namespace segpt;
-  if (check_paged_sizes(p, false) != SEGPT_OK) return 0;
+  if (check_paged_sizes(p, PagedCall::kAttend) != SEGPT_OK) return 0;
   PagedArgs a{};
   const size_t n = plan(*p, a, target_of(*p));
   return n > SIZE_MAX - 256 ? 0 : up256(n);
@@ -697,7 +697,7 @@ size_t segpt_paged_workspace_bytes(const segpt_paged_params* p) {
 
 int segpt_paged_attn(const segpt_paged_params* p, void* stream) {
   using namespace segpt;
-  const int rc = check_paged(p, false);
+  const int rc = check_paged(p, PagedCall::kAttend);
   if (rc) return rc;
   PagedArgs a{};
   const int bad = prepare_call(p, a, target_of(*p));

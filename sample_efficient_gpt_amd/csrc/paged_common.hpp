@@ -5,8 +5,11 @@
 
 namespace segpt {
 
-int check_paged_sizes(const segpt_paged_params* p, bool append);
-int check_paged(const segpt_paged_params* p, bool append);
+enum class PagedCall { kAppend, kRead, kAttend };
+int check_paged_sizes(const segpt_paged_params* p, PagedCall call);
+// row, whole: elements of the pool's rows and elements of 16 bytes; 0: the pool holds rows of p's dtype
+int check_paged(const segpt_paged_params* p, PagedCall call, int64_t row = 0, int64_t whole = 0);
+int check_pool(const segpt_tensor4& t, const segpt_paged_params& p, int64_t row, int64_t whole, int bytes, bool out);
 // keys a sequence may hold (checked: fits an int)
 __host__ __device__ inline int paged_capacity(const segpt_paged_params& p) {
   const int64_t room = (int64_t)p.table_width * p.page_size;
@@ -23,6 +26,32 @@ __device__ __forceinline__ void sequence_rows(const segpt_paged_params& p, int r
   const int r0 = min(max(p.seq_start[b], 0), p.T), r1 = min(max(p.seq_start[b + 1], 0), p.T);
   *first = r0;
   *n = max(r1 - r0, 0);
+}
+
+// Sequence of row t, for a whole wave: the number of the last sequence that starts at or before it.  64 starts are looked at a time, so
+// that a batch of up to 64 sequences is one load, of up to 4096 two one after the other.
+__device__ __forceinline__ int sequence_of_row(const segpt_paged_params& p, int t, int lane) {
+  int lo = 0, n = p.B;
+  while (true) {
+    const int step = (n + 63) / 64, i = lane * step;
+    const bool before = i < n && p.seq_start[lo + i] <= t;
+    const int k = __popcll(__builtin_amdgcn_ballot_w64(before));
+    if (k > 0) lo += (k - 1) * step;
+    if (step == 1) return lo;
+    n = min(step, p.B - lo);
+  }
+}
+
+// the same for lanes whose rows t begin with the wave's row t0 and follow it
+__device__ __forceinline__ int lane_sequence(const segpt_paged_params& p, int rows_each, int t0, int t, int lane) {
+  if (!p.seq_start) return t / rows_each;
+  int b = sequence_of_row(p, t0, lane);
+  // a later row of the wave: mostly the next sequence, but any number without rows may lie between
+  int step = 1;
+  for (; b + step < p.B && p.seq_start[b + step] <= t; step *= 2) b += step;
+  while (step >>= 1)
+    if (b + step < p.B && p.seq_start[b + step] <= t) b += step;
+  return b;
 }
 
 // byte address of row (page, head, slot) of a pool

@@ -1,0 +1,762 @@
+// Attention over a paged key/value cache of 8 or 4 bits, forward only: what paged_attn.hip does for pools of bf16 and fp32, with the same
+// division of the work (paged_work.hpp), for pools whose rows are codes in blocks of 32 components with a power-of-two scale each.
+//
+//   y_i = sum_j exp(s_ij - lse_i) v'_j      s_ij = qhat_i . k'_j      k'_j, v'_j = code * 2^e, exact in bf16
+//
+// A code times its scale is a bf16 number, so the codes are made bf16 operands in registers (one instruction a pair of components, the scale as
+// its operand) and everything behind that is bf16 matrix products with fp32 sums, whatever the rows are: bf16 rows bring their queries in two bf16
+// parts, fp32 rows queries and probabilities in three, and neither loses anything of the keys and values as stored.
+#include "paged_quant.hpp"
+#include "paged_work.hpp"
+
+namespace segpt {
+namespace {
+
+
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// PARTS bf16 parts of a pair of values: the first ones cut off (two_parts), the last one rounded
+template <int PARTS>
+__device__ __forceinline__ void parts_of(float a, float b, uint32_t (&w)[PARTS]) {
+  if constexpr (PARTS == 1) {
+    w[0] = pack_bf16x2(a, b);
+  } else {
+    constexpr float kBelow = 1.f - 0x1p-9f;
+#pragma unroll
+    for (int i = 0; i < PARTS - 1; ++i) {
+      const uint32_t x = __float_as_uint(a * kBelow) & 0xffff0000u, y = __float_as_uint(b * kBelow) & 0xffff0000u;
+      w[i] = x >> 16 | y;
+      a -= __uint_as_float(x);
+      b -= __uint_as_float(y);
+    }
+    w[PARTS - 1] = pack_bf16x2(a, b);
+  }
+}
+template <typename E>
+constexpr int kQueryParts = sizeof(E) == 2 ? 2 : 3;
+
+// eight elements of a row
+__device__ __forceinline__ void load8(const uint16_t* p, float (&x)[8]) { load16(p, x); }
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+  const float4 u = *reinterpret_cast<const float4*>(p), v = *reinterpret_cast<const float4*>(p + 4);
+  x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+}
+
+// ---- the pages of an item, walked from its first key on by one wave.  Lane l holds the number of page base + l, and of page base + 64 + l, asked
+// for when the window before it was taken up; a number that is not in the pool is replaced by 0 and remembered.
+struct Pages {
+  const int* ids;
+  int n_pages, log_page, last;  // last: last page of the item's keys
+  int base, now, next;
+  bool bad;
+  __device__ __forceinline__ int ask(int from, int lane) const { return from + lane <= last ? ids[from + lane] : 0; }
+  __device__ __forceinline__ void start(const PagedArgs& a, const Item& it, int lane) {
+    ids = it.ids;
+    n_pages = a.p.n_pages;
+    log_page = a.log_page;
+    base = it.k0 >> log_page;
+    last = it.nk ? (it.k0 + it.nk - 1) >> log_page : -1;
+    now = ask(base, lane);
+    next = ask(base + 64, lane);
+    bad = false;
+  }
+  __device__ __forceinline__ void check(int& id) {
+    if ((uint32_t)id >= (uint32_t)n_pages) { id = 0; bad = true; }
+  }
+  __device__ __forceinline__ void arrived() { check(now); }  // before the first of()
+  __device__ __forceinline__ void reach(int key, int lane) {
+    if ((key >> log_page) - base >= 64) {
+      base += 64;
+      now = next;
+      check(now);
+      next = ask(base + 64, lane);
+    }
+  }
+  __device__ __forceinline__ int of(int key) const { return lane_value(now, (key >> log_page) - base); }
+  __device__ __forceinline__ bool any_bad() {
+    check(next);
+    return __builtin_amdgcn_ballot_w64(bad) != 0;
+  }
+};
+
+// What a lane asks for of one row of keys or values: WORDS words of codes, and the scales of the whole row
+template <int WORDS>
+struct RowPart {
+  uint32_t w[WORDS];
+  uint32_t s;
+};
+template <int D>
+__device__ __forceinline__ uint32_t load_scales(const char* at) {  // D / 32 bytes, aligned to them
+  if constexpr (D == 128) return *reinterpret_cast<const uint32_t*>(at);
+  else return *reinterpret_cast<const uint16_t*>(at);
+}
+template <int BYTES>
+__device__ __forceinline__ void load_words(const char* at, uint32_t* w) {
+  if constexpr (BYTES == 16) { const u32x4 x = *reinterpret_cast<const u32x4*>(at); w[0] = x[0]; w[1] = x[1]; w[2] = x[2]; w[3] = x[3]; }
+  else { const u32x2 x = *reinterpret_cast<const u32x2*>(at); w[0] = x[0]; w[1] = x[1]; }
+}
+__device__ __forceinline__ float scale_at(uint32_t scales, int block) { return __uint_as_float((scales >> (8 * block) & 255u) << 23); }
+
+// Rows key .. key + rows - 1 of keys and values, `rows` of them a power of two up to 16 and key a multiple: one page, or two of eight.  A lane's
+// row stands at most `most` rows behind the first.  NP pieces of P bytes a lane, 4 P apart, the first at byte `from`.
+template <int D, int NP, int P>
+struct Source {
+  const char *k, *v, *ks, *vs;  // first rows of the kv head
+  int64_t kb, vb, ksb, vsb;     // bytes from page to page
+  uint32_t kr, vr, ksr, vsr;    // from row to row
+  __device__ __forceinline__ void start(const QuantArgs& a, int g) {
+    k = byte_row(a.p.k_pages, 0, g, 0);
+    v = byte_row(a.p.v_pages, 0, g, 0);
+    ks = byte_row(a.k_scales, 0, g, 0);
+    vs = byte_row(a.v_scales, 0, g, 0);
+    kb = a.p.k_pages.stride_b; vb = a.p.v_pages.stride_b; ksb = a.k_scales.stride_b; vsb = a.v_scales.stride_b;
+    kr = (uint32_t)a.p.k_pages.stride_s; vr = (uint32_t)a.p.v_pages.stride_s; ksr = (uint32_t)a.k_scales.stride_s; vsr = (uint32_t)a.v_scales.stride_s;
+  }
+  template <int ROWS>
+  __device__ __forceinline__ void ask(const Pages& pages, int key, int row, uint32_t from, RowPart<NP * P / 4>& x, RowPart<NP * P / 4>& y) const {
+    const int id = pages.of(key);
+    const uint32_t slot = (uint32_t)(key & ((1 << pages.log_page) - 1));
+    auto begin = [&](const char* first, int64_t page, uint32_t step) { return first + (int64_t)id * page + (int64_t)((uint64_t)slot * step); };
+    const char *kp = begin(k, kb, kr), *vp = begin(v, vb, vr), *ksp = begin(ks, ksb, ksr), *vsp = begin(vs, vsb, vsr);
+    auto get = [&](const char* kp, const char* vp, const char* ksp, const char* vsp, uint32_t r) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) load_words<P>(kp + (r * kr + from + i * 4 * P), x.w + i * P / 4);
+      x.s = load_scales<D>(ksp + r * ksr);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) load_words<P>(vp + (r * vr + from + i * 4 * P), y.w + i * P / 4);
+      y.s = load_scales<D>(vsp + r * vsr);
+    };
+    if (ROWS <= 8 || pages.log_page > 3) {
+      get(kp, vp, ksp, vsp, (uint32_t)row);
+    } else {  // the second eight rows lie in a page of their own (or nowhere, and no lane's row is among them)
+      const int64_t by = (int64_t)pages.of(key + 8) - id;
+      const bool second = row >= 8;
+      get(kp + (second ? by * kb : 0), vp + (second ? by * vb : 0), ksp + (second ? by * ksb : 0), vsp + (second ? by * vsb : 0), (uint32_t)(second ? row - 8 : row));
+    }
+  }
+};
+
+// ---- FEW: one wave, CT tiles of 16 columns.  A score tile is 16 keys by 16 columns; a lane takes a quarter of a key's row, so that a row is read
+// whole by four lanes and is the A operand as it is decoded, no LDS in between: the components that a lane contributes to a step are not those of
+// the instruction's own order, but the queries' are the same, and a sum does not ask.
+template <int D, int FMT>
+struct Quarter {
+  static constexpr int kBytes = Codes<FMT>::row_bytes(D) / 4;   // of a lane
+  static constexpr int P = kBytes < 16 ? kBytes : 16, NP = kBytes / P, kWords = kBytes / 4;
+  static constexpr int EP = P * 8 / Codes<FMT>::kBits;          // components of a piece: 16 or 32, of one block
+  static constexpr int KS = D / 32;                             // steps of the product
+  static constexpr int kWordsOf8 = Codes<FMT>::kBits / 4;       // words of eight components
+  static __device__ __forceinline__ int component(int step, int quarter) { return (step * 8 / EP) * 4 * EP + quarter * EP + step * 8 % EP; }
+  static __device__ __forceinline__ int block(int piece, int quarter) { return (piece * 4 * EP + quarter * EP) / SEGPT_SCALE_BLOCK; }
+  // the row's part as operands, 8 components each
+  static __device__ __forceinline__ void decode(const RowPart<kWords>& x, int quarter, u32x4 (&out)[KS]) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const float scale = scale_at(x.s, block(i, quarter));
+#pragma unroll
+      for (int u = 0; u < EP / 8; ++u) {
+        uint32_t r[4];
+        decode8<FMT>(x.w + i * (P / 4) + u * kWordsOf8, scale, r);
+        out[i * (EP / 8) + u] = u32x4{r[0], r[1], r[2], r[3]};
+      }
+    }
+  }
+};
+template <typename E, int D, int FMT>
+struct Query16 {
+  using L = Quarter<D, FMT>;
+  static constexpr int KS = L::KS, kCols = 16, kLogCols = 4, PARTS = kQueryParts<E>;
+  bf16x8 part[PARTS][KS];
+  float x[KS][8], other[KS][8], cs[KS][8], sn[KS][8];
+  __device__ __forceinline__ void fetch(const segpt_paged_params& p, const E* row, int64_t angle, int quarter) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) load8(row + L::component(ks, quarter), x[ks]);
+    if (!p.rope_cos) return;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int d = L::component(ks, quarter), j = d % (D / 2);
+      load8(row + (d + D / 2) % D, other[ks]);
+      load8(p.rope_cos + angle + j, cs[ks]);
+      load8(p.rope_sin + angle + j, sn[ks]);
+    }
+  }
+  __device__ __forceinline__ void finish(const segpt_paged_params& p, bool live, int quarter, const float* gsm) {
+    if (p.rope_cos) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const float sign = L::component(ks, quarter) < D / 2 ? -1.f : 1.f;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) x[ks][t] = x[ks][t] * cs[ks][t] + sign * (other[ks][t] * sn[ks][t]);
+      }
+    }
+    float sq[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int t = 0; t < 8; ++t) sq[t % 4] += x[ks][t] * x[ks][t];
+    float ss = (sq[0] + sq[1]) + (sq[2] + sq[3]);
+    ss += __shfl_xor(ss, 16, 64);
+    ss = half_sum(ss);
+    const float alpha = (p.flags & SEGPT_FLAG_NO_NORM) ? 1.f : 1.0f / sqrtf(ss * (1.0f / D) + p.eps);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      float g[8];
+      load8(gsm + L::component(ks, quarter), g);
+      u32x4 w[PARTS];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t part_i[PARTS];
+        parts_of<PARTS>(x[ks][2 * i] * alpha * g[2 * i], x[ks][2 * i + 1] * alpha * g[2 * i + 1], part_i);
+#pragma unroll
+        for (int u = 0; u < PARTS; ++u) w[u][i] = live ? part_i[u] : 0u;
+      }
+#pragma unroll
+      for (int u = 0; u < PARTS; ++u) part[u][ks] = as_bf16x8(w[u]);
+    }
+  }
+};
+// The values of a block of 32 keys in LDS, bf16: chunk c (16 bytes) of row r lies at chunk c ^ f(r).  Sixteen lanes write one chunk of 16 rows, and a
+// transposing read takes two chunks of eight rows at a time; either way all banks are met once.
+template <int D>
+struct ValueTile {
+  static constexpr int kRB = 2 * D, kBytes = kBlock * kRB;
+  static __device__ __forceinline__ int f(int row) { return (D == 64 ? 2 * (row >> 1 & 3) : 2 * (row & 7)) | (row >> 3 & 1); }
+  static __device__ __forceinline__ uint32_t write_at(int row, int chunk) { return row * kRB + ((chunk ^ f(row & 15)) << 4); }
+  // where lane's address lies for the operand of components 16 db .. and, of each quarter of the wave, its four keys of the first 16
+  static __device__ __forceinline__ uint32_t read_at(int lane, int db) {
+    const int r = lane & 15, row = 4 * (lane >> 4) + (r >> 2);
+    return row * kRB + (((2 * db + (r >> 1 & 1)) ^ f(row)) << 4) + ((r & 1) << 3);
+  }
+  static __device__ __forceinline__ u32x4 read(uint32_t tile, int lane, int db) {
+    typedef s16x4 __attribute__((address_space(3))) * lds_s16x4_ptr;
+    const uint32_t at = tile + read_at(lane, db);
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(at));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(at + 16 * kRB));
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    const s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(u32x4, v);
+  }
+};
+__device__ __forceinline__ void lds_write16(uint32_t addr, u32x4 v) { *(__attribute__((address_space(3))) u32x4*)addr = v; }
+
+// A value that is no number must reach the rows that see its key, and not the others as 0 * NaN: in a block that not all rows see it is made 0 and
+// noted, and put back behind the loop
+__device__ __forceinline__ bool clear_nan(u32x4& v) {
+  typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+  uint32_t all = ~0u;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {  // sign of |x| - inf: all ones where x is finite
+    const uint32_t finite = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(i16x2, v[e] & 0x7fff7fffu) - (int16_t)0x7f80) >> 15);
+    v[e] &= finite;
+    all &= finite;
+  }
+  asm volatile("" : "+v"(v));  // whole registers again: as bf16 vectors they would be taken apart, element by element
+  return all != ~0u;
+}
+// calls `found(block)` for every block of components that is no number in the value of a key from j0 on that the lane's row sees (keys counted from k0)
+template <int D, typename F>
+__device__ __forceinline__ void odd_values(const QuantArgs& qa, const PagedArgs& a, const Item& it, const Column& c, int j0, F found) {
+  for (int j = j0; j <= c.any; ++j) {
+    const int key = it.k0 + j, page = it.ids[key >> a.log_page];
+    if ((uint32_t)page >= (uint32_t)a.p.n_pages) continue;  // the rows are NaN as a whole
+    const uint32_t s = load_scales<D>(byte_row(qa.v_scales, page, it.g, key & ((1 << a.log_page) - 1)));
+#pragma unroll
+    for (int b = 0; b < D / SEGPT_SCALE_BLOCK; ++b)
+      if (j <= c.lim && (s >> (8 * b) & 255u) == kNoNumber) found(b);
+  }
+}
+
+// this wave's LDS reads have returned (before what they came from is written over), its LDS writes are there
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0) only
+}
+
+template <typename E, int D, int FMT, int CT>
+__device__ __forceinline__ void few_columns(const QuantArgs& qa, const PagedArgs& a, const Item& it, int rep, int lane, uint32_t lds, float* gsm) {
+  using L = Quarter<D, FMT>;
+  using V = ValueTile<D>;
+  constexpr int KS = L::KS, DB = D / 16, PARTS = kQueryParts<E>;
+  const segpt_paged_params& p = a.p;
+  const int quarter = lane >> 4, r16 = lane & 15;
+  const int last = it.k0 + it.nk - 1, blocks = (it.nk + kBlock - 1) / kBlock;
+  // one round trip: gain, query rows and angles, page numbers
+  Pages pages;
+  pages.start(a, it, lane);
+  Gain gain[(D + 63) / 64];
+#pragma unroll
+  for (int i = 0; i < (D + 63) / 64; ++i) gain[i] = fetch_gain(p, (64 * i + lane) % D);
+  Query16<E, D, FMT> q[CT];
+  Column c[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) c[ct] = column_of<E, D>(a, it, rep, it.tile * kFew + 16 * ct, lane, q[ct]);
+  Source<D, L::NP, L::P> src;
+  src.start(qa, it.g);
+  pages.arrived();
+  struct Block {
+    RowPart<L::kWords> k[2], v[2];
+  };
+  auto ask = [&](Block& b, int j) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int key = min(it.k0 + j * kBlock + 16 * t, last & ~15);  // past the last key: the last row once more
+      pages.reach(key, lane);
+      src.template ask<16>(pages, key, min(r16, last - key), (uint32_t)quarter * L::P, b.k[t], b.v[t]);
+    }
+  };
+  Block b0, b1;
+  if (blocks > 0) ask(b0, 0);
+  if (blocks > 1) ask(b1, 1);
+#pragma unroll
+  for (int i = 0; i < (D + 63) / 64; ++i)
+    if (64 * i + lane < D) gsm[64 * i + lane] = scale_of(p, gain[i]);
+  wave_sync();
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) q[ct].finish(p, c[ct].live, quarter, gsm);
+
+  f32x4 o[CT][DB];
+  float m[CT], limit[CT], l[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    m[ct] = 0.f;
+    limit[ct] = -INFINITY;
+    l[ct] = 0.f;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) o[ct][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  int all = c[0].all;
+#pragma unroll
+  for (int ct = 1; ct < CT; ++ct) all = min(all, c[ct].all);
+  bool odd = false;
+  auto step = [&](Block& b, int j) {
+    u32x4 k[2][KS];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      L::decode(b.k[t], quarter, k[t]);
+      u32x4 v[KS];
+      L::decode(b.v[t], quarter, v);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) lds_write16(lds + V::write_at(16 * t + r16, L::component(ks, quarter) / 8), v[ks]);
+    }
+    if (j + 2 < blocks) ask(b, j + 2);
+    const bool masked = j * kBlock + kBlock - 1 > all;
+    f32x4 s[CT][2];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        s[ct][t] = f32x4{-m[ct], -m[ct], -m[ct], -m[ct]};
+#pragma unroll
+        for (int u = PARTS - 1; u >= 0; --u)
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) s[ct][t] = mfma16(as_bf16x8(k[t][ks]), q[ct].part[u][ks], s[ct][t]);
+        if (masked) {
+          const int seen = c[ct].lim - j * kBlock - 16 * t - 4 * quarter;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (r > seen) s[ct][t][r] = -INFINITY;
+        }
+      }
+    u32x4 pb[CT][PARTS];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      float top = s[ct][0][0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) top = fmaxf(top, s[ct][i / 4][i % 4]);
+      if (__builtin_amdgcn_ballot_w64(top > limit[ct]) != 0) {  // a lane's own keys may tell; the column's reference is one for its four lanes
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = half_max(top);
+        const float up = top > limit[ct] ? top : 0.f, corr = limit[ct] == -INFINITY ? 1.f : fast_exp2(-up);
+        m[ct] += up;
+        if (top > limit[ct]) limit[ct] = kLazy;
+        l[ct] *= corr;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[ct][db][r] *= corr;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[ct][i / 4][i % 4] -= up;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        s[ct][i / 4][i % 4] = fast_exp2(s[ct][i / 4][i % 4]);
+        l[ct] += s[ct][i / 4][i % 4];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t w[PARTS];
+        parts_of<PARTS>(s[ct][i / 2][i % 2 * 2], s[ct][i / 2][i % 2 * 2 + 1], w);
+#pragma unroll
+        for (int u = 0; u < PARTS; ++u) pb[ct][u][i] = w[u];
+      }
+    }
+    wave_sync();
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      u32x4 v = V::read(lds, lane, db);
+      if (masked) odd |= clear_nan(v);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int u = PARTS - 1; u >= 0; --u) o[ct][db] = mfma16(as_bf16x8(v), as_bf16x8(pb[ct][u]), o[ct][db]);
+    }
+    wave_sync();
+  };
+  for (int j = 0; j < blocks; j += 2) {
+    step(b0, j);
+    if (j + 1 < blocks) step(b1, j + 1);
+  }
+  const bool bad = it.x.broken | pages.any_bad();
+  if (__builtin_amdgcn_ballot_w64(odd) != 0) {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+      odd_values<D>(qa, a, it, c[ct], (max(all, -1) + 1) / kBlock * kBlock, [&](int b) {
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+          if (db / 2 == b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[ct][db][r] = __builtin_nanf("");
+      });
+  }
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    float sum = l[ct] + __shfl_xor(l[ct], 16, 64), ref = limit[ct] == -INFINITY ? -INFINITY : m[ct];
+    sum = half_sum(sum);
+    if (bad) { sum = __builtin_nanf(""); ref = 0.f; }
+    if (!c[ct].live) continue;
+    if (!it.direct) {
+      const int64_t at = (int64_t)it.slot * 32 + 16 * ct + r16;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(a.part + at * D + 16 * db + 4 * quarter) = o[ct][db];
+      if (quarter == 0) a.stat[at] = make_float2(ref, sum);
+      continue;
+    }
+    float f = sum == 0.f ? 0.f : 1.0f / sum;
+    if (p.lse && quarter == 0) p.lse[(int64_t)c[ct].t * p.H + c[ct].h] = sum == 0.f ? -INFINITY : (ref + __log2f(sum)) * kLn2;
+    if (p.gate.ptr) f *= gate_factor<E, D>(p, c[ct].t, c[ct].h);
+    E* out = row_of<E>(p.o, c[ct].t, c[ct].h) + 4 * quarter;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      const float y[4] = {o[ct][db][0] * f, o[ct][db][1] * f, o[ct][db][2] * f, o[ct][db][3] * f};
+      if constexpr (sizeof(E) == 2) *reinterpret_cast<u32x2*>(out + 16 * db) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+      else store16(out + 16 * db, y);
+    }
+  }
+}
+
+// ---- MANY: four waves of 32 columns around a ring of three stages (K' tile, V' tile of bf16); tile jt lives in stage jt % 3.  The codes of a tile are
+// asked for four turns before its products, two tiles ahead of the ring in registers, and decoded into LDS two turns before.  A turn computes the
+// scores of tile jt + 1 beside the exponentials of tile jt and its product with the values.
+template <int D>
+struct ManyShape {
+  static constexpr int kBK = D == 64 ? 64 : 32, kTileBytes = kBK * 2 * D, kStageBytes = 2 * kTileBytes, kStages = 3;
+  static constexpr int kLanes = D / 16, kRows = 64 / kLanes;  // lanes of a row (16 components each), rows of a wave
+};
+template <typename E, int D>
+struct Query32 {
+  static constexpr int KS = D / 16, kCols = 32, kLogCols = 5, PARTS = kQueryParts<E>;
+  bf16x8 part[PARTS][KS];
+  float x[KS][8], cs[KS / 2][8], sn[KS / 2][8];
+  __device__ __forceinline__ void fetch(const segpt_paged_params& p, const E* row, int64_t angle, int hh) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) load8(row + 16 * ks + 8 * hh, x[ks]);
+    if (!p.rope_cos) return;
+#pragma unroll
+    for (int ks = 0; ks < KS / 2; ++ks) {
+      load8(p.rope_cos + angle + 16 * ks + 8 * hh, cs[ks]);
+      load8(p.rope_sin + angle + 16 * ks + 8 * hh, sn[ks]);
+    }
+  }
+  __device__ __forceinline__ void finish(const segpt_paged_params& p, bool live, int hh, const float* gsm) {
+    if (p.rope_cos) {
+#pragma unroll
+      for (int ks = 0; ks < KS / 2; ++ks)
+#pragma unroll
+        for (int t = 0; t < 8; ++t) rope_pair(x[ks][t], x[ks + KS / 2][t], cs[ks][t], sn[ks][t]);
+    }
+    float sq[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int t = 0; t < 8; ++t) sq[t % 4] += x[ks][t] * x[ks][t];
+    const float ss = half_sum((sq[0] + sq[1]) + (sq[2] + sq[3]));
+    const float alpha = (p.flags & SEGPT_FLAG_NO_NORM) ? 1.f : 1.0f / sqrtf(ss * (1.0f / D) + p.eps);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      float g[8];
+      load8(gsm + 16 * ks + 8 * hh, g);
+      u32x4 w[PARTS];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t part_i[PARTS];
+        parts_of<PARTS>(x[ks][2 * i] * alpha * g[2 * i], x[ks][2 * i + 1] * alpha * g[2 * i + 1], part_i);
+#pragma unroll
+        for (int u = 0; u < PARTS; ++u) w[u][i] = live ? part_i[u] : 0u;
+      }
+#pragma unroll
+      for (int u = 0; u < PARTS; ++u) part[u][ks] = as_bf16x8(w[u]);
+    }
+  }
+};
+
+template <typename E, int D, int FMT>
+__device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArgs& a, const Item& it, int rep, int tid, uint32_t lds, float* gsm) {
+  using S = ManyShape<D>;
+  constexpr int BK = S::kBK, N = BK / 32, MB = D / 32, KS = D / 16, PARTS = kQueryParts<E>, PROBS = sizeof(E) == 2 ? 1 : 3;
+  constexpr int P = 16 * Codes<FMT>::kBits / 8;  // bytes of a lane's 16 components
+  const segpt_paged_params& p = a.p;
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
+  const int own_row = lane / S::kLanes, own_part = lane % S::kLanes, last = it.k0 + it.nk - 1, n_kt = (it.nk + BK - 1) / BK;
+  // one round trip: gain, query row and angles, page numbers
+  Pages pages;
+  pages.start(a, it, lane);
+  const Gain gain = fetch_gain(p, tid % D);
+  Query32<E, D> q;
+  const Column c = column_of<E, D>(a, it, rep, it.tile * kMany + wave * 32, lane, q);
+  Source<D, 1, P> src;
+  src.start(qa, it.g);
+  pages.arrived();
+  struct Raw2 {
+    RowPart<P / 4> k, v;
+  };
+  auto ask = [&](Raw2& x, int jt) {
+    if (jt >= n_kt) return;
+    const int key = min(it.k0 + jt * BK + wave * S::kRows, last & ~(S::kRows - 1));
+    pages.reach(key, lane);
+    src.template ask<S::kRows>(pages, key, min(own_row, last - key), (uint32_t)own_part * P, x.k, x.v);
+  };
+  auto put = [&](const Raw2& x, int jt, uint32_t stage) {
+    if (jt >= n_kt) return;
+    const int row = wave * S::kRows + own_row, f = Swz<D>::f(row);
+    auto tensor = [&](const RowPart<P / 4>& r, uint32_t at) {
+      const float scale = scale_at(r.s, own_part / 2);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        uint32_t w[4];
+        decode8<FMT>(r.w + u * (P / 8), scale, w);
+        lds_write16(at + row * S::kTileBytes / BK + (((2 * own_part + u) ^ f) << 4), u32x4{w[0], w[1], w[2], w[3]});
+      }
+    };
+    tensor(x.k, lds + stage);
+    tensor(x.v, lds + stage + S::kTileBytes);
+  };
+  Raw2 x0, x1;
+  ask(x0, 0);
+  ask(x1, 1);
+  if (tid < D) gsm[tid] = scale_of(p, gain);
+  __syncthreads();
+  q.finish(p, c.live, hh, gsm);
+  put(x0, 0, 0);
+  ask(x0, 2);
+  put(x1, 1, S::kStageBytes);
+  ask(x1, 3);
+  State<MB> st;
+  st.clear();
+  bool odd = false;
+  typedef f32x16 Scores[N];
+  auto scores = [&](auto masked_c, uint32_t stage, Scores& s, int jb) {  // of the tile whose keys begin at jb, from k0 on
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      s[n] = st.less;
+      bf16x8 k[KS];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) k[ks] = swz_frag_rm<D>(lds + stage + n * 64 * D + swz_off_rm<D>(lane), 0, ks);
+#pragma unroll
+      for (int u = PARTS - 1; u >= 0; --u)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s[n] = mfma32(k[ks], q.part[u][ks], s[n]);
+    }
+    if (decltype(masked_c)::value != 0) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) hide_unseen(s[n], c.lim - jb - 32 * n, hh);
+    }
+  };
+  auto products = [&](auto masked_c, uint32_t stage, Scores& s) {
+    st.exponentials(s);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      u32x4 pb[PROBS][2];
+      if constexpr (PROBS == 1) {
+        pb[0][0] = __builtin_bit_cast(u32x4, pack_c_half_sum(s[n], 0, st.l));
+        pb[0][1] = __builtin_bit_cast(u32x4, pack_c_half_sum(s[n], 1, st.l));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t w[PROBS];
+          parts_of<PROBS>(s[n][2 * i], s[n][2 * i + 1], w);
+#pragma unroll
+          for (int u = 0; u < PROBS; ++u) pb[u][i / 4][i % 4] = w[u];
+          st.l[0] += s[n][2 * i];
+          st.l[1] += s[n][2 * i + 1];
+        }
+      }
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+          u32x4 v = __builtin_bit_cast(u32x4, swz_frag_tr<D>(lds + stage + S::kTileBytes + n * 64 * D + swz_off_tr<D>(lane), mb, s2));
+          if (decltype(masked_c)::value != 0) odd |= clear_nan(v);
+#pragma unroll
+          for (int u = PROBS - 1; u >= 0; --u) st.o[mb] = mfma32(as_bf16x8(v), as_bf16x8(pb[u][s2]), st.o[mb]);
+        }
+    }
+  };
+  uint32_t stage = 0;  // of tile jt
+  auto stage_from = [&](int steps) {  // of tile jt + steps
+    const uint32_t x = stage + steps * S::kStageBytes;
+    return x >= S::kStages * S::kStageBytes ? x - S::kStages * S::kStageBytes : x;
+  };
+  auto active = [&](int jt) { return jt < n_kt && jt * BK <= c.any; };  // some column of the wave sees a key of the tile
+  const int n_whole = max(min((c.all + 1) / BK, n_kt), 0);  // tiles that all columns of the wave see whole
+  Scores s0, s1;
+  __syncthreads();
+  if (active(0)) {
+    scores(IC<1>{}, 0, s0, 0);
+    st.raise(s0);
+  }
+  auto turn = [&](int jt, Raw2& x) {
+    __syncthreads();  // tile jt + 1 is there; everyone has left tile jt - 1
+    put(x, jt + 2, stage_from(2));
+    ask(x, jt + 4);
+  };
+  auto whole = [&](int jt, Raw2& x, Scores& s, Scores& ahead) {  // neither tile jt nor the next needs a mask
+    turn(jt, x);
+    scores(IC<0>{}, stage_from(1), ahead, 0);
+    products(IC<0>{}, stage, s);
+    st.raise(ahead);
+    stage = stage_from(1);
+  };
+  auto any_tiles = [&](int jt, Raw2& x, Scores& s, Scores& ahead) {
+    turn(jt, x);
+    if (active(jt)) {
+      if (jt >= n_whole) products(IC<1>{}, stage, s);
+      else products(IC<0>{}, stage, s);
+    }
+    if (active(jt + 1)) {
+      scores(IC<1>{}, stage_from(1), ahead, (jt + 1) * BK);
+      st.raise(ahead);
+    }
+    stage = stage_from(1);
+  };
+  // two turns a round, so that scores and codes change places without being copied
+  int jt = 0;
+  for (; jt + 2 < n_whole; jt += 2) {
+    whole(jt, x0, s0, s1);
+    whole(jt + 1, x1, s1, s0);
+  }
+  for (; jt < n_kt; jt += 2) {
+    any_tiles(jt, x0, s0, s1);
+    if (jt + 1 < n_kt) any_tiles(jt + 1, x1, s1, s0);
+  }
+  const bool bad = it.x.broken | pages.any_bad();
+  if (__builtin_amdgcn_ballot_w64(odd) != 0)
+    odd_values<D>(qa, a, it, c, (max(c.all, -1) + 1) / BK * BK, [&](int b) {
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+        if (mb == b) st.o[mb] = splat16(__builtin_nanf(""));
+    });
+  store_result<E, D>(a, it, c, st, bad, wave * 32 + (lane & 31), hh);
+}
+
+struct Args {
+  PagedArgs w;
+  segpt_tensor4 k_scales, v_scales;
+};
+__device__ __forceinline__ QuantArgs quant_of(const Args& a) { return {a.w.p, a.k_scales, a.v_scales}; }
+
+// Launches whose entries are all FEW: a workgroup is one wave
+template <typename E, int D, int FMT>
+__global__ __launch_bounds__(64, 2) void paged_quant_few_kernel(Args args) {
+  const PagedArgs& a = args.w;
+  __shared__ __attribute__((aligned(1024))) char lds[ValueTile<D>::kBytes];
+  __shared__ __attribute__((aligned(16))) float gsm[D];
+  const int lane = threadIdx.x, rep = a.rep.d;
+  clear_rest<E>(a, lane, 64, D);
+  const Entries mine = kept_entries(a, lane, rep);
+  const Shares share = share_blocks(a, mine);
+  leave_plan(a, lane, rep, share, mine);
+  const Item it = locate<false>(a, lane, rep, share, mine, blockIdx.x);
+  if (!it.valid) return;
+  const QuantArgs qa = quant_of(args);
+  if (it.cols <= 16) few_columns<E, D, FMT, 1>(qa, a, it, rep, lane, lds_addr_of(lds), gsm);
+  else few_columns<E, D, FMT, 2>(qa, a, it, rep, lane, lds_addr_of(lds), gsm);
+}
+
+// Any launch: the first workgroups are items of many columns, the next four items each of few, the rest have none
+template <typename E, int D, int FMT>
+__global__ __launch_bounds__(256, (sizeof(E) == 2 || D == 64 ? 2 : 1)) void paged_quant_any_kernel(Args args) {
+  const PagedArgs& a = args.w;
+  using S = ManyShape<D>;
+  constexpr int kLds = std::max(S::kStages * S::kStageBytes, 4 * ValueTile<D>::kBytes);
+  __shared__ __attribute__((aligned(1024))) char lds[kLds];
+  __shared__ __attribute__((aligned(16))) float gsm[4][D];
+  const int tid = threadIdx.x, lane = tid & 63, rep = a.rep.d;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  clear_rest<E>(a, tid, 256, D);
+  const Entries mine = kept_entries(a, lane, rep);
+  const Shares share = share_blocks(a, mine);
+  leave_plan(a, lane, rep, share, mine);
+  const QuantArgs qa = quant_of(args);
+  const Item it = locate<true>(a, lane, rep, share, mine, blockIdx.x);
+  if (it.x.entry >= 0) {
+    if (it.valid) many_columns<E, D, FMT>(qa, a, it, rep, tid, lds_addr_of(lds), gsm[0]);
+  } else {
+    const Item it4 = locate<false>(a, lane, rep, share, mine, ((int)blockIdx.x - it.x.base) * 4 + wave);
+    if (!it4.valid) return;
+    const uint32_t at = lds_addr_of(lds) + wave * ValueTile<D>::kBytes;
+    if (it4.cols <= 16) few_columns<E, D, FMT, 1>(qa, a, it4, rep, lane, at, gsm[wave]);
+    else few_columns<E, D, FMT, 2>(qa, a, it4, rep, lane, at, gsm[wave]);
+  }
+}
+
+// ---- host side
+int target_of(const segpt_paged_params& p) {
+  const int rep = p.H / p.Hkv;
+  const bool wide = p.prefix_table || (!p.seq_start && (int64_t)rep * (p.T / p.B) > kFew);
+  return wide ? 384 : p.seq_start ? 480 : 496;
+}
+
+template <typename E, int D, int FMT>
+int launch(const Args& args, hipStream_t st) {
+  const PagedArgs& a = args.w;
+  int rc = launch_plan(a, st);
+  if (rc) return rc;
+  if (all_few(a.p)) hipLaunchKernelGGL((paged_quant_few_kernel<E, D, FMT>), dim3((unsigned)a.n_few), dim3(64), 0, st, args);
+  else hipLaunchKernelGGL((paged_quant_any_kernel<E, D, FMT>), dim3((unsigned)(a.n_many + (a.n_few + 3) / 4)), dim3(256), 0, st, args);
+  rc = (int)hipGetLastError();
+  if (rc) return rc;
+  return launch_merge<E, D>(a, st);
+}
+
+}  // namespace
+}  // namespace segpt
+
+extern "C" {
+
+size_t segpt_paged_quant_workspace_bytes(const segpt_paged_params* p, const segpt_paged_quant* q) {
+  using namespace segpt;
+  if (check_paged_sizes(p, PagedCall::kAttend) != SEGPT_OK || !q || q->struct_bytes != sizeof(segpt_paged_quant)) return 0;
+  if ((q->format != SEGPT_POOL_E4M3 && q->format != SEGPT_POOL_E2M1) || (p->D != 64 && p->D != 128)) return 0;
+  PagedArgs a{};
+  const size_t n = plan(*p, a, target_of(*p));
+  return n > SIZE_MAX - 256 ? 0 : up256(n);
+}
+
+int segpt_paged_attn_quant(const segpt_paged_params* p, const segpt_paged_quant* q, void* stream) {
+  using namespace segpt;
+  int rc = check_quant(p, q, PagedCall::kAttend);
+  if (rc) return rc;
+  Args args{{}, q->k_scales, q->v_scales};
+  if ((rc = prepare_call(p, args.w, target_of(*p)))) return rc;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const bool e4m3 = q->format == SEGPT_POOL_E4M3;
+  if (p->dtype == SEGPT_DTYPE_BF16) {
+    if (p->D == 64) return e4m3 ? launch<uint16_t, 64, SEGPT_POOL_E4M3>(args, st) : launch<uint16_t, 64, SEGPT_POOL_E2M1>(args, st);
+    return e4m3 ? launch<uint16_t, 128, SEGPT_POOL_E4M3>(args, st) : launch<uint16_t, 128, SEGPT_POOL_E2M1>(args, st);
+  }
+  if (p->D == 64) return e4m3 ? launch<float, 64, SEGPT_POOL_E4M3>(args, st) : launch<float, 64, SEGPT_POOL_E2M1>(args, st);
+  return e4m3 ? launch<float, 128, SEGPT_POOL_E4M3>(args, st) : launch<float, 128, SEGPT_POOL_E2M1>(args, st);
+}
+
+}  // extern "C"

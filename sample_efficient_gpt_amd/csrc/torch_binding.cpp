@@ -506,16 +506,51 @@ void no_gradient_asked(const char* what, std::initializer_list<const Tensor*> al
       throw CheckFailed(std::string(what) + " has no derivative: call it under torch.no_grad() or on detached tensors");
   if (const auto& transforms = at::functorch::functorchTLSAccessor()) transforms->checkSupportsCppAutogradFunction();
 }
-// What appending and attending have in common: pool, table, lengths, angles.  rows: k or q
-void fill_paged(segpt_paged_params& p, const Tensor& rows, const char* name, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
-                const Tensor& kv_len, const Tensor& seq_start, const Tensor& cos, const Tensor& sin, int64_t pos0, std::optional<int64_t> max_len,
-                double eps, bool qk_norm) {
+// Format and scales of a pool of 8 or 4 bits; neither scales: the pool holds rows of the call's dtype
+struct Scales {
+  Tensor k, v;
+  bool any() const { return k.defined() || v.defined(); }
+};
+segpt_paged_quant fill_quant(const Scales& scales, const Tensor& k_pages) {
+  segpt_paged_quant q{};
+  q.struct_bytes = sizeof(q);
+  q.format = k_pages.scalar_type() == at::kFloat8_e4m3fn ? SEGPT_POOL_E4M3 : SEGPT_POOL_E2M1;
+  q.k_scales = view4(scales.k, 0); q.v_scales = view4(scales.v, 0);
+  return q;
+}
+void check_scaled_pool(const Scales& scales, const Tensor& k_pages, const Tensor& v_pages, int64_t head_dim, const at::Device& dev) {
+  check(scales.k.defined() && scales.v.defined(), "k_scales and v_scales go together");
+  const auto dt = k_pages.scalar_type();
+  const bool e4m3 = dt == at::kFloat8_e4m3fn;
+  if (!e4m3 && dt != at::kByte && dt != at::kFloat4_e2m1fn_x2)
+    throw BadType(std::string("pages with scales must be float8_e4m3fn, or uint8 or float4_e2m1fn_x2 (two codes a byte), got ") + c10::toString(dt));
+  if (v_pages.scalar_type() != dt) throw BadType(std::string("the pages have dtypes ") + c10::toString(dt) + " and " + c10::toString(v_pages.scalar_type()));
+  const int64_t row = e4m3 ? head_dim : head_dim / 2;
+  for (const Tensor* t : {&k_pages, &v_pages}) {
+    check(t->device() == dev, "all tensors must be on one device");
+    check(t->dim() == 4 && t->sizes() == k_pages.sizes() && t->size(3) == row && (t->stride(3) == 1 || t->size(3) == 1),
+          "the pages must be [pages, kv heads, page size, head_dim (4 bits: head_dim / 2)], contiguous in the last");
+  }
+  for (const Tensor* t : {&scales.k, &scales.v}) {
+    if (t->scalar_type() != at::kByte && t->scalar_type() != at::kFloat8_e8m0fnu)
+      throw BadType(std::string("scales must be uint8 or float8_e8m0fnu, got ") + c10::toString(t->scalar_type()));
+    check(t->device() == dev, "all tensors must be on one device");
+    check(t->dim() == 4 && t->size(0) == k_pages.size(0) && t->size(1) == k_pages.size(1) && t->size(2) == k_pages.size(2) &&
+              t->size(3) == head_dim / SEGPT_SCALE_BLOCK && (t->stride(3) == 1 || t->size(3) == 1),
+          "scales must be [pages, kv heads, page size, head_dim / 32], contiguous in the last");
+  }
+}
+// What appending, reading and attending have in common: pool, table, lengths, angles.  rows: k or q
+void fill_paged(segpt_paged_params& p, const Tensor& rows, const char* name, const Tensor& k_pages, const Tensor& v_pages, const Scales& scales,
+                const Tensor& table, const Tensor& kv_len, const Tensor& seq_start, const Tensor& cos, const Tensor& sin, int64_t pos0,
+                std::optional<int64_t> max_len, double eps, bool qk_norm) {
   const auto dt = rows.scalar_type();
   const auto dev = rows.device();
   if (dt != at::kBFloat16 && dt != at::kFloat) throw BadType(std::string("the paged cache supports bfloat16 and float32 tensors, got ") + c10::toString(dt));
   check(rows.is_cuda(), "the paged cache works on device tensors");
   check(rows.dim() == 3, (std::string(name) + " must be [rows, heads, head_dim]").c_str());
-  for (const Tensor* t : {&k_pages, &v_pages}) {
+  if (scales.any()) check_scaled_pool(scales, k_pages, v_pages, rows.size(2), dev);
+  else for (const Tensor* t : {&k_pages, &v_pages}) {
     if (t->scalar_type() != dt) throw BadType(std::string("the pages have dtype ") + c10::toString(t->scalar_type()) + ", expected " + c10::toString(dt));
     check(t->device() == dev, "all tensors must be on one device");
     check(t->dim() == 4 && t->sizes() == k_pages.sizes() && t->size(3) == rows.size(2) && (t->stride(3) == 1 || t->size(3) == 1),
@@ -560,16 +595,16 @@ void fill_paged(segpt_paged_params& p, const Tensor& rows, const char* name, con
   }
 }
 
-void paged_append(const Tensor& k_in, const Tensor& v_in, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& kv_len,
-                  const OptTensor& seq_start, const OptTensor& ov_first, const OptTensor& ocoef, double eps, bool qk_norm, const OptTensor& ocos,
-                  const OptTensor& osin, int64_t pos0, std::optional<int64_t> max_len) {
+void append_to(const Scales& scales, const Tensor& k_in, const Tensor& v_in, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
+               const Tensor& kv_len, const OptTensor& seq_start, const OptTensor& ov_first, const OptTensor& ocoef, double eps, bool qk_norm,
+               const OptTensor& ocos, const OptTensor& osin, int64_t pos0, std::optional<int64_t> max_len) {
   const Tensor first_in = defined_or_none(ov_first), coef = defined_or_none(ocoef);
   no_gradient_asked("paged_kv_append", {&k_in, &v_in, &k_pages, &v_pages, &first_in, &coef});
   const auto dev = k_in.device();
   const Tensor k = last_dim_contiguous(k_in), v = last_dim_contiguous(v_in), v_first = last_dim_contiguous(first_in);
   const Tensor cos = f32_table(defined_or_none(ocos), dev), sin = f32_table(defined_or_none(osin), dev), c32 = f32_vector(coef, dev);
   segpt_paged_params p{};
-  fill_paged(p, k, "k", k_pages, v_pages, table, kv_len, defined_or_none(seq_start), cos, sin, pos0, max_len, eps, qk_norm);
+  fill_paged(p, k, "k", k_pages, v_pages, scales, table, kv_len, defined_or_none(seq_start), cos, sin, pos0, max_len, eps, qk_norm);
   check(k.size(1) == k_pages.size(1), "k must have the pages' number of kv heads");
   check(v_first.defined() == coef.defined(), "v_first and vr_coef go together");
   for (const Tensor* t : {&v, &v_first})
@@ -580,21 +615,90 @@ void paged_append(const Tensor& k_in, const Tensor& v_in, const Tensor& k_pages,
     }
   if (coef.defined()) check(coef.numel() == 2, "vr_coef must have two elements");
   if (at::has_internal_overlap(k_pages) != at::MemOverlap::Yes) check_apart(k_pages, "k_pages", v_pages, "v_pages");  // the entry refuses the other kind
+  if (scales.any()) {
+    if (at::has_internal_overlap(scales.k) != at::MemOverlap::Yes) check_apart(scales.k, "k_scales", scales.v, "v_scales");
+    for (const Tensor* t : {&scales.k, &scales.v})
+      for (const Tensor* pool : {&k_pages, &v_pages}) check_apart(*pool, "the pages", *t, "the scales");
+  }
+  const std::initializer_list<const Tensor*> written = {&k_pages, &v_pages, &scales.k, &scales.v};
   for (const Tensor* t : {&k, &v, &v_first})
-    for (const Tensor* pool : {&k_pages, &v_pages}) check_apart(*pool, "the pages", *t, "k, v or v_first");
-  for (const Tensor* t : {&k_pages, &v_pages})
-    check(!t->is_inference() || c10::InferenceMode::is_enabled(), "pages made in inference mode can be appended to in inference mode only");
+    for (const Tensor* pool : written) check_apart(*pool, "the pages", *t, "k, v or v_first");
+  for (const Tensor* t : written)
+    check(!t->defined() || !t->is_inference() || c10::InferenceMode::is_enabled(), "pages made in inference mode can be appended to in inference mode only");
   if (k.numel() == 0) return;
   p.k = view_rows(k); p.v = view_rows(v); p.v_first = view_rows(v_first);
   p.vr_coef = ptr_of<float>(c32);
   const c10::DeviceGuard guard(dev);
-  const int rc = segpt_paged_append(&p, current_stream(dev));
-  if (rc) throw LibraryError(rc, "segpt_paged_append");
-  for (const Tensor* t : {&k_pages, &v_pages})
-    if (!t->is_inference()) torch::autograd::impl::bump_version(*t);
+  if (scales.any()) {
+    const segpt_paged_quant q = fill_quant(scales, k_pages);
+    const int rc = segpt_paged_append_quant(&p, &q, current_stream(dev));
+    if (rc) throw LibraryError(rc, "segpt_paged_append_quant");
+  } else {
+    const int rc = segpt_paged_append(&p, current_stream(dev));
+    if (rc) throw LibraryError(rc, "segpt_paged_append");
+  }
+  for (const Tensor* t : written)
+    if (t->defined() && !t->is_inference()) torch::autograd::impl::bump_version(*t);
 }
 
-std::pair<Tensor, Tensor> paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& v_pages, const OptTensor& oprefix, int64_t prefix_len,
+void paged_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& kv_len,
+                  const OptTensor& seq_start, const OptTensor& v_first, const OptTensor& coef, double eps, bool qk_norm, const OptTensor& cos,
+                  const OptTensor& sin, int64_t pos0, std::optional<int64_t> max_len) {
+  append_to({}, k, v, k_pages, v_pages, table, kv_len, seq_start, v_first, coef, eps, qk_norm, cos, sin, pos0, max_len);
+}
+void paged_append_scaled(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const OptTensor& k_scales, const OptTensor& v_scales,
+                         const Tensor& table, const Tensor& kv_len, const OptTensor& seq_start, const OptTensor& v_first, const OptTensor& coef, double eps,
+                         bool qk_norm, const OptTensor& cos, const OptTensor& sin, int64_t pos0, std::optional<int64_t> max_len) {
+  append_to({defined_or_none(k_scales), defined_or_none(v_scales)}, k, v, k_pages, v_pages, table, kv_len, seq_start, v_first, coef, eps, qk_norm, cos, sin,
+            pos0, max_len);
+}
+
+// rows (k, v) of what the pages hold; both allocated here unless given
+std::pair<Tensor, Tensor> paged_read(const Tensor& k_pages, const Tensor& v_pages, const OptTensor& ok_scales, const OptTensor& ov_scales, const Tensor& table,
+                                     const Tensor& kv_len, int64_t rows, const OptTensor& seq_start, at::ScalarType dtype, std::optional<int64_t> max_len,
+                                     const OptTensor& ok, const OptTensor& ov) {
+  const Scales scales{defined_or_none(ok_scales), defined_or_none(ov_scales)};
+  no_gradient_asked("paged_kv_read", {&k_pages, &v_pages});
+  const auto dev = k_pages.device();
+  check(k_pages.is_cuda(), "the paged cache works on device tensors");
+  check(k_pages.dim() == 4, "the pages must be [pages, kv heads, page size, head_dim (4 bits: head_dim / 2)], contiguous in the last");
+  check(rows >= 0 && rows < (int64_t{1} << 30), "rows must not be negative, nor 2^30 or more");
+  check(ok.has_value() == ov.has_value(), "out is a pair");
+  const int64_t head_dim = k_pages.size(3) * (scales.any() && k_pages.scalar_type() != at::kFloat8_e4m3fn ? 2 : 1);
+  const bool given = ok.has_value();
+  const auto options = at::TensorOptions().dtype(dtype).device(dev);
+  if (dtype != at::kBFloat16 && dtype != at::kFloat) throw BadType(std::string("the paged cache supports bfloat16 and float32 tensors, got ") + c10::toString(dtype));
+  const Tensor k = given ? *ok : at::empty({rows, k_pages.size(1), head_dim}, options), v = given ? *ov : at::empty({rows, k_pages.size(1), head_dim}, options);
+  segpt_paged_params p{};
+  const Tensor starts = defined_or_none(seq_start);
+  for (const Tensor* t : {&k, &v}) {
+    if (t->scalar_type() != dtype) throw BadType(std::string("out must have the dtype asked for, got ") + c10::toString(t->scalar_type()));
+    check(t->device() == dev && t->dim() == 3 && t->size(0) == rows && t->size(1) == k_pages.size(1) && t->size(2) == head_dim && (t->stride(2) == 1 || t->size(2) == 1),
+          "out must be [rows, kv heads, head_dim], contiguous in head_dim");
+  }
+  fill_paged(p, k, "out", k_pages, v_pages, scales, table, kv_len, starts, Tensor(), Tensor(), 0, max_len, 0.0, true);
+  if (given) {
+    check_apart(k, "k", v, "v");
+    for (const Tensor* o : {&k, &v}) {
+      for (const Tensor* t : {&k_pages, &v_pages, &scales.k, &scales.v, &table, &kv_len, &starts}) check_apart(*o, "out", *t, "an input");
+      check(!o->is_inference() || c10::InferenceMode::is_enabled(), "out made in inference mode can be written in inference mode only");
+      check(!(at::GradMode::is_enabled() && o->requires_grad()), "paged_kv_read has no derivative: call it under torch.no_grad() or on detached tensors");
+    }
+  } else {
+    p.flags |= SEGPT_FLAG_ZERO_REST;
+  }
+  if (k.numel() == 0) return {k, v};
+  p.k = view_rows(k); p.v = view_rows(v);
+  const c10::DeviceGuard guard(dev);
+  const segpt_paged_quant q = scales.any() ? fill_quant(scales, k_pages) : segpt_paged_quant{};
+  const int rc = segpt_paged_read(&p, scales.any() ? &q : nullptr, current_stream(dev));
+  if (rc) throw LibraryError(rc, "segpt_paged_read");
+  for (const Tensor* t : {&k, &v})
+    if (given && !t->is_inference()) torch::autograd::impl::bump_version(*t);
+  return {k, v};
+}
+
+std::pair<Tensor, Tensor> attend_over(const Scales& scales, const Tensor& q_in, const Tensor& k_pages, const Tensor& v_pages, const OptTensor& oprefix, int64_t prefix_len,
                                           const Tensor& table, const Tensor& kv_len, const Tensor& g_q, const OptTensor& og_k, const OptTensor& seq_start,
                                           const OptTensor& ogate, double gate_scale, double eps, std::optional<double> sm_scale, bool qk_norm,
                                           const OptTensor& ocos, const OptTensor& osin, int64_t pos0, std::optional<int64_t> max_len,
@@ -606,7 +710,7 @@ std::pair<Tensor, Tensor> paged_attention(const Tensor& q_in, const Tensor& k_pa
   const Tensor cos = f32_table(defined_or_none(ocos), dev), sin = f32_table(defined_or_none(osin), dev);
   const Tensor gq32 = f32_vector(g_q, dev), gk32 = f32_vector(g_k, dev);
   segpt_paged_params p{};
-  fill_paged(p, q, "q", k_pages, v_pages, table, kv_len, defined_or_none(seq_start), cos, sin, pos0, max_len, eps, qk_norm);
+  fill_paged(p, q, "q", k_pages, v_pages, scales, table, kv_len, defined_or_none(seq_start), cos, sin, pos0, max_len, eps, qk_norm);
   check(k_pages.size(1) > 0 && q.size(1) % k_pages.size(1) == 0, "number of query heads must be a multiple of the kv heads");
   check(gq32.numel() == 1 || gq32.numel() == q.size(2), "gain must have 1 or head_dim elements");
   check(!gk32.defined() || gk32.numel() == 1 || gk32.numel() == q.size(2), "k_gain must have 1 or head_dim elements");
@@ -628,7 +732,7 @@ std::pair<Tensor, Tensor> paged_attention(const Tensor& q_in, const Tensor& k_pa
     check(out.device() == dev && out.sizes() == q.sizes() && (out.stride(2) == 1 || out.size(2) == 1), "out must have q's shape and device, contiguous in head_dim");
     check(out.data_ptr() != q.data_ptr() || q.numel() == 0, "out must not be q: a row is read again after others are written");
     const Tensor starts = defined_or_none(seq_start);
-    for (const Tensor* t : {&q, &k_pages, &v_pages, &gate, &table, &kv_len, &starts, &prefix, &gq32, &gk32, &cos, &sin}) check_apart(out, "out", *t, "an input");
+    for (const Tensor* t : {&q, &k_pages, &v_pages, &scales.k, &scales.v, &gate, &table, &kv_len, &starts, &prefix, &gq32, &gk32, &cos, &sin}) check_apart(out, "out", *t, "an input");
     check(!out.is_inference() || c10::InferenceMode::is_enabled(), "out made in inference mode can be written in inference mode only");
   }
   const Tensor y = out.defined() ? out : at::empty(q.sizes(), q.options());
@@ -646,14 +750,31 @@ std::pair<Tensor, Tensor> paged_attention(const Tensor& q_in, const Tensor& k_pa
   p.q = view_rows(q); p.o = view_rows(y); p.gate = view_rows(gate);
   p.lse = ptr_of<float>(lse);
   p.g_q = ptr_of<float>(gq32); p.g_k = ptr_of<float>(gk32);
-  const size_t bytes = segpt_paged_workspace_bytes(&p);
+  const segpt_paged_quant quant = scales.any() ? fill_quant(scales, k_pages) : segpt_paged_quant{};
+  const size_t bytes = scales.any() ? segpt_paged_quant_workspace_bytes(&p, &quant) : segpt_paged_workspace_bytes(&p);
   const Tensor ws = at::empty({(int64_t)(bytes < 256 ? 256 : bytes)}, at::TensorOptions().dtype(at::kByte).device(dev));
   p.workspace = ws.data_ptr(); p.workspace_bytes = (size_t)ws.numel();
   const c10::DeviceGuard guard(dev);
-  const int rc = segpt_paged_attn(&p, current_stream(dev));
-  if (rc) throw LibraryError(rc, "segpt_paged_attn");
+  const int rc = scales.any() ? segpt_paged_attn_quant(&p, &quant, current_stream(dev)) : segpt_paged_attn(&p, current_stream(dev));
+  if (rc) throw LibraryError(rc, scales.any() ? "segpt_paged_attn_quant" : "segpt_paged_attn");
   if (out.defined() && !out.is_inference()) torch::autograd::impl::bump_version(out);
   return {y, lse};
+}
+
+std::pair<Tensor, Tensor> paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const OptTensor& prefix, int64_t prefix_len, const Tensor& table, const Tensor& kv_len,
+                                          const Tensor& g_q, const OptTensor& g_k, const OptTensor& seq_start, const OptTensor& gate, double gate_scale, double eps,
+                                          std::optional<double> sm_scale, bool qk_norm, const OptTensor& cos, const OptTensor& sin, int64_t pos0, std::optional<int64_t> max_len,
+                                          const OptTensor& out, bool with_lse) {
+  return attend_over({}, q, k_pages, v_pages, prefix, prefix_len, table, kv_len, g_q, g_k, seq_start, gate, gate_scale, eps, sm_scale, qk_norm, cos, sin, pos0,
+                     max_len, out, with_lse);
+}
+std::pair<Tensor, Tensor> paged_attention_scaled(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const OptTensor& k_scales, const OptTensor& v_scales,
+                                                 const OptTensor& prefix, int64_t prefix_len, const Tensor& table, const Tensor& kv_len,
+                                                 const Tensor& g_q, const OptTensor& g_k, const OptTensor& seq_start, const OptTensor& gate, double gate_scale, double eps,
+                                                 std::optional<double> sm_scale, bool qk_norm, const OptTensor& cos, const OptTensor& sin, int64_t pos0, std::optional<int64_t> max_len,
+                                                 const OptTensor& out, bool with_lse) {
+  return attend_over({defined_or_none(k_scales), defined_or_none(v_scales)}, q, k_pages, v_pages, prefix, prefix_len, table, kv_len, g_q, g_k, seq_start, gate, gate_scale, eps, sm_scale, qk_norm, cos, sin, pos0,
+                     max_len, out, with_lse);
 }
 
 // What torch raises (out of memory, an error from a saved-tensor hook) keeps its Python type across the binding
@@ -697,4 +818,7 @@ PYBIND11_MODULE(_segpt_torch, m) {
   m.def("generation_step", bound(&generation_step));
   m.def("paged_append", bound(&paged_append));
   m.def("paged_attention", bound(&paged_attention));
+  m.def("paged_append_scaled", bound(&paged_append_scaled));
+  m.def("paged_attention_scaled", bound(&paged_attention_scaled));
+  m.def("paged_read", bound(&paged_read));
 }

@@ -6,6 +6,7 @@
 // A code times its scale is a bf16 number, so the codes are made bf16 operands in registers (one instruction a pair of components, the scale as
 // its operand) and everything behind that is bf16 matrix products with fp32 sums, whatever the rows are: bf16 rows bring their queries in two bf16
 // parts, fp32 rows queries and probabilities in three, and neither loses anything of the keys and values as stored.
+#define SEGPT_FEW_COLUMNS 16
 #include "paged_quant.hpp"
 #include "paged_work.hpp"
 
@@ -42,40 +43,51 @@ __device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
   x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
 }
 
-// ---- the pages of an item, walked from its first key on by one wave.  Lane l holds the number of page base + l, and of page base + 64 + l, asked
-// for when the window before it was taken up; a number that is not in the pool is replaced by 0 and remembered.
-struct Pages {
+// ---- where the rows of an item lie.  One wave goes through tiles of rows that stand side by side, `STEP` keys from one tile's first to the next one's; a
+// lane works out the places of one tile, 64 tiles at a time, from a page number that was asked for 64 tiles before.  A page number that is not in the
+// pool is replaced by 0 and remembered.  A tile past the item's last key is the last one there is once more.
+template <int D, int ROWS, int STEP>  // ROWS: of a tile, which begins at a multiple of them: of one page, or 16 of two pages of eight
+struct Walk {
   const int* ids;
-  int n_pages, log_page, last;  // last: last page of the item's keys
-  int base, now, next;
+  int first, last, log_page, tiles;  // keys of the first tile and of the item's last; tiles there are
+  int upto;                          // tiles that have been worked out, the last 64 of them kept
+  int next;                          // page number of tile upto + lane
+  int64_t k, v, ks, vs;              // byte offsets of tile upto - 64 + lane from the kv head's first rows
+  int apart;                         // pages of eight: from the first eight rows' page to that of the others
   bool bad;
-  __device__ __forceinline__ int ask(int from, int lane) const { return from + lane <= last ? ids[from + lane] : 0; }
-  __device__ __forceinline__ void start(const PagedArgs& a, const Item& it, int lane) {
+  __device__ __forceinline__ int key_of(int tile) const { return min(first + tile * STEP, last & ~(ROWS - 1)); }
+  __device__ __forceinline__ int ask(int tile) const { return tiles ? ids[key_of(tile) >> log_page] : 0; }
+  __device__ __forceinline__ void start(const PagedArgs& a, const Item& it, int offset, int n, int lane) {
     ids = it.ids;
-    n_pages = a.p.n_pages;
+    first = it.k0 + offset;
+    last = it.k0 + it.nk - 1;
     log_page = a.log_page;
-    base = it.k0 >> log_page;
-    last = it.nk ? (it.k0 + it.nk - 1) >> log_page : -1;
-    now = ask(base, lane);
-    next = ask(base + 64, lane);
+    tiles = n;
+    upto = 0;
     bad = false;
+    next = ask(lane);
   }
-  __device__ __forceinline__ void check(int& id) {
-    if ((uint32_t)id >= (uint32_t)n_pages) { id = 0; bad = true; }
+  __device__ __forceinline__ int checked(const PagedArgs& a, int id) {
+    if ((uint32_t)id < (uint32_t)a.p.n_pages) return id;
+    bad = true;
+    return 0;
   }
-  __device__ __forceinline__ void arrived() { check(now); }  // before the first of()
-  __device__ __forceinline__ void reach(int key, int lane) {
-    if ((key >> log_page) - base >= 64) {
-      base += 64;
-      now = next;
-      check(now);
-      next = ask(base + 64, lane);
-    }
+  __device__ __forceinline__ void work_out(const QuantArgs& qa, const PagedArgs& a, int lane) {
+    const segpt_paged_params& p = qa.p;
+    const int key = key_of(upto + lane), id = checked(a, next);
+    const uint32_t slot = (uint32_t)(key & ((1 << log_page) - 1));
+    auto place = [&](const segpt_tensor4& t) { return (int64_t)id * t.stride_b + (int64_t)slot * t.stride_s; };
+    k = place(p.k_pages);
+    v = place(p.v_pages);
+    ks = place(qa.k_scales);
+    vs = place(qa.v_scales);
+    if (ROWS > 8 && log_page == 3) apart = key + 8 <= last && tiles ? checked(a, ids[(key + 8) >> 3]) - id : 0;
+    upto += 64;
+    if (upto < tiles) next = ask(upto + lane);
   }
-  __device__ __forceinline__ int of(int key) const { return lane_value(now, (key >> log_page) - base); }
-  __device__ __forceinline__ bool any_bad() {
-    check(next);
-    return __builtin_amdgcn_ballot_w64(bad) != 0;
+  static __device__ __forceinline__ const char* at(const char* base, int64_t off, int l) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)off, l), hi = __builtin_amdgcn_readlane((int)(off >> 32), l);
+    return base + (int64_t)((uint64_t)hi << 32 | lo);
   }
 };
 
@@ -97,46 +109,57 @@ __device__ __forceinline__ void load_words(const char* at, uint32_t* w) {
 }
 __device__ __forceinline__ float scale_at(uint32_t scales, int block) { return __uint_as_float((scales >> (8 * block) & 255u) << 23); }
 
-// Rows key .. key + rows - 1 of keys and values, `rows` of them a power of two up to 16 and key a multiple: one page, or two of eight.  A lane's
-// row stands at most `most` rows behind the first.  NP pieces of P bytes a lane, 4 P apart, the first at byte `from`.
+// A lane's part of a row of every tile: NP pieces of P bytes, 4 P apart, the first at byte `from`
 template <int D, int NP, int P>
 struct Source {
   const char *k, *v, *ks, *vs;  // first rows of the kv head
-  int64_t kb, vb, ksb, vsb;     // bytes from page to page
-  uint32_t kr, vr, ksr, vsr;    // from row to row
-  __device__ __forceinline__ void start(const QuantArgs& a, int g) {
+  uint32_t kr, vr, ksr, vsr;    // bytes from row to row
+  uint32_t from, klane, vlane, kslane, vslane;  // what a lane adds in a whole tile
+  int row;
+  __device__ __forceinline__ void start(const QuantArgs& a, int g, int own_row, uint32_t own_from) {
     k = byte_row(a.p.k_pages, 0, g, 0);
     v = byte_row(a.p.v_pages, 0, g, 0);
     ks = byte_row(a.k_scales, 0, g, 0);
     vs = byte_row(a.v_scales, 0, g, 0);
-    kb = a.p.k_pages.stride_b; vb = a.p.v_pages.stride_b; ksb = a.k_scales.stride_b; vsb = a.v_scales.stride_b;
     kr = (uint32_t)a.p.k_pages.stride_s; vr = (uint32_t)a.p.v_pages.stride_s; ksr = (uint32_t)a.k_scales.stride_s; vsr = (uint32_t)a.v_scales.stride_s;
+    row = own_row;
+    from = own_from;
+    klane = row * kr + from; vlane = row * vr + from; kslane = row * ksr; vslane = row * vsr;
   }
-  template <int ROWS>
-  __device__ __forceinline__ void ask(const Pages& pages, int key, int row, uint32_t from, RowPart<NP * P / 4>& x, RowPart<NP * P / 4>& y) const {
-    const int id = pages.of(key);
-    const uint32_t slot = (uint32_t)(key & ((1 << pages.log_page) - 1));
-    auto begin = [&](const char* first, int64_t page, uint32_t step) { return first + (int64_t)id * page + (int64_t)((uint64_t)slot * step); };
-    const char *kp = begin(k, kb, kr), *vp = begin(v, vb, vr), *ksp = begin(ks, ksb, ksr), *vsp = begin(vs, vsb, vsr);
-    auto get = [&](const char* kp, const char* vp, const char* ksp, const char* vsp, uint32_t r) {
+  static __device__ __forceinline__ void get(const char* base, uint32_t off, uint32_t (&w)[NP * P / 4]) {
 #pragma unroll
-      for (int i = 0; i < NP; ++i) load_words<P>(kp + (r * kr + from + i * 4 * P), x.w + i * P / 4);
-      x.s = load_scales<D>(ksp + r * ksr);
-#pragma unroll
-      for (int i = 0; i < NP; ++i) load_words<P>(vp + (r * vr + from + i * 4 * P), y.w + i * P / 4);
-      y.s = load_scales<D>(vsp + r * vsr);
-    };
-    if (ROWS <= 8 || pages.log_page > 3) {
-      get(kp, vp, ksp, vsp, (uint32_t)row);
-    } else {  // the second eight rows lie in a page of their own (or nowhere, and no lane's row is among them)
-      const int64_t by = (int64_t)pages.of(key + 8) - id;
-      const bool second = row >= 8;
-      get(kp + (second ? by * kb : 0), vp + (second ? by * vb : 0), ksp + (second ? by * ksb : 0), vsp + (second ? by * vsb : 0), (uint32_t)(second ? row - 8 : row));
+    for (int i = 0; i < NP; ++i) load_words<P>(base + (off + i * 4 * P), w + i * P / 4);
+  }
+  // tile: of the 64 that were worked out last
+  template <int ROWS, int STEP>
+  __device__ __forceinline__ void ask(const Walk<D, ROWS, STEP>& w, const QuantArgs& qa, int tile, RowPart<NP * P / 4>& x, RowPart<NP * P / 4>& y) const {
+    using W = Walk<D, ROWS, STEP>;
+    const int l = tile & 63, left = w.last - w.key_of(tile);
+    const char *kp = W::at(k, w.k, l), *vp = W::at(v, w.v, l), *ksp = W::at(ks, w.ks, l), *vsp = W::at(vs, w.vs, l);
+    uint32_t ko = klane, vo = vlane, kso = kslane, vso = vslane;
+    if (left < ROWS - 1) {  // past the last key: its row once more
+      const uint32_t r = min(row, left);
+      ko = r * kr + from; vo = r * vr + from; kso = r * ksr; vso = r * vsr;
+    }
+    if (ROWS > 8 && w.log_page == 3) {  // the second eight rows lie in a page of their own
+      const bool second = min(row, left) >= 8;
+      const int pages = lane_value(w.apart, l);  // outside the condition: the lane that is asked need not be among those that want it
+      const int64_t by = second ? pages : 0;
+      auto moved = [&](const char* base, int64_t page, uint32_t step) { return base + (by * page - (second ? (int64_t)8 * step : 0)); };
+      get(moved(kp, qa.p.k_pages.stride_b, kr), ko, x.w);
+      x.s = load_scales<D>(moved(ksp, qa.k_scales.stride_b, ksr) + kso);
+      get(moved(vp, qa.p.v_pages.stride_b, vr), vo, y.w);
+      y.s = load_scales<D>(moved(vsp, qa.v_scales.stride_b, vsr) + vso);
+    } else {
+      get(kp, ko, x.w);
+      x.s = load_scales<D>(ksp + kso);
+      get(vp, vo, y.w);
+      y.s = load_scales<D>(vsp + vso);
     }
   }
 };
 
-// ---- FEW: one wave, CT tiles of 16 columns.  A score tile is 16 keys by 16 columns; a lane takes a quarter of a key's row, so that a row is read
+// ---- FEW: one wave, up to 16 columns.  A score tile is 16 keys by 16 columns; a lane takes a quarter of a key's row, so that a row is read
 // whole by four lanes and is the A operand as it is decoded, no LDS in between: the components that a lane contributes to a step are not those of
 // the instruction's own order, but the queries' are the same, and a sum does not ask.
 template <int D, int FMT>
@@ -159,59 +182,6 @@ struct Quarter {
         decode8<FMT>(x.w + i * (P / 4) + u * kWordsOf8, scale, r);
         out[i * (EP / 8) + u] = u32x4{r[0], r[1], r[2], r[3]};
       }
-    }
-  }
-};
-template <typename E, int D, int FMT>
-struct Query16 {
-  using L = Quarter<D, FMT>;
-  static constexpr int KS = L::KS, kCols = 16, kLogCols = 4, PARTS = kQueryParts<E>;
-  bf16x8 part[PARTS][KS];
-  float x[KS][8], other[KS][8], cs[KS][8], sn[KS][8];
-  __device__ __forceinline__ void fetch(const segpt_paged_params& p, const E* row, int64_t angle, int quarter) {
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) load8(row + L::component(ks, quarter), x[ks]);
-    if (!p.rope_cos) return;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const int d = L::component(ks, quarter), j = d % (D / 2);
-      load8(row + (d + D / 2) % D, other[ks]);
-      load8(p.rope_cos + angle + j, cs[ks]);
-      load8(p.rope_sin + angle + j, sn[ks]);
-    }
-  }
-  __device__ __forceinline__ void finish(const segpt_paged_params& p, bool live, int quarter, const float* gsm) {
-    if (p.rope_cos) {
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const float sign = L::component(ks, quarter) < D / 2 ? -1.f : 1.f;
-#pragma unroll
-        for (int t = 0; t < 8; ++t) x[ks][t] = x[ks][t] * cs[ks][t] + sign * (other[ks][t] * sn[ks][t]);
-      }
-    }
-    float sq[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int t = 0; t < 8; ++t) sq[t % 4] += x[ks][t] * x[ks][t];
-    float ss = (sq[0] + sq[1]) + (sq[2] + sq[3]);
-    ss += __shfl_xor(ss, 16, 64);
-    ss = half_sum(ss);
-    const float alpha = (p.flags & SEGPT_FLAG_NO_NORM) ? 1.f : 1.0f / sqrtf(ss * (1.0f / D) + p.eps);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      float g[8];
-      load8(gsm + L::component(ks, quarter), g);
-      u32x4 w[PARTS];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t part_i[PARTS];
-        parts_of<PARTS>(x[ks][2 * i] * alpha * g[2 * i], x[ks][2 * i + 1] * alpha * g[2 * i + 1], part_i);
-#pragma unroll
-        for (int u = 0; u < PARTS; ++u) w[u][i] = live ? part_i[u] : 0u;
-      }
-#pragma unroll
-      for (int u = 0; u < PARTS; ++u) part[u][ks] = as_bf16x8(w[u]);
     }
   }
 };
@@ -238,6 +208,85 @@ struct ValueTile {
   }
 };
 __device__ __forceinline__ void lds_write16(uint32_t addr, u32x4 v) { *(__attribute__((address_space(3))) u32x4*)addr = v; }
+
+// this wave's LDS reads have returned (before what they came from is written over), its LDS writes are there
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0) only
+}
+
+// The queries of 16 columns: a lane has a quarter of a column's pairs, works them out, and the parts reach the operand's order through LDS (the
+// value tile's, which is not in use yet)
+template <typename E, int D, int FMT>
+struct Query16 {
+  using L = Quarter<D, FMT>;
+  static constexpr int KS = L::KS, kCols = 16, kLogCols = 4, PARTS = kQueryParts<E>, N = D / 64;
+  bf16x8 part[PARTS][KS];
+  struct Row {
+    float x[2][N][8], cs[N][8], sn[N][8];  // pairs (quarter * N + n) * 8 .. + 7
+  };
+  Row row;
+  __device__ __forceinline__ void fetch(const segpt_paged_params& p, const E* at, int64_t angle, int quarter) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int j = (quarter * N + n) * 8;
+      load8(at + j, row.x[0][n]);
+      load8(at + j + D / 2, row.x[1][n]);
+      if (p.rope_cos) {
+        load8(p.rope_cos + angle + j, row.cs[n]);
+        load8(p.rope_sin + angle + j, row.sn[n]);
+      }
+    }
+  }
+  __device__ __forceinline__ void finish(const segpt_paged_params& p, bool live, int lane, const float* gsm, uint32_t lds) {
+    using V = ValueTile<D>;
+    const int quarter = lane >> 4, col = lane & 15;
+    if (p.rope_cos) {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int t = 0; t < 8; ++t) rope_pair(row.x[0][n][t], row.x[1][n][t], row.cs[n][t], row.sn[n][t]);
+    }
+    float sq[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int t = 0; t < 8; ++t) sq[t % 4] += row.x[h][n][t] * row.x[h][n][t];
+    float ss = (sq[0] + sq[1]) + (sq[2] + sq[3]);
+    ss += __shfl_xor(ss, 16, 64);
+    ss = half_sum(ss);
+    const float alpha = !live ? 0.f : (p.flags & SEGPT_FLAG_NO_NORM) ? 1.f : 1.0f / sqrtf(ss * (1.0f / D) + p.eps);
+    u32x4 w[PARTS][2][N];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        float g[8];
+        load8(gsm + (quarter * N + n) * 8 + h * (D / 2), g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t part_i[PARTS];
+          parts_of<PARTS>(live ? row.x[h][n][2 * i] * alpha * g[2 * i] : 0.f, live ? row.x[h][n][2 * i + 1] * alpha * g[2 * i + 1] : 0.f, part_i);
+#pragma unroll
+          for (int u = 0; u < PARTS; ++u) w[u][h][n][i] = part_i[u];
+        }
+      }
+#pragma unroll
+    for (int u = 0; u < PARTS; ++u) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int n = 0; n < N; ++n) lds_write16(lds + V::write_at(col, quarter * N + n + h * (D / 16)), w[u][h][n]);
+      wave_sync();
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) part[u][ks] = as_bf16x8(lds_read16(lds + V::write_at(col, L::component(ks, quarter) / 8)));
+      wave_sync();
+    }
+  }
+};
 
 // A value that is no number must reach the rows that see its key, and not the others as 0 * NaN: in a block that not all rows see it is made 0 and
 // noted, and put back behind the loop
@@ -266,70 +315,47 @@ __device__ __forceinline__ void odd_values(const QuantArgs& qa, const PagedArgs&
   }
 }
 
-// this wave's LDS reads have returned (before what they came from is written over), its LDS writes are there
-__device__ __forceinline__ void wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0) only
-}
-
-template <typename E, int D, int FMT, int CT>
+template <typename E, int D, int FMT>
 __device__ __forceinline__ void few_columns(const QuantArgs& qa, const PagedArgs& a, const Item& it, int rep, int lane, uint32_t lds, float* gsm) {
   using L = Quarter<D, FMT>;
   using V = ValueTile<D>;
   constexpr int KS = L::KS, DB = D / 16, PARTS = kQueryParts<E>;
   const segpt_paged_params& p = a.p;
   const int quarter = lane >> 4, r16 = lane & 15;
-  const int last = it.k0 + it.nk - 1, blocks = (it.nk + kBlock - 1) / kBlock;
+  const int blocks = (it.nk + kBlock - 1) / kBlock;
   // one round trip: gain, query rows and angles, page numbers
-  Pages pages;
-  pages.start(a, it, lane);
-  Gain gain[(D + 63) / 64];
+  Walk<D, 16, 16> walk;
+  walk.start(a, it, 0, 2 * blocks, lane);
+  Gain gain[D / 64];
 #pragma unroll
-  for (int i = 0; i < (D + 63) / 64; ++i) gain[i] = fetch_gain(p, (64 * i + lane) % D);
-  Query16<E, D, FMT> q[CT];
-  Column c[CT];
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) c[ct] = column_of<E, D>(a, it, rep, it.tile * kFew + 16 * ct, lane, q[ct]);
+  for (int i = 0; i < D / 64; ++i) gain[i] = fetch_gain(p, 64 * i + lane);
+  Query16<E, D, FMT> q;
+  const Column c = column_of<E, D>(a, it, rep, it.tile * kFew, lane, q);
   Source<D, L::NP, L::P> src;
-  src.start(qa, it.g);
-  pages.arrived();
+  src.start(qa, it.g, r16, (uint32_t)quarter * L::P);
   struct Block {
     RowPart<L::kWords> k[2], v[2];
   };
   auto ask = [&](Block& b, int j) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int key = min(it.k0 + j * kBlock + 16 * t, last & ~15);  // past the last key: the last row once more
-      pages.reach(key, lane);
-      src.template ask<16>(pages, key, min(r16, last - key), (uint32_t)quarter * L::P, b.k[t], b.v[t]);
-    }
+    for (int t = 0; t < 2; ++t) src.ask(walk, qa, 2 * j + t, b.k[t], b.v[t]);
   };
   Block b0, b1;
+  walk.work_out(qa, a, lane);
   if (blocks > 0) ask(b0, 0);
   if (blocks > 1) ask(b1, 1);
 #pragma unroll
-  for (int i = 0; i < (D + 63) / 64; ++i)
-    if (64 * i + lane < D) gsm[64 * i + lane] = scale_of(p, gain[i]);
+  for (int i = 0; i < D / 64; ++i) gsm[64 * i + lane] = scale_of(p, gain[i]);
   wave_sync();
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) q[ct].finish(p, c[ct].live, quarter, gsm);
+  q.finish(p, c.live, lane, gsm, lds);
 
-  f32x4 o[CT][DB];
-  float m[CT], limit[CT], l[CT];
+  f32x4 o[DB];
+  float m = 0.f, limit = -INFINITY, l = 0.f;  // reference (log2 units); by how much a score may exceed it; sum over this lane's keys
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    m[ct] = 0.f;
-    limit[ct] = -INFINITY;
-    l[ct] = 0.f;
-#pragma unroll
-    for (int db = 0; db < DB; ++db) o[ct][db] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  int all = c[0].all;
-#pragma unroll
-  for (int ct = 1; ct < CT; ++ct) all = min(all, c[ct].all);
+  for (int db = 0; db < DB; ++db) o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
   bool odd = false;
   auto step = [&](Block& b, int j) {
+    const bool masked = j * kBlock + kBlock - 1 > c.all;
     u32x4 k[2][KS];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -340,108 +366,97 @@ __device__ __forceinline__ void few_columns(const QuantArgs& qa, const PagedArgs
       for (int ks = 0; ks < KS; ++ks) lds_write16(lds + V::write_at(16 * t + r16, L::component(ks, quarter) / 8), v[ks]);
     }
     if (j + 2 < blocks) ask(b, j + 2);
-    const bool masked = j * kBlock + kBlock - 1 > all;
-    f32x4 s[CT][2];
+    f32x4 s[2];
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
+    for (int t = 0; t < 2; ++t) {
+      s[t] = f32x4{-m, -m, -m, -m};
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        s[ct][t] = f32x4{-m[ct], -m[ct], -m[ct], -m[ct]};
+      for (int u = PARTS - 1; u >= 0; --u)
 #pragma unroll
-        for (int u = PARTS - 1; u >= 0; --u)
+        for (int ks = 0; ks < KS; ++ks) s[t] = mfma16(as_bf16x8(k[t][ks]), q.part[u][ks], s[t]);
+      if (masked) {
+        const int seen = c.lim - j * kBlock - 16 * t - 4 * quarter;
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) s[ct][t] = mfma16(as_bf16x8(k[t][ks]), q[ct].part[u][ks], s[ct][t]);
-        if (masked) {
-          const int seen = c[ct].lim - j * kBlock - 16 * t - 4 * quarter;
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (r > seen) s[ct][t][r] = -INFINITY;
-        }
+        for (int r = 0; r < 4; ++r)
+          if (r > seen) s[t][r] = -INFINITY;
       }
-    u32x4 pb[CT][PARTS];
+    }
+    float top = s[0][0];
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      float top = s[ct][0][0];
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i / 4][i % 4]);
+    if (__builtin_amdgcn_ballot_w64(top > limit) != 0) {  // a lane's own keys may tell; the column's reference is one for its four lanes
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = half_max(top);
+      const float up = top > limit ? top : 0.f, corr = limit == -INFINITY ? 1.f : fast_exp2(-up);  // nothing to scale before the first key
+      m += up;
+      if (top > limit) limit = kLazy;
+      l *= corr;
 #pragma unroll
-      for (int i = 1; i < 8; ++i) top = fmaxf(top, s[ct][i / 4][i % 4]);
-      if (__builtin_amdgcn_ballot_w64(top > limit[ct]) != 0) {  // a lane's own keys may tell; the column's reference is one for its four lanes
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = half_max(top);
-        const float up = top > limit[ct] ? top : 0.f, corr = limit[ct] == -INFINITY ? 1.f : fast_exp2(-up);
-        m[ct] += up;
-        if (top > limit[ct]) limit[ct] = kLazy;
-        l[ct] *= corr;
+      for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
+        for (int r = 0; r < 4; ++r) o[db][r] *= corr;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) o[ct][db][r] *= corr;
+      for (int i = 0; i < 8; ++i) s[i / 4][i % 4] -= up;
+    }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[ct][i / 4][i % 4] -= up;
-      }
+    for (int i = 0; i < 8; ++i) {
+      s[i / 4][i % 4] = fast_exp2(s[i / 4][i % 4]);
+      l += s[i / 4][i % 4];
+    }
+    u32x4 pb[PARTS];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        s[ct][i / 4][i % 4] = fast_exp2(s[ct][i / 4][i % 4]);
-        l[ct] += s[ct][i / 4][i % 4];
-      }
+    for (int i = 0; i < 4; ++i) {
+      uint32_t w[PARTS];
+      parts_of<PARTS>(s[i / 2][i % 2 * 2], s[i / 2][i % 2 * 2 + 1], w);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t w[PARTS];
-        parts_of<PARTS>(s[ct][i / 2][i % 2 * 2], s[ct][i / 2][i % 2 * 2 + 1], w);
-#pragma unroll
-        for (int u = 0; u < PARTS; ++u) pb[ct][u][i] = w[u];
-      }
+      for (int u = 0; u < PARTS; ++u) pb[u][i] = w[u];
     }
     wave_sync();
+    u32x4 v[DB];
 #pragma unroll
-    for (int db = 0; db < DB; ++db) {
-      u32x4 v = V::read(lds, lane, db);
-      if (masked) odd |= clear_nan(v);
+    for (int db = 0; db < DB; ++db) v[db] = V::read(lds, lane, db);
+    if (masked) {
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-        for (int u = PARTS - 1; u >= 0; --u) o[ct][db] = mfma16(as_bf16x8(v), as_bf16x8(pb[ct][u]), o[ct][db]);
+      for (int db = 0; db < DB; ++db) odd |= clear_nan(v[db]);
     }
+#pragma unroll
+    for (int u = PARTS - 1; u >= 0; --u)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db] = mfma16(as_bf16x8(v[db]), as_bf16x8(pb[u]), o[db]);
     wave_sync();
   };
   for (int j = 0; j < blocks; j += 2) {
+    if ((2 * j + 4) % 64 == 0 && j + 2 < blocks) walk.work_out(qa, a, lane);  // the next tiles asked for: 2 j + 4 .. 2 j + 7
     step(b0, j);
     if (j + 1 < blocks) step(b1, j + 1);
   }
-  const bool bad = it.x.broken | pages.any_bad();
-  if (__builtin_amdgcn_ballot_w64(odd) != 0) {
+  const bool bad = it.x.broken | (__builtin_amdgcn_ballot_w64(walk.bad) != 0);
+  if (__builtin_amdgcn_ballot_w64(odd) != 0)
+    odd_values<D>(qa, a, it, c, (max(c.all, -1) + 1) / kBlock * kBlock, [&](int b) {
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
-      odd_values<D>(qa, a, it, c[ct], (max(all, -1) + 1) / kBlock * kBlock, [&](int b) {
+      for (int db = 0; db < DB; ++db)
+        if (db / 2 == b) o[db] = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+    });
+  float sum = l + __shfl_xor(l, 16, 64), ref = limit == -INFINITY ? -INFINITY : m;
+  sum = half_sum(sum);
+  if (bad) { sum = __builtin_nanf(""); ref = 0.f; }
+  if (!c.live) return;
+  if (!it.direct) {
+    const int64_t at = (int64_t)it.slot * 32 + r16;
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
-          if (db / 2 == b)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[ct][db][r] = __builtin_nanf("");
-      });
+    for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(a.part + at * D + 16 * db + 4 * quarter) = o[db];
+    if (quarter == 0) a.stat[at] = make_float2(ref, sum);
+    return;
   }
+  float f = sum == 0.f ? 0.f : 1.0f / sum;
+  if (p.lse && quarter == 0) p.lse[(int64_t)c.t * p.H + c.h] = sum == 0.f ? -INFINITY : (ref + __log2f(sum)) * kLn2;
+  if (p.gate.ptr) f *= gate_factor<E, D>(p, c.t, c.h);
+  E* out = row_of<E>(p.o, c.t, c.h) + 4 * quarter;
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    float sum = l[ct] + __shfl_xor(l[ct], 16, 64), ref = limit[ct] == -INFINITY ? -INFINITY : m[ct];
-    sum = half_sum(sum);
-    if (bad) { sum = __builtin_nanf(""); ref = 0.f; }
-    if (!c[ct].live) continue;
-    if (!it.direct) {
-      const int64_t at = (int64_t)it.slot * 32 + 16 * ct + r16;
-#pragma unroll
-      for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(a.part + at * D + 16 * db + 4 * quarter) = o[ct][db];
-      if (quarter == 0) a.stat[at] = make_float2(ref, sum);
-      continue;
-    }
-    float f = sum == 0.f ? 0.f : 1.0f / sum;
-    if (p.lse && quarter == 0) p.lse[(int64_t)c[ct].t * p.H + c[ct].h] = sum == 0.f ? -INFINITY : (ref + __log2f(sum)) * kLn2;
-    if (p.gate.ptr) f *= gate_factor<E, D>(p, c[ct].t, c[ct].h);
-    E* out = row_of<E>(p.o, c[ct].t, c[ct].h) + 4 * quarter;
-#pragma unroll
-    for (int db = 0; db < DB; ++db) {
-      const float y[4] = {o[ct][db][0] * f, o[ct][db][1] * f, o[ct][db][2] * f, o[ct][db][3] * f};
-      if constexpr (sizeof(E) == 2) *reinterpret_cast<u32x2*>(out + 16 * db) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
-      else store16(out + 16 * db, y);
-    }
+  for (int db = 0; db < DB; ++db) {
+    const float y[4] = {o[db][0] * f, o[db][1] * f, o[db][2] * f, o[db][3] * f};
+    if constexpr (sizeof(E) == 2) *reinterpret_cast<u32x2*>(out + 16 * db) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+    else store16(out + 16 * db, y);
   }
 }
 
@@ -507,24 +522,21 @@ __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArg
   constexpr int P = 16 * Codes<FMT>::kBits / 8;  // bytes of a lane's 16 components
   const segpt_paged_params& p = a.p;
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
-  const int own_row = lane / S::kLanes, own_part = lane % S::kLanes, last = it.k0 + it.nk - 1, n_kt = (it.nk + BK - 1) / BK;
+  const int own_row = lane / S::kLanes, own_part = lane % S::kLanes, n_kt = (it.nk + BK - 1) / BK;
   // one round trip: gain, query row and angles, page numbers
-  Pages pages;
-  pages.start(a, it, lane);
+  Walk<D, S::kRows, BK> walk;
+  walk.start(a, it, wave * S::kRows, n_kt, lane);
   const Gain gain = fetch_gain(p, tid % D);
   Query32<E, D> q;
   const Column c = column_of<E, D>(a, it, rep, it.tile * kMany + wave * 32, lane, q);
   Source<D, 1, P> src;
-  src.start(qa, it.g);
-  pages.arrived();
+  src.start(qa, it.g, own_row, (uint32_t)own_part * P);
   struct Raw2 {
     RowPart<P / 4> k, v;
   };
   auto ask = [&](Raw2& x, int jt) {
     if (jt >= n_kt) return;
-    const int key = min(it.k0 + jt * BK + wave * S::kRows, last & ~(S::kRows - 1));
-    pages.reach(key, lane);
-    src.template ask<S::kRows>(pages, key, min(own_row, last - key), (uint32_t)own_part * P, x.k, x.v);
+    src.ask(walk, qa, jt, x.k, x.v);
   };
   auto put = [&](const Raw2& x, int jt, uint32_t stage) {
     if (jt >= n_kt) return;
@@ -542,6 +554,7 @@ __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArg
     tensor(x.v, lds + stage + S::kTileBytes);
   };
   Raw2 x0, x1;
+  walk.work_out(qa, a, lane);
   ask(x0, 0);
   ask(x1, 1);
   if (tid < D) gsm[tid] = scale_of(p, gain);
@@ -641,15 +654,20 @@ __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArg
   };
   // two turns a round, so that scores and codes change places without being copied
   int jt = 0;
+  auto places = [&] {  // of the next two tiles asked for
+    if ((jt + 4) % 64 == 0 && jt + 4 < n_kt) walk.work_out(qa, a, lane);
+  };
   for (; jt + 2 < n_whole; jt += 2) {
+    places();
     whole(jt, x0, s0, s1);
     whole(jt + 1, x1, s1, s0);
   }
   for (; jt < n_kt; jt += 2) {
+    places();
     any_tiles(jt, x0, s0, s1);
     if (jt + 1 < n_kt) any_tiles(jt + 1, x1, s1, s0);
   }
-  const bool bad = it.x.broken | pages.any_bad();
+  const bool bad = it.x.broken | (__builtin_amdgcn_ballot_w64(walk.bad) != 0);
   if (__builtin_amdgcn_ballot_w64(odd) != 0)
     odd_values<D>(qa, a, it, c, (max(c.all, -1) + 1) / BK * BK, [&](int b) {
 #pragma unroll
@@ -679,8 +697,7 @@ __global__ __launch_bounds__(64, 2) void paged_quant_few_kernel(Args args) {
   const Item it = locate<false>(a, lane, rep, share, mine, blockIdx.x);
   if (!it.valid) return;
   const QuantArgs qa = quant_of(args);
-  if (it.cols <= 16) few_columns<E, D, FMT, 1>(qa, a, it, rep, lane, lds_addr_of(lds), gsm);
-  else few_columns<E, D, FMT, 2>(qa, a, it, rep, lane, lds_addr_of(lds), gsm);
+  few_columns<E, D, FMT>(qa, a, it, rep, lane, lds_addr_of(lds), gsm);
 }
 
 // Any launch: the first workgroups are items of many columns, the next four items each of few, the rest have none
@@ -704,9 +721,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 2 || D == 64 ? 2 : 1)) void page
   } else {
     const Item it4 = locate<false>(a, lane, rep, share, mine, ((int)blockIdx.x - it.x.base) * 4 + wave);
     if (!it4.valid) return;
-    const uint32_t at = lds_addr_of(lds) + wave * ValueTile<D>::kBytes;
-    if (it4.cols <= 16) few_columns<E, D, FMT, 1>(qa, a, it4, rep, lane, at, gsm[wave]);
-    else few_columns<E, D, FMT, 2>(qa, a, it4, rep, lane, at, gsm[wave]);
+    few_columns<E, D, FMT>(qa, a, it4, rep, lane, lds_addr_of(lds) + wave * ValueTile<D>::kBytes, gsm[wave]);
   }
 }
 

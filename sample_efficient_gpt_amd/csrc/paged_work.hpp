@@ -53,7 +53,10 @@ struct PagedArgs {
 };
 
 constexpr int kBlock = 32;          // keys of a score tile
-constexpr int kFew = 32, kMany = 128;  // columns of a tile
+#ifndef SEGPT_FEW_COLUMNS
+#define SEGPT_FEW_COLUMNS 32
+#endif
+constexpr int kFew = SEGPT_FEW_COLUMNS, kMany = 128;  // columns of a tile; kFew: up to 32, set where another number suits the kernels
 constexpr float kLazy = 8.f;        // the reference is raised where a score exceeds it by 2^8: probabilities stay below 2^8
 
 // ---- the plan, computed by every wave for itself or, for many entries, by paged_plan_kernel
@@ -333,7 +336,7 @@ struct Item {
 };
 template <bool MANY>
 __device__ __forceinline__ Item locate(const PagedArgs& a, int lane, int rep, const Shares& share, const Entries& mine, int number) {
-  constexpr int COLS = MANY ? kMany : kFew;
+  constexpr int COLS = MANY ? kMany : kFew, SLOTS = MANY ? kMany / 32 : 1;
   Item it;
   it.x = find_entry<MANY ? kFindMany : kFindFew>(a, lane, rep, share, mine, number);
   const Found& x = it.x;
@@ -348,9 +351,9 @@ __device__ __forceinline__ Item locate(const PagedArgs& a, int lane, int rep, co
   it.tile = n_tiles - 1 - from_last;  // the last tiles see the most keys: they start first
   it.prefix = a.shared && x.entry == 0;
   it.direct = !a.shared && x.shares == 1;
-  it.slot = x.slot + ((it.tile * x.shares + it.part) * a.p.Hkv + it.g) * (COLS / 32);
+  it.slot = x.slot + ((it.tile * x.shares + it.part) * a.p.Hkv + it.g) * SLOTS;
   // row ranges that overlap may add up to more than 32 bits hold: nothing is written outside the scratch
-  it.valid = it.tile >= 0 && (it.direct || (it.slot >= 0 && it.slot <= a.n_slots - COLS / 32));
+  it.valid = it.tile >= 0 && (it.direct || (it.slot >= 0 && it.slot <= a.n_slots - SLOTS));
   it.past = x.len - x.n;
   const int per = shares.of(x.blocks + x.shares - 1) * kBlock;  // shares as even as whole blocks allow
   const int last_col = min(it.cols, (it.tile + 1) * COLS) - 1, sees = it.prefix ? x.len : min(x.len, it.past + a.rep.of(last_col) + 1);

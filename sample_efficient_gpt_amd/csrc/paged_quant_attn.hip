@@ -43,21 +43,32 @@ __device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
   x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
 }
 
+// this wave's LDS reads have returned (before what they came from is written over), its LDS writes are there
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0) only
+}
+
 // ---- where the rows of an item lie.  One wave goes through tiles of rows that stand side by side, `STEP` keys from one tile's first to the next one's; a
 // lane works out the places of one tile, 64 tiles at a time, from a page number that was asked for 64 tiles before.  A page number that is not in the
 // pool is replaced by 0 and remembered.  A tile past the item's last key is the last one there is once more.
-template <int D, int ROWS, int STEP>  // ROWS: of a tile, which begins at a multiple of them: of one page, or 16 of two pages of eight
+// In LDS, or where registers are at hand in those.
+template <int ROWS, int STEP, bool LDS>  // ROWS: of a tile, which begins at a multiple of them: of one page, or 16 of two pages of eight
 struct Walk {
+  static constexpr int kBytes = 64 * 4 * 8;  // of LDS
   const int* ids;
   int first, last, log_page, tiles;  // keys of the first tile and of the item's last; tiles there are
   int upto;                          // tiles that have been worked out, the last 64 of them kept
   int next;                          // page number of tile upto + lane
-  int64_t k, v, ks, vs;              // byte offsets of tile upto - 64 + lane from the kv head's first rows
+  int64_t place[LDS ? 1 : 4];        // byte offsets of tile upto - 64 + lane from the kv head's first rows: keys, values, their scales
+  uint32_t lds;
   int apart;                         // pages of eight: from the first eight rows' page to that of the others
   bool bad;
   __device__ __forceinline__ int key_of(int tile) const { return min(first + tile * STEP, last & ~(ROWS - 1)); }
   __device__ __forceinline__ int ask(int tile) const { return tiles ? ids[key_of(tile) >> log_page] : 0; }
-  __device__ __forceinline__ void start(const PagedArgs& a, const Item& it, int offset, int n, int lane) {
+  __device__ __forceinline__ void start(const PagedArgs& a, const Item& it, int offset, int n, int lane, uint32_t lds_at) {
+    lds = lds_at;
     ids = it.ids;
     first = it.k0 + offset;
     last = it.k0 + it.nk - 1;
@@ -76,17 +87,29 @@ struct Walk {
     const segpt_paged_params& p = qa.p;
     const int key = key_of(upto + lane), id = checked(a, next);
     const uint32_t slot = (uint32_t)(key & ((1 << log_page) - 1));
-    auto place = [&](const segpt_tensor4& t) { return (int64_t)id * t.stride_b + (int64_t)slot * t.stride_s; };
-    k = place(p.k_pages);
-    v = place(p.v_pages);
-    ks = place(qa.k_scales);
-    vs = place(qa.v_scales);
+    const segpt_tensor4* all[4] = {&p.k_pages, &p.v_pages, &qa.k_scales, &qa.v_scales};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t at = (int64_t)id * all[i]->stride_b + (int64_t)slot * all[i]->stride_s;
+      if constexpr (LDS) *(__attribute__((address_space(3))) int64_t*)(lds + 512 * i + 8 * lane) = at;
+      else place[i] = at;
+    }
+    if constexpr (LDS) wave_sync();
     if (ROWS > 8 && log_page == 3) apart = key + 8 <= last && tiles ? checked(a, ids[(key + 8) >> 3]) - id : 0;
     upto += 64;
     if (upto < tiles) next = ask(upto + lane);
   }
-  static __device__ __forceinline__ const char* at(const char* base, int64_t off, int l) {
-    const uint32_t lo = __builtin_amdgcn_readlane((int)off, l), hi = __builtin_amdgcn_readlane((int)(off >> 32), l);
+  // first row of tile l of those, in tensor i
+  __device__ __forceinline__ const char* at(int i, const char* base, int l) const {
+    uint32_t lo, hi;
+    if constexpr (LDS) {
+      const u32x2 off = *(const __attribute__((address_space(3))) u32x2*)(lds + 512 * i + 8 * l);
+      lo = __builtin_amdgcn_readfirstlane((int)off[0]);
+      hi = __builtin_amdgcn_readfirstlane((int)off[1]);
+    } else {
+      lo = __builtin_amdgcn_readlane((int)place[i], l);
+      hi = __builtin_amdgcn_readlane((int)(place[i] >> 32), l);
+    }
     return base + (int64_t)((uint64_t)hi << 32 | lo);
   }
 };
@@ -131,11 +154,10 @@ struct Source {
     for (int i = 0; i < NP; ++i) load_words<P>(base + (off + i * 4 * P), w + i * P / 4);
   }
   // tile: of the 64 that were worked out last
-  template <int ROWS, int STEP>
-  __device__ __forceinline__ void ask(const Walk<D, ROWS, STEP>& w, const QuantArgs& qa, int tile, RowPart<NP * P / 4>& x, RowPart<NP * P / 4>& y) const {
-    using W = Walk<D, ROWS, STEP>;
+  template <int ROWS, int STEP, bool LDS>
+  __device__ __forceinline__ void ask(const Walk<ROWS, STEP, LDS>& w, const QuantArgs& qa, int tile, RowPart<NP * P / 4>& x, RowPart<NP * P / 4>& y) const {
     const int l = tile & 63, left = w.last - w.key_of(tile);
-    const char *kp = W::at(k, w.k, l), *vp = W::at(v, w.v, l), *ksp = W::at(ks, w.ks, l), *vsp = W::at(vs, w.vs, l);
+    const char *kp = w.at(0, k, l), *vp = w.at(1, v, l), *ksp = w.at(2, ks, l), *vsp = w.at(3, vs, l);
     uint32_t ko = klane, vo = vlane, kso = kslane, vso = vslane;
     if (left < ROWS - 1) {  // past the last key: its row once more
       const uint32_t r = min(row, left);
@@ -208,13 +230,6 @@ struct ValueTile {
   }
 };
 __device__ __forceinline__ void lds_write16(uint32_t addr, u32x4 v) { *(__attribute__((address_space(3))) u32x4*)addr = v; }
-
-// this wave's LDS reads have returned (before what they came from is written over), its LDS writes are there
-__device__ __forceinline__ void wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0) only
-}
 
 // The queries of 16 columns: a lane has a quarter of a column's pairs, works them out, and the parts reach the operand's order through LDS (the
 // value tile's, which is not in use yet)
@@ -324,8 +339,8 @@ __device__ __forceinline__ void few_columns(const QuantArgs& qa, const PagedArgs
   const int quarter = lane >> 4, r16 = lane & 15;
   const int blocks = (it.nk + kBlock - 1) / kBlock;
   // one round trip: gain, query rows and angles, page numbers
-  Walk<D, 16, 16> walk;
-  walk.start(a, it, 0, 2 * blocks, lane);
+  Walk<16, 16, false> walk;
+  walk.start(a, it, 0, 2 * blocks, lane, 0);
   Gain gain[D / 64];
 #pragma unroll
   for (int i = 0; i < D / 64; ++i) gain[i] = fetch_gain(p, 64 * i + lane);
@@ -461,8 +476,8 @@ __device__ __forceinline__ void few_columns(const QuantArgs& qa, const PagedArgs
 }
 
 // ---- MANY: four waves of 32 columns around a ring of three stages (K' tile, V' tile of bf16); tile jt lives in stage jt % 3.  The codes of a tile are
-// asked for four turns before its products, two tiles ahead of the ring in registers, and decoded into LDS two turns before.  A turn computes the
-// scores of tile jt + 1 beside the exponentials of tile jt and its product with the values.
+// asked for three turns before its products, kept in registers for one, and decoded into LDS.  The scores of a block of 32 keys are computed beside the
+// exponentials of the block before it and its product with the values.
 template <int D>
 struct ManyShape {
   static constexpr int kBK = D == 64 ? 64 : 32, kTileBytes = kBK * 2 * D, kStageBytes = 2 * kTileBytes, kStages = 3;
@@ -516,7 +531,7 @@ struct Query32 {
 };
 
 template <typename E, int D, int FMT>
-__device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArgs& a, const Item& it, int rep, int tid, uint32_t lds, float* gsm) {
+__device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArgs& a, const Item& it, int rep, int tid, uint32_t lds, uint32_t places, float* gsm) {
   using S = ManyShape<D>;
   constexpr int BK = S::kBK, N = BK / 32, MB = D / 32, KS = D / 16, PARTS = kQueryParts<E>, PROBS = sizeof(E) == 2 ? 1 : 3;
   constexpr int P = 16 * Codes<FMT>::kBits / 8;  // bytes of a lane's 16 components
@@ -524,8 +539,8 @@ __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArg
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
   const int own_row = lane / S::kLanes, own_part = lane % S::kLanes, n_kt = (it.nk + BK - 1) / BK;
   // one round trip: gain, query row and angles, page numbers
-  Walk<D, S::kRows, BK> walk;
-  walk.start(a, it, wave * S::kRows, n_kt, lane);
+  Walk<S::kRows, BK, true> walk;
+  walk.start(a, it, wave * S::kRows, n_kt, lane, places + wave * decltype(walk)::kBytes);
   const Gain gain = fetch_gain(p, tid % D);
   Query32<E, D> q;
   const Column c = column_of<E, D>(a, it, rep, it.tile * kMany + wave * 32, lane, q);
@@ -553,119 +568,108 @@ __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArg
     tensor(x.k, lds + stage);
     tensor(x.v, lds + stage + S::kTileBytes);
   };
-  Raw2 x0, x1;
+  Raw2 x, x1;
   walk.work_out(qa, a, lane);
-  ask(x0, 0);
+  ask(x, 0);
   ask(x1, 1);
   if (tid < D) gsm[tid] = scale_of(p, gain);
   __syncthreads();
   q.finish(p, c.live, hh, gsm);
-  put(x0, 0, 0);
-  ask(x0, 2);
+  put(x, 0, 0);
+  ask(x, 2);
   put(x1, 1, S::kStageBytes);
-  ask(x1, 3);
   State<MB> st;
   st.clear();
   bool odd = false;
-  typedef f32x16 Scores[N];
-  auto scores = [&](auto masked_c, uint32_t stage, Scores& s, int jb) {  // of the tile whose keys begin at jb, from k0 on
+  typedef f32x16 Scores[1];
+  auto scores = [&](bool masked, uint32_t block, Scores& s, int jb) {  // of the block of 32 keys at `block` in LDS, jb on from k0
+    s[0] = st.less;
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      s[n] = st.less;
-      bf16x8 k[KS];
+    for (int ks = 0; ks < KS; ++ks) {
+      const bf16x8 k = swz_frag_rm<D>(lds + block + swz_off_rm<D>(lane), 0, ks);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) k[ks] = swz_frag_rm<D>(lds + stage + n * 64 * D + swz_off_rm<D>(lane), 0, ks);
-#pragma unroll
-      for (int u = PARTS - 1; u >= 0; --u)
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s[n] = mfma32(k[ks], q.part[u][ks], s[n]);
+      for (int u = PARTS - 1; u >= 0; --u) s[0] = mfma32(k, q.part[u][ks], s[0]);
     }
-    if (decltype(masked_c)::value != 0) {
-#pragma unroll
-      for (int n = 0; n < N; ++n) hide_unseen(s[n], c.lim - jb - 32 * n, hh);
-    }
+    if (masked) hide_unseen(s[0], c.lim - jb, hh);
   };
-  auto products = [&](auto masked_c, uint32_t stage, Scores& s) {
+  auto products = [&](bool masked, uint32_t block, Scores& s) {
     st.exponentials(s);
+    u32x4 pb[PROBS][2];
+    if constexpr (PROBS == 1) {
+      pb[0][0] = __builtin_bit_cast(u32x4, pack_c_half_sum(s[0], 0, st.l));
+      pb[0][1] = __builtin_bit_cast(u32x4, pack_c_half_sum(s[0], 1, st.l));
+    } else {
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      u32x4 pb[PROBS][2];
-      if constexpr (PROBS == 1) {
-        pb[0][0] = __builtin_bit_cast(u32x4, pack_c_half_sum(s[n], 0, st.l));
-        pb[0][1] = __builtin_bit_cast(u32x4, pack_c_half_sum(s[n], 1, st.l));
-      } else {
+      for (int i = 0; i < 8; ++i) {
+        uint32_t w[PROBS];
+        parts_of<PROBS>(s[0][2 * i], s[0][2 * i + 1], w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint32_t w[PROBS];
-          parts_of<PROBS>(s[n][2 * i], s[n][2 * i + 1], w);
-#pragma unroll
-          for (int u = 0; u < PROBS; ++u) pb[u][i / 4][i % 4] = w[u];
-          st.l[0] += s[n][2 * i];
-          st.l[1] += s[n][2 * i + 1];
-        }
+        for (int u = 0; u < PROBS; ++u) pb[u][i / 4][i % 4] = w[u];
+        st.l[0] += s[0][2 * i];
+        st.l[1] += s[0][2 * i + 1];
       }
-#pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
-          u32x4 v = __builtin_bit_cast(u32x4, swz_frag_tr<D>(lds + stage + S::kTileBytes + n * 64 * D + swz_off_tr<D>(lane), mb, s2));
-          if (decltype(masked_c)::value != 0) odd |= clear_nan(v);
-#pragma unroll
-          for (int u = PROBS - 1; u >= 0; --u) st.o[mb] = mfma32(as_bf16x8(v), as_bf16x8(pb[u][s2]), st.o[mb]);
-        }
     }
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        u32x4 v = __builtin_bit_cast(u32x4, swz_frag_tr<D>(lds + block + S::kTileBytes + swz_off_tr<D>(lane), mb, s2));
+        if (masked) odd |= clear_nan(v);
+#pragma unroll
+        for (int u = PROBS - 1; u >= 0; --u) st.o[mb] = mfma32(as_bf16x8(v), as_bf16x8(pb[u][s2]), st.o[mb]);
+      }
   };
-  uint32_t stage = 0;  // of tile jt
-  auto stage_from = [&](int steps) {  // of tile jt + steps
-    const uint32_t x = stage + steps * S::kStageBytes;
-    return x >= S::kStages * S::kStageBytes ? x - S::kStages * S::kStageBytes : x;
+  uint32_t stage = 0;  // of the tile that the turn is about
+  auto stage_from = [&](int steps) {
+    const uint32_t at = stage + steps * S::kStageBytes;
+    return at >= S::kStages * S::kStageBytes ? at - S::kStages * S::kStageBytes : at;
   };
-  auto active = [&](int jt) { return jt < n_kt && jt * BK <= c.any; };  // some column of the wave sees a key of the tile
-  const int n_whole = max(min((c.all + 1) / BK, n_kt), 0);  // tiles that all columns of the wave see whole
+  const int n_blocks = n_kt * N;
+  auto active = [&](int b) { return b < n_blocks && b * 32 <= c.any; };  // some column of the wave sees a key of the block
+  const int n_whole = max(min((c.all + 1) / 32, n_blocks), 0);             // blocks that all columns of the wave see whole
   Scores s0, s1;
   __syncthreads();
   if (active(0)) {
-    scores(IC<1>{}, 0, s0, 0);
+    scores(true, 0, s0, 0);
     st.raise(s0);
   }
-  auto turn = [&](int jt, Raw2& x) {
+  auto turn = [&](int jt) {
     __syncthreads();  // tile jt + 1 is there; everyone has left tile jt - 1
     put(x, jt + 2, stage_from(2));
-    ask(x, jt + 4);
+    if ((jt + 3) % 64 == 0 && jt + 3 < n_kt) walk.work_out(qa, a, lane);
+    ask(x, jt + 3);
   };
-  auto whole = [&](int jt, Raw2& x, Scores& s, Scores& ahead) {  // neither tile jt nor the next needs a mask
-    turn(jt, x);
-    scores(IC<0>{}, stage_from(1), ahead, 0);
-    products(IC<0>{}, stage, s);
+  // block b of s, and the scores of the next one beside it; HALF: b is the first of a tile of two
+  auto whole = [&](auto half, Scores& s, Scores& ahead) {
+    constexpr bool HALF = decltype(half)::value != 0;
+    scores(false, HALF ? stage + 64 * D : stage_from(1), ahead, 0);
+    products(false, HALF || N == 1 ? stage : stage + 64 * D, s);
     st.raise(ahead);
-    stage = stage_from(1);
+    if (!HALF) stage = stage_from(1);
   };
-  auto any_tiles = [&](int jt, Raw2& x, Scores& s, Scores& ahead) {
-    turn(jt, x);
-    if (active(jt)) {
-      if (jt >= n_whole) products(IC<1>{}, stage, s);
-      else products(IC<0>{}, stage, s);
-    }
-    if (active(jt + 1)) {
-      scores(IC<1>{}, stage_from(1), ahead, (jt + 1) * BK);
+  auto any = [&](auto half, int b, Scores& s, Scores& ahead) {
+    constexpr bool HALF = decltype(half)::value != 0;
+    if (active(b)) products(b >= n_whole, HALF || N == 1 ? stage : stage + 64 * D, s);
+    if (active(b + 1)) {
+      scores(true, HALF ? stage + 64 * D : stage_from(1), ahead, (b + 1) * 32);
       st.raise(ahead);
     }
-    stage = stage_from(1);
+    if (!HALF) stage = stage_from(1);
   };
-  // two turns a round, so that scores and codes change places without being copied
-  int jt = 0;
-  auto places = [&] {  // of the next two tiles asked for
-    if ((jt + 4) % 64 == 0 && jt + 4 < n_kt) walk.work_out(qa, a, lane);
-  };
-  for (; jt + 2 < n_whole; jt += 2) {
-    places();
-    whole(jt, x0, s0, s1);
-    whole(jt + 1, x1, s1, s0);
+  // two blocks a round, so that the scores change places without being copied
+  int b = 0;
+  for (; b + 2 < n_whole; b += 2) {
+    turn(b / N);
+    whole(IC<N == 2>{}, s0, s1);
+    if (N == 1) turn(b + 1);
+    whole(IC<0>{}, s1, s0);
   }
-  for (; jt < n_kt; jt += 2) {
-    places();
-    any_tiles(jt, x0, s0, s1);
-    if (jt + 1 < n_kt) any_tiles(jt + 1, x1, s1, s0);
+  for (; b < n_blocks; b += 2) {
+    turn(b / N);
+    any(IC<N == 2>{}, b, s0, s1);
+    if (b + 1 >= n_blocks) break;
+    if (N == 1) turn(b + 1);
+    any(IC<0>{}, b + 1, s1, s0);
   }
   const bool bad = it.x.broken | (__builtin_amdgcn_ballot_w64(walk.bad) != 0);
   if (__builtin_amdgcn_ballot_w64(odd) != 0)
@@ -708,6 +712,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 2 || D == 64 ? 2 : 1)) void page
   constexpr int kLds = std::max(S::kStages * S::kStageBytes, 4 * ValueTile<D>::kBytes);
   __shared__ __attribute__((aligned(1024))) char lds[kLds];
   __shared__ __attribute__((aligned(16))) float gsm[4][D];
+  __shared__ __attribute__((aligned(16))) char places[4 * Walk<S::kRows, S::kBK, true>::kBytes];
   const int tid = threadIdx.x, lane = tid & 63, rep = a.rep.d;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   clear_rest<E>(a, tid, 256, D);
@@ -717,7 +722,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 2 || D == 64 ? 2 : 1)) void page
   const QuantArgs qa = quant_of(args);
   const Item it = locate<true>(a, lane, rep, share, mine, blockIdx.x);
   if (it.x.entry >= 0) {
-    if (it.valid) many_columns<E, D, FMT>(qa, a, it, rep, tid, lds_addr_of(lds), gsm[0]);
+    if (it.valid) many_columns<E, D, FMT>(qa, a, it, rep, tid, lds_addr_of(lds), lds_addr_of(places), gsm[0]);
   } else {
     const Item it4 = locate<false>(a, lane, rep, share, mine, ((int)blockIdx.x - it.x.base) * 4 + wave);
     if (!it4.valid) return;

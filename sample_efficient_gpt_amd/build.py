@@ -23,7 +23,7 @@ SOURCES = ["api.hip", "f32_path.hip", "f32_split.hip", "pre_post.hip", "fwd_mfma
 EXTRA_FLAGS = {"fwd_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-mllvm", "-amdgpu-sched-strategy=max-ilp"],
                "decode_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
                "paged_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
-               "paged_quant_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+               "paged_quant_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
                # one workgroup per CU at head_dim 128 as above: dK/dV 49 -> 43 us at B = 2, H = 4, S = 500
                "f32_path.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
                "f32_split.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}

@@ -530,6 +530,45 @@ struct Query32 {
   }
 };
 
+// Sums of a column at head_dim 128.  State keeps the reference's negative in sixteen registers, so that scores come out of the product less it; here
+// those registers hold keys on their way to it, and the reference is taken off behind the product, beside matrix instructions that take longer.
+template <int MB>
+struct StateLess {
+  f32x16 o[MB], less;  // less: 0
+  float m, top_allowed;  // reference (log2 units), and by what a score may exceed it
+  float l[2];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) o[mb] = splat16(0.f);
+    less = splat16(0.f);
+    m = 0.f;
+    top_allowed = -INFINITY;
+    l[0] = l[1] = 0.f;
+  }
+  __device__ __forceinline__ float reference() const { return top_allowed == -INFINITY ? -INFINITY : m; }
+  __device__ __forceinline__ void raise(f32x16 (&s)[1]) {
+    float top = s[0][0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, s[0][r]);
+    top = half_max(top);
+    if (__builtin_amdgcn_ballot_w64(top > top_allowed) != 0) {
+      const bool up = top > top_allowed;
+      const float corr = !up || top_allowed == -INFINITY ? 1.f : fast_exp2(m - top);  // nothing to scale before the first key
+      if (up) { m = top; top_allowed = top + kLazy; }
+      l[0] *= corr;
+      l[1] *= corr;
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[mb][r] *= corr;
+    }
+  }
+  __device__ __forceinline__ void exponentials(f32x16 (&s)[1]) const {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[0][r] = fast_exp2(s[0][r] - m);
+  }
+};
+
 template <typename E, int D, int FMT>
 __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArgs& a, const Item& it, int rep, int tid, uint32_t lds, uint32_t places, float* gsm) {
   using S = ManyShape<D>;
@@ -578,18 +617,24 @@ __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArg
   put(x, 0, 0);
   ask(x, 2);
   put(x1, 1, S::kStageBytes);
-  State<MB> st;
+  std::conditional_t<D == 64, State<MB>, StateLess<MB>> st;
   st.clear();
   bool odd = false;
   typedef f32x16 Scores[1];
-  auto scores = [&](bool masked, uint32_t block, Scores& s, int jb) {  // of the block of 32 keys at `block` in LDS, jb on from k0
+  // Keys of the block after this one: at head_dim 64 read as soon as they are there, beside the decoding of a later tile's codes; at 128 there are no
+  // registers for that (with them in scratch six prompts take 301 us instead of 288).
+  constexpr bool EARLY = D == 64;
+  typedef bf16x8 Keys[KS];
+  auto read_keys = [&](uint32_t block, Keys& k) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) k[ks] = swz_frag_rm<D>(lds + block + swz_off_rm<D>(lane), 0, ks);
+  };
+  auto scores = [&](bool masked, const Keys& k, Scores& s, int jb) {  // of the block of 32 keys k, jb on from k0
     s[0] = st.less;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const bf16x8 k = swz_frag_rm<D>(lds + block + swz_off_rm<D>(lane), 0, ks);
+    for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int u = PARTS - 1; u >= 0; --u) s[0] = mfma32(k, q.part[u][ks], s[0]);
-    }
+      for (int u = PARTS - 1; u >= 0; --u) s[0] = mfma32(k[ks], q.part[u][ks], s[0]);
     if (masked) hide_unseen(s[0], c.lim - jb, hh);
   };
   auto products = [&](bool masked, uint32_t block, Scores& s) {
@@ -630,11 +675,15 @@ __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArg
   Scores s0, s1;
   __syncthreads();
   if (active(0)) {
-    scores(true, 0, s0, 0);
+    Keys k;
+    read_keys(0, k);
+    scores(true, k, s0, 0);
     st.raise(s0);
   }
-  auto turn = [&](int jt) {
+  Keys ahead_k;
+  auto turn = [&](int jt, uint32_t block) {  // block: whose keys are wanted next
     __syncthreads();  // tile jt + 1 is there; everyone has left tile jt - 1
+    if (EARLY) read_keys(block, ahead_k);
     put(x, jt + 2, stage_from(2));
     if ((jt + 3) % 64 == 0 && jt + 3 < n_kt) walk.work_out(qa, a, lane);
     ask(x, jt + 3);
@@ -642,7 +691,8 @@ __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArg
   // block b of s, and the scores of the next one beside it; HALF: b is the first of a tile of two
   auto whole = [&](auto half, Scores& s, Scores& ahead) {
     constexpr bool HALF = decltype(half)::value != 0;
-    scores(false, HALF ? stage + 64 * D : stage_from(1), ahead, 0);
+    if (!EARLY || !HALF) read_keys(HALF ? stage + 64 * D : stage_from(1), ahead_k);
+    scores(false, ahead_k, ahead, 0);
     products(false, HALF || N == 1 ? stage : stage + 64 * D, s);
     st.raise(ahead);
     if (!HALF) stage = stage_from(1);
@@ -651,7 +701,8 @@ __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArg
     constexpr bool HALF = decltype(half)::value != 0;
     if (active(b)) products(b >= n_whole, HALF || N == 1 ? stage : stage + 64 * D, s);
     if (active(b + 1)) {
-      scores(true, HALF ? stage + 64 * D : stage_from(1), ahead, (b + 1) * 32);
+      if (!EARLY || !HALF) read_keys(HALF ? stage + 64 * D : stage_from(1), ahead_k);
+      scores(true, ahead_k, ahead, (b + 1) * 32);
       st.raise(ahead);
     }
     if (!HALF) stage = stage_from(1);
@@ -659,16 +710,16 @@ __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArg
   // two blocks a round, so that the scores change places without being copied
   int b = 0;
   for (; b + 2 < n_whole; b += 2) {
-    turn(b / N);
+    turn(b / N, N == 2 ? stage + 64 * D : stage_from(1));
     whole(IC<N == 2>{}, s0, s1);
-    if (N == 1) turn(b + 1);
+    if (N == 1) turn(b + 1, stage_from(1));
     whole(IC<0>{}, s1, s0);
   }
   for (; b < n_blocks; b += 2) {
-    turn(b / N);
+    turn(b / N, N == 2 ? stage + 64 * D : stage_from(1));
     any(IC<N == 2>{}, b, s0, s1);
     if (b + 1 >= n_blocks) break;
-    if (N == 1) turn(b + 1);
+    if (N == 1) turn(b + 1, stage_from(1));
     any(IC<0>{}, b + 1, s1, s0);
   }
   const bool bad = it.x.broken | (__builtin_amdgcn_ballot_w64(walk.bad) != 0);
@@ -689,7 +740,7 @@ __device__ __forceinline__ QuantArgs quant_of(const Args& a) { return {a.w.p, a.
 
 // Launches whose entries are all FEW: a workgroup is one wave
 template <typename E, int D, int FMT>
-__global__ __launch_bounds__(64, 2) void paged_quant_few_kernel(Args args) {
+__global__ __launch_bounds__(64, (D == 64 ? 3 : 2)) void paged_quant_few_kernel(Args args) {
   const PagedArgs& a = args.w;
   __shared__ __attribute__((aligned(1024))) char lds[ValueTile<D>::kBytes];
   __shared__ __attribute__((aligned(16))) float gsm[D];
@@ -734,6 +785,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 2 || D == 64 ? 2 : 1)) void page
 int target_of(const segpt_paged_params& p) {
   const int rep = p.H / p.Hkv;
   const bool wide = p.prefix_table || (!p.seq_start && (int64_t)rep * (p.T / p.B) > kFew);
+  if (all_few(p)) return p.D == 64 ? 744 : 496;
   return wide ? 384 : p.seq_start ? 480 : 496;
 }
 

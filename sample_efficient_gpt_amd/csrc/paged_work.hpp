@@ -478,8 +478,8 @@ __device__ __forceinline__ void hide_unseen(f32x16& s, int seen, int hh) {  // r
 }
 
 // What an item leaves: y where it is its tile's only one, else a partial result
-template <typename E, int D>
-__device__ __forceinline__ void store_result(const PagedArgs& a, const Item& it, const Column& c, State<D / 32>& st, bool bad, int slot_col, int hh) {
+template <typename E, int D, typename S>
+__device__ __forceinline__ void store_result(const PagedArgs& a, const Item& it, const Column& c, S& st, bool bad, int slot_col, int hh) {
   const segpt_paged_params& p = a.p;
   constexpr int MB = D / 32;
   float l = half_sum(st.l[0] + st.l[1]), m = st.reference();

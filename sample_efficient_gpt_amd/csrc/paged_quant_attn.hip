@@ -36,8 +36,28 @@ __device__ __forceinline__ void parts_of(float a, float b, uint32_t (&w)[PARTS])
 template <typename E>
 constexpr int kQueryParts = sizeof(E) == 2 ? 2 : 3;
 
-// eight elements of a row
-__device__ __forceinline__ void load8(const uint16_t* p, float (&x)[8]) { load16(p, x); }
+// eight elements of a row, as they are stored
+template <typename E>
+struct Eight;
+template <>
+struct Eight<uint16_t> {
+  u32x4 w;
+  __device__ __forceinline__ void load(const uint16_t* p) { w = *reinterpret_cast<const u32x4*>(p); }
+  __device__ __forceinline__ void values(float (&x)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[2 * i] = bf16lo(w[i]); x[2 * i + 1] = bf16hi(w[i]); }
+  }
+};
+template <>
+struct Eight<float> {
+  f32x4 u, v;
+  __device__ __forceinline__ void load(const float* p) { u = *reinterpret_cast<const f32x4*>(p); v = *reinterpret_cast<const f32x4*>(p + 4); }
+  __device__ __forceinline__ void values(float (&x)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[i] = u[i]; x[4 + i] = v[i]; }
+  }
+};
+// and of a table
 __device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
   const float4 u = *reinterpret_cast<const float4*>(p), v = *reinterpret_cast<const float4*>(p + 4);
   x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
@@ -238,30 +258,33 @@ struct Query16 {
   using L = Quarter<D, FMT>;
   static constexpr int KS = L::KS, kCols = 16, kLogCols = 4, PARTS = kQueryParts<E>, N = D / 64;
   bf16x8 part[PARTS][KS];
-  struct Row {
-    float x[2][N][8], cs[N][8], sn[N][8];  // pairs (quarter * N + n) * 8 .. + 7
-  };
-  Row row;
+  Eight<E> raw[2][N];
+  float cs[N][8], sn[N][8];  // pairs (quarter * N + n) * 8 .. + 7
   __device__ __forceinline__ void fetch(const segpt_paged_params& p, const E* at, int64_t angle, int quarter) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int j = (quarter * N + n) * 8;
-      load8(at + j, row.x[0][n]);
-      load8(at + j + D / 2, row.x[1][n]);
+      raw[0][n].load(at + j);
+      raw[1][n].load(at + j + D / 2);
       if (p.rope_cos) {
-        load8(p.rope_cos + angle + j, row.cs[n]);
-        load8(p.rope_sin + angle + j, row.sn[n]);
+        load8(p.rope_cos + angle + j, cs[n]);
+        load8(p.rope_sin + angle + j, sn[n]);
       }
     }
   }
   __device__ __forceinline__ void finish(const segpt_paged_params& p, bool live, int lane, const float* gsm, uint32_t lds) {
     using V = ValueTile<D>;
     const int quarter = lane >> 4, col = lane & 15;
+    float x[2][N][8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int n = 0; n < N; ++n) raw[h][n].values(x[h][n]);
     if (p.rope_cos) {
 #pragma unroll
       for (int n = 0; n < N; ++n)
 #pragma unroll
-        for (int t = 0; t < 8; ++t) rope_pair(row.x[0][n][t], row.x[1][n][t], row.cs[n][t], row.sn[n][t]);
+        for (int t = 0; t < 8; ++t) rope_pair(x[0][n][t], x[1][n][t], cs[n][t], sn[n][t]);
     }
     float sq[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -269,7 +292,7 @@ struct Query16 {
 #pragma unroll
       for (int n = 0; n < N; ++n)
 #pragma unroll
-        for (int t = 0; t < 8; ++t) sq[t % 4] += row.x[h][n][t] * row.x[h][n][t];
+        for (int t = 0; t < 8; ++t) sq[t % 4] += x[h][n][t] * x[h][n][t];
     float ss = (sq[0] + sq[1]) + (sq[2] + sq[3]);
     ss += __shfl_xor(ss, 16, 64);
     ss = half_sum(ss);
@@ -284,7 +307,7 @@ struct Query16 {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           uint32_t part_i[PARTS];
-          parts_of<PARTS>(live ? row.x[h][n][2 * i] * alpha * g[2 * i] : 0.f, live ? row.x[h][n][2 * i + 1] * alpha * g[2 * i + 1] : 0.f, part_i);
+          parts_of<PARTS>(live ? x[h][n][2 * i] * alpha * g[2 * i] : 0.f, live ? x[h][n][2 * i + 1] * alpha * g[2 * i + 1] : 0.f, part_i);
 #pragma unroll
           for (int u = 0; u < PARTS; ++u) w[u][h][n][i] = part_i[u];
         }
@@ -358,11 +381,11 @@ __device__ __forceinline__ void few_columns(const QuantArgs& qa, const PagedArgs
   Block b0, b1;
   walk.work_out(qa, a, lane);
   if (blocks > 0) ask(b0, 0);
-  if (blocks > 1) ask(b1, 1);
 #pragma unroll
   for (int i = 0; i < D / 64; ++i) gsm[64 * i + lane] = scale_of(p, gain[i]);
   wave_sync();
   q.finish(p, c.live, lane, gsm, lds);
+  if (blocks > 1) ask(b1, 1);
 
   f32x4 o[DB];
   float m = 0.f, limit = -INFINITY, l = 0.f;  // reference (log2 units); by how much a score may exceed it; sum over this lane's keys
@@ -371,25 +394,28 @@ __device__ __forceinline__ void few_columns(const QuantArgs& qa, const PagedArgs
   bool odd = false;
   auto step = [&](Block& b, int j) {
     const bool masked = j * kBlock + kBlock - 1 > c.all;
-    u32x4 k[2][KS];
+    f32x4 s[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      L::decode(b.k[t], quarter, k[t]);
+      u32x4 k[KS];
+      L::decode(b.k[t], quarter, k);
+      s[t] = f32x4{-m, -m, -m, -m};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int u = PARTS - 1; u >= 0; --u) s[t] = mfma16(as_bf16x8(k[ks]), q.part[u][ks], s[t]);
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
       u32x4 v[KS];
       L::decode(b.v[t], quarter, v);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) lds_write16(lds + V::write_at(16 * t + r16, L::component(ks, quarter) / 8), v[ks]);
     }
     if (j + 2 < blocks) ask(b, j + 2);
-    f32x4 s[2];
+    if (masked) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      s[t] = f32x4{-m, -m, -m, -m};
-#pragma unroll
-      for (int u = PARTS - 1; u >= 0; --u)
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s[t] = mfma16(as_bf16x8(k[t][ks]), q.part[u][ks], s[t]);
-      if (masked) {
+      for (int t = 0; t < 2; ++t) {
         const int seen = c.lim - j * kBlock - 16 * t - 4 * quarter;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -487,10 +513,11 @@ template <typename E, int D>
 struct Query32 {
   static constexpr int KS = D / 16, kCols = 32, kLogCols = 5, PARTS = kQueryParts<E>;
   bf16x8 part[PARTS][KS];
-  float x[KS][8], cs[KS / 2][8], sn[KS / 2][8];
+  Eight<E> raw[KS];
+  float cs[KS / 2][8], sn[KS / 2][8];
   __device__ __forceinline__ void fetch(const segpt_paged_params& p, const E* row, int64_t angle, int hh) {
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) load8(row + 16 * ks + 8 * hh, x[ks]);
+    for (int ks = 0; ks < KS; ++ks) raw[ks].load(row + 16 * ks + 8 * hh);
     if (!p.rope_cos) return;
 #pragma unroll
     for (int ks = 0; ks < KS / 2; ++ks) {
@@ -499,6 +526,9 @@ struct Query32 {
     }
   }
   __device__ __forceinline__ void finish(const segpt_paged_params& p, bool live, int hh, const float* gsm) {
+    float x[KS][8];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) raw[ks].values(x[ks]);
     if (p.rope_cos) {
 #pragma unroll
       for (int ks = 0; ks < KS / 2; ++ks)
@@ -739,8 +769,10 @@ struct Args {
 __device__ __forceinline__ QuantArgs quant_of(const Args& a) { return {a.w.p, a.k_scales, a.v_scales}; }
 
 // Launches whose entries are all FEW: a workgroup is one wave
+template <typename E, int D>
+constexpr int kFewWaves = sizeof(E) == 2 && D == 64 ? 3 : 2;  // waves a SIMD: what their registers leave room for
 template <typename E, int D, int FMT>
-__global__ __launch_bounds__(64, (D == 64 ? 3 : 2)) void paged_quant_few_kernel(Args args) {
+__global__ __launch_bounds__(64, (kFewWaves<E, D>)) void paged_quant_few_kernel(Args args) {
   const PagedArgs& a = args.w;
   __shared__ __attribute__((aligned(1024))) char lds[ValueTile<D>::kBytes];
   __shared__ __attribute__((aligned(16))) float gsm[D];
@@ -785,7 +817,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 2 || D == 64 ? 2 : 1)) void page
 int target_of(const segpt_paged_params& p) {
   const int rep = p.H / p.Hkv;
   const bool wide = p.prefix_table || (!p.seq_start && (int64_t)rep * (p.T / p.B) > kFew);
-  if (all_few(p)) return p.D == 64 ? 744 : 496;
+  if (all_few(p)) return p.D == 64 && p.dtype == SEGPT_DTYPE_BF16 ? 744 : 496;
   return wide ? 384 : p.seq_start ? 480 : 496;
 }
 

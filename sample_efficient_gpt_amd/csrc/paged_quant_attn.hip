@@ -7,6 +7,7 @@
 // its operand) and everything behind that is bf16 matrix products with fp32 sums, whatever the rows are: bf16 rows bring their queries in two bf16
 // parts, fp32 rows queries and probabilities in three, and neither loses anything of the keys and values as stored.
 #define SEGPT_FEW_COLUMNS 16
+#define SEGPT_JOIN_COLUMNS
 #include "paged_quant.hpp"
 #include "paged_work.hpp"
 

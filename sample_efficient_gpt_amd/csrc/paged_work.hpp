@@ -43,7 +43,8 @@ struct PagedArgs {
   int32_t target;                 // workgroups of four waves there are to be
   int32_t min_few, min_many;      // shortest shares, in blocks of 32 keys
   int32_t n_many, n_few;          // items there may be of either kind
-  int32_t n_joins;                // tiles and kv heads whose partial results there may be to join
+  int32_t n_joins;                // tiles and kv heads whose partial results there may be to join; kJoinColumns: groups of columns of a kv head
+  int32_t joined;                 // kJoinColumns: columns of a group, a power of two up to kMany
   int32_t n_slots;                // partial results there is room for, 32 columns each
   size_t planned_bytes;           // of upto
   int32_t* lens;                  // blocks of a share (few, many) and tiles and kv heads to join, left for the merge
@@ -57,6 +58,13 @@ constexpr int kBlock = 32;          // keys of a score tile
 #define SEGPT_FEW_COLUMNS 32
 #endif
 constexpr int kFew = SEGPT_FEW_COLUMNS, kMany = 128;  // columns of a tile; kFew: up to 32, set where another number suits the kernels
+// What a workgroup of the merge has: by tiles, some of the columns there may be of a tile, whether there are so many or not; by columns, `a.joined` of
+// those that there are.  The latter for new callers: the order of a column's sums follows from the number of its units, and what was there keeps its own.
+#ifdef SEGPT_JOIN_COLUMNS
+constexpr bool kJoinColumns = true;
+#else
+constexpr bool kJoinColumns = false;
+#endif
 constexpr float kLazy = 8.f;        // the reference is raised where a score exceeds it by 2^8: probabilities stay below 2^8
 
 // ---- the plan, computed by every wave for itself or, for many entries, by paged_plan_kernel
@@ -186,7 +194,8 @@ struct Counts {
 __device__ __forceinline__ Counts counts_of(const PagedArgs& a, int e, const Entry& x, const Shares& share) {
   const int shares = shares_of(x, share), items = x.tiles * shares * a.p.Hkv;
   const bool partial = a.shared || shares > 1;
-  return {{x.many ? 0 : items, x.many ? items : 0, partial && e >= a.shared ? x.tiles * a.p.Hkv : 0, partial ? items * (x.many ? kMany / 32 : 1) : 0}, shares};
+  const int joins = kJoinColumns ? (x.n * (int)a.rep.d + a.joined - 1) >> __builtin_ctz(a.joined) : x.tiles;
+  return {{x.many ? 0 : items, x.many ? items : 0, partial && e >= a.shared ? joins * a.p.Hkv : 0, partial ? items * (x.many ? kMany / 32 : 1) : 0}, shares};
 }
 // an entry as the whole wave sees it
 struct Found {
@@ -317,12 +326,13 @@ __device__ __forceinline__ void two_parts(float a, float b, uint32_t& first, uin
 }
 
 template <typename E, int D>
-__device__ __forceinline__ float gate_factor(const segpt_paged_params& p, int t, int h) {
-  const E z = row_of<E>(p.gate, t, h)[0];
+__device__ __forceinline__ float gate_factor(const segpt_paged_params& p, E z) {
   float x;
   if constexpr (sizeof(E) == 2) x = bf16_to_f32(z); else x = z;
   return p.gate_scale / (1.0f + __expf(-x));
 }
+template <typename E, int D>
+__device__ __forceinline__ float gate_factor(const segpt_paged_params& p, int t, int h) { return gate_factor<E, D>(p, row_of<E>(p.gate, t, h)[0]); }
 
 // ---- an item
 struct Item {
@@ -540,7 +550,7 @@ __device__ __forceinline__ void leave_plan(const PagedArgs& a, int lane, int rep
 // row; as many units stand side by side over the shares of a column as leave each one batch of kBatch that is requested together, and
 // their sums meet in LDS.  Fixed order: deterministic.  4.9 us for one token of 18 heads (launch and two round trips), 5.9 for 32 of them, 12 for
 // 128 tokens of 16 heads of 128 behind a prefix (25 MB).
-constexpr int kMergeThreads = 256;
+constexpr int kMergeThreads = 256, kMergeGroups = 2048;
 template <typename E, int D>
 __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedArgs a, int subs, int per_sub) {
   const segpt_paged_params& p = a.p;
@@ -551,12 +561,13 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedArgs a,
   const int rep = a.rep.d;
   const int few = a.lens[0], many = a.lens[1], joins = a.lens[2];
   const Entries mine = kept_entries(a, lane, rep);
-  const int which = blockIdx.x / subs, sub = blockIdx.x - which * subs;
+  const int which = kJoinColumns ? blockIdx.x : blockIdx.x / subs, sub = blockIdx.x - which * subs;
   if (which >= joins) return;
   const Shares share = shares_from(few, many);
   const Found own = find_entry<kFindJoin>(a, lane, rep, share, mine, which);
   if (own.entry < 0) return;
-  const int tile = a.hkv.of(which - own.base), g = which - own.base - tile * p.Hkv, cols = own.n * rep, tile_cols = own.many ? kMany : kFew;
+  const int number = a.hkv.of(which - own.base), g = which - own.base - number * p.Hkv, cols = own.n * rep, tile_cols = own.many ? kMany : kFew;
+  const int tile = kJoinColumns ? number * per_sub / tile_cols : number, from = kJoinColumns ? number * per_sub - tile * tile_cols : sub * per_sub;
   Found pre{-1, 0, 0, 0, 0, 0, 0, 0, false, false};
   if (a.shared) pre = find_entry<kFindFirst>(a, lane, rep, share, mine, 0);
   const int pre_cols = pre.many ? kMany : kFew;
@@ -564,10 +575,10 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedArgs a,
   int step = min(per_sub, kUnits);  // columns at a time
   while (step > 1 && kUnits / step * kBatch < n) step >>= 1;
   const int wide = kUnits / step;  // units of a column
-  for (int c0 = sub * per_sub; c0 < min((sub + 1) * per_sub, tile_cols); c0 += step) {  // the same for all threads
+  for (int c0 = from; c0 < min(from + per_sub, tile_cols); c0 += step) {  // the same for all threads
     if (tile * tile_cols + c0 >= cols) return;
     const int col = tile * tile_cols + min(c0 + unit % step, tile_cols - 1);
-    const bool live = col < cols && c0 + unit % step < min((sub + 1) * per_sub, tile_cols);
+    const bool live = col < cols && c0 + unit % step < min(from + per_sub, tile_cols);
     const int i = a.rep.of(min(col, cols - 1)), t = own.first + i, h = g * rep + (min(col, cols - 1) - i * rep);
     const int pcol = (t - pre.first) * rep + h - g * rep, ptile = pcol / pre_cols;
     auto place = [&](int s) {  // row of share s among all partial results; none: there is no room for it
@@ -576,6 +587,8 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedArgs a,
       const int slot = x.slot + (((is_own ? tile : ptile) * x.shares + (is_own ? s : s - own.shares)) * p.Hkv + g) * (x.many ? kMany / 32 : 1);
       return slot < a.n_slots - (x.many ? kMany / 32 - 1 : 0) ? (int64_t)slot * 32 + (is_own ? col - tile * tile_cols : pcol - ptile * pre_cols) : (int64_t)-1;
     };
+    E gate{};  // on its way while the results are joined
+    if (p.gate.ptr) gate = row_of<E>(p.gate, t, h)[0];
     float m = -INFINITY, l = 0.f;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
     if (live)
@@ -628,7 +641,7 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedArgs a,
     if (own.broken) l = __builtin_nanf("");
     float f = l == 0.f ? 0.f : 1.0f / l;
     if (p.lse && c == 0) p.lse[(int64_t)t * p.H + h] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
-    if (p.gate.ptr) f *= gate_factor<E, D>(p, t, h);
+    if (p.gate.ptr) f *= gate_factor<E, D>(p, gate);
     E* out = row_of<E>(p.o, t, h) + 4 * c;
     const float v[4] = {y.x * f, y.y * f, y.z * f, y.w * f};
     if constexpr (sizeof(E) == 2) *reinterpret_cast<u32x2*>(out) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
@@ -676,7 +689,17 @@ size_t plan(const segpt_paged_params& p, PagedArgs& a, int target) {
   const int64_t most = (int64_t)a.target + slack;
   const int64_t slots = kMany / 32 * (a.shared ? n_many : std::min(n_many, 2 * most)) + (a.shared ? n_few : std::min(n_few, 8 * most));
   a.n_slots = (int32_t)std::min<int64_t>(slots, INT32_MAX / 32);
-  const int64_t joins = a.shared ? own * p.Hkv : std::min(own_many * p.Hkv, most) + std::min((own - own_many) * p.Hkv, 4 * most);
+  const int64_t tiles = a.shared ? own * p.Hkv : std::min(own_many * p.Hkv, most) + std::min((own - own_many) * p.Hkv, 4 * most);
+  int64_t joins = tiles;
+  if (kJoinColumns) {
+    // groups of so many columns that the card holds their workgroups at once, if there are not even more of them; what is begun counts as one
+    const int64_t each = cols / p.B, many_tiles = a.shared ? own_many * p.Hkv : std::min(own_many * p.Hkv, most);
+    for (a.joined = 1;; a.joined *= 2) {
+      const int64_t j = a.joined, all = p.seq_start ? cols / j + std::min<int64_t>(p.B, p.T) : (each + j - 1) / j * p.B;
+      joins = std::min(all * p.Hkv, many_tiles * (kMany / j) + (tiles - many_tiles) * std::max<int64_t>(kFew / j, 1));
+      if (joins <= kMergeGroups || j == kMany) break;
+    }
+  }
   a.n_joins = (int32_t)std::min<int64_t>(joins, INT32_MAX);
   a.planned_bytes = a.entries > kKept * 64 ? (size_t)4 * a.entries * sizeof(int32_t) : 0;
   // a launch has fewer than 2^32 threads (the merge: a workgroup a join at least)
@@ -707,6 +730,10 @@ int launch_plan(const PagedArgs& a, hipStream_t st) {
 template <typename E, int D>
 int launch_merge(const PagedArgs& a, hipStream_t st) {
   const segpt_paged_params& p = a.p;
+  if (kJoinColumns) {
+    hipLaunchKernelGGL((paged_merge_kernel<E, D>), dim3((unsigned)a.n_joins), dim3(kMergeThreads), 0, st, a, 1, a.joined);
+    return (int)hipGetLastError();
+  }
   // a column a workgroup, or so many that there are not more workgroups than the card holds a few times over
   const int64_t all = (int64_t)p.T * (p.H / p.Hkv);
   const bool any_many = p.seq_start ? all > kFew : all / p.B > kFew;

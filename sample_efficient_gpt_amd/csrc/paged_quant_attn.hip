@@ -817,7 +817,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 2 || D == 64 ? 2 : 1)) void page
 // ---- host side
 int target_of(const segpt_paged_params& p) {
   const int rep = p.H / p.Hkv;
-  const bool wide = p.prefix_table || (!p.seq_start && (int64_t)rep * (p.T / p.B) > kFew);
+  const bool wide = p.prefix_table || (!p.seq_start && (int64_t)rep * (p.T / p.B) > kMostFew);
   if (all_few(p)) return p.D == 64 && p.dtype == SEGPT_DTYPE_BF16 ? 744 : 496;
   return wide ? 384 : p.seq_start ? 480 : 496;
 }

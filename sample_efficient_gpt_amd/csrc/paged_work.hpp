@@ -58,6 +58,7 @@ constexpr int kBlock = 32;          // keys of a score tile
 #define SEGPT_FEW_COLUMNS 32
 #endif
 constexpr int kFew = SEGPT_FEW_COLUMNS, kMany = 128;  // columns of a tile; kFew: up to 32, set where another number suits the kernels
+constexpr int kMostFew = 32;                          // an entry of more columns has tiles of kMany
 // What a workgroup of the merge has: by tiles, some of the columns there may be of a tile, whether there are so many or not; by columns, `a.joined` of
 // those that there are.  The latter for new callers: the order of a column's sums follows from the number of its units, and what was there keeps its own.
 #ifdef SEGPT_JOIN_COLUMNS
@@ -99,8 +100,8 @@ __device__ __forceinline__ Entry entry_of(const PagedArgs& a, int e, int rep, co
   x.n = e < a.entries ? max(r1 - r0, 0) : 0;
   x.len = len;
   const int cols = x.n * rep;
-  x.many = cols > kFew;
-  x.tiles = x.many ? (cols + kMany - 1) / kMany : cols > 0;
+  x.many = cols > kMostFew;
+  x.tiles = x.many ? (cols + kMany - 1) / kMany : (cols + kFew - 1) / kFew;
   x.blocks = (x.len + kBlock - 1) / kBlock;
   x.broken = broken;
   return x;
@@ -194,7 +195,7 @@ struct Counts {
 __device__ __forceinline__ Counts counts_of(const PagedArgs& a, int e, const Entry& x, const Shares& share) {
   const int shares = shares_of(x, share), items = x.tiles * shares * a.p.Hkv;
   const bool partial = a.shared || shares > 1;
-  const int joins = kJoinColumns ? (x.n * (int)a.rep.d + a.joined - 1) >> __builtin_ctz(a.joined) : x.tiles;
+  const int joined = x.many ? a.joined : min(a.joined, kFew), joins = kJoinColumns ? (x.n * a.rep.d + joined - 1) >> __builtin_ctz(joined) : x.tiles;
   return {{x.many ? 0 : items, x.many ? items : 0, partial && e >= a.shared ? joins * a.p.Hkv : 0, partial ? items * (x.many ? kMany / 32 : 1) : 0}, shares};
 }
 // an entry as the whole wave sees it
@@ -567,6 +568,7 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedArgs a,
   const Found own = find_entry<kFindJoin>(a, lane, rep, share, mine, which);
   if (own.entry < 0) return;
   const int number = a.hkv.of(which - own.base), g = which - own.base - number * p.Hkv, cols = own.n * rep, tile_cols = own.many ? kMany : kFew;
+  if (kJoinColumns) per_sub = min(per_sub, tile_cols);
   const int tile = kJoinColumns ? number * per_sub / tile_cols : number, from = kJoinColumns ? number * per_sub - tile * tile_cols : sub * per_sub;
   Found pre{-1, 0, 0, 0, 0, 0, 0, 0, false, false};
   if (a.shared) pre = find_entry<kFindFirst>(a, lane, rep, share, mine, 0);
@@ -651,7 +653,7 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedArgs a,
 
 // ---- host side
 bool all_few(const segpt_paged_params& p) {  // known on the host
-  return !p.prefix_table && !p.seq_start && (int64_t)p.H / p.Hkv * (p.T / p.B) <= kFew;
+  return !p.prefix_table && !p.seq_start && (int64_t)p.H / p.Hkv * (p.T / p.B) <= kMostFew;
 }
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -670,17 +672,20 @@ size_t plan(const segpt_paged_params& p, PagedArgs& a, int target) {
   a.target = target;
   a.min_few = 2;
   a.min_many = 4;
-  // Tiles: whole ones of the columns there are, and one begun an entry.  Items: a tile's part of what the target stands for, and one begun.
+  // Tiles: whole ones of the columns there are, and one begun an entry (of few columns: one, and another where a tile does not hold them).  Items: a
+  // tile's part of what the target stands for, and one begun.
   const int64_t cols = (int64_t)p.T * rep;
-  int64_t many = cols / kMany + std::min<int64_t>(p.B, cols / (kFew + 1)), few = std::min<int64_t>(p.B, p.T);
+  int64_t many = cols / kMany + std::min<int64_t>(p.B, cols / (kMostFew + 1)), few = std::min<int64_t>(p.B, p.T);
+  static_assert(kFew <= kMostFew && 2 * kFew >= kMostFew);
+  if (kFew < kMostFew) few += std::min<int64_t>(few, cols / (kFew + 1));
   if (!p.seq_start) {
     const int64_t each = cols / p.B;
-    many = each > kFew ? (each + kMany - 1) / kMany * p.B : 0;
-    few = each > kFew ? 0 : p.B;
+    many = each > kMostFew ? (each + kMany - 1) / kMany * p.B : 0;
+    few = each > kMostFew ? 0 : (each + kFew - 1) / kFew * p.B;
   }
   const int64_t own = many + few, own_many = many;
-  if (a.shared && cols > kFew) many += (cols + kMany - 1) / kMany;
-  else if (a.shared) few += 1;
+  if (a.shared && cols > kMostFew) many += (cols + kMany - 1) / kMany;
+  else if (a.shared) few += (cols + kFew - 1) / kFew;
   const int64_t slack = 64;  // the sum that gives the length of a share is rounded
   const int64_t n_many = many ? many * p.Hkv + a.target + slack : 0, n_few = few ? few * p.Hkv + 4 * a.target + slack : 0;
   a.n_many = (int32_t)std::min<int64_t>(n_many, INT32_MAX);
@@ -695,8 +700,9 @@ size_t plan(const segpt_paged_params& p, PagedArgs& a, int target) {
     // groups of so many columns that the card holds their workgroups at once, if there are not even more of them; what is begun counts as one
     const int64_t each = cols / p.B, many_tiles = a.shared ? own_many * p.Hkv : std::min(own_many * p.Hkv, most);
     for (a.joined = 1;; a.joined *= 2) {
-      const int64_t j = a.joined, all = p.seq_start ? cols / j + std::min<int64_t>(p.B, p.T) : (each + j - 1) / j * p.B;
-      joins = std::min(all * p.Hkv, many_tiles * (kMany / j) + (tiles - many_tiles) * std::max<int64_t>(kFew / j, 1));
+      const int64_t j = a.joined, jf = std::min<int64_t>(j, kFew), own_j = each > kMostFew ? j : jf, begun = std::min<int64_t>(p.B, p.T);
+      const int64_t all = p.seq_start ? cols / j + begun + (j > jf ? std::min(begun, cols / (kFew + 1)) : 0) : (each + own_j - 1) / own_j * p.B;
+      joins = std::min(all * p.Hkv, many_tiles * (kMany / j) + (tiles - many_tiles) * (kFew / jf));
       if (joins <= kMergeGroups || j == kMany) break;
     }
   }

@@ -115,6 +115,24 @@ def test_shared_prefix(gpu_device, rows, lens, prefix, H, Hkv, D, dtype, page, f
     check_y(x, y, lse, x.attended(gate=True))
 
 
+# 17 .. 32 columns of a kv head are two tiles of one wave each, 33 are a tile of four waves
+@both_formats
+@pytest.mark.parametrize("H,Hkv,D,dtype", [(16, 1, 64, BF16), (17, 1, 128, BF16), (32, 1, 64, BF16), (32, 1, 128, F32), (33, 1, 64, F32)])
+@pytest.mark.parametrize("rows,lens,prefix", [([1], [2500], 0), ([1, 1], [100, 1], 0), ([1, 2, 1], [900, 77, 1300], 0), ([2], [600], 0), ([1], [40], 1500), ([1, 1], [0, 9], 16)])
+def test_two_tiles_of_few_columns(gpu_device, rows, lens, prefix, H, Hkv, D, dtype, fmt):
+    x = QuantBatch(fmt, rows, lens, H, Hkv, D, 16, dtype, gpu_device, prefix=prefix, seed=41, uniform=len(set(rows)) == 1)
+    y, lse = attend(x, gate_logits=x.gate, return_lse=True)
+    check_y(x, y, lse, x.attended(gate=True))
+
+
+# so many columns that a workgroup of the merge has more than a tile of 16 holds
+@both_formats
+def test_merge_of_many_small_tiles(gpu_device, fmt):
+    x = QuantBatch(fmt, [2] * 1100, [2 + i % 20 for i in range(1100)], 16, 1, 64, 8, BF16, gpu_device, prefix=40, seed=42, uniform=True)
+    y, lse = attend(x, return_lse=True)
+    check_y(x, y, lse, x.attended())
+
+
 @both_formats
 @pytest.mark.parametrize("H,Hkv,D,dtype", [(18, 6, 64, BF16), (16, 4, 128, BF16), (8, 4, 64, F32), (4, 2, 128, F32)])
 @pytest.mark.parametrize("rows,lens,page", [

@@ -6,6 +6,10 @@
 // A code times its scale is a bf16 number, so the codes are made bf16 operands in registers (one instruction a pair of components, the scale as
 // its operand) and everything behind that is bf16 matrix products with fp32 sums, whatever the rows are: bf16 rows bring their queries in two bf16
 // parts, fp32 rows queries and probabilities in three, and neither loses anything of the keys and values as stored.
+//
+// Single tokens are bound by the bytes of the rows that they read behind a start of 8 us (plan, page numbers, query), longer calls by the issue of vector
+// and matrix instructions together.  Tiles of few columns are of 16 here: a wave reads a block of keys with half the registers of 32 and three of them
+// fit a SIMD, and two tiles that read the same rows meet in the cache.
 #define SEGPT_FEW_COLUMNS 16
 #define SEGPT_JOIN_COLUMNS
 #include "paged_quant.hpp"
@@ -13,7 +17,6 @@
 
 namespace segpt {
 namespace {
-
 
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
@@ -204,7 +207,10 @@ struct Source {
 
 // ---- FEW: one wave, up to 16 columns.  A score tile is 16 keys by 16 columns; a lane takes a quarter of a key's row, so that a row is read
 // whole by four lanes and is the A operand as it is decoded, no LDS in between: the components that a lane contributes to a step are not those of
-// the instruction's own order, but the queries' are the same, and a sum does not ask.
+// the instruction's own order, but the queries' are the same, and a sum does not ask.  Probabilities go to the values in two bf16 parts, fp32 rows' in
+// three.  Two blocks of codes are under way while a third is worked on.  32 tokens of 18 / 6 heads of 64, 200 .. 8192 keys, 8 bits: 25.5 us, 110 MB at
+// 4.3 TB/s; 48 tokens of 16 / 4 heads of 128, 255 .. 16000 keys, 4 bits: 51 us, 214 MB at 4.2 TB/s; one token, 4096 keys: 7.9.  Of the vector
+// instructions of the 32 tokens two fifths are the start of the items, of nine blocks each; fewer and longer ones leave the memory idle (target_of).
 template <int D, int FMT>
 struct Quarter {
   static constexpr int kBytes = Codes<FMT>::row_bytes(D) / 4;   // of a lane
@@ -504,7 +510,9 @@ __device__ __forceinline__ void few_columns(const QuantArgs& qa, const PagedArgs
 
 // ---- MANY: four waves of 32 columns around a ring of three stages (K' tile, V' tile of bf16); tile jt lives in stage jt % 3.  The codes of a tile are
 // asked for three turns before its products, kept in registers for one, and decoded into LDS.  The scores of a block of 32 keys are computed beside the
-// exponentials of the block before it and its product with the values.
+// exponentials of the block before it and its product with the values.  bf16 rows' probabilities are rounded once: with their second part the error of y
+// would go from 2.3e-3 to its own rounding's 1.7e-3, for half as many matrix instructions again.  One prompt of 8192 rows, 18 / 6 heads of 64: 246 us,
+// 0.94 PFLOP/s with the queries' second part; 512 rows beside 31 tokens, 100 .. 8192 keys: 62 us, vector instructions half of it, matrix a quarter.
 template <int D>
 struct ManyShape {
   static constexpr int kBK = D == 64 ? 64 : 32, kTileBytes = kBK * 2 * D, kStageBytes = 2 * kTileBytes, kStages = 3;
@@ -771,7 +779,7 @@ __device__ __forceinline__ QuantArgs quant_of(const Args& a) { return {a.w.p, a.
 
 // Launches whose entries are all FEW: a workgroup is one wave
 template <typename E, int D>
-constexpr int kFewWaves = sizeof(E) == 2 && D == 64 ? 3 : 2;  // waves a SIMD: what their registers leave room for
+constexpr int kFewWaves = sizeof(E) == 2 && D == 64 ? 3 : 2;  // waves a SIMD that registers leave room for (128 tokens of up to 3000 keys: 62 us with two, 53)
 template <typename E, int D, int FMT>
 __global__ __launch_bounds__(64, (kFewWaves<E, D>)) void paged_quant_few_kernel(Args args) {
   const PagedArgs& a = args.w;
@@ -815,6 +823,10 @@ __global__ __launch_bounds__(256, (sizeof(E) == 2 || D == 64 ? 2 : 1)) void page
 }
 
 // ---- host side
+// Workgroups of four waves that the items are to fill.  Tokens alone: as many waves as are resident (32 tokens 31 us; for 496 workgroups 32, 384 36, 1000 37;
+// heads of 128, where two waves fit a SIMD, 55, for 744 69).  Tiles of many columns: 512 are resident, but one a CU runs faster than two, and what
+// rounding adds must not wait for a place (32 tokens behind 8192 keys 22.1, for 496 23.9, 256 24.1; four prompts of 512 22.3, for 496 34.7).  Ragged rows:
+// few and many columns, and many workgroups of the first kind (512 rows beside 31 tokens 63, for 384 85, 640 69).
 int target_of(const segpt_paged_params& p) {
   const int rep = p.H / p.Hkv;
   const bool wide = p.prefix_table || (!p.seq_start && (int64_t)rep * (p.T / p.B) > kMostFew);

@@ -551,6 +551,7 @@ __device__ __forceinline__ void leave_plan(const PagedArgs& a, int lane, int rep
 // row; as many units stand side by side over the shares of a column as leave each one batch of kBatch that is requested together, and
 // their sums meet in LDS.  Fixed order: deterministic.  4.9 us for one token of 18 heads (launch and two round trips), 5.9 for 32 of them, 12 for
 // 128 tokens of 16 heads of 128 behind a prefix (25 MB).
+// By columns (kJoinColumns): 223 rows of 16 heads of 128 behind 5001 keys 16.2 -> 9.5 us, 2891 rows of fp32, 8 / 4 heads of 64, 11.4 -> 7.4; single tokens as before.
 constexpr int kMergeThreads = 256, kMergeGroups = 2048;
 template <typename E, int D>
 __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedArgs a, int subs, int per_sub) {

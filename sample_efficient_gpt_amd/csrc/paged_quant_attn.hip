@@ -235,7 +235,8 @@ struct Quarter {
   }
 };
 // The values of a block of 32 keys in LDS, bf16: chunk c (16 bytes) of row r lies at chunk c ^ f(r).  Sixteen lanes write one chunk of 16 rows, and a
-// transposing read takes two chunks of eight rows at a time; either way all banks are met once.
+// transposing read takes two chunks of eight rows at a time; as groups of sixteen lanes both meet all banks once.  (Two fifths of the LDS cycles are counted
+// as conflicts all the same; the LDS is busy for 17 % of the time at head_dim 64, 30 % at 128.)
 template <int D>
 struct ValueTile {
   static constexpr int kRB = 2 * D, kBytes = kBlock * kRB;

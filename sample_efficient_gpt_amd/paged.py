@@ -365,6 +365,9 @@ class PageTable:
         self.kv_len[b] = 0
 
 
+_ROWS_AT_ONCE = 1 << 18  # of a cache that is turned into one of another dtype
+
+
 class PagedKVCache:
     """Pages of keys and values of one layer, ``[n_pages, Hkv, page size, D]`` each, under a ``PageTable`` that all layers share.
 
@@ -418,26 +421,38 @@ class PagedKVCache:
 
     def read(self, dtype=None):
         """Everything the table's sequences hold, packed: ``(k, v, seq_start)``, keys as the attention multiplies them."""
+        return self._read(0, len(self.pages.lengths), dtype)
+
+    def _read(self, first, end, dtype=None):
         t = self.pages
         starts = [0]
-        for n in t.lengths:
+        for n in t.lengths[first:end]:
             starts.append(starts[-1] + n)
         seq_start = torch.tensor(starts, dtype=torch.int32).to(t.kv_len.device)
-        k, v = paged_kv_read(self.k_pages, self.v_pages, t.block_table, t.kv_len, starts[-1], seq_start=seq_start, k_scales=self.k_scales, v_scales=self.v_scales,
-                             dtype=dtype, max_len=t.max_len)
+        k, v = paged_kv_read(self.k_pages, self.v_pages, t.block_table[first:end], t.kv_len[first:end], starts[-1], seq_start=seq_start, k_scales=self.k_scales,
+                             v_scales=self.v_scales, dtype=dtype, max_len=t.max_len)
         return k, v, seq_start
 
     def to(self, dtype):
-        """A cache of this dtype in pages of its own, under the same table and with the same keys and values (the shared prefix's among them)."""
+        """A cache of this dtype in pages of its own, under the same table and with the same keys and values (the shared prefix's among them).  Rows
+        pass through memory of their own, some sequences at a time."""
         if dtype == self.dtype:
             return self
         other = PagedKVCache(self.pages, self.k_pages.shape[1], self.head_dim, dtype)
         rows = dtype if other.k_scales is None else torch.float32 if self.dtype == torch.float32 else torch.bfloat16
         for t in (self.pages, self.pages.prefix):
-            if t is None or not any(t.lengths):
+            if t is None:
                 continue
-            k, v, seq_start = (x if x.dtype == torch.int32 else x.to(rows) for x in self.of(t).read())
-            with torch.no_grad():
-                paged_kv_append(k, v, other.k_pages, other.v_pages, t.block_table, t.kv_len, seq_start=seq_start, qk_norm=False, max_len=t.max_len,
-                                k_scales=other.k_scales, v_scales=other.v_scales)
+            source, b = self.of(t), 0
+            while b < len(t.lengths):
+                e, n = b + 1, t.lengths[b]
+                while e < len(t.lengths) and n + t.lengths[e] <= _ROWS_AT_ONCE:
+                    n += t.lengths[e]
+                    e += 1
+                if n:
+                    k, v, seq_start = source._read(b, e)
+                    with torch.no_grad():
+                        paged_kv_append(k.to(rows), v.to(rows), other.k_pages, other.v_pages, t.block_table[b:e], t.kv_len[b:e], seq_start=seq_start,
+                                        qk_norm=False, max_len=t.max_len, k_scales=other.k_scales, v_scales=other.v_scales)
+                b = e
         return other

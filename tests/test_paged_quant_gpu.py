@@ -350,6 +350,24 @@ def test_run_of_steps(gpu_device, fmt, dtype):
 
 
 @both_formats
+@pytest.mark.parametrize("at_once", [1, 40, 61, 1 << 18])
+def test_another_dtype_some_sequences_at_a_time(gpu_device, fmt, at_once, monkeypatch):
+    from sample_efficient_gpt_amd import paged
+
+    monkeypatch.setattr(paged, "_ROWS_AT_ONCE", at_once)
+    pages = PageTable(5, 64, 8, device=gpu_device, prefix_len=11)
+    cache = PagedKVCache(pages, 2, 64)
+    g = torch.Generator().manual_seed(5)
+    for table, rows in ((pages.prefix, 11), (pages, [20, 0, 41, 1, 33])):
+        table.extend(rows)
+        cache.of(table).append(*(torch.randn(table.rows, 2, 64, generator=g).to(BF16).to(gpu_device) for _ in "kv"))
+    small = cache.to(DTYPES[fmt])
+    for table in (pages.prefix, pages):
+        for got, ref in zip(small.of(table).read()[:2], cache.of(table).read()[:2]):
+            assert torch.equal(got.to(F64), decode(*encode(ref.to(F64), fmt), fmt))
+
+
+@both_formats
 @pytest.mark.parametrize("prefix", [0, 70])
 def test_module(gpu_device, fmt, prefix):
     """The attention module over such a cache, against the same module over a bf16 cache that holds the very values: what this one reads back."""

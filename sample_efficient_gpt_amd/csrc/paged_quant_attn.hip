@@ -208,7 +208,7 @@ struct Source {
 // ---- FEW: one wave, up to 16 columns.  A score tile is 16 keys by 16 columns; a lane takes a quarter of a key's row, so that a row is read
 // whole by four lanes and is the A operand as it is decoded, no LDS in between: the components that a lane contributes to a step are not those of
 // the instruction's own order, but the queries' are the same, and a sum does not ask.  Probabilities go to the values in two bf16 parts, fp32 rows' in
-// three.  Two blocks of codes are under way while a third is worked on.  32 tokens of 18 / 6 heads of 64, 200 .. 8192 keys, 8 bits: 25.5 us, 110 MB at
+// three.  One or two blocks of codes are under way while another is worked on.  32 tokens of 18 / 6 heads of 64, 200 .. 8192 keys, 8 bits: 25.5 us, 110 MB at
 // 4.3 TB/s; 48 tokens of 16 / 4 heads of 128, 255 .. 16000 keys, 4 bits: 51 us, 214 MB at 4.2 TB/s; one token, 4096 keys: 7.9.  Of the vector
 // instructions of the 32 tokens two fifths are the start of the items, of nine blocks each; fewer and longer ones leave the memory idle (target_of).
 template <int D, int FMT>
@@ -361,7 +361,8 @@ __device__ __forceinline__ void odd_values(const QuantArgs& qa, const PagedArgs&
   }
 }
 
-template <typename E, int D, int FMT>
+// AHEAD: blocks under way
+template <typename E, int D, int FMT, int AHEAD>
 __device__ __forceinline__ void few_columns(const QuantArgs& qa, const PagedArgs& a, const Item& it, int rep, int lane, uint32_t lds, float* gsm) {
   using L = Quarter<D, FMT>;
   using V = ValueTile<D>;
@@ -393,7 +394,7 @@ __device__ __forceinline__ void few_columns(const QuantArgs& qa, const PagedArgs
   for (int i = 0; i < D / 64; ++i) gsm[64 * i + lane] = scale_of(p, gain[i]);
   wave_sync();
   q.finish(p, c.live, lane, gsm, lds);
-  if (blocks > 1) ask(b1, 1);
+  if (AHEAD == 2 && blocks > 1) ask(b1, 1);
 
   f32x4 o[DB];
   float m = 0.f, limit = -INFINITY, l = 0.f;  // reference (log2 units); by how much a score may exceed it; sum over this lane's keys
@@ -420,7 +421,7 @@ __device__ __forceinline__ void few_columns(const QuantArgs& qa, const PagedArgs
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) lds_write16(lds + V::write_at(16 * t + r16, L::component(ks, quarter) / 8), v[ks]);
     }
-    if (j + 2 < blocks) ask(b, j + 2);
+    if (j + AHEAD < blocks) ask(b, j + AHEAD);
     if (masked) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -474,10 +475,10 @@ __device__ __forceinline__ void few_columns(const QuantArgs& qa, const PagedArgs
       for (int db = 0; db < DB; ++db) o[db] = mfma16(as_bf16x8(v[db]), as_bf16x8(pb[u]), o[db]);
     wave_sync();
   };
-  for (int j = 0; j < blocks; j += 2) {
-    if ((2 * j + 4) % 64 == 0 && j + 2 < blocks) walk.work_out(qa, a, lane);  // the next tiles asked for: 2 j + 4 .. 2 j + 7
+  for (int j = 0; j < blocks; j += AHEAD) {
+    if ((2 * j + 2 * AHEAD) % 64 == 0 && j + AHEAD < blocks) walk.work_out(qa, a, lane);  // the next tiles asked for: 2 AHEAD of them from 2 j + 2 AHEAD on
     step(b0, j);
-    if (j + 1 < blocks) step(b1, j + 1);
+    if (AHEAD == 2 && j + 1 < blocks) step(b1, j + 1);
   }
   const bool bad = it.x.broken | (__builtin_amdgcn_ballot_w64(walk.bad) != 0);
   if (__builtin_amdgcn_ballot_w64(odd) != 0)
@@ -779,10 +780,10 @@ struct Args {
 __device__ __forceinline__ QuantArgs quant_of(const Args& a) { return {a.w.p, a.k_scales, a.v_scales}; }
 
 // Launches whose entries are all FEW: a workgroup is one wave
-template <typename E, int D>
-constexpr int kFewWaves = sizeof(E) == 2 && D == 64 ? 3 : 2;  // waves a SIMD that registers leave room for (128 tokens of up to 3000 keys: 62 us with two, 53)
+template <int D>
+constexpr int kFewWaves = D == 64 ? 3 : 2;  // waves a SIMD that registers leave room for (128 tokens of up to 3000 keys: 62 us with two, 53)
 template <typename E, int D, int FMT>
-__global__ __launch_bounds__(64, (kFewWaves<E, D>)) void paged_quant_few_kernel(Args args) {
+__global__ __launch_bounds__(64, kFewWaves<D>) void paged_quant_few_kernel(Args args) {
   const PagedArgs& a = args.w;
   __shared__ __attribute__((aligned(1024))) char lds[ValueTile<D>::kBytes];
   __shared__ __attribute__((aligned(16))) float gsm[D];
@@ -794,7 +795,10 @@ __global__ __launch_bounds__(64, (kFewWaves<E, D>)) void paged_quant_few_kernel(
   const Item it = locate<false>(a, lane, rep, share, mine, blockIdx.x);
   if (!it.valid) return;
   const QuantArgs qa = quant_of(args);
-  few_columns<E, D, FMT>(qa, a, it, rep, lane, lds_addr_of(lds), gsm);
+  // one where a second would not leave the registers for the waves: 48 tokens of heads of 128 at 8 bits 97 -> 89 us, with fp32 rows 142 -> 91, at 4 bits the
+  // other way for bf16 rows (57 and 58); 128 tokens of heads of 64 in fp32 59 -> 52 with the third wave, 32 in bf16 the other way (30.7 and 32.1)
+  constexpr int AHEAD = sizeof(E) == 2 && Codes<FMT>::row_bytes(D) <= 64 ? 2 : 1;
+  few_columns<E, D, FMT, AHEAD>(qa, a, it, rep, lane, lds_addr_of(lds), gsm);
 }
 
 // Any launch: the first workgroups are items of many columns, the next four items each of few, the rest have none
@@ -819,7 +823,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 2 || D == 64 ? 2 : 1)) void page
   } else {
     const Item it4 = locate<false>(a, lane, rep, share, mine, ((int)blockIdx.x - it.x.base) * 4 + wave);
     if (!it4.valid) return;
-    few_columns<E, D, FMT>(qa, a, it4, rep, lane, lds_addr_of(lds) + wave * ValueTile<D>::kBytes, gsm[wave]);
+    few_columns<E, D, FMT, 2>(qa, a, it4, rep, lane, lds_addr_of(lds) + wave * ValueTile<D>::kBytes, gsm[wave]);
   }
 }
 
@@ -831,7 +835,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 2 || D == 64 ? 2 : 1)) void page
 int target_of(const segpt_paged_params& p) {
   const int rep = p.H / p.Hkv;
   const bool wide = p.prefix_table || (!p.seq_start && (int64_t)rep * (p.T / p.B) > kMostFew);
-  if (all_few(p)) return p.D == 64 && p.dtype == SEGPT_DTYPE_BF16 ? 744 : 496;
+  if (all_few(p)) return p.D == 64 ? 744 : 496;
   return wide ? 384 : p.seq_start ? 480 : 496;
 }
 

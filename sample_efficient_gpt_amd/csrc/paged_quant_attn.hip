@@ -611,7 +611,8 @@ struct StateLess {
 };
 
 template <typename E, int D, int FMT>
-__device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArgs& a, const Item& it, int rep, int tid, uint32_t lds, uint32_t places, float* gsm) {
+__device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArgs& a, const Item& it, int rep, int tid, uint32_t lds, uint32_t places, float* gsm,
+                                             int* any_bad) {
   using S = ManyShape<D>;
   constexpr int BK = S::kBK, N = BK / 32, MB = D / 32, KS = D / 16, PARTS = kQueryParts<E>, PROBS = sizeof(E) == 2 ? 1 : 3;
   constexpr int P = 16 * Codes<FMT>::kBits / 8;  // bytes of a lane's 16 components
@@ -763,7 +764,11 @@ __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArg
     if (N == 1) turn(b + 1, stage_from(1));
     any(IC<0>{}, b + 1, s1, s0);
   }
-  const bool bad = it.x.broken | (__builtin_amdgcn_ballot_w64(walk.bad) != 0);
+  // a wave looks up the pages of its own rows of a tile, and multiplies by all of them
+  const bool mine = __builtin_amdgcn_ballot_w64(walk.bad) != 0;
+  if (lane == 0) any_bad[wave] = mine;
+  __syncthreads();
+  const bool bad = it.x.broken | ((any_bad[0] | any_bad[1] | any_bad[2] | any_bad[3]) != 0);
   if (__builtin_amdgcn_ballot_w64(odd) != 0)
     odd_values<D>(qa, a, it, c, (max(c.all, -1) + 1) / BK * BK, [&](int b) {
 #pragma unroll
@@ -810,6 +815,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 2 || D == 64 ? 2 : 1)) void page
   __shared__ __attribute__((aligned(1024))) char lds[kLds];
   __shared__ __attribute__((aligned(16))) float gsm[4][D];
   __shared__ __attribute__((aligned(16))) char places[4 * Walk<S::kRows, S::kBK, true>::kBytes];
+  __shared__ int any_bad[4];
   const int tid = threadIdx.x, lane = tid & 63, rep = a.rep.d;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   clear_rest<E>(a, tid, 256, D);
@@ -819,7 +825,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 2 || D == 64 ? 2 : 1)) void page
   const QuantArgs qa = quant_of(args);
   const Item it = locate<true>(a, lane, rep, share, mine, blockIdx.x);
   if (it.x.entry >= 0) {
-    if (it.valid) many_columns<E, D, FMT>(qa, a, it, rep, tid, lds_addr_of(lds), lds_addr_of(places), gsm[0]);
+    if (it.valid) many_columns<E, D, FMT>(qa, a, it, rep, tid, lds_addr_of(lds), lds_addr_of(places), gsm[0], any_bad);
   } else {
     const Item it4 = locate<false>(a, lane, rep, share, mine, ((int)blockIdx.x - it.x.base) * 4 + wave);
     if (!it4.valid) return;

@@ -365,6 +365,8 @@ int segpt_paged_attn(const segpt_paged_params* p, void* stream);
  * The scale is held as the byte e + 127.  Rows are prepared in 64 bits, so that the codes are those of the exact value.  A block with a
  * component that is not finite, or beyond top 2^119 (E2M1: top 2^125), has the scale 255 and is NaN as a whole, when it is read and
  * in the attention; everything else that is stored is finite, and exact in bf16.  The reference has no such cache.
+ * (Pools that something else filled: scales from 17 to 255.  A code of E4M3 that is NaN, 0x7F or 0xFF, is NaN here, and what a scale carries beyond the
+ * largest bf16 number is an infinity.)
  *
  * The calls below are those above with such pools: segpt_paged_params as there, dtype that of the rows, head_dim 64 or 128, and
  * k_pages, v_pages [n_pages, Hkv, page_size, D (E2M1: D / 2)] of bytes, strides in BYTES, rows 16-byte aligned. */

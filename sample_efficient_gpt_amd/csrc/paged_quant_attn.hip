@@ -138,6 +138,18 @@ struct Walk {
   }
 };
 
+struct Args {
+  PagedArgs w;
+  segpt_tensor4 k_scales, v_scales;
+};
+__device__ __forceinline__ QuantArgs quant_of(const Args& a) { return {a.w.p, a.k_scales, a.v_scales}; }
+// The kernel's arguments (its only ones) from memory once more, for what is hardly ever needed: else they wait in registers from the start
+__device__ __forceinline__ const Args& arguments() {
+  auto at = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(at));
+  return *(const Args*)at;
+}
+
 // What a lane asks for of one row of keys or values: WORDS words of codes, and the scales of the whole row
 template <int WORDS>
 struct RowPart {
@@ -334,9 +346,9 @@ struct Query16 {
   }
 };
 
-// A value that is no number must reach the rows that see its key, and not the others as 0 * NaN: in a block that not all rows see it is made 0 and
-// noted, and put back behind the loop
-__device__ __forceinline__ bool clear_nan(u32x4& v) {
+// A value that is not finite (NaN by its scale or code, or beyond the largest number) must reach the rows that see its key, and not the others as 0 * NaN:
+// in a block that not all rows see it is made 0 and noted, and put back behind the loop
+__device__ __forceinline__ bool clear_odd(u32x4& v) {
   typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
   uint32_t all = ~0u;
 #pragma unroll
@@ -348,16 +360,39 @@ __device__ __forceinline__ bool clear_nan(u32x4& v) {
   asm volatile("" : "+v"(v));  // whole registers again: as bf16 vectors they would be taken apart, element by element
   return all != ~0u;
 }
-// calls `found(block)` for every block of components that is no number in the value of a key from j0 on that the lane's row sees (keys counted from k0)
-template <int D, typename F>
-__device__ __forceinline__ void odd_values(const QuantArgs& qa, const PagedArgs& a, const Item& it, const Column& c, int j0, F found) {
-  for (int j = j0; j <= c.any; ++j) {
-    const int key = it.k0 + j, page = it.ids[key >> a.log_page];
-    if ((uint32_t)page >= (uint32_t)a.p.n_pages) continue;  // the rows are NaN as a whole
-    const uint32_t s = load_scales<D>(byte_row(qa.v_scales, page, it.g, key & ((1 << a.log_page) - 1)));
+// Adds those that clear_odd() left out to what the item has left, y or a partial result, key by key from j0 on (counted from k0) for the rows that see them:
+// their probability is positive, so a sum with one is that value, or NaN where signs meet.  A lane has the components that it wrote: four of every STEP,
+// from `from` on.  Behind the results, in memory, and with the arguments read again, so that the loop before has the registers to itself (32 tokens 30.2 us;
+// added to the sums before they are written 32.2).
+template <typename E, int D, int FMT, int STEP>
+__device__ __forceinline__ void add_odd_values(const Item& it, const Column& c, int j0, int slot_col, int from) {
+  if (!c.live) return;
+  const Args& qa = arguments();
+  const PagedArgs& a = qa.w;
+  float* part = a.part + ((int64_t)it.slot * 32 + slot_col) * D;
+  E* out = row_of<E>(a.p.o, c.t, c.h);
+  const float f = it.direct && a.p.gate.ptr ? gate_factor<E, D>(a.p, c.t, c.h) : 1.f;
+  for (int j = j0; j <= c.lim; ++j) {
+    const int key = it.k0 + j, page = it.ids[key >> a.log_page], slot = key & ((1 << a.log_page) - 1);
+    if ((uint32_t)page >= (uint32_t)a.p.n_pages) continue;  // the row is NaN as a whole
+    const char* row = byte_row(a.p.v_pages, page, it.g, slot);
+    const uint32_t scales = load_scales<D>(byte_row(qa.v_scales, page, it.g, slot));
+#pragma unroll 1
+    for (int at = from; at < D; at += STEP) {
+      const float scale = scale_at(scales, at / SEGPT_SCALE_BLOCK);
+      uint32_t w;
+      if constexpr (Codes<FMT>::k8) w = *reinterpret_cast<const uint32_t*>(row + at);
+      else w = *reinterpret_cast<const uint16_t*>(row + at / 2);
+      const uint32_t x[2] = {decode_bf16x2<FMT, 0>(w, scale), decode_bf16x2<FMT, 1>(w, scale)};
 #pragma unroll
-    for (int b = 0; b < D / SEGPT_SCALE_BLOCK; ++b)
-      if (j <= c.lim && (s >> (8 * b) & 255u) == kNoNumber) found(b);
+      for (int r = 0; r < 4; ++r) {
+        const float v = r & 1 ? bf16hi(x[r / 2]) : bf16lo(x[r / 2]);
+        if (fabsf(v) < INFINITY) continue;
+        if (!it.direct) part[at + r] += v;
+        else if constexpr (sizeof(E) == 2) out[at + r] = f32_to_bf16(bf16_to_f32(out[at + r]) + v * f);
+        else out[at + r] += v * f;
+      }
+    }
   }
 }
 
@@ -467,7 +502,7 @@ __device__ __forceinline__ void few_columns(const QuantArgs& qa, const PagedArgs
     for (int db = 0; db < DB; ++db) v[db] = V::read(lds, lane, db);
     if (masked) {
 #pragma unroll
-      for (int db = 0; db < DB; ++db) odd |= clear_nan(v[db]);
+      for (int db = 0; db < DB; ++db) odd |= clear_odd(v[db]);
     }
 #pragma unroll
     for (int u = PARTS - 1; u >= 0; --u)
@@ -481,33 +516,27 @@ __device__ __forceinline__ void few_columns(const QuantArgs& qa, const PagedArgs
     if (AHEAD == 2 && j + 1 < blocks) step(b1, j + 1);
   }
   const bool bad = it.x.broken | (__builtin_amdgcn_ballot_w64(walk.bad) != 0);
-  if (__builtin_amdgcn_ballot_w64(odd) != 0)
-    odd_values<D>(qa, a, it, c, (max(c.all, -1) + 1) / kBlock * kBlock, [&](int b) {
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-        if (db / 2 == b) o[db] = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
-    });
   float sum = l + __shfl_xor(l, 16, 64), ref = limit == -INFINITY ? -INFINITY : m;
   sum = half_sum(sum);
   if (bad) { sum = __builtin_nanf(""); ref = 0.f; }
-  if (!c.live) return;
-  if (!it.direct) {
+  if (c.live && !it.direct) {
     const int64_t at = (int64_t)it.slot * 32 + r16;
 #pragma unroll
     for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(a.part + at * D + 16 * db + 4 * quarter) = o[db];
     if (quarter == 0) a.stat[at] = make_float2(ref, sum);
-    return;
-  }
-  float f = sum == 0.f ? 0.f : 1.0f / sum;
-  if (p.lse && quarter == 0) p.lse[(int64_t)c.t * p.H + c.h] = sum == 0.f ? -INFINITY : (ref + __log2f(sum)) * kLn2;
-  if (p.gate.ptr) f *= gate_factor<E, D>(p, c.t, c.h);
-  E* out = row_of<E>(p.o, c.t, c.h) + 4 * quarter;
+  } else if (c.live) {
+    float f = sum == 0.f ? 0.f : 1.0f / sum;
+    if (p.lse && quarter == 0) p.lse[(int64_t)c.t * p.H + c.h] = sum == 0.f ? -INFINITY : (ref + __log2f(sum)) * kLn2;
+    if (p.gate.ptr) f *= gate_factor<E, D>(p, c.t, c.h);
+    E* out = row_of<E>(p.o, c.t, c.h) + 4 * quarter;
 #pragma unroll
-  for (int db = 0; db < DB; ++db) {
-    const float y[4] = {o[db][0] * f, o[db][1] * f, o[db][2] * f, o[db][3] * f};
-    if constexpr (sizeof(E) == 2) *reinterpret_cast<u32x2*>(out + 16 * db) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
-    else store16(out + 16 * db, y);
+    for (int db = 0; db < DB; ++db) {
+      const float y[4] = {o[db][0] * f, o[db][1] * f, o[db][2] * f, o[db][3] * f};
+      if constexpr (sizeof(E) == 2) *reinterpret_cast<u32x2*>(out + 16 * db) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+      else store16(out + 16 * db, y);
+    }
   }
+  if (__builtin_amdgcn_ballot_w64(odd) != 0) add_odd_values<E, D, FMT, 16>(it, c, (max(c.all, -1) + 1) / kBlock * kBlock, r16, 4 * quarter);
 }
 
 // ---- MANY: four waves of 32 columns around a ring of three stages (K' tile, V' tile of bf16); tile jt lives in stage jt % 3.  The codes of a tile are
@@ -701,7 +730,7 @@ __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArg
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) {
         u32x4 v = __builtin_bit_cast(u32x4, swz_frag_tr<D>(lds + block + S::kTileBytes + swz_off_tr<D>(lane), mb, s2));
-        if (masked) odd |= clear_nan(v);
+        if (masked) odd |= clear_odd(v);
 #pragma unroll
         for (int u = PROBS - 1; u >= 0; --u) st.o[mb] = mfma32(as_bf16x8(v), as_bf16x8(pb[u][s2]), st.o[mb]);
       }
@@ -769,20 +798,9 @@ __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArg
   if (lane == 0) any_bad[wave] = mine;
   __syncthreads();
   const bool bad = it.x.broken | ((any_bad[0] | any_bad[1] | any_bad[2] | any_bad[3]) != 0);
-  if (__builtin_amdgcn_ballot_w64(odd) != 0)
-    odd_values<D>(qa, a, it, c, (max(c.all, -1) + 1) / BK * BK, [&](int b) {
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
-        if (mb == b) st.o[mb] = splat16(__builtin_nanf(""));
-    });
   store_result<E, D>(a, it, c, st, bad, wave * 32 + (lane & 31), hh);
+  if (__builtin_amdgcn_ballot_w64(odd) != 0) add_odd_values<E, D, FMT, 8>(it, c, (max(c.all, -1) + 1) / BK * BK, wave * 32 + (lane & 31), 4 * hh);
 }
-
-struct Args {
-  PagedArgs w;
-  segpt_tensor4 k_scales, v_scales;
-};
-__device__ __forceinline__ QuantArgs quant_of(const Args& a) { return {a.w.p, a.k_scales, a.v_scales}; }
 
 // Launches whose entries are all FEW: a workgroup is one wave
 template <int D>

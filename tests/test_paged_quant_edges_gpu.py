@@ -37,3 +37,60 @@ def test_a_bad_page_number_reaches_every_row_that_sees_it(gpu_device, H, Hkv, D,
         assert attend(x).isnan().all(), j
         x.prefix_table[j] = was
     assert torch.equal(attend(x), clean)
+
+
+@pytest.mark.parametrize("fmt,kind", [("e4m3", "nan"), ("e4m3", "-nan"), ("e4m3", "large"), ("e2m1", "large")])
+@pytest.mark.parametrize("H,Hkv,D,dtype", [(6, 2, 64, BF16), (4, 2, 128, BF16), (4, 2, 64, F32), (4, 2, 128, F32)])
+@pytest.mark.parametrize("rows,lens,prefix", [([1, 1], [37, 64], 0), ([70, 1], [70, 40], 0), ([45, 3], [300, 50], 0), ([1, 50], [5, 50], 40)])
+def test_a_value_that_is_none_by_its_code(gpu_device, rows, lens, prefix, H, Hkv, D, dtype, fmt, kind):
+    """Pools that something else filled: the code that is NaN in 8 bits, and a scale that carries codes beyond the largest number.  Wherever the key stands
+    (in a block that all rows see, or one that some do), the rows that see it have its value, and nothing else changes."""
+    x = QuantBatch(fmt, rows, lens, H, Hkv, D, 16, dtype, gpu_device, seed=51, prefix=prefix)
+    clean = attend(x)
+    codes, rep = x.v_pages.view(torch.uint8), H // Hkv
+    for b, (n, L) in enumerate(zip(rows, lens)):
+        for p in sorted({0, L // 2, L // 32 * 32, L - n, L - 2, L - 1} & set(range(L))):
+            page, slot = int(x.block_table[b, p // 16]), p % 16
+            was = codes[page, 1, slot].clone(), x.v_scales[page, 1, slot].clone()
+            if kind == "large":  # a whole block, beyond what bf16 and fp32 hold
+                codes[page, 1, slot, 32 * codes.shape[3] // D:] = 0x7E if fmt == "e4m3" else 0x77
+                x.v_scales[page, 1, slot, 1:] = 254
+                none = torch.arange(D) >= 32
+            else:
+                codes[page, 1, slot, 37] = 0x7F if kind == "nan" else 0xFF
+                none = torch.arange(D) == 37
+            y = attend(x)
+            codes[page, 1, slot], x.v_scales[page, 1, slot] = was
+            first, end = x.starts[b] + max(0, p - (L - n)), x.starts[b + 1]
+            hit = torch.zeros(y.shape, dtype=torch.bool, device=gpu_device)
+            hit[first:end, rep:2 * rep] = none.to(gpu_device)
+            assert torch.equal(y.isnan() if kind != "large" else ~y.isfinite(), hit), (b, p)
+            assert torch.equal(y[~hit], clean[~hit]), (b, p)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,lens", [([1, 1], [37, 64]), ([70, 1], [70, 40])])
+def test_a_key_that_is_none_by_its_code(gpu_device, rows, lens, dtype):
+    x = QuantBatch("e4m3", rows, lens, 6, 2, 64, 16, dtype, gpu_device, seed=52)
+    clean = attend(x)
+    for b, (n, L) in enumerate(zip(rows, lens)):
+        for p in sorted({0, L // 2, L // 32 * 32, L - 1} & set(range(L))):
+            at = x.k_pages.view(torch.uint8)[int(x.block_table[b, p // 16]), 1, p % 16, 5:6]
+            was = at.clone()
+            at.fill_(0x7F)
+            y = attend(x)
+            at.copy_(was)
+            hit = torch.zeros(y.shape, dtype=torch.bool, device=gpu_device)
+            hit[x.starts[b] + max(0, p - (L - n)):x.starts[b + 1], 3:] = True
+            assert torch.equal(y.isnan(), hit) and torch.equal(y[~hit], clean[~hit]), (b, p)
+
+
+def test_rows_back_from_codes_that_are_none(gpu_device):
+    x = QuantBatch("e4m3", [40], [40], 2, 1, 64, 16, BF16, gpu_device, seed=53)
+    codes = x.v_pages.view(torch.uint8)
+    for t, (code, scale) in enumerate([(0x7F, 127), (0xFF, 127), (0x7E, 254), (0xFE, 254)]):
+        at = int(x.block_table[0, t // 16]), 0, t % 16
+        codes[(*at, slice(32))], x.v_scales[(*at, 0)] = code, scale
+    for dtype in (BF16, F32):
+        v = read(x, dtype=dtype)[1][:, 0, :32]
+        assert v[:2].isnan().all() and v[2:4].isinf().all() and (v[2] > 0).all() and (v[3] < 0).all() and v[4:].isfinite().all()

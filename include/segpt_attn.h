@@ -297,6 +297,7 @@ int segpt_linear_rows(const segpt_linear_rows_params* p, void* stream);
  *     those of its keys, gives NaN in every row that sees one of these (it may give NaN in its other rows).
  * Row ranges must not overlap, and two rows of one append must not name one slot: which of them is kept is undefined.  No output (o, lse; the pools
  * of an append) may overlap an input or another output: rows are read again after others are written. */
+#define SEGPT_FLAG_HEAD_32 64    /* pools of 8 and 4 bits: D may be 32, with fp32 rows (without it SEGPT_E_HEAD_DIM, and 0 bytes of scratch) */
 #define SEGPT_FLAG_ZERO_REST 32  /* segpt_paged_attn: rows of o that belong to no sequence are set to zero, their lse to -inf */
 
 /* [T, heads, D] tensor view; the D axis is contiguous. Strides in ELEMENTS. */
@@ -314,7 +315,7 @@ typedef struct segpt_paged_params {
   int32_t max_len;            /* no sequence holds more keys; 0 = table_width * page_size, and never more than that */
   int32_t prefix_len;         /* segpt_paged_attn: keys of the shared prefix, 0 = none */
   int32_t gq_numel, gk_numel;
-  int32_t flags; /* SEGPT_FLAG_NO_NORM, SEGPT_FLAG_ZERO_REST */
+  int32_t flags; /* SEGPT_FLAG_NO_NORM, SEGPT_FLAG_ZERO_REST, SEGPT_FLAG_HEAD_32 */
   float eps, sm_scale, gate_scale;
   int32_t rope_len, rope_pos0; /* rope_pos0 + prefix_len + max_len must not exceed rope_len */
 
@@ -368,7 +369,7 @@ int segpt_paged_attn(const segpt_paged_params* p, void* stream);
  * (Pools that something else filled: scales from 17 to 255.  A code of E4M3 that is NaN, 0x7F or 0xFF, is NaN here, and what a scale carries beyond the
  * largest bf16 number is an infinity.)
  *
- * The calls below are those above with such pools: segpt_paged_params as there, dtype that of the rows, head_dim 64 or 128, and
+ * The calls below are those above with such pools: segpt_paged_params as there, dtype that of the rows, head_dim 64 or 128 (SEGPT_FLAG_HEAD_32: 32), and
  * k_pages, v_pages [n_pages, Hkv, page_size, D (E2M1: D / 2)] of bytes, strides in BYTES, rows 16-byte aligned. */
 #define SEGPT_SCALE_BLOCK 32
 #define SEGPT_POOL_E4M3 1

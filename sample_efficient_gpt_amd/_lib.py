@@ -21,6 +21,7 @@ SEGPT_FLAG_DECODE = 4
 SEGPT_FLAG_NO_NORM = 8
 SEGPT_FLAG_F32_SPLIT = 16
 SEGPT_FLAG_ZERO_REST = 32
+SEGPT_FLAG_HEAD_32 = 64
 SEGPT_SCALE_BLOCK = 32
 SEGPT_POOL_E4M3 = 1
 SEGPT_POOL_E2M1 = 2

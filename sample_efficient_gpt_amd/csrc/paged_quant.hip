@@ -45,14 +45,18 @@ __device__ __forceinline__ float scaled(double x, int e) {
 }
 __device__ __forceinline__ float scaled(float x, int e) { return x * __uint_as_float((uint32_t)(127 - e) << 23); }
 
-// VEC components of a block spread over 32 / VEC lanes: their codes, VEC * bits / 8 bytes, and the block's scale
-template <int FMT, int VEC, typename T>
-__device__ __forceinline__ uint32_t encode(const T (&x)[VEC], uint32_t (&w)[2]) {
+template <int VEC, typename T>
+__device__ __forceinline__ uint32_t largest_of(const T (&x)[VEC]) {
   uint32_t largest = 0;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) largest = max(largest, size_of(x[i]));
+  return largest;
+}
+// VEC components of a block spread over LANES lanes: their codes, VEC * bits / 8 bytes, and the block's scale; largest: of this lane's
+template <int FMT, int VEC, int LANES, typename T>
+__device__ __forceinline__ uint32_t encode(const T (&x)[VEC], uint32_t largest, uint32_t (&w)[2]) {
 #pragma unroll
-  for (int o = 1; o < SEGPT_SCALE_BLOCK / VEC; o <<= 1) largest = max(largest, (uint32_t)__shfl_xor((int)largest, o, 64));
+  for (int o = 1; o < LANES; o <<= 1) largest = max(largest, (uint32_t)__shfl_xor((int)largest, o, 64));
   const int e = max(exponent_of<FMT, T>(largest), kLeastExponent);
   const bool none = e > Codes<FMT>::kMostExponent;
   float y[VEC];
@@ -73,6 +77,16 @@ __device__ __forceinline__ uint32_t encode(const T (&x)[VEC], uint32_t (&w)[2]) 
   }
   if (none) w[0] = w[1] = 0u;
   return none ? kNoNumber : (uint32_t)(e + 127);
+}
+// a lane's components of either half of a row: codes and scales
+template <int FMT, int D, int VEC, typename T>
+__device__ __forceinline__ void encode_halves(const T (&x)[2][VEC], uint32_t (&w)[2][2], uint32_t (&scale)[2]) {
+  constexpr bool kOneBlock = D == SEGPT_SCALE_BLOCK;  // both halves are of one block
+  constexpr int kLanes = (kOneBlock ? D / 2 : SEGPT_SCALE_BLOCK) / VEC;
+  uint32_t largest[2] = {largest_of(x[0]), largest_of(x[1])};
+  if (kOneBlock) largest[0] = largest[1] = max(largest[0], largest[1]);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) scale[h] = encode<FMT, VEC, kLanes>(x[h], largest[h], w[h]);
 }
 template <int BYTES>
 __device__ __forceinline__ void store_codes(char* at, const uint32_t (&w)[2]) {
@@ -147,20 +161,17 @@ __global__ __launch_bounds__(kThreads) void paged_append_quant_kernel(QuantArgs 
     for (int i = 0; i < VEC; ++i) { kd[0][i] *= beta; kd[1][i] *= beta; }
   }
   uint32_t kw[2][2], vw[2][2], ks[2], vs[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) ks[h] = encode<FMT, VEC>(kd[h], kw[h]);
+  encode_halves<FMT, D>(kd, kw, ks);
   if constexpr (MIX) {
     const double c1 = p.vr_coef[0], c2 = p.vr_coef[1];
+    double x[2][VEC];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      double x[VEC];
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) x[i] = fma(c2, (double)f[h][i], c1 * v[h][i]);
-      vs[h] = encode<FMT, VEC>(x, vw[h]);
-    }
+      for (int i = 0; i < VEC; ++i) x[h][i] = fma(c2, (double)f[h][i], c1 * v[h][i]);
+    encode_halves<FMT, D>(x, vw, vs);
   } else {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) vs[h] = encode<FMT, VEC>(v[h], vw[h]);
+    encode_halves<FMT, D>(v, vw, vs);
   }
   if (!placed || (uint32_t)page >= (uint32_t)p.n_pages) return;
   const int slot = at & ((1 << log_page) - 1);
@@ -175,7 +186,7 @@ __global__ __launch_bounds__(kThreads) void paged_append_quant_kernel(QuantArgs 
     char* kb = byte_row(a.k_scales, page, g, slot) + c / SEGPT_SCALE_BLOCK;
     char* vb = byte_row(a.v_scales, page, g, slot) + c / SEGPT_SCALE_BLOCK;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < (D == SEGPT_SCALE_BLOCK ? 1 : 2); ++h) {
       kb[h * (D / 2 / SEGPT_SCALE_BLOCK)] = (char)ks[h];
       vb[h * (D / 2 / SEGPT_SCALE_BLOCK)] = (char)vs[h];
     }
@@ -271,13 +282,16 @@ int launch_read(const QuantArgs& a, hipStream_t st) {
 
 }  // namespace
 
+// heads of 32 are an extension that a caller asks for: the entries' first callers go by the refusal
+bool quant_head_dim(const segpt_paged_params& p) { return p.D == 64 || p.D == 128 || (p.D == 32 && (p.flags & SEGPT_FLAG_HEAD_32)); }
+
 int check_quant(const segpt_paged_params* p, const segpt_paged_quant* q, PagedCall call) {
   int rc = check_paged_sizes(p, call);
   if (rc) return rc;
   if (!q) return SEGPT_E_NULL;
   if (q->struct_bytes != sizeof(segpt_paged_quant)) return SEGPT_E_STRUCT;
   if (q->format != SEGPT_POOL_E4M3 && q->format != SEGPT_POOL_E2M1) return SEGPT_E_DTYPE;
-  if (p->D != 64 && p->D != 128) return SEGPT_E_HEAD_DIM;
+  if (!quant_head_dim(*p)) return SEGPT_E_HEAD_DIM;
   if ((rc = check_paged(p, call, q->format == SEGPT_POOL_E4M3 ? p->D : p->D / 2, 16))) return rc;
   if (p->n_pages <= 0) return SEGPT_E_PAGES;
   const int scales = p->D / SEGPT_SCALE_BLOCK;
@@ -301,6 +315,7 @@ int segpt_paged_append_quant(const segpt_paged_params* p, const segpt_paged_quan
     if (p->D == 64) return e4m3 ? launch_append<uint16_t, 64, SEGPT_POOL_E4M3>(a, st) : launch_append<uint16_t, 64, SEGPT_POOL_E2M1>(a, st);
     return e4m3 ? launch_append<uint16_t, 128, SEGPT_POOL_E4M3>(a, st) : launch_append<uint16_t, 128, SEGPT_POOL_E2M1>(a, st);
   }
+  if (p->D == 32) return e4m3 ? launch_append<float, 32, SEGPT_POOL_E4M3>(a, st) : launch_append<float, 32, SEGPT_POOL_E2M1>(a, st);
   if (p->D == 64) return e4m3 ? launch_append<float, 64, SEGPT_POOL_E4M3>(a, st) : launch_append<float, 64, SEGPT_POOL_E2M1>(a, st);
   return e4m3 ? launch_append<float, 128, SEGPT_POOL_E4M3>(a, st) : launch_append<float, 128, SEGPT_POOL_E2M1>(a, st);
 }
@@ -316,8 +331,7 @@ int segpt_paged_read(const segpt_paged_params* p, const segpt_paged_quant* q, vo
     using E = decltype(elem);
     constexpr int D = decltype(dim)::value;
     if (format == 0) return launch_read<E, D, 0>(a, st);
-    if constexpr (D >= 64) return format == SEGPT_POOL_E4M3 ? launch_read<E, D, SEGPT_POOL_E4M3>(a, st) : launch_read<E, D, SEGPT_POOL_E2M1>(a, st);
-    else return (int)SEGPT_E_HEAD_DIM;
+    return format == SEGPT_POOL_E4M3 ? launch_read<E, D, SEGPT_POOL_E4M3>(a, st) : launch_read<E, D, SEGPT_POOL_E2M1>(a, st);
   };
   if (p->dtype == SEGPT_DTYPE_BF16) return p->D == 64 ? go(uint16_t{}, std::integral_constant<int, 64>{}) : go(uint16_t{}, std::integral_constant<int, 128>{});
   return p->D == 32 ? go(0.f, std::integral_constant<int, 32>{}) : p->D == 64 ? go(0.f, std::integral_constant<int, 64>{}) : go(0.f, std::integral_constant<int, 128>{});

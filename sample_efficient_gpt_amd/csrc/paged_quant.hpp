@@ -11,6 +11,7 @@ struct QuantArgs {
   segpt_tensor4 k_scales, v_scales;
 };
 int check_quant(const segpt_paged_params* p, const segpt_paged_quant* q, PagedCall call);
+bool quant_head_dim(const segpt_paged_params& p);
 
 constexpr int kLeastExponent = -110;  // of a scale: the smallest code times it is a normal bf16 number
 constexpr int kNoNumber = 255;        // scale of a block with a component that cannot be held

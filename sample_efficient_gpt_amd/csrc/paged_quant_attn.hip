@@ -159,11 +159,13 @@ struct RowPart {
 template <int D>
 __device__ __forceinline__ uint32_t load_scales(const char* at) {  // D / 32 bytes, aligned to them
   if constexpr (D == 128) return *reinterpret_cast<const uint32_t*>(at);
-  else return *reinterpret_cast<const uint16_t*>(at);
+  else if constexpr (D == 64) return *reinterpret_cast<const uint16_t*>(at);
+  else return *reinterpret_cast<const uint8_t*>(at);
 }
 template <int BYTES>
 __device__ __forceinline__ void load_words(const char* at, uint32_t* w) {
   if constexpr (BYTES == 16) { const u32x4 x = *reinterpret_cast<const u32x4*>(at); w[0] = x[0]; w[1] = x[1]; w[2] = x[2]; w[3] = x[3]; }
+  else if constexpr (BYTES == 4) w[0] = *reinterpret_cast<const uint32_t*>(at);
   else { const u32x2 x = *reinterpret_cast<const u32x2*>(at); w[0] = x[0]; w[1] = x[1]; }
 }
 __device__ __forceinline__ float scale_at(uint32_t scales, int block) { return __uint_as_float((scales >> (8 * block) & 255u) << 23); }
@@ -227,7 +229,7 @@ template <int D, int FMT>
 struct Quarter {
   static constexpr int kBytes = Codes<FMT>::row_bytes(D) / 4;   // of a lane
   static constexpr int P = kBytes < 16 ? kBytes : 16, NP = kBytes / P, kWords = kBytes / 4;
-  static constexpr int EP = P * 8 / Codes<FMT>::kBits;          // components of a piece: 16 or 32, of one block
+  static constexpr int EP = P * 8 / Codes<FMT>::kBits;          // components of a piece: 8, 16 or 32, of one block
   static constexpr int KS = D / 32;                             // steps of the product
   static constexpr int kWordsOf8 = Codes<FMT>::kBits / 4;       // words of eight components
   static __device__ __forceinline__ int component(int step, int quarter) { return (step * 8 / EP) * 4 * EP + quarter * EP + step * 8 % EP; }
@@ -246,6 +248,9 @@ struct Quarter {
     }
   }
 };
+// Rows of 32 components lie in LDS as the first halves of rows of 64.
+template <int D>
+constexpr int kTileDim = D < 64 ? 64 : D;
 // The values of a block of 32 keys in LDS, bf16: chunk c (16 bytes) of row r lies at chunk c ^ f(r).  Sixteen lanes write one chunk of 16 rows, and a
 // transposing read takes two chunks of eight rows at a time; as groups of sixteen lanes both meet all banks once.  (Two fifths of the LDS cycles are counted
 // as conflicts all the same; the LDS is busy for 17 % of the time at head_dim 64, 30 % at 128.)
@@ -276,14 +281,15 @@ __device__ __forceinline__ void lds_write16(uint32_t addr, u32x4 v) { *(__attrib
 template <typename E, int D, int FMT>
 struct Query16 {
   using L = Quarter<D, FMT>;
-  static constexpr int KS = L::KS, kCols = 16, kLogCols = 4, PARTS = kQueryParts<E>, N = D / 64;
+  static constexpr int KS = L::KS, kCols = 16, kLogCols = 4, PARTS = kQueryParts<E>, N = D < 64 ? 1 : D / 64;
   bf16x8 part[PARTS][KS];
   Eight<E> raw[2][N];
-  float cs[N][8], sn[N][8];  // pairs (quarter * N + n) * 8 .. + 7
+  float cs[N][8], sn[N][8];  // pairs of(quarter, n) .. + 7
+  static __device__ __forceinline__ int of(int quarter, int n) { return D < 64 ? (quarter & 1) * 8 : (quarter * N + n) * 8; }  // 16 pairs: twice each
   __device__ __forceinline__ void fetch(const segpt_paged_params& p, const E* at, int64_t angle, int quarter) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int j = (quarter * N + n) * 8;
+      const int j = of(quarter, n);
       raw[0][n].load(at + j);
       raw[1][n].load(at + j + D / 2);
       if (p.rope_cos) {
@@ -293,7 +299,7 @@ struct Query16 {
     }
   }
   __device__ __forceinline__ void finish(const segpt_paged_params& p, bool live, int lane, const float* gsm, uint32_t lds) {
-    using V = ValueTile<D>;
+    using V = ValueTile<kTileDim<D>>;
     const int quarter = lane >> 4, col = lane & 15;
     float x[2][N][8];
 #pragma unroll
@@ -315,7 +321,7 @@ struct Query16 {
         for (int t = 0; t < 8; ++t) sq[t % 4] += x[h][n][t] * x[h][n][t];
     float ss = (sq[0] + sq[1]) + (sq[2] + sq[3]);
     ss += __shfl_xor(ss, 16, 64);
-    ss = half_sum(ss);
+    if (D >= 64) ss = half_sum(ss);
     const float alpha = !live ? 0.f : (p.flags & SEGPT_FLAG_NO_NORM) ? 1.f : 1.0f / sqrtf(ss * (1.0f / D) + p.eps);
     u32x4 w[PARTS][2][N];
 #pragma unroll
@@ -323,7 +329,7 @@ struct Query16 {
 #pragma unroll
       for (int n = 0; n < N; ++n) {
         float g[8];
-        load8(gsm + (quarter * N + n) * 8 + h * (D / 2), g);
+        load8(gsm + of(quarter, n) + h * (D / 2), g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           uint32_t part_i[PARTS];
@@ -337,7 +343,7 @@ struct Query16 {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int n = 0; n < N; ++n) lds_write16(lds + V::write_at(col, quarter * N + n + h * (D / 16)), w[u][h][n]);
+        for (int n = 0; n < N; ++n) lds_write16(lds + V::write_at(col, of(quarter, n) / 8 + h * (D / 16)), w[u][h][n]);
       wave_sync();
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) part[u][ks] = as_bf16x8(lds_read16(lds + V::write_at(col, L::component(ks, quarter) / 8)));
@@ -400,7 +406,7 @@ __device__ __forceinline__ void add_odd_values(const Item& it, const Column& c, 
 template <typename E, int D, int FMT, int AHEAD>
 __device__ __forceinline__ void few_columns(const QuantArgs& qa, const PagedArgs& a, const Item& it, int rep, int lane, uint32_t lds, float* gsm) {
   using L = Quarter<D, FMT>;
-  using V = ValueTile<D>;
+  using V = ValueTile<kTileDim<D>>;
   constexpr int KS = L::KS, DB = D / 16, PARTS = kQueryParts<E>;
   const segpt_paged_params& p = a.p;
   const int quarter = lane >> 4, r16 = lane & 15;
@@ -408,9 +414,9 @@ __device__ __forceinline__ void few_columns(const QuantArgs& qa, const PagedArgs
   // one round trip: gain, query rows and angles, page numbers
   Walk<16, 16, false> walk;
   walk.start(a, it, 0, 2 * blocks, lane, 0);
-  Gain gain[D / 64];
+  Gain gain[(D + 63) / 64];
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) gain[i] = fetch_gain(p, 64 * i + lane);
+  for (int i = 0; i < (D + 63) / 64; ++i) gain[i] = fetch_gain(p, (64 * i + lane) % D);
   Query16<E, D, FMT> q;
   const Column c = column_of<E, D>(a, it, rep, it.tile * kFew, lane, q);
   Source<D, L::NP, L::P> src;
@@ -426,7 +432,8 @@ __device__ __forceinline__ void few_columns(const QuantArgs& qa, const PagedArgs
   walk.work_out(qa, a, lane);
   if (blocks > 0) ask(b0, 0);
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) gsm[64 * i + lane] = scale_of(p, gain[i]);
+  for (int i = 0; i < (D + 63) / 64; ++i)
+    if (64 * i + lane < D) gsm[64 * i + lane] = scale_of(p, gain[i]);
   wave_sync();
   q.finish(p, c.live, lane, gsm, lds);
   if (AHEAD == 2 && blocks > 1) ask(b1, 1);
@@ -546,8 +553,9 @@ __device__ __forceinline__ void few_columns(const QuantArgs& qa, const PagedArgs
 // 0.94 PFLOP/s with the queries' second part; 512 rows beside 31 tokens, 100 .. 8192 keys: 62 us, vector instructions half of it, matrix a quarter.
 template <int D>
 struct ManyShape {
-  static constexpr int kBK = D == 64 ? 64 : 32, kTileBytes = kBK * 2 * D, kStageBytes = 2 * kTileBytes, kStages = 3;
-  static constexpr int kLanes = D / 16, kRows = 64 / kLanes;  // lanes of a row (16 components each), rows of a wave
+  static constexpr int kBK = D == 128 ? 32 : 64, kRB = 2 * kTileDim<D>, kTileBytes = kBK * kRB, kStageBytes = 2 * kTileBytes, kStages = 3;
+  static constexpr int kPart = D == 32 ? 8 : 16, kLanes = D / kPart, kRows = 64 / kLanes;  // components of a lane, lanes of a row, rows of a wave
+  static_assert(4 * kRows == kBK);
 };
 template <typename E, int D>
 struct Query32 {
@@ -644,7 +652,7 @@ __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArg
                                              int* any_bad) {
   using S = ManyShape<D>;
   constexpr int BK = S::kBK, N = BK / 32, MB = D / 32, KS = D / 16, PARTS = kQueryParts<E>, PROBS = sizeof(E) == 2 ? 1 : 3;
-  constexpr int P = 16 * Codes<FMT>::kBits / 8;  // bytes of a lane's 16 components
+  constexpr int P = S::kPart * Codes<FMT>::kBits / 8, TD = kTileDim<D>;  // P: bytes of a lane's components
   const segpt_paged_params& p = a.p;
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
   const int own_row = lane / S::kLanes, own_part = lane % S::kLanes, n_kt = (it.nk + BK - 1) / BK;
@@ -665,14 +673,14 @@ __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArg
   };
   auto put = [&](const Raw2& x, int jt, uint32_t stage) {
     if (jt >= n_kt) return;
-    const int row = wave * S::kRows + own_row, f = Swz<D>::f(row);
+    const int row = wave * S::kRows + own_row, f = Swz<TD>::f(row);
     auto tensor = [&](const RowPart<P / 4>& r, uint32_t at) {
-      const float scale = scale_at(r.s, own_part / 2);
+      const float scale = scale_at(r.s, own_part * S::kPart / SEGPT_SCALE_BLOCK);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < S::kPart / 8; ++u) {
         uint32_t w[4];
-        decode8<FMT>(r.w + u * (P / 8), scale, w);
-        lds_write16(at + row * S::kTileBytes / BK + (((2 * own_part + u) ^ f) << 4), u32x4{w[0], w[1], w[2], w[3]});
+        decode8<FMT>(r.w + u * (Codes<FMT>::kBits / 4), scale, w);
+        lds_write16(at + row * S::kRB + (((S::kPart / 8 * own_part + u) ^ f) << 4), u32x4{w[0], w[1], w[2], w[3]});
       }
     };
     tensor(x.k, lds + stage);
@@ -688,17 +696,17 @@ __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArg
   put(x, 0, 0);
   ask(x, 2);
   put(x1, 1, S::kStageBytes);
-  std::conditional_t<D == 64, State<MB>, StateLess<MB>> st;
+  std::conditional_t<D != 128, State<MB>, StateLess<MB>> st;
   st.clear();
   bool odd = false;
   typedef f32x16 Scores[1];
   // Keys of the block after this one: at head_dim 64 read as soon as they are there, beside the decoding of a later tile's codes; at 128 there are no
   // registers for that (with them in scratch six prompts take 301 us instead of 288).
-  constexpr bool EARLY = D == 64;
+  constexpr bool EARLY = D != 128;
   typedef bf16x8 Keys[KS];
   auto read_keys = [&](uint32_t block, Keys& k) {
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) k[ks] = swz_frag_rm<D>(lds + block + swz_off_rm<D>(lane), 0, ks);
+    for (int ks = 0; ks < KS; ++ks) k[ks] = swz_frag_rm<TD>(lds + block + swz_off_rm<TD>(lane), 0, ks);
   };
   auto scores = [&](bool masked, const Keys& k, Scores& s, int jb) {  // of the block of 32 keys k, jb on from k0
     s[0] = st.less;
@@ -729,7 +737,7 @@ __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArg
     for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) {
-        u32x4 v = __builtin_bit_cast(u32x4, swz_frag_tr<D>(lds + block + S::kTileBytes + swz_off_tr<D>(lane), mb, s2));
+        u32x4 v = __builtin_bit_cast(u32x4, swz_frag_tr<TD>(lds + block + S::kTileBytes + swz_off_tr<TD>(lane), mb, s2));
         if (masked) odd |= clear_odd(v);
 #pragma unroll
         for (int u = PROBS - 1; u >= 0; --u) st.o[mb] = mfma32(as_bf16x8(v), as_bf16x8(pb[u][s2]), st.o[mb]);
@@ -762,17 +770,17 @@ __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArg
   // block b of s, and the scores of the next one beside it; HALF: b is the first of a tile of two
   auto whole = [&](auto half, Scores& s, Scores& ahead) {
     constexpr bool HALF = decltype(half)::value != 0;
-    if (!EARLY || !HALF) read_keys(HALF ? stage + 64 * D : stage_from(1), ahead_k);
+    if (!EARLY || !HALF) read_keys(HALF ? stage + 32 * S::kRB : stage_from(1), ahead_k);
     scores(false, ahead_k, ahead, 0);
-    products(false, HALF || N == 1 ? stage : stage + 64 * D, s);
+    products(false, HALF || N == 1 ? stage : stage + 32 * S::kRB, s);
     st.raise(ahead);
     if (!HALF) stage = stage_from(1);
   };
   auto any = [&](auto half, int b, Scores& s, Scores& ahead) {
     constexpr bool HALF = decltype(half)::value != 0;
-    if (active(b)) products(b >= n_whole, HALF || N == 1 ? stage : stage + 64 * D, s);
+    if (active(b)) products(b >= n_whole, HALF || N == 1 ? stage : stage + 32 * S::kRB, s);
     if (active(b + 1)) {
-      if (!EARLY || !HALF) read_keys(HALF ? stage + 64 * D : stage_from(1), ahead_k);
+      if (!EARLY || !HALF) read_keys(HALF ? stage + 32 * S::kRB : stage_from(1), ahead_k);
       scores(true, ahead_k, ahead, (b + 1) * 32);
       st.raise(ahead);
     }
@@ -781,13 +789,13 @@ __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArg
   // two blocks a round, so that the scores change places without being copied
   int b = 0;
   for (; b + 2 < n_whole; b += 2) {
-    turn(b / N, N == 2 ? stage + 64 * D : stage_from(1));
+    turn(b / N, N == 2 ? stage + 32 * S::kRB : stage_from(1));
     whole(IC<N == 2>{}, s0, s1);
     if (N == 1) turn(b + 1, stage_from(1));
     whole(IC<0>{}, s1, s0);
   }
   for (; b < n_blocks; b += 2) {
-    turn(b / N, N == 2 ? stage + 64 * D : stage_from(1));
+    turn(b / N, N == 2 ? stage + 32 * S::kRB : stage_from(1));
     any(IC<N == 2>{}, b, s0, s1);
     if (b + 1 >= n_blocks) break;
     if (N == 1) turn(b + 1, stage_from(1));
@@ -804,11 +812,11 @@ __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArg
 
 // Launches whose entries are all FEW: a workgroup is one wave
 template <int D>
-constexpr int kFewWaves = D == 64 ? 3 : 2;  // waves a SIMD that registers leave room for (128 tokens of up to 3000 keys: 62 us with two, 53)
+constexpr int kFewWaves = D == 128 ? 2 : 3;  // waves a SIMD that registers leave room for (128 tokens of up to 3000 keys: 62 us with two, 53)
 template <typename E, int D, int FMT>
 __global__ __launch_bounds__(64, kFewWaves<D>) void paged_quant_few_kernel(Args args) {
   const PagedArgs& a = args.w;
-  __shared__ __attribute__((aligned(1024))) char lds[ValueTile<D>::kBytes];
+  __shared__ __attribute__((aligned(1024))) char lds[ValueTile<kTileDim<D>>::kBytes];
   __shared__ __attribute__((aligned(16))) float gsm[D];
   const int lane = threadIdx.x, rep = a.rep.d;
   clear_rest<E>(a, lane, 64, D);
@@ -826,10 +834,10 @@ __global__ __launch_bounds__(64, kFewWaves<D>) void paged_quant_few_kernel(Args 
 
 // Any launch: the first workgroups are items of many columns, the next four items each of few, the rest have none
 template <typename E, int D, int FMT>
-__global__ __launch_bounds__(256, (sizeof(E) == 2 || D == 64 ? 2 : 1)) void paged_quant_any_kernel(Args args) {
+__global__ __launch_bounds__(256, (sizeof(E) == 2 || D != 128 ? 2 : 1)) void paged_quant_any_kernel(Args args) {
   const PagedArgs& a = args.w;
   using S = ManyShape<D>;
-  constexpr int kLds = std::max(S::kStages * S::kStageBytes, 4 * ValueTile<D>::kBytes);
+  constexpr int kLds = std::max(S::kStages * S::kStageBytes, 4 * ValueTile<kTileDim<D>>::kBytes);
   __shared__ __attribute__((aligned(1024))) char lds[kLds];
   __shared__ __attribute__((aligned(16))) float gsm[4][D];
   __shared__ __attribute__((aligned(16))) char places[4 * Walk<S::kRows, S::kBK, true>::kBytes];
@@ -847,7 +855,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 2 || D == 64 ? 2 : 1)) void page
   } else {
     const Item it4 = locate<false>(a, lane, rep, share, mine, ((int)blockIdx.x - it.x.base) * 4 + wave);
     if (!it4.valid) return;
-    few_columns<E, D, FMT, 2>(qa, a, it4, rep, lane, lds_addr_of(lds) + wave * ValueTile<D>::kBytes, gsm[wave]);
+    few_columns<E, D, FMT, 2>(qa, a, it4, rep, lane, lds_addr_of(lds) + wave * ValueTile<kTileDim<D>>::kBytes, gsm[wave]);
   }
 }
 
@@ -859,7 +867,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 2 || D == 64 ? 2 : 1)) void page
 int target_of(const segpt_paged_params& p) {
   const int rep = p.H / p.Hkv;
   const bool wide = p.prefix_table || (!p.seq_start && (int64_t)rep * (p.T / p.B) > kMostFew);
-  if (all_few(p)) return p.D == 64 ? 744 : 496;
+  if (all_few(p)) return p.D == 128 ? 496 : 744;
   return wide ? 384 : p.seq_start ? 480 : 496;
 }
 
@@ -883,7 +891,7 @@ extern "C" {
 size_t segpt_paged_quant_workspace_bytes(const segpt_paged_params* p, const segpt_paged_quant* q) {
   using namespace segpt;
   if (check_paged_sizes(p, PagedCall::kAttend) != SEGPT_OK || !q || q->struct_bytes != sizeof(segpt_paged_quant)) return 0;
-  if ((q->format != SEGPT_POOL_E4M3 && q->format != SEGPT_POOL_E2M1) || (p->D != 64 && p->D != 128)) return 0;
+  if ((q->format != SEGPT_POOL_E4M3 && q->format != SEGPT_POOL_E2M1) || !quant_head_dim(*p)) return 0;
   PagedArgs a{};
   const size_t n = plan(*p, a, target_of(*p));
   return n > SIZE_MAX - 256 ? 0 : up256(n);
@@ -901,6 +909,7 @@ int segpt_paged_attn_quant(const segpt_paged_params* p, const segpt_paged_quant*
     if (p->D == 64) return e4m3 ? launch<uint16_t, 64, SEGPT_POOL_E4M3>(args, st) : launch<uint16_t, 64, SEGPT_POOL_E2M1>(args, st);
     return e4m3 ? launch<uint16_t, 128, SEGPT_POOL_E4M3>(args, st) : launch<uint16_t, 128, SEGPT_POOL_E2M1>(args, st);
   }
+  if (p->D == 32) return e4m3 ? launch<float, 32, SEGPT_POOL_E4M3>(args, st) : launch<float, 32, SEGPT_POOL_E2M1>(args, st);
   if (p->D == 64) return e4m3 ? launch<float, 64, SEGPT_POOL_E4M3>(args, st) : launch<float, 64, SEGPT_POOL_E2M1>(args, st);
   return e4m3 ? launch<float, 128, SEGPT_POOL_E4M3>(args, st) : launch<float, 128, SEGPT_POOL_E2M1>(args, st);
 }

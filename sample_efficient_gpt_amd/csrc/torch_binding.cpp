@@ -579,7 +579,7 @@ void fill_paged(segpt_paged_params& p, const Tensor& rows, const char* name, con
   p.n_pages = (int32_t)k_pages.size(0); p.page_size = (int32_t)k_pages.size(2);
   p.table_width = (int32_t)table.size(1);
   p.max_len = max_len.has_value() ? (int32_t)std::min<int64_t>(*max_len, INT32_MAX) : 0;
-  p.flags = qk_norm ? 0 : SEGPT_FLAG_NO_NORM;
+  p.flags = (qk_norm ? 0 : SEGPT_FLAG_NO_NORM) | (scales.any() ? SEGPT_FLAG_HEAD_32 : 0);
   p.eps = (float)eps;
   p.k_pages = view4(k_pages, 0); p.v_pages = view4(v_pages, 0);
   p.block_table = ptr_of<int32_t>(table);

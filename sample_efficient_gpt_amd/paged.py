@@ -24,7 +24,7 @@ components with one power of two each: twice or four times as many keys in the s
   with which no component exceeds the largest code (448, 6).  255: the block is NaN, as one with a component that is not finite becomes.
 
 A component is the nearest code of its exact value, ties to the even one.  What is attended to is the stored value, exactly.  Rows may be bfloat16 or
-float32, head_dim 64 or 128.
+float32, head_dim 64 or 128, with float32 rows also 32.
 """
 
 from __future__ import annotations
@@ -264,7 +264,7 @@ def paged_kv_read(k_pages, v_pages, block_table, kv_len, rows, *, seq_start=None
     for the same pages (pages, scales, tables, lengths and row ranges as there).  Row i of n of sequence b is its key ``kv_len[b] - n + i``;
     rows is the number of all rows, ``seq_start[-1]`` or a multiple of the sequences.
 
-    dtype: of the rows; bfloat16 by default, or float32 (both exact) where the pages have scales, else the pages' own.  out: a pair of tensors to write to
+    dtype: of the rows; bfloat16 by default, or float32 (both exact; heads of 32 are float32) where the pages have scales, else the pages' own.  out: a pair of tensors to write to
     (any strides, last dim contiguous, rows 16 B aligned; no overlap with inputs or each other, RuntimeError), whose dtype counts.
 
     A row before its sequence's first key is 0.  A sequence whose length is negative or above max_len gives NaN, and so does a row whose page number is
@@ -429,6 +429,8 @@ class PagedKVCache:
         for n in t.lengths[first:end]:
             starts.append(starts[-1] + n)
         seq_start = torch.tensor(starts, dtype=torch.int32).to(t.kv_len.device)
+        if dtype is None and self.k_scales is not None and self.head_dim == 32:
+            dtype = torch.float32  # the only rows of 32 that there are
         k, v = paged_kv_read(self.k_pages, self.v_pages, t.block_table[first:end], t.kv_len[first:end], starts[-1], seq_start=seq_start, k_scales=self.k_scales,
                              v_scales=self.v_scales, dtype=dtype, max_len=t.max_len)
         return k, v, seq_start
@@ -439,7 +441,7 @@ class PagedKVCache:
         if dtype == self.dtype:
             return self
         other = PagedKVCache(self.pages, self.k_pages.shape[1], self.head_dim, dtype)
-        rows = dtype if other.k_scales is None else torch.float32 if self.dtype == torch.float32 else torch.bfloat16
+        rows = dtype if other.k_scales is None else torch.float32 if self.dtype == torch.float32 or self.head_dim == 32 else torch.bfloat16
         for t in (self.pages, self.pages.prefix):
             if t is None:
                 continue

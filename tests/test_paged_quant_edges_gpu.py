@@ -13,7 +13,7 @@ pytestmark = pytest.mark.gpu
 
 
 @both_formats
-@pytest.mark.parametrize("H,Hkv,D,dtype", [(6, 2, 64, BF16), (4, 2, 128, BF16), (4, 2, 64, F32), (4, 2, 128, F32)])
+@pytest.mark.parametrize("H,Hkv,D,dtype", [(6, 2, 64, BF16), (4, 2, 128, BF16), (4, 2, 32, F32), (4, 2, 64, F32), (4, 2, 128, F32)])
 @pytest.mark.parametrize("page", [8, 16, 32, 64])
 @pytest.mark.parametrize("prefix", [0, 45])
 def test_a_bad_page_number_reaches_every_row_that_sees_it(gpu_device, H, Hkv, D, dtype, page, prefix, fmt):
@@ -40,7 +40,7 @@ def test_a_bad_page_number_reaches_every_row_that_sees_it(gpu_device, H, Hkv, D,
 
 
 @pytest.mark.parametrize("fmt,kind", [("e4m3", "nan"), ("e4m3", "-nan"), ("e4m3", "large"), ("e2m1", "large")])
-@pytest.mark.parametrize("H,Hkv,D,dtype", [(6, 2, 64, BF16), (4, 2, 128, BF16), (4, 2, 64, F32), (4, 2, 128, F32)])
+@pytest.mark.parametrize("H,Hkv,D,dtype", [(6, 2, 64, BF16), (4, 2, 128, BF16), (4, 2, 32, F32), (4, 2, 64, F32), (4, 2, 128, F32)])
 @pytest.mark.parametrize("rows,lens,prefix", [([1, 1], [37, 64], 0), ([70, 1], [70, 40], 0), ([45, 3], [300, 50], 0), ([1, 50], [5, 50], 40)])
 def test_a_value_that_is_none_by_its_code(gpu_device, rows, lens, prefix, H, Hkv, D, dtype, fmt, kind):
     """Pools that something else filled: the code that is NaN in 8 bits, and a scale that carries codes beyond the largest number.  Wherever the key stands
@@ -53,12 +53,12 @@ def test_a_value_that_is_none_by_its_code(gpu_device, rows, lens, prefix, H, Hkv
             page, slot = int(x.block_table[b, p // 16]), p % 16
             was = codes[page, 1, slot].clone(), x.v_scales[page, 1, slot].clone()
             if kind == "large":  # a whole block, beyond what bf16 and fp32 hold
-                codes[page, 1, slot, 32 * codes.shape[3] // D:] = 0x7E if fmt == "e4m3" else 0x77
-                x.v_scales[page, 1, slot, 1:] = 254
-                none = torch.arange(D) >= 32
+                codes[page, 1, slot, (D - 32) * codes.shape[3] // D:] = 0x7E if fmt == "e4m3" else 0x77
+                x.v_scales[page, 1, slot, -1] = 254
+                none = torch.arange(D) >= D - 32
             else:
-                codes[page, 1, slot, 37] = 0x7F if kind == "nan" else 0xFF
-                none = torch.arange(D) == 37
+                codes[page, 1, slot, D - 27] = 0x7F if kind == "nan" else 0xFF
+                none = torch.arange(D) == D - 27
             y = attend(x)
             codes[page, 1, slot], x.v_scales[page, 1, slot] = was
             first, end = x.starts[b] + max(0, p - (L - n)), x.starts[b + 1]

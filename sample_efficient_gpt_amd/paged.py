@@ -372,28 +372,23 @@ class PagedKVCache:
     """Pages of keys and values of one layer, ``[n_pages, Hkv, page size, D]`` each, under a ``PageTable`` that all layers share.
 
     dtype: bfloat16 or float32, that of the rows; or float8_e4m3fn or float4_e2m1fn_x2, for rows of either: pages of 8 or 4 bits, with ``k_scales`` and
-    ``v_scales`` beside them.  Pools that are handed in say themselves what they are: their type and shape count, of their own number of pages.
+    ``v_scales`` beside them.
 
     A step: ``pages.extend(rows)`` once, then for every layer ``append`` and ``attend`` (``MultiHeadSelfAttention`` does both when it is given
     the cache).  ``of(table)`` is the same pool under another table, as ``cache.of(pages.prefix)`` to fill the shared prefix.  ``read()`` is what it
     holds; ``to(dtype)`` is a cache of another dtype with the same keys and values, as of a prompt that was worked out in bfloat16 and goes on at 4 bits."""
 
     def __init__(self, pages, n_kv_heads, head_dim, dtype=torch.bfloat16, k_pages=None, v_pages=None, k_scales=None, v_scales=None):
-        self.pages = pages
-        device = pages.kv_len.device
-        if k_pages is None:
-            row = head_dim // 2 if dtype == torch.float4_e2m1fn_x2 else head_dim
-            k_pages = torch.empty(pages.n_pages, n_kv_heads, pages.page_size, row, dtype=dtype, device=device)
-        self.k_pages = k_pages
-        self.v_pages = torch.empty(k_pages.shape, dtype=k_pages.dtype, device=device) if v_pages is None else v_pages
-        if self.v_pages.shape != k_pages.shape or self.v_pages.dtype != k_pages.dtype:
-            raise ValueError(f"the pages must be alike, got {tuple(k_pages.shape)} of {k_pages.dtype} and {tuple(self.v_pages.shape)} of {self.v_pages.dtype}")
-        if k_pages.shape[2] != pages.page_size:
-            raise ValueError(f"the table has a page size of {pages.page_size}, the pool one of {k_pages.shape[2]}")
-        self.head_dim = k_pages.shape[3] * (2 if k_pages.dtype == torch.float4_e2m1fn_x2 else 1)
+        self.pages, self.head_dim = pages, head_dim
+        device, rows = pages.kv_len.device, (pages.n_pages, n_kv_heads, pages.page_size)
+        shape = (*rows, head_dim // 2 if dtype == torch.float4_e2m1fn_x2 else head_dim)
+        self.k_pages = torch.empty(shape, dtype=dtype, device=device) if k_pages is None else k_pages
+        self.v_pages = torch.empty(shape, dtype=dtype, device=device) if v_pages is None else v_pages
+        if self.k_pages.shape != shape or self.v_pages.shape != shape:
+            raise ValueError(f"pages must be {shape}, got {tuple(self.k_pages.shape)} and {tuple(self.v_pages.shape)}")
         self.k_scales = self.v_scales = None
-        if k_pages.dtype in (torch.float8_e4m3fn, torch.float4_e2m1fn_x2):
-            shape = (*k_pages.shape[:3], self.head_dim // 32)
+        if dtype in (torch.float8_e4m3fn, torch.float4_e2m1fn_x2):
+            shape = (*rows, head_dim // 32)
             self.k_scales = torch.empty(shape, dtype=torch.uint8, device=device) if k_scales is None else k_scales
             self.v_scales = torch.empty(shape, dtype=torch.uint8, device=device) if v_scales is None else v_scales
             if self.k_scales.shape != shape or self.v_scales.shape != shape:

@@ -371,21 +371,27 @@ _ROWS_AT_ONCE = 1 << 18  # of a cache that is turned into one of another dtype
 class PagedKVCache:
     """Pages of keys and values of one layer, ``[n_pages, Hkv, page size, D]`` each, under a ``PageTable`` that all layers share.
 
-    dtype: bfloat16 or float32, that of the rows; or float8_e4m3fn or float4_e2m1fn_x2, for rows of either: pages of 8 or 4 bits, with ``k_scales`` and
-    ``v_scales`` beside them.
+    dtype: bfloat16 or float32, that of the rows; or float8_e4m3fn or float4_e2m1fn_x2 (or uint8, the same), for rows of either: pages of 8 or 4 bits, with
+    ``k_scales`` and ``v_scales`` beside them.  Pools that are handed in are of the table's shape; codes say themselves what they are.
 
     A step: ``pages.extend(rows)`` once, then for every layer ``append`` and ``attend`` (``MultiHeadSelfAttention`` does both when it is given
     the cache).  ``of(table)`` is the same pool under another table, as ``cache.of(pages.prefix)`` to fill the shared prefix.  ``read()`` is what it
     holds; ``to(dtype)`` is a cache of another dtype with the same keys and values, as of a prompt that was worked out in bfloat16 and goes on at 4 bits."""
 
     def __init__(self, pages, n_kv_heads, head_dim, dtype=torch.bfloat16, k_pages=None, v_pages=None, k_scales=None, v_scales=None):
+        if k_pages is not None and k_pages.dtype in (torch.uint8, torch.float8_e4m3fn, torch.float4_e2m1fn_x2):
+            dtype = k_pages.dtype  # pools say themselves what they are
+        if dtype == torch.uint8:
+            dtype = torch.float4_e2m1fn_x2  # two codes a byte, as in the functions
         self.pages, self.head_dim = pages, head_dim
         device, rows = pages.kv_len.device, (pages.n_pages, n_kv_heads, pages.page_size)
         shape = (*rows, head_dim // 2 if dtype == torch.float4_e2m1fn_x2 else head_dim)
         self.k_pages = torch.empty(shape, dtype=dtype, device=device) if k_pages is None else k_pages
-        self.v_pages = torch.empty(shape, dtype=dtype, device=device) if v_pages is None else v_pages
+        self.v_pages = torch.empty(shape, dtype=self.k_pages.dtype, device=device) if v_pages is None else v_pages
         if self.k_pages.shape != shape or self.v_pages.shape != shape:
             raise ValueError(f"pages must be {shape}, got {tuple(self.k_pages.shape)} and {tuple(self.v_pages.shape)}")
+        if self.k_pages.dtype != self.v_pages.dtype:
+            raise ValueError(f"pages must have one dtype, got {self.k_pages.dtype} and {self.v_pages.dtype}")
         self.k_scales = self.v_scales = None
         if dtype in (torch.float8_e4m3fn, torch.float4_e2m1fn_x2):
             shape = (*rows, head_dim // 32)
@@ -393,10 +399,13 @@ class PagedKVCache:
             self.v_scales = torch.empty(shape, dtype=torch.uint8, device=device) if v_scales is None else v_scales
             if self.k_scales.shape != shape or self.v_scales.shape != shape:
                 raise ValueError(f"scales must be {shape}, got {tuple(self.k_scales.shape)} and {tuple(self.v_scales.shape)}")
+        elif k_scales is not None or v_scales is not None:
+            raise ValueError(f"pages of {dtype} have no scales")
 
     @property
     def dtype(self):
-        return self.k_pages.dtype
+        """float4_e2m1fn_x2 also where the pages are bytes."""
+        return torch.float4_e2m1fn_x2 if self.k_pages.dtype == torch.uint8 else self.k_pages.dtype
 
     def of(self, pages):
         return PagedKVCache(pages, self.k_pages.shape[1], self.head_dim, self.dtype, self.k_pages, self.v_pages, self.k_scales, self.v_scales)
@@ -438,6 +447,8 @@ class PagedKVCache:
     def to(self, dtype):
         """A cache of this dtype in pages of its own, under the same table and with the same keys and values (the shared prefix's among them).  Rows
         pass through memory of their own, some sequences at a time."""
+        if dtype == torch.uint8:
+            dtype = torch.float4_e2m1fn_x2
         if dtype == self.dtype:
             return self
         other = PagedKVCache(self.pages, self.k_pages.shape[1], self.head_dim, dtype)

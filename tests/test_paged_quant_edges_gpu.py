@@ -7,7 +7,8 @@ import pytest
 import torch
 
 from paged_quant_util import QuantBatch
-from test_paged_quant_gpu import BF16, F32, attend, both_formats, read
+from sample_efficient_gpt_amd import PagedKVCache, PageTable
+from test_paged_quant_gpu import BF16, DTYPES, F32, attend, both_formats, read
 
 pytestmark = pytest.mark.gpu
 
@@ -94,3 +95,28 @@ def test_rows_back_from_codes_that_are_none(gpu_device):
     for dtype in (BF16, F32):
         v = read(x, dtype=dtype)[1][:, 0, :32]
         assert v[:2].isnan().all() and v[2:4].isinf().all() and (v[2] > 0).all() and (v[3] < 0).all() and v[4:].isfinite().all()
+
+
+@both_formats
+def test_a_cache_around_pools_of_bytes(gpu_device, fmt):
+    """Pools that a program made itself, as bytes where they are of 4 bits: under the prefix's table, turned into other types, attended to."""
+    pages = PageTable(2, 40, 8, prefix_len=19, device=gpu_device)
+    codes = [torch.empty(pages.n_pages, 2, 8, 64 if fmt == "e4m3" else 32, dtype=torch.uint8, device=gpu_device) for _ in "kv"]
+    scales = [torch.empty(pages.n_pages, 2, 8, 2, dtype=torch.uint8, device=gpu_device) for _ in "kv"]
+    mine = PagedKVCache(pages, 2, 64, DTYPES[fmt], *([t.view(DTYPES[fmt]) for t in codes] if fmt == "e4m3" else codes), *scales)
+    plain = PagedKVCache(pages, 2, 64, DTYPES[fmt])
+    g = torch.Generator().manual_seed(54)
+    n = lambda *s: torch.randn(*s, generator=g).to(BF16).to(gpu_device)
+    for table, rows in ((pages.prefix, 19), (pages, [30, 7])):
+        table.extend(rows)
+        k, v = n(table.rows, 2, 64), n(table.rows, 2, 64)
+        for c in (mine, plain):
+            c.of(table).append(k, v)
+    q = n(pages.rows, 6, 64)
+    gain = torch.ones(1, device=gpu_device)
+    assert torch.equal(mine.attend(q, gain), plain.attend(q, gain))
+    for dtype in (BF16, *DTYPES.values(), torch.uint8):
+        a, b = mine.to(dtype), plain.to(dtype)
+        assert a.dtype == b.dtype
+        for table in (pages, pages.prefix):
+            assert all(torch.equal(x, y) for x, y in zip(a.of(table).read()[:2], b.of(table).read()[:2]))

@@ -383,6 +383,9 @@ class PagedKVCache:
             dtype = k_pages.dtype  # pools say themselves what they are
         if dtype == torch.uint8:
             dtype = torch.float4_e2m1fn_x2  # two codes a byte, as in the functions
+        scaled = dtype in (torch.float8_e4m3fn, torch.float4_e2m1fn_x2)
+        if scaled and head_dim not in (32, 64, 128):
+            raise ValueError(f"pages of 8 and 4 bits have a head_dim of 32, 64 or 128, got {head_dim}")
         self.pages, self.head_dim = pages, head_dim
         device, rows = pages.kv_len.device, (pages.n_pages, n_kv_heads, pages.page_size)
         shape = (*rows, head_dim // 2 if dtype == torch.float4_e2m1fn_x2 else head_dim)
@@ -393,7 +396,7 @@ class PagedKVCache:
         if self.k_pages.dtype != self.v_pages.dtype:
             raise ValueError(f"pages must have one dtype, got {self.k_pages.dtype} and {self.v_pages.dtype}")
         self.k_scales = self.v_scales = None
-        if dtype in (torch.float8_e4m3fn, torch.float4_e2m1fn_x2):
+        if scaled:
             shape = (*rows, head_dim // 32)
             self.k_scales = torch.empty(shape, dtype=torch.uint8, device=device) if k_scales is None else k_scales
             self.v_scales = torch.empty(shape, dtype=torch.uint8, device=device) if v_scales is None else v_scales
@@ -451,6 +454,10 @@ class PagedKVCache:
             dtype = torch.float4_e2m1fn_x2
         if dtype == self.dtype:
             return self
+        if dtype not in (torch.bfloat16, torch.float32, torch.float8_e4m3fn, torch.float4_e2m1fn_x2):
+            raise ValueError(f"no cache has the dtype {dtype}")
+        if dtype == torch.bfloat16 and self.head_dim == 32:
+            raise ValueError("a head_dim of 32 is one of float32 rows")
         other = PagedKVCache(self.pages, self.k_pages.shape[1], self.head_dim, dtype)
         rows = dtype if other.k_scales is None else torch.float32 if self.dtype == torch.float32 or self.head_dim == 32 else torch.bfloat16
         for t in (self.pages, self.pages.prefix):

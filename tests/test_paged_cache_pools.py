@@ -51,3 +51,19 @@ def test_pools_that_do_not_fit_are_refused():
     rows = _pools(t.n_pages, 2, 16, 64, torch.bfloat16)
     with pytest.raises(ValueError, match="scales"):
         PagedKVCache(t, 2, 64, torch.bfloat16, *rows, torch.zeros(t.n_pages, 2, 16, 2, dtype=torch.uint8))
+
+
+def test_types_that_no_call_has_are_refused_before_anything_is_made():
+    c = PagedKVCache(PageTable(2, 40, 16, device="cpu"), 2, 64)
+    for dtype in (torch.float16, torch.int8, torch.float8_e5m2):
+        with pytest.raises(ValueError, match="dtype"):
+            c.to(dtype)
+    small = PagedKVCache(PageTable(2, 40, 16, device="cpu"), 2, 32, torch.float32)
+    assert small.to(E4M3).head_dim == 32
+    with pytest.raises(ValueError, match="head_dim"):
+        small.to(torch.bfloat16)
+    with pytest.raises(ValueError, match="head_dim"):
+        PagedKVCache(PageTable(2, 40, 16, device="cpu"), 2, 48, torch.float32).to(E4M3)
+    for d in (16, 48, 96, 256):
+        with pytest.raises(ValueError, match="head_dim"):
+            PagedKVCache(PageTable(2, 40, 16, device="cpu"), 2, d, E4M3)

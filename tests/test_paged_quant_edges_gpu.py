@@ -8,7 +8,7 @@ import torch
 
 from paged_quant_util import QuantBatch
 from sample_efficient_gpt_amd import PagedKVCache, PageTable
-from test_paged_quant_gpu import BF16, DTYPES, F32, attend, both_formats, read
+from test_paged_quant_gpu import BF16, DTYPES, F32, attend, both_formats, check_y, read
 
 pytestmark = pytest.mark.gpu
 
@@ -120,3 +120,33 @@ def test_a_cache_around_pools_of_bytes(gpu_device, fmt):
         assert a.dtype == b.dtype
         for table in (pages, pages.prefix):
             assert all(torch.equal(x, y) for x, y in zip(a.of(table).read()[:2], b.of(table).read()[:2]))
+
+
+# Items of more than 64 tiles: a wave goes through tiles of 16 keys (more than 32 columns a kv head: 64, at heads of 128 32) and works out the places of 64 at a
+# time.  How long an item is follows from the number of blocks of 32 keys, all tiles of columns and kv heads together, over 744 workgroups (heads of 128 496,
+# ragged rows 480): 100 to 150 tiles in the first two, 78 and 91 in the third.  All sequences have the same pages; some rows are looked at.
+@both_formats
+@pytest.mark.parametrize("page", [8, 64])
+@pytest.mark.parametrize("D,dtype", [(64, BF16), (128, BF16), (32, F32), (64, F32), (128, F32)])
+@pytest.mark.parametrize("kind", ["tokens", "ragged tokens", "prompt"])
+def test_items_of_more_tiles_than_a_wave_holds_places_for(gpu_device, kind, D, dtype, page, fmt):
+    if kind == "prompt":
+        H, Hkv, B, rows, lens = 32, 4, 1, [2500 if D == 128 else 4500], [2900 if D == 128 else 5000]
+    else:
+        H, Hkv, B = 8, 8, 64
+        rows, lens = [1] * 63 + [1 if kind == "tokens" else 2], [9600 - 3 * b for b in range(64)]
+    x = QuantBatch(fmt, rows[-1:], [max(lens)], H, Hkv, D, page, dtype, gpu_device, seed=55)
+    x.rows, x.lens = rows, lens
+    x.starts = [sum(rows[:b]) for b in range(B + 1)]
+    x.q = torch.randn(sum(rows), H, D, generator=torch.Generator().manual_seed(56)).to(dtype).to(gpu_device)
+    x.block_table, x.kv_len = x.block_table.repeat(B, 1), torch.tensor(lens, dtype=torch.int32, device=gpu_device)
+    x.seq_start = None if kind == "tokens" else torch.tensor(x.starts, dtype=torch.int32, device=gpu_device)
+    y, lse = attend(x, return_lse=True)
+    some = [(0, i) for i in (0, 1, rows[0] // 2, rows[0] - 1)] if kind == "prompt" else [(b, rows[b] - 1) for b in (0, 1, 40, 63)]
+    at = [x.starts[b] + i for b, i in some]
+    part = QuantBatch(fmt, [1] * 4, [1] * 4, H, Hkv, D, page, dtype, gpu_device)  # the same rows as sequences of their own
+    part.lens, part.q, part.block_table = [lens[b] - rows[b] + i + 1 for b, i in some], x.q[at], x.block_table[[b for b, _ in some]]
+    for name in ("g_q", "cos", "sin", "k_pages", "v_pages", "k_scales", "v_scales"):
+        setattr(part, name, getattr(x, name))
+    check_y(part, y[at], lse[at], part.attended())
+    assert torch.equal(y, attend(x))

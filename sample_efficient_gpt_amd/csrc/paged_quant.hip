@@ -98,7 +98,7 @@ __device__ __forceinline__ void store_codes(char* at, const uint32_t (&w)[2]) {
 // A row is D * sizeof(E) / 32 lanes, as in the append of whole numbers: a lane holds 16 bytes of the first half and the 16 bytes of the second half
 // that they rotate with, and the lanes of a block stand side by side.  Bound by what a wave waits for, one after the other: its sequence, the page number
 // and the angles, then the sum of squares and the blocks' largest.  One token 3.4 us; 16 ragged prompts of head_dim 128, 69 MB with the codes: 20.8 us,
-// 3.3 TB/s.  Fewer instructions for scales and codes did not change that.  (Eight bytes of each, so that every SIMD holds its eight waves and not four: the
+// 3.3 TB/s.  Fewer instructions for scales and codes did not change that.  At head_dim 32 both halves are of one block.  (Eight bytes of each, so that every SIMD holds its eight waves and not four: the
 // prompts below take 24.4 us, since a lane's share of finding its row and its block's scale does not halve.  Rows kept as stored and values first, for
 // five waves: 21.4.)
 template <typename E, int D, int FMT, bool ROPE, bool MIX>
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(kThreads) void paged_append_quant_kernel(QuantArgs 
 }
 
 // ---- stored rows back as rows.  FMT 0: rows of E.  A lane writes 16 bytes of a row of keys and of one of values; bound by the bytes that it moves.
-// Eight sequences of 28 .. 4,100 positions, head_dim 64, 91 MB with what is written: 19 us, 4.8 TB/s, the rate of a large copy.
+// Eight sequences of 1,641 .. 8,185 positions, head_dim 64, 91 MB with what is written: 19 us, 4.8 TB/s, the rate of a large copy.
 template <typename E, int D, int FMT>
 __global__ __launch_bounds__(kThreads) void paged_read_kernel(QuantArgs a, int log_page, int rows_each, int capacity) {
   const segpt_paged_params& p = a.p;

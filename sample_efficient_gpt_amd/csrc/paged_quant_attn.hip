@@ -223,7 +223,7 @@ struct Source {
 // whole by four lanes and is the A operand as it is decoded, no LDS in between: the components that a lane contributes to a step are not those of
 // the instruction's own order, but the queries' are the same, and a sum does not ask.  Probabilities go to the values in two bf16 parts, fp32 rows' in
 // three.  One or two blocks of codes are under way while another is worked on.  32 tokens of 18 / 6 heads of 64, 200 .. 8192 keys, 8 bits: 25.5 us, 110 MB at
-// 4.3 TB/s; 48 tokens of 16 / 4 heads of 128, 255 .. 16000 keys, 4 bits: 51 us, 214 MB at 4.2 TB/s; one token, 4096 keys: 7.9.  Of the vector
+// 4.3 TB/s; 48 tokens of 16 / 4 heads of 128, 255 .. 16000 keys, 4 bits: 49 us, 214 MB at 4.3 TB/s; one token, 4096 keys: 7.5.  Of the vector
 // instructions of the 32 tokens two fifths are the start of the items, of nine blocks each; fewer and longer ones leave the memory idle (target_of).
 template <int D, int FMT>
 struct Quarter {
@@ -551,6 +551,7 @@ __device__ __forceinline__ void few_columns(const QuantArgs& qa, const PagedArgs
 // exponentials of the block before it and its product with the values.  bf16 rows' probabilities are rounded once: with their second part the error of y
 // would go from 2.3e-3 to its own rounding's 1.7e-3, for half as many matrix instructions again.  One prompt of 8192 rows, 18 / 6 heads of 64: 246 us,
 // 0.94 PFLOP/s with the queries' second part; 512 rows beside 31 tokens, 100 .. 8192 keys: 62 us, vector instructions half of it, matrix a quarter.
+// At heads of 128 with bf16 rows, two workgroups a CU, 57 (8 bits) and 39 (4 bits) vector registers live in scratch, 168 and 156 bytes a lane.
 template <int D>
 struct ManyShape {
   static constexpr int kBK = D == 128 ? 32 : 64, kRB = 2 * kTileDim<D>, kTileBytes = kBK * kRB, kStageBytes = 2 * kTileBytes, kStages = 3;
@@ -700,8 +701,8 @@ __device__ __forceinline__ void many_columns(const QuantArgs& qa, const PagedArg
   st.clear();
   bool odd = false;
   typedef f32x16 Scores[1];
-  // Keys of the block after this one: at head_dim 64 read as soon as they are there, beside the decoding of a later tile's codes; at 128 there are no
-  // registers for that (with them in scratch six prompts take 301 us instead of 288).
+  // Keys of the block after this one: read as soon as they are there, beside the decoding of a later tile's codes; at head_dim 128 there are no
+  // registers for that (with more of them in scratch six prompts take 301 us instead of 288).
   constexpr bool EARLY = D != 128;
   typedef bf16x8 Keys[KS];
   auto read_keys = [&](uint32_t block, Keys& k) {
@@ -827,7 +828,8 @@ __global__ __launch_bounds__(64, kFewWaves<D>) void paged_quant_few_kernel(Args 
   if (!it.valid) return;
   const QuantArgs qa = quant_of(args);
   // one where a second would not leave the registers for the waves: 48 tokens of heads of 128 at 8 bits 97 -> 89 us, with fp32 rows 142 -> 91, at 4 bits the
-  // other way for bf16 rows (57 and 58); 128 tokens of heads of 64 in fp32 59 -> 52 with the third wave, 32 in bf16 the other way (30.7 and 32.1)
+  // other way for bf16 rows (57 and 58); 128 tokens of heads of 64 in fp32 59 -> 52 with the third wave, 32 in bf16 the other way (30.7 and 32.1).
+  // The kernel below has two for all: its registers go by the items of many columns.
   constexpr int AHEAD = sizeof(E) == 2 && Codes<FMT>::row_bytes(D) <= 64 ? 2 : 1;
   few_columns<E, D, FMT, AHEAD>(qa, a, it, rep, lane, lds_addr_of(lds), gsm);
 }
